@@ -251,6 +251,46 @@ FGG_API int fgg_mx_grouped_gemm(const FggMxProblem* p, void* workspace, size_t w
                         void* stream);
 
 /* ------------------------------------------------------------------------ */
+/* bf16 / fp16 products grouped by expert, forward and both gradients        */
+/* ------------------------------------------------------------------------ */
+
+/* No counterpart in the reference operator (FP4 only, forward only): the same
+ * contiguous M-grouped layout for experts that stay in 16 bits, and for their
+ * training.  Group g owns rows [offsets[g], offsets[g+1]) of the token tensors;
+ * the offsets may be written by an earlier kernel on the stream.
+ *   direction 0, forward  a = x  [max_rows, K], b = w [G, N, K]:
+ *                         out[r, :] = W_g x_r, [max_rows, N]
+ *   direction 1, dgrad    a = dy [max_rows, N], b = w [G, N, K]:
+ *                         out[r, :] = W_g^T dy_r, [max_rows, K]
+ *   direction 2, wgrad    a = dy [max_rows, N], b = x [max_rows, K]:
+ *                         out[g] = sum_r dy_r x_r^T, [G, N, K]; an empty group's
+ *                         is zero; with accumulate != 0 (fp32 only) it is added
+ *                         to what out holds.
+ * N and K are multiples of 8; every tensor is contiguous and 16-byte aligned.
+ * Sums are held in fp32 and rounded once (fp16 results past 65504 become
+ * infinite).  Rows outside every group are neither read for any output nor
+ * written.  Malformed offsets (decreasing, negative, past max_rows) run no
+ * tile and leave status 0x203 in the workspace. */
+typedef struct FggF16RowsProblem {
+  int32_t num_groups;
+  int32_t n;
+  int32_t k;
+  int32_t max_rows;
+  int32_t dtype;      /* operands: 1 bf16, 2 fp16                               */
+  int32_t out_dtype;  /* as dtype; wgrad also 0 = fp32                          */
+  int32_t accumulate; /* wgrad with out_dtype 0: add to out                     */
+  const int32_t* offsets; /* device int32 [G + 1], nondecreasing, <= max_rows   */
+  const void* a;
+  const void* b;
+  void* out;
+} FggF16RowsProblem;
+
+/* Workspace (128-byte aligned) of one call; 0 for a bad problem. */
+FGG_API size_t fgg_f16_rows_workspace_bytes(const FggF16RowsProblem* p, int32_t direction);
+FGG_API int fgg_f16_grouped_gemm_rows(const FggF16RowsProblem* p, int32_t direction,
+                                      void* workspace, size_t ws_bytes, void* stream);
+
+/* ------------------------------------------------------------------------ */
 /* Expert-parallel MoE: the byte-moving kernels around the grouped GEMM      */
 /* ------------------------------------------------------------------------ */
 

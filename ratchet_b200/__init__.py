@@ -6,6 +6,7 @@ per-group-list operator `nvfp4_grouped_gemm`, both on one hand-written tcgen05
 kernel behind the C ABI in include/fgg_api.h.
 """
 from ._lib import FggError
+from .f16 import grouped_gemm_rows, grouped_gemm_rows_dgrad, grouped_gemm_rows_wgrad
 from .ops import (WeightPack, clear_caches, fp4_grouped_gemm, interleave_gate_up, last_status,
                   nvfp4_expert_mlp, nvfp4_grouped_gemm, nvfp4_grouped_gemm_rows,
                   nvfp4_grouped_gemm_silu_mul, pack_weights, quantize_nvfp4)
@@ -13,5 +14,6 @@ from .ops import (WeightPack, clear_caches, fp4_grouped_gemm, interleave_gate_up
 __all__ = ["fp4_grouped_gemm", "nvfp4_grouped_gemm", "nvfp4_grouped_gemm_rows",
            "nvfp4_grouped_gemm_silu_mul",
            "interleave_gate_up", "nvfp4_expert_mlp", "pack_weights", "WeightPack",
+           "grouped_gemm_rows", "grouped_gemm_rows_dgrad", "grouped_gemm_rows_wgrad",
            "quantize_nvfp4", "last_status", "clear_caches", "FggError"]
 __version__ = "0.2.0"

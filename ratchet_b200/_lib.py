@@ -52,6 +52,13 @@ class FggMxProblem(ctypes.Structure):
                 ("reuse_prepared", ctypes.c_int32)]
 
 
+class FggF16RowsProblem(ctypes.Structure):
+    _fields_ = [("num_groups", ctypes.c_int32), ("n", ctypes.c_int32), ("k", ctypes.c_int32),
+                ("max_rows", ctypes.c_int32), ("dtype", ctypes.c_int32),
+                ("out_dtype", ctypes.c_int32), ("accumulate", ctypes.c_int32),
+                ("offsets", _VOIDP), ("a", _VOIDP), ("b", _VOIDP), ("out", _VOIDP)]
+
+
 class FggMoeTokens(ctypes.Structure):
     _fields_ = [("num_tokens", ctypes.c_int32), ("topk", ctypes.c_int32), ("k", ctypes.c_int32),
                 ("codes", _VOIDP), ("codes_stride", ctypes.c_int64),
@@ -94,6 +101,8 @@ _SIGS = {
     "fgg_nvfp4_rows_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(FggNvfp4RowsProblem)]),
     "fgg_nvfp4_grouped_gemm_rows": (ctypes.c_int, [ctypes.POINTER(FggNvfp4RowsProblem), _VOIDP, _VOIDP, ctypes.c_size_t, _VOIDP]),
     "fgg_nvfp4_grouped_gemm_noalloc": (ctypes.c_int, [ctypes.POINTER(FggNvfp4Problem), _VOIDP, _VOIDP, _VOIDP]),
+    "fgg_f16_rows_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(FggF16RowsProblem), ctypes.c_int32]),
+    "fgg_f16_grouped_gemm_rows": (ctypes.c_int, [ctypes.POINTER(FggF16RowsProblem), ctypes.c_int32, _VOIDP, ctypes.c_size_t, _VOIDP]),
     "fgg_moe_plan": (ctypes.c_int, [_VOIDP, ctypes.c_int32, ctypes.c_int32, _VOIDP, _VOIDP, ctypes.c_int32,
                                     ctypes.c_int32, ctypes.c_int32, _VOIDP, _VOIDP, _VOIDP, _VOIDP, _VOIDP]),
     "fgg_moe_gather_rows": (ctypes.c_int, [_VOIDP, _VOIDP, ctypes.c_int64, ctypes.c_int32, ctypes.c_int32,

@@ -1,0 +1,885 @@
+// fgg_f16.cu - products grouped by expert in bf16 / fp16, over contiguous token
+// rows with the group offsets on the device: the forward product and its two
+// gradients.
+//
+//   forward  y[r, n]    = sum_k x[r, k]  W_g[n, k]     r in group g
+//   dgrad    dx[r, k]   = sum_n dy[r, n] W_g[n, k]
+//   wgrad    dW_g[n, k] = sum_{r in g} dy[r, n] x[r, k]
+//
+// All three run one persistent kernel of CTA pairs (tcgen05 .cta_group::2,
+// .kind::f16, fp32 accumulators in TMEM).  The tensor core's M axis is the
+// weights' output axis (n forward, k dgrad, n wgrad), 256 per pair; its N axis
+// is the group's tokens (forward, dgrad: up to 256, in steps of 32, so that a
+// ragged group costs what its rows cost) or k (wgrad, 256).  No operand is
+// transposed in memory: where the contraction is not the contiguous axis
+// (W in dgrad, both operands in wgrad) the tiles are read MN-major, boxes of
+// 64 x 64 whose descriptor names the major axis.
+//
+// Ragged edges cost no branches in the main loop:
+//   * tokens behind a group's end (forward, dgrad) are the next group's: they
+//     only reach accumulator columns that are not stored;
+//   * in wgrad they would enter the sum, so every group has its own tensor maps
+//     (written on the device by the prepare kernel: base = the group's first
+//     row, extent = its rows) and TMA fills zeros behind the group's end,
+//     whatever the next group's rows hold;
+//   * n and k need not be multiples of the tile: TMA fills zeros, and the
+//     epilogues clip.
+//
+// What bounds it: the tensor pipe for groups of about 200 tokens and more, the
+// weights' HBM stream below that, the gradient's write for wgrad with short
+// groups.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+#include <cstring>
+
+#include "fgg_engine.cuh"
+#include "fgg_host.cuh"
+
+namespace fgg {
+namespace {
+
+constexpr int kFwd = 0, kDgrad = 1, kWgrad = 2;
+constexpr int kF16BadOffsets = 0x203;  // offsets decreasing, negative or past max_rows
+
+// Token boxes of 16, 32, ..., 128 rows: a CTA loads half of its tile's tokens.
+constexpr int kTokenMaps = 8;
+
+struct F16Slot {
+  int32_t g;     // group, -1 = no more tiles
+  int32_t mt;    // tile of the M axis
+  int32_t row0;  // first token row of the tile (forward, dgrad)
+  int32_t rows;  // tokens of the tile (forward, dgrad) / of the group (wgrad)
+  int32_t ct;    // tile of the N axis (wgrad)
+  int32_t pad[3];
+};
+static_assert(sizeof(F16Slot) == 32, "slot is 8 words");
+
+struct F16Params {
+  CUtensorMap tmap_w;                // forward, dgrad: [G, N, K] weights
+  CUtensorMap tmap_tok[kTokenMaps];  // forward, dgrad: [rows, contraction] tokens
+  CUtensorMap tmap_out;              // wgrad: [G, N, K] gradient
+  const CUtensorMap* tmap_a;         // wgrad: [G] maps of each group's dy rows
+  const CUtensorMap* tmap_b;         // wgrad: [G] maps of each group's x rows
+  const uint64_t* tiles;             // forward, dgrad: group << 48 | mt << 32 | first row
+  const int32_t* tile_rows;          // forward, dgrad: tokens of each tile
+  const int32_t* offsets;
+  void* out;
+  int* status;  // [0] status [1] tile counter [2] finished CTAs [3] tile count
+  int32_t num_groups;
+  int32_t m_ext;   // extent of the M axis (the output's columns; wgrad: its rows n)
+  int32_t c_ext;   // wgrad: extent of the N axis (k)
+  int32_t ksteps;  // forward, dgrad: 64-element steps of the contraction
+  int32_t mts, cts;
+  int32_t grid_tiles;  // host bound on the tiles
+  int32_t bf16;        // operands bf16 (1) or fp16 (0)
+  int32_t out_fp32;    // wgrad: fp32 gradient
+  int32_t accumulate;  // wgrad, fp32: add to the gradient
+  int32_t debug_flags;
+};
+
+__device__ __forceinline__ uint32_t pack_16(float lo, float hi, bool bf16) {
+  if (bf16) return pack_bf16x2(lo, hi);
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+template <int MODE_>
+struct F16Cfg {
+  static constexpr int MODE = MODE_;
+  static constexpr bool A_MN = MODE_ != kFwd;
+  static constexpr bool B_MN = MODE_ == kWgrad;
+  static constexpr int BN = 256;   // N axis of a pair tile
+  static constexpr int KS = 64;    // contraction per stage: one 128-byte swizzle row
+  static constexpr uint32_t A_BYTES = 128 * 128;
+  static constexpr uint32_t B_BYTES = 128 * 128;  // half of 256 columns
+  static constexpr uint32_t STAGE_BYTES = A_BYTES + B_BYTES;
+  static constexpr int STAGES = 6;
+  static constexpr uint32_t TMEM_COLS = 512;  // two accumulators of 256 columns
+  static constexpr int SCHED = 8;
+  // readers of a slot: leader producer, MMA warp, 4 epilogue warps; follower
+  // producer and 4 epilogue warps
+  static constexpr uint32_t SCHED_READERS = 11;
+  static constexpr uint32_t NBARS = 2 * STAGES + 4 + 2 * SCHED + 3;
+  // epilogue staging: forward, dgrad 1 KB per warp; wgrad two 4 KB boxes per warp
+  static constexpr uint32_t EPI_WARP = MODE_ == kWgrad ? 2 * 4096 : 1024;
+  static constexpr uint32_t EPI_REGION = STAGES * STAGE_BYTES;  // 1024 B aligned
+  static constexpr uint32_t BAR_REGION = EPI_REGION + 4 * EPI_WARP;
+  static constexpr uint32_t SMEM_BYTES = 1024 + BAR_REGION + 8 * NBARS + 32 * SCHED + 16;
+  static_assert(SMEM_BYTES <= 232448, "shared memory budget exceeded");
+};
+
+// ------------------------------------------------------------- epilogues
+// Forward, dgrad.  The warp's 32 TMEM lanes are the output columns m0 + lane,
+// its TMEM columns the tile's tokens.  Sixteen tokens at a time are transposed
+// through 1 KB of the warp's shared memory so that every lane stores 16
+// contiguous bytes (see epilogue_tile of the block-scaled kernels, whose
+// layout this shares); columns past the output's edge are not stored.
+__device__ __forceinline__ void f16_epilogue_rows(void* out, int ldn, int m0, size_t row0, int rows,
+                                                  int ncols, bool bf16, uint32_t taddr,
+                                                  uint32_t* stage) {
+  const int lane = threadIdx.x & 31;
+  const bool odd = lane & 1;
+  const int seg = lane & 3;
+  const bool col_ok = m0 + 8 * seg < ldn;
+  uint16_t* const o = static_cast<uint16_t*>(out);
+  for (int c0 = 0; c0 < ncols; c0 += 16) {
+    uint32_t r[16];
+    tmem_ld16(taddr + c0, r);
+    tmem_wait_ld();
+#pragma unroll
+    for (int j = 0; j < 16; j += 2) {
+      const float v0 = __uint_as_float(r[j]), v1 = __uint_as_float(r[j + 1]);
+      const float got = __shfl_xor_sync(kFullMask, odd ? v0 : v1, 1);
+      stage[(j + (odd ? 1 : 0)) * 16 + (lane >> 1)] =
+          odd ? pack_16(got, v1, bf16) : pack_16(v0, got, bf16);
+    }
+    __syncwarp();
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int t = (lane >> 2) + 8 * h;
+      const uint4 q = *reinterpret_cast<const uint4*>(stage + t * 16 + 4 * seg);
+      if (c0 + t < rows && col_ok)
+        *reinterpret_cast<uint4*>(o + (row0 + size_t(c0 + t)) * size_t(ldn) + size_t(m0 + 8 * seg)) =
+            q;
+    }
+    __syncwarp();
+  }
+}
+
+// Wgrad.  The warp's TMEM lanes are gradient rows n0 + lane, its columns k.
+// 128 bytes of every row at a time go through one of two 4 KB boxes (written
+// in the 128-byte swizzle, free of bank conflicts) into a TMA store, which
+// clips at the gradient's bounds; or into an adding store.
+__device__ __forceinline__ void f16_epilogue_wgrad(const F16Params& p, int g, int n0, int k0,
+                                                   bool empty, uint32_t taddr, uint32_t stage,
+                                                   uint32_t& box) {
+  const int lane = threadIdx.x & 31;
+  const int cw = p.out_fp32 ? 32 : 64;  // columns per box
+  const int kcols = min(256, p.c_ext - k0);
+  if (n0 >= p.m_ext) return;
+  for (int c0 = 0; c0 < kcols; c0 += cw) {
+    uint32_t v[32];
+    if (empty) {
+#pragma unroll
+      for (int j = 0; j < 32; ++j) v[j] = 0u;
+    } else if (p.out_fp32) {
+      tmem_ld32(taddr + c0, v);
+      tmem_wait_ld();
+    } else {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t r[32];
+        tmem_ld32(taddr + c0 + 32 * h, r);
+        tmem_wait_ld();
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          v[16 * h + j] = pack_16(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]),
+                                  p.bf16 != 0);
+      }
+    }
+    // the store issued from this box two steps ago has read it
+    if (lane == 0) bulk_wait_read<1>();
+    __syncwarp();
+    const uint32_t at = stage + (box & 1u) * 4096u + uint32_t(lane) * 128u;
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + ((u ^ (lane & 7)) << 4)),
+                   "r"(v[4 * u]), "r"(v[4 * u + 1]), "r"(v[4 * u + 2]), "r"(v[4 * u + 3])
+                   : "memory");
+    fence_async_shared();
+    __syncwarp();
+    if (lane == 0) {
+      const uint32_t src = stage + (box & 1u) * 4096u;
+      if (p.accumulate)
+        tma_add_3d(&p.tmap_out, src, k0 + c0, n0, g);
+      else
+        tma_store_3d(&p.tmap_out, src, k0 + c0, n0, g);
+      bulk_commit();
+    }
+    ++box;
+  }
+}
+
+// ------------------------------------------------------------ the kernel
+__device__ __forceinline__ F16Slot f16_read_slot(const volatile F16Slot* ring, int slot) {
+  F16Slot s;
+  s.g = ring[slot].g;
+  s.mt = ring[slot].mt;
+  s.row0 = ring[slot].row0;
+  s.rows = ring[slot].rows;
+  s.ct = ring[slot].ct;
+  return s;
+}
+
+template <int MODE>
+__device__ __forceinline__ F16Slot f16_make_slot(const F16Params& p, int t, int num_tiles) {
+  F16Slot s;
+  s.g = -1;
+  s.mt = s.row0 = s.rows = s.ct = 0;
+  if (t >= num_tiles) return s;
+  if constexpr (MODE == kWgrad) {
+    const int per = p.mts * p.cts;
+    s.g = t / per;
+    const int local = t - s.g * per;
+    s.mt = local / p.cts;
+    s.ct = local - s.mt * p.cts;
+    s.rows = __ldg(p.offsets + s.g + 1) - __ldg(p.offsets + s.g);
+  } else {
+    const uint64_t tile = __ldg(p.tiles + t);
+    s.g = int(tile >> 48);
+    s.mt = int((tile >> 32) & 0xFFFFu);
+    s.row0 = int(uint32_t(tile));
+    s.rows = __ldg(p.tile_rows + t);
+  }
+  return s;
+}
+
+// Roles as in the block-scaled pair kernel (fgg_engine.cuh): warp 0 producer in
+// both CTAs, warp 1 MMA issuer in the leader, warp 2 TMEM, warp 3 scheduler in
+// the leader, warps 4-7 epilogue.
+template <class C>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
+    f16_pair_kernel(const __grid_constant__ F16Params p) {
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  uint8_t* const gbase = smem_raw + (base - raw);
+
+  const uint32_t bars = base + C::BAR_REGION;
+  auto full_bar = [&](int s) { return bars + 8u * s; };
+  auto empty_bar = [&](int s) { return bars + 8u * (C::STAGES + s); };
+  auto accf_bar = [&](int b) { return bars + 8u * (2 * C::STAGES + b); };
+  auto acce_bar = [&](int b) { return bars + 8u * (2 * C::STAGES + 2 + b); };
+  auto schedf_bar = [&](int i) { return bars + 8u * (2 * C::STAGES + 4 + i); };
+  auto schede_bar = [&](int i) { return bars + 8u * (2 * C::STAGES + 4 + C::SCHED + i); };
+  const uint32_t tmem_ready_bar = bars + 8u * (2 * C::STAGES + 4 + 2 * C::SCHED);
+  const uint32_t drain_bar = tmem_ready_bar + 8u;
+  const uint32_t taken_bar = tmem_ready_bar + 16u;
+  uint8_t* const misc = gbase + C::BAR_REGION + 8 * C::NBARS;
+  volatile F16Slot* const ring = reinterpret_cast<volatile F16Slot*>(misc);
+  volatile uint32_t* const tmem_holder =
+      reinterpret_cast<volatile uint32_t*>(misc + 32 * C::SCHED);
+  volatile int* const abort_flag = reinterpret_cast<volatile int*>(misc + 32 * C::SCHED + 4);
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const bool leader = (rank == 0);
+  const uint32_t peer = rank ^ 1u;
+
+  auto sA = [&](int s) { return base + s * C::STAGE_BYTES; };
+  auto sB = [&](int s) { return base + s * C::STAGE_BYTES + C::A_BYTES; };
+  // MMA N of a tile: multiples of 32, so that each CTA holds a multiple of 16 rows
+  auto tile_ncols = [&](int rows) -> int {
+    return C::MODE == kWgrad ? C::BN : min(C::BN, (rows + 31) & ~31);
+  };
+  auto tile_ksteps = [&](int rows) -> int {
+    return C::MODE == kWgrad ? (rows + C::KS - 1) / C::KS : p.ksteps;
+  };
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::STAGES; ++s) {
+      mbar_init(full_bar(s), 1);
+      mbar_init(empty_bar(s), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(accf_bar(b), 1);
+      mbar_init(acce_bar(b), 8);  // 4 epilogue warps in each CTA (leader's barrier)
+    }
+    for (int i = 0; i < C::SCHED; ++i) {
+      mbar_init(schedf_bar(i), 1);
+      mbar_init(schede_bar(i), C::SCHED_READERS);  // used on the leader
+    }
+    mbar_init(tmem_ready_bar, 1);
+    mbar_init(drain_bar, 1);
+    mbar_init(taken_bar, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  cluster_sync();
+
+  if (warp == 2) {
+    tmem_alloc_pair(smem_u32(const_cast<uint32_t*>(tmem_holder)), C::TMEM_COLS);
+    tmem_relinquish_pair();
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(tmem_ready_bar);
+  }
+
+  // the tile list, the tensor maps and the status words come from the prepare
+  // kernel just before this launch, which it may overlap until here
+  griddep_wait();
+  const uint32_t leader_schede0 = mapa_shared(schede_bar(0), 0);
+  const uint32_t leader_acce0 = mapa_shared(acce_bar(0), 0);
+  const uint32_t leader_full0 = mapa_shared(full_bar(0), 0);
+  auto release_slot = [&](int slot) {
+    if (leader)
+      mbar_arrive(schede_bar(slot));
+    else
+      mbar_arrive_remote(leader_schede0 + 8u * slot);
+  };
+
+  if (warp == 3) {
+    // ---------------------------------------------- scheduler (leader only)
+    if (lane == 0 && leader) {
+      int slot = 0;
+      uint32_t sphase = 0;
+      const int num_tiles = p.status[3];
+      const uint32_t remote_ring0 = mapa_shared(smem_u32(const_cast<F16Slot*>(ring)), peer);
+      const uint32_t remote_schedf0 = mapa_shared(schedf_bar(0), peer);
+      for (uint32_t n = 0;; ++n) {
+        // at most one tile per pair that it has not started
+        if (n > 0 && !mbar_wait1(taken_bar, (n - 1) & 1u, abort_flag, p.status,
+                                 kStatusTimeoutProducer))
+          break;
+        const int t = atomicAdd(p.status + 1, 1);
+        const F16Slot s = f16_make_slot<C::MODE>(p, t, num_tiles);
+        if (!mbar_wait1<true>(schede_bar(slot), sphase ^ 1, abort_flag, p.status,
+                              kStatusTimeoutProducer))
+          break;
+        const uint32_t words[5] = {uint32_t(s.g), uint32_t(s.mt), uint32_t(s.row0),
+                                   uint32_t(s.rows), uint32_t(s.ct)};
+#pragma unroll
+        for (int i = 0; i < 5; ++i) {
+          reinterpret_cast<volatile uint32_t*>(ring + slot)[i] = words[i];
+          st_shared_remote_u32(remote_ring0 + 32u * slot + 4u * i, words[i]);
+        }
+        mbar_arrive(schedf_bar(slot));
+        mbar_arrive_remote(remote_schedf0 + 8u * slot);
+        if (++slot == C::SCHED) {
+          slot = 0;
+          sphase ^= 1;
+        }
+        if (s.g < 0) break;
+      }
+    }
+    __syncwarp();
+  } else if (warp == 0) {
+    // ------------------------------------------------- producer (both CTAs)
+    int stage = 0;
+    uint32_t phase = 0;
+    int slot = 0;
+    uint32_t sphase = 0;
+    uint32_t arms = 0;
+    if (C::MODE != kWgrad && lane == 0) {
+      prefetch_tensormap(&p.tmap_w);
+      prefetch_tensormap(&p.tmap_tok[kTokenMaps - 1]);
+    }
+    while (true) {
+      if (!mbar_wait<true>(schedf_bar(slot), sphase, abort_flag, p.status,
+                           kStatusTimeoutProducer))
+        break;
+      const int g = __shfl_sync(kFullMask, ring[slot].g, 0);
+      const int mt = __shfl_sync(kFullMask, ring[slot].mt, 0);
+      const int row0 = __shfl_sync(kFullMask, ring[slot].row0, 0);
+      const int rows = __shfl_sync(kFullMask, ring[slot].rows, 0);
+      const int ct = __shfl_sync(kFullMask, ring[slot].ct, 0);
+      if (lane == 0) {
+        release_slot(slot);
+        if (leader) mbar_arrive(taken_bar);
+      }
+      if (++slot == C::SCHED) {
+        slot = 0;
+        sphase ^= 1;
+      }
+      if (g < 0) {
+        if (lane == 0) griddep_launch_dependents();  // no new tiles for this CTA
+        break;
+      }
+      if (g >= p.num_groups) {  // the group indexes descriptor arrays: never trusted blindly
+        if (lane == 0) {
+          atomicCAS(p.status, 0, kStatusBadTile);
+          *abort_flag = 1;
+        }
+        break;
+      }
+      const int half = tile_ncols(rows) >> 1;
+      const int ksteps = tile_ksteps(rows);
+      // bytes that both CTAs' loads of one step deliver to the leader's barrier
+      const uint32_t tx_step = 2u * (C::A_BYTES + uint32_t(half) * 128u);
+      const int m0 = mt * 256 + int(rank) * 128;     // this CTA's rows of the M axis
+      const int tok = row0 + int(rank) * half;       // forward, dgrad: its tokens
+      const int c0 = ct * 256 + int(rank) * 128;     // wgrad: its columns k
+      const CUtensorMap* ta = nullptr;
+      const CUtensorMap* tb = nullptr;
+      if constexpr (C::MODE == kWgrad) {
+        ta = p.tmap_a + g;
+        tb = p.tmap_b + g;
+        tensormap_acquire(ta);
+        tensormap_acquire(tb);
+      } else {
+        tb = &p.tmap_tok[half / 16 - 1];
+      }
+      bool ok = true;
+      for (int ks = 0; ks < ksteps; ++ks) {
+        if (!mbar_wait(empty_bar(stage), phase ^ 1, abort_flag, p.status,
+                       kStatusTimeoutProducer)) {
+          ok = false;
+          break;
+        }
+        const uint32_t fb = leader_full0 + 8u * stage;
+        const int x = ks * C::KS;
+        const bool arm = (p.debug_flags & kDebugNoLoads) == 0;
+        if (arm && elect_one()) {
+          if (leader) mbar_arrive_expect_tx(full_bar(stage), tx_step);
+          if constexpr (C::MODE == kFwd) {
+            tma_load_3d_pair(sA(stage), &p.tmap_w, fb, x, m0, g);
+            tma_load_2d_pair(sB(stage), tb, fb, x, tok);
+          } else if constexpr (C::MODE == kDgrad) {
+            tma_load_3d_pair(sA(stage), &p.tmap_w, fb, m0, x, g);
+            tma_load_3d_pair(sA(stage) + 8192u, &p.tmap_w, fb, m0 + 64, x, g);
+            tma_load_2d_pair(sB(stage), tb, fb, x, tok);
+          } else {
+            tma_load_2d_pair(sA(stage), ta, fb, m0, x);
+            tma_load_2d_pair(sA(stage) + 8192u, ta, fb, m0 + 64, x);
+            tma_load_2d_pair(sB(stage), tb, fb, c0, x);
+            tma_load_2d_pair(sB(stage) + 8192u, tb, fb, c0 + 64, x);
+          }
+        }
+        __syncwarp();
+        if (arm) ++arms;
+        if (++stage == C::STAGES) {
+          stage = 0;
+          phase ^= 1;
+        }
+      }
+      if (!ok) break;
+    }
+    // the leader's full barriers cover both CTAs' bytes: they land before exit
+    if (leader && lane == 0) {
+      const uint32_t first = arms > uint32_t(C::STAGES) ? arms - C::STAGES : 0u;
+      for (uint32_t a = first; a < arms; ++a)
+        mbar_wait_one(full_bar(int(a % C::STAGES)), (a / C::STAGES) & 1u, 200000000ull);
+    }
+    __syncwarp();
+  } else if (warp == 1 && leader) {
+    // ------------------------------------------------------- MMA issuer
+    bool ok = mbar_wait(tmem_ready_bar, 0, abort_flag, p.status, kStatusTimeoutMma);
+    tc_fence_after();
+    const uint32_t tmem = __shfl_sync(kFullMask, *tmem_holder, 0);
+    int stage = 0;
+    uint32_t phase = 0;
+    int slot = 0;
+    uint32_t sphase = 0;
+    uint32_t lt = 0;
+    bool issued_any = false;
+    while (ok) {
+      if (!mbar_wait<true>(schedf_bar(slot), sphase, abort_flag, p.status, kStatusTimeoutMma))
+        break;
+      const int g = __shfl_sync(kFullMask, ring[slot].g, 0);
+      const int rows = __shfl_sync(kFullMask, ring[slot].rows, 0);
+      if (lane == 0) mbar_arrive(schede_bar(slot));
+      if (++slot == C::SCHED) {
+        slot = 0;
+        sphase ^= 1;
+      }
+      if (g < 0) break;
+      const int ncols = tile_ncols(rows);
+      const int ksteps = tile_ksteps(rows);
+      const uint32_t b = lt & 1u;
+      if (!mbar_wait(acce_bar(b), ((lt >> 1) & 1u) ^ 1u, abort_flag, p.status, kStatusTimeoutMma))
+        break;
+      tc_fence_after();
+      const uint32_t d_tmem = tmem + b * C::BN;
+      const uint32_t idesc =
+          idesc_f16(p.bf16 ? 1u : 0u, C::A_MN ? 1u : 0u, C::B_MN ? 1u : 0u, 256, ncols);
+      for (int ks = 0; ks < ksteps; ++ks) {
+        if (!mbar_wait(full_bar(stage), phase, abort_flag, p.status, kStatusTimeoutMma)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint64_t adesc = C::A_MN ? desc_mn_sw128(sA(stage), 8192u) : desc_k_sw128(sA(stage));
+        const uint64_t bdesc = C::B_MN ? desc_mn_sw128(sB(stage), 8192u) : desc_k_sw128(sB(stage));
+        // 16 of the contraction: 32 bytes of a K-major row, 16 rows of an MN-major tile
+        constexpr uint32_t kStepA = C::A_MN ? 2048u >> 4 : 32u >> 4;
+        constexpr uint32_t kStepB = C::B_MN ? 2048u >> 4 : 32u >> 4;
+        if (elect_one()) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            tc_mma_f16_pair(d_tmem, adesc + kStepA * j, bdesc + kStepB * j, idesc,
+                            (ks | j) != 0 ? 1u : 0u);
+          tc_commit_pair(empty_bar(stage), 0x3);
+          if (ks + 1 == ksteps) tc_commit_pair(accf_bar(b), 0x3);
+        }
+        __syncwarp();
+        issued_any = true;
+        if (++stage == C::STAGES) {
+          stage = 0;
+          phase ^= 1;
+        }
+      }
+      if (!ok) break;
+      // an empty group's gradient tile (wgrad): nothing to multiply, zeros to store
+      if (ksteps == 0) {
+        if (elect_one()) tc_commit_pair(accf_bar(b), 0x3);
+        __syncwarp();
+        issued_any = true;
+      }
+      ++lt;
+    }
+    if (issued_any) {
+      if (elect_one()) {
+        tc_commit_pair(drain_bar, 0x1);
+        if (!mbar_wait_one(drain_bar, 0, 200000000ull))
+          atomicCAS(p.status, 0, kStatusTimeoutDrain);
+      }
+    }
+    __syncwarp();
+  } else if (warp >= 4) {
+    // --------------------------------------------------------- epilogue
+    const int q = warp & 3;
+    bool ok = mbar_wait(tmem_ready_bar, 0, abort_flag, p.status, kStatusTimeoutEpilogue);
+    tc_fence_after();
+    const uint32_t tmem = *tmem_holder;
+    const uint32_t stage_off = C::EPI_REGION + uint32_t(q) * C::EPI_WARP;
+    int slot = 0;
+    uint32_t sphase = 0;
+    uint32_t lt = 0;
+    uint32_t box = 0;
+    while (ok) {
+      if (!mbar_wait<true>(schedf_bar(slot), sphase, abort_flag, p.status,
+                           kStatusTimeoutEpilogue))
+        break;
+      const F16Slot s = f16_read_slot(ring, slot);
+      __syncwarp();
+      if (lane == 0) release_slot(slot);
+      if (++slot == C::SCHED) {
+        slot = 0;
+        sphase ^= 1;
+      }
+      if (s.g < 0) break;
+      const uint32_t b = lt & 1u;
+      if (!mbar_wait(accf_bar(b), (lt >> 1) & 1u, abort_flag, p.status, kStatusTimeoutEpilogue))
+        break;
+      tc_fence_after();
+      const int m0 = s.mt * 256 + int(rank) * 128 + q * 32;
+      const uint32_t taddr = tmem + (uint32_t(q * 32) << 16) + b * C::BN;
+      if constexpr (C::MODE == kWgrad) {
+        if (s.rows > 0 || !p.accumulate)
+          f16_epilogue_wgrad(p, s.g, m0, s.ct * 256, s.rows == 0, taddr, base + stage_off, box);
+      } else {
+        if (m0 < p.m_ext)
+          f16_epilogue_rows(p.out, p.m_ext, m0, size_t(s.row0), s.rows, tile_ncols(s.rows),
+                            p.bf16 != 0, taddr, reinterpret_cast<uint32_t*>(gbase + stage_off));
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if (leader)
+          mbar_arrive(acce_bar(b));
+        else
+          mbar_arrive_remote(leader_acce0 + 8u * b);
+      }
+      ++lt;
+    }
+    // stores in flight read this CTA's shared memory
+    if (C::MODE == kWgrad && lane == 0) bulk_wait<0>();
+  }
+
+  __syncthreads();
+  // the leader's MMAs write the follower's TMEM and read its shared memory
+  cluster_sync();
+  if (warp == 2) {
+    tc_fence_after();
+    tmem_dealloc_pair(*tmem_holder, C::TMEM_COLS);
+  }
+}
+
+// ---------------------------------------------------------------- prepare
+struct F16PrepParams {
+  CUtensorMap tmpl_a, tmpl_b;  // wgrad: one group's geometry
+  const int32_t* offsets;
+  const uint8_t* a;  // wgrad: dy, x
+  const uint8_t* b;
+  CUtensorMap* tmap_a;
+  CUtensorMap* tmap_b;
+  uint64_t* tiles;
+  int32_t* tile_rows;
+  int* status;
+  int64_t row_bytes_a, row_bytes_b;
+  int32_t num_groups, max_rows, mts, tile_cap;
+  int32_t wgrad_tiles;  // wgrad: every group's tiles; 0 = forward, dgrad
+};
+
+// Token tiles of a group of m rows: the fewest of at most 256 rows, of equal
+// size up to a multiple of 32 (two of 160 and 140 for 300 rows, not 256 and 44:
+// an MMA of 44 columns takes the time of 64).
+__device__ __forceinline__ int f16_tile_count(int m) { return (m + 255) / 256; }
+__device__ __forceinline__ int f16_tile_height(int m, int count) {
+  return ((m + count - 1) / count + 31) & ~31;
+}
+
+// Every block scans the groups' tile counts (at most 512) in shared memory and
+// writes its share of the tile list, group by group, a weight tile's token
+// tiles next to each other (they share it in L2); or its share of the groups'
+// tensor maps (wgrad).
+__global__ void __launch_bounds__(256) f16_prepare_kernel(const __grid_constant__ F16PrepParams p) {
+  griddep_launch_dependents();
+  griddep_wait();
+  __shared__ int32_t soff[FGG_MAX_GROUPS + 1];
+  __shared__ int32_t sbegin[FGG_MAX_GROUPS + 1];
+  __shared__ int32_t swarp[8];
+  __shared__ int s_bad;
+  __shared__ alignas(128) CUtensorMap smap[8];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int G = p.num_groups;
+  if (threadIdx.x == 0) s_bad = 0;
+  for (int i = threadIdx.x; i <= G; i += 256) soff[i] = __ldg(p.offsets + i);
+  __syncthreads();
+  // two groups per thread cover FGG_MAX_GROUPS
+  static_assert(FGG_MAX_GROUPS <= 512, "two groups per thread");
+  int cnt[2], run = 0;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int g = 2 * threadIdx.x + i;
+    cnt[i] = 0;
+    if (g < G) {
+      const int lo = soff[g], hi = soff[g + 1];
+      if (lo < 0 || hi < lo || hi > p.max_rows)
+        s_bad = 1;
+      else
+        cnt[i] = f16_tile_count(hi - lo);
+    }
+    run += cnt[i];
+  }
+  int incl = run;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(kFullMask, incl, o);
+    if (lane >= o) incl += y;
+  }
+  if (lane == 31) swarp[warp] = incl;
+  __syncthreads();
+  int acc = incl - run;
+  for (int w = 0; w < warp; ++w) acc += swarp[w];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int g = 2 * threadIdx.x + i;
+    if (g <= G) sbegin[g] = acc;
+    acc += cnt[i];
+  }
+  if (threadIdx.x == 255 && G == 512) sbegin[512] = acc;
+  __syncthreads();
+  int num_tiles = p.wgrad_tiles > 0 ? p.wgrad_tiles : sbegin[G] * p.mts;
+  if (s_bad || num_tiles > p.tile_cap) num_tiles = 0;
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    p.status[0] = s_bad ? kF16BadOffsets : 0;
+    p.status[1] = 0;
+    p.status[2] = 0;
+    p.status[3] = num_tiles;
+  }
+  if (num_tiles == 0) return;
+  if (p.wgrad_tiles > 0) {
+    for (int i = blockIdx.x * 8 + warp; i < 2 * G; i += gridDim.x * 8) {
+      const int g = i >> 1;
+      const bool is_b = i & 1;
+      const uint32_t* src = reinterpret_cast<const uint32_t*>(is_b ? &p.tmpl_b : &p.tmpl_a);
+      reinterpret_cast<uint32_t*>(&smap[warp])[lane] = src[lane];
+      __syncwarp();
+      if (lane == 0) {
+        const uint8_t* at = is_b ? p.b + int64_t(soff[g]) * p.row_bytes_b
+                                 : p.a + int64_t(soff[g]) * p.row_bytes_a;
+        // an empty group's maps are never used: any valid address will do
+        const int m = soff[g + 1] - soff[g];
+        tmap_replace_address(smem_u32(&smap[warp]),
+                             reinterpret_cast<uint64_t>(m > 0 ? at : (is_b ? p.b : p.a)));
+        tmap_replace_dim1(smem_u32(&smap[warp]), max(m, 1));
+      }
+      __syncwarp();
+      tmap_publish((is_b ? p.tmap_b : p.tmap_a) + g, smem_u32(&smap[warp]));
+      __syncwarp();
+    }
+    return;
+  }
+  for (int t = blockIdx.x * 256 + threadIdx.x; t < num_tiles; t += gridDim.x * 256) {
+    // the group whose tiles (token tiles x mts) hold t
+    int lo = 0, hi = G;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (sbegin[mid] * p.mts <= t)
+        lo = mid;
+      else
+        hi = mid;
+    }
+    const int m = soff[lo + 1] - soff[lo];
+    const int count = sbegin[lo + 1] - sbegin[lo];
+    const int height = f16_tile_height(m, count);
+    const int local = t - sbegin[lo] * p.mts;
+    const int mt = local / count, xt = local - mt * count;
+    p.tiles[t] = (uint64_t(lo) << 48) | (uint64_t(mt) << 32) | uint32_t(soff[lo] + xt * height);
+    p.tile_rows[t] = min(height, m - xt * height);
+  }
+}
+
+// ------------------------------------------------------------------- host
+struct F16Layout {
+  int mts = 0, cts = 0, tile_cap = 0;
+  size_t status = 0, tiles = 0, tile_rows = 0, tmap_a = 0, tmap_b = 0, total = 0;
+};
+
+int plan_f16(const FggF16RowsProblem* p, int direction, F16Layout* L) {
+  if (p == nullptr) return set_error(FGG_EINVAL, "problem is null");
+  if (direction < kFwd || direction > kWgrad)
+    return set_error(FGG_EINVAL, "direction=%d must be 0 (forward), 1 (dgrad) or 2 (wgrad)",
+                     direction);
+  const int G = p->num_groups;
+  if (G < 1 || G > FGG_MAX_GROUPS)
+    return set_error(FGG_EINVAL, "num_groups=%d outside [1, %d]", G, FGG_MAX_GROUPS);
+  if (p->n < 8 || p->n % 8 != 0 || p->k < 8 || p->k % 8 != 0)
+    return set_error(FGG_EBADSHAPE, "N=%d and K=%d must be positive multiples of 8", p->n, p->k);
+  if (p->max_rows < 0) return set_error(FGG_EINVAL, "max_rows=%d is negative", p->max_rows);
+  if (p->dtype != 1 && p->dtype != 2)
+    return set_error(FGG_EINVAL, "dtype=%d must be 1 (bf16) or 2 (fp16)", p->dtype);
+  if (p->out_dtype != p->dtype && !(direction == kWgrad && p->out_dtype == 0))
+    return set_error(FGG_EINVAL, "out_dtype=%d must be the operands' type%s", p->out_dtype,
+                     direction == kWgrad ? " or 0 (fp32)" : "");
+  if (p->accumulate != 0 && (direction != kWgrad || p->out_dtype != 0))
+    return set_error(FGG_EINVAL, "accumulate needs a weight gradient in fp32");
+  const int m_ext = direction == kDgrad ? p->k : p->n;
+  L->mts = (m_ext + 255) / 256;
+  L->cts = (p->k + 255) / 256;
+  if (L->mts > 0xFFFF) return set_error(FGG_EBADSHAPE, "N=%d or K=%d too large", p->n, p->k);
+  Carver cv;
+  L->status = cv.take(kStatusBytes, 256);
+  int64_t cap;
+  if (direction == kWgrad) {
+    cap = int64_t(G) * L->mts * L->cts;
+    L->tmap_a = cv.take(size_t(G) * sizeof(CUtensorMap), 128);
+    L->tmap_b = cv.take(size_t(G) * sizeof(CUtensorMap), 128);
+  } else {
+    // sum over groups of ceil(m / 256) <= rows / 256 + groups (and <= rows)
+    cap = std::min<int64_t>(int64_t(p->max_rows) / 256 + G, p->max_rows) * L->mts;
+    L->tiles = cv.take(size_t(std::max<int64_t>(cap, 1)) * 8, 256);
+    L->tile_rows = cv.take(size_t(std::max<int64_t>(cap, 1)) * 4, 256);
+  }
+  // the tile counter runs past the last tile by one claim per pair
+  if (cap > INT32_MAX - 4096) return set_error(FGG_EBADSHAPE, "problem too large");
+  L->tile_cap = int(cap);
+  L->total = cv.off;
+  return FGG_OK;
+}
+
+constexpr CUtensorMapDataType kMap16 = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;  // moved as bits
+
+template <int MODE>
+int launch_f16(const F16Params& gp, const DeviceInfo& dev, cudaStream_t s) {
+  using C = F16Cfg<MODE>;
+  if (int rc = ensure_max_dynamic_smem(reinterpret_cast<const void*>(f16_pair_kernel<C>),
+                                       int(C::SMEM_BYTES)))
+    return rc;
+  const int pairs = std::max(1, std::min(gp.grid_tiles, dev.sm_count / 2));
+  const cudaError_t e = launch_dependent(f16_pair_kernel<C>, 2 * pairs, C::SMEM_BYTES, s, gp);
+  if (e != cudaSuccess) return set_error(FGG_ECUDA, "GEMM launch failed: %s", cudaGetErrorString(e));
+  return FGG_OK;
+}
+
+}  // namespace
+}  // namespace fgg
+
+using namespace fgg;
+
+extern "C" {
+
+size_t fgg_f16_rows_workspace_bytes(const FggF16RowsProblem* p, int32_t direction) {
+  F16Layout L;
+  if (plan_f16(p, direction, &L) != FGG_OK) return 0;
+  return L.total;
+}
+
+int fgg_f16_grouped_gemm_rows(const FggF16RowsProblem* p, int32_t direction, void* workspace,
+                              size_t ws_bytes, void* stream) {
+  F16Layout L;
+  if (int rc = plan_f16(p, direction, &L)) return rc;
+  if (workspace == nullptr) return set_error(FGG_EINVAL, "workspace is null");
+  if ((reinterpret_cast<uintptr_t>(workspace) & 127u) != 0)
+    return set_error(FGG_EALIGN, "workspace must be 128-byte aligned");
+  if (ws_bytes < L.total)
+    return set_error(FGG_EWORKSPACE, "workspace has %zu bytes, needs %zu", ws_bytes, L.total);
+  if (p->offsets == nullptr || p->out == nullptr) {
+    // without rows the token tensors may be null, and so may an empty output
+    if (p->offsets == nullptr || direction == kWgrad || p->max_rows > 0)
+      return set_error(FGG_EINVAL, "offsets / out is null");
+  }
+  if (p->max_rows > 0 && (p->a == nullptr || p->b == nullptr))
+    return set_error(FGG_EINVAL, "a / b is null");
+  if (!aligned16(p->a) || !aligned16(p->b) || !aligned16(p->out))
+    return set_error(FGG_EALIGN, "a, b and out must be 16-byte aligned");
+  if (!aligned4(p->offsets)) return set_error(FGG_EALIGN, "offsets must be 4-byte aligned");
+  DeviceInfo dev;
+  if (int rc = current_device(&dev)) return rc;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  const uint64_t G = uint64_t(p->num_groups), N = uint64_t(p->n), K = uint64_t(p->k);
+  if (p->max_rows == 0) {
+    // no rows: nothing to write but an overwritten gradient, which is zero
+    FGG_CUDA_CHECK(cudaMemsetAsync(ws + L.status, 0, kStatusBytes, s));
+    if (direction == kWgrad && !p->accumulate)
+      FGG_CUDA_CHECK(cudaMemsetAsync(p->out, 0, G * N * K * (p->out_dtype == 0 ? 4 : 2), s));
+    return FGG_OK;
+  }
+  const uint64_t R = uint64_t(p->max_rows);
+
+  F16PrepParams pp;
+  memset(&pp, 0, sizeof(pp));
+  F16Params gp;
+  memset(&gp, 0, sizeof(gp));
+  pp.offsets = gp.offsets = p->offsets;
+  pp.status = gp.status = reinterpret_cast<int*>(ws + L.status);
+  pp.num_groups = gp.num_groups = p->num_groups;
+  pp.max_rows = p->max_rows;
+  pp.mts = gp.mts = L.mts;
+  gp.cts = L.cts;
+  pp.tile_cap = gp.grid_tiles = L.tile_cap;
+  gp.bf16 = p->dtype == 1 ? 1 : 0;
+  gp.out = p->out;
+  gp.debug_flags = debug_flags();
+  int blocks;
+  if (direction == kWgrad) {
+    // one group's maps: the prepare kernel sets each group's base and rows
+    if (int rc = encode_2d(&pp.tmpl_a, kMap16, p->a, N, R, N * 2, 64, 64)) return rc;
+    if (int rc = encode_2d(&pp.tmpl_b, kMap16, p->b, K, R, K * 2, 64, 64)) return rc;
+    pp.a = static_cast<const uint8_t*>(p->a);
+    pp.b = static_cast<const uint8_t*>(p->b);
+    pp.row_bytes_a = int64_t(N) * 2;
+    pp.row_bytes_b = int64_t(K) * 2;
+    pp.tmap_a = reinterpret_cast<CUtensorMap*>(ws + L.tmap_a);
+    pp.tmap_b = reinterpret_cast<CUtensorMap*>(ws + L.tmap_b);
+    pp.wgrad_tiles = L.tile_cap;
+    gp.tmap_a = pp.tmap_a;
+    gp.tmap_b = pp.tmap_b;
+    gp.m_ext = p->n;
+    gp.c_ext = p->k;
+    gp.out_fp32 = p->out_dtype == 0 ? 1 : 0;
+    gp.accumulate = p->accumulate != 0 ? 1 : 0;
+    const uint64_t eb = gp.out_fp32 ? 4 : 2;
+    if (int rc = encode_3d(&gp.tmap_out, gp.out_fp32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : kMap16,
+                           p->out, K, N, G, K * eb, N * K * eb, gp.out_fp32 ? 32 : 64, 32, 1))
+      return rc;
+    blocks = (2 * p->num_groups + 7) / 8;
+  } else {
+    const uint64_t ck = direction == kFwd ? K : N;  // contraction: the tokens' row length
+    if (int rc = encode_3d(&gp.tmap_w, kMap16, p->b, K, N, G, K * 2, N * K * 2, 64,
+                           direction == kFwd ? 128 : 64, 1))
+      return rc;
+    for (int i = 0; i < kTokenMaps; ++i)
+      if (int rc = encode_2d(&gp.tmap_tok[i], kMap16, p->a, ck, R, ck * 2, 64,
+                             uint32_t(16 * (i + 1))))
+        return rc;
+    pp.tiles = reinterpret_cast<uint64_t*>(ws + L.tiles);
+    pp.tile_rows = reinterpret_cast<int32_t*>(ws + L.tile_rows);
+    gp.tiles = pp.tiles;
+    gp.tile_rows = pp.tile_rows;
+    gp.m_ext = direction == kFwd ? p->n : p->k;
+    gp.ksteps = int((ck + 63) / 64);
+    blocks = std::min((L.tile_cap + 255) / 256, dev.sm_count);
+  }
+  FGG_CUDA_CHECK(launch_dependent(f16_prepare_kernel, std::max(blocks, 1), 0, s, pp));
+  if (direction == kFwd) return launch_f16<kFwd>(gp, dev, s);
+  if (direction == kDgrad) return launch_f16<kDgrad>(gp, dev, s);
+  return launch_f16<kWgrad>(gp, dev, s);
+}
+
+}  // extern "C"

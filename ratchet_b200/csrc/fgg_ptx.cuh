@@ -162,6 +162,41 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
       "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z)
       : "memory");
 }
+// Tiled store shared -> global, clipped at the tensor's bounds, and its
+// adding form (fp32 maps: every element is added once, in memory).
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, uint32_t src, int32_t x,
+                                             int32_t y, int32_t z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(
+          reinterpret_cast<uint64_t>(map)),
+      "r"(src), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+__device__ __forceinline__ void tma_add_3d(const CUtensorMap* map, uint32_t src, int32_t x,
+                                           int32_t y, int32_t z) {
+  asm volatile(
+      "cp.reduce.async.bulk.tensor.3d.global.shared::cta.add.bulk_group"
+      " [%0, {%2, %3, %4}], [%1];" ::"l"(reinterpret_cast<uint64_t>(map)),
+      "r"(src), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+__device__ __forceinline__ void bulk_commit() {
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+// At most N of this thread's bulk groups still read their shared memory / are
+// still incomplete.
+template <int N>
+__device__ __forceinline__ void bulk_wait_read() {
+  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void bulk_wait() {
+  asm volatile("cp.async.bulk.wait_group %0;" ::"n"(N) : "memory");
+}
+// This thread's shared-memory writes become visible to the async proxy (TMA).
+__device__ __forceinline__ void fence_async_shared() {
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
 // Plain (untiled) bulk copy global -> shared; 16-byte aligned, size % 16 == 0.
 __device__ __forceinline__ void bulk_g2s(uint32_t dst, const void* src, uint32_t bytes,
                                          uint32_t bar) {
@@ -372,6 +407,32 @@ __device__ __forceinline__ void tc_mma_mxf8f6f4_pair(uint32_t d_tmem, uint64_t a
       : "memory");
 }
 
+// 16-bit operands (bf16 x bf16 or fp16 x fp16), fp32 accumulation, K 16 per
+// instruction; the pair form computes 256 rows over both CTAs.
+__device__ __forceinline__ void tc_mma_f16_pair(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc,
+                                                uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// Each thread reads 32 consecutive 32-bit columns of its own TMEM lane.
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32"
+      " {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19,"
+      " %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
+        "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]),
+        "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+
 // Each thread reads 16 consecutive 32-bit columns of its own TMEM lane.
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
@@ -405,6 +466,12 @@ constexpr uint32_t kLayoutNone = 0;
 __device__ __forceinline__ uint64_t desc_k_sw128(uint32_t saddr) {
   return smem_desc(saddr, 16, 1024, kLayoutSwizzle128);
 }
+// MN-major 16-bit operand tile written by TMA with 128-byte swizzle in boxes of
+// 64 (M or N) elements x K rows: a K row is 128 bytes, 8 of them 1024 B, and the
+// next 64 elements follow `chunk_bytes` later.  Stepping K by 16 adds 2048 B.
+__device__ __forceinline__ uint64_t desc_mn_sw128(uint32_t saddr, uint32_t chunk_bytes) {
+  return smem_desc(saddr, chunk_bytes, 1024, kLayoutSwizzle128);
+}
 // Scale-factor atom (512 B = 32 rows x 16 B, core matrices of 8 x 16 B).
 __device__ __forceinline__ uint64_t desc_sf_atom(uint32_t saddr) {
   return smem_desc(saddr, 128, 128, kLayoutNone);
@@ -420,6 +487,14 @@ __host__ __device__ constexpr uint32_t idesc_block_scaled(uint32_t afmt, uint32_
                                                           uint32_t a_sf_id, uint32_t b_sf_id) {
   return (b_sf_id << 4) | (afmt << 7) | (bfmt << 10) | (uint32_t(n >> 3) << 17) |
          (scale_ue8m0 << 23) | (uint32_t(m >> 4) << 24) | (a_sf_id << 29);
+}
+// Instruction descriptor of .kind::f16 (same table): [4,6) accumulator (1 fp32)
+//   [7,10) A format  [10,13) B format (0 fp16, 1 bf16)  [15] A MN-major
+//   [16] B MN-major  [17,23) N>>3  [24,29) M>>4
+__host__ __device__ constexpr uint32_t idesc_f16(uint32_t fmt, uint32_t a_mn, uint32_t b_mn, int m,
+                                                 int n) {
+  return (1u << 4) | (fmt << 7) | (fmt << 10) | (a_mn << 15) | (b_mn << 16) |
+         (uint32_t(n >> 3) << 17) | (uint32_t(m >> 4) << 24);
 }
 constexpr uint32_t kFmtNvf4E2M1 = 1;   // .kind::mxf4nvf4 operand format E2M1
 constexpr uint32_t kFmtF8E4M3 = 0;     // .kind::mxf8f6f4 E4M3

@@ -21,6 +21,7 @@ Everything runs on the current CUDA stream; nothing here synchronises the host.
 from __future__ import annotations
 
 from collections import OrderedDict
+from contextlib import nullcontext
 from typing import Sequence
 
 import numpy as np
@@ -61,6 +62,11 @@ def _is_current(device: torch.device) -> bool:
     """True when `device` is the current CUDA device (no context switch needed)."""
     cur = _get_device() if _get_device is not None else torch.cuda.current_device()
     return device.index is None or device.index == cur
+
+
+def _on(device: torch.device):
+    """Context that makes `device` current (nothing to do when it is)."""
+    return nullcontext() if _is_current(device) else torch.cuda.device(device)
 
 
 # Workspaces reused per (device, stream): calls on one stream are ordered, so
