@@ -18,10 +18,10 @@
 // Ragged edges cost no branches in the main loop:
 //   * tokens behind a group's end (forward, dgrad) are the next group's: they
 //     only reach accumulator columns that are not stored;
-//   * in wgrad they would enter the sum, so every group has its own tensor maps
-//     (written on the device by the prepare kernel: base = the group's first
-//     row, extent = its rows) and TMA fills zeros behind the group's end,
-//     whatever the next group's rows hold;
+//   * in wgrad they would enter the sum (and an infinity there spoil it, even
+//     against a zero), so a group's last rows % 16 rows are read from a copy with
+//     zeros behind them, which the prepare kernel makes (16 rows per group and
+//     operand); the step before it multiplies only its whole sixteens of rows;
 //   * n and k need not be multiples of the tile: TMA fills zeros, and the
 //     epilogues clip.
 //
@@ -49,7 +49,7 @@ constexpr int kTokenMaps = 8;
 struct F16Slot {
   int32_t g;     // group, -1 = no more tiles
   int32_t mt;    // tile of the M axis
-  int32_t row0;  // first token row of the tile (forward, dgrad)
+  int32_t row0;  // first token row of the tile (wgrad: of the group)
   int32_t rows;  // tokens of the tile (forward, dgrad) / of the group (wgrad)
   int32_t ct;    // tile of the N axis (wgrad)
   int32_t pad[3];
@@ -59,9 +59,8 @@ static_assert(sizeof(F16Slot) == 32, "slot is 8 words");
 struct F16Params {
   CUtensorMap tmap_w;                // forward, dgrad: [G, N, K] weights
   CUtensorMap tmap_tok[kTokenMaps];  // forward, dgrad: [rows, contraction] tokens
-  CUtensorMap tmap_out;              // wgrad: [G, N, K] gradient
-  const CUtensorMap* tmap_a;         // wgrad: [G] maps of each group's dy rows
-  const CUtensorMap* tmap_b;         // wgrad: [G] maps of each group's x rows
+  CUtensorMap tmap_a, tmap_b;        // wgrad: dy [rows, N], x [rows, K]
+  CUtensorMap tmap_ta, tmap_tb;      // wgrad: the groups' last rows, [16 G, N], [16 G, K]
   const uint64_t* tiles;             // forward, dgrad: group << 48 | mt << 32 | first row
   const int32_t* tile_rows;          // forward, dgrad: tokens of each tile
   const int32_t* offsets;
@@ -102,8 +101,8 @@ struct F16Cfg {
   // producer and 4 epilogue warps
   static constexpr uint32_t SCHED_READERS = 11;
   static constexpr uint32_t NBARS = 2 * STAGES + 4 + 2 * SCHED + 3;
-  // epilogue staging: forward, dgrad 1 KB per warp; wgrad two 4 KB boxes per warp
-  static constexpr uint32_t EPI_WARP = MODE_ == kWgrad ? 2 * 4096 : 1024;
+  // epilogue staging of a warp: 16 tokens x 64 bytes; wgrad 32 rows x 128 bytes
+  static constexpr uint32_t EPI_WARP = MODE_ == kWgrad ? 4096 : 1024;
   static constexpr uint32_t EPI_REGION = STAGES * STAGE_BYTES;  // 1024 B aligned
   static constexpr uint32_t BAR_REGION = EPI_REGION + 4 * EPI_WARP;
   static constexpr uint32_t SMEM_BYTES = 1024 + BAR_REGION + 8 * NBARS + 32 * SCHED + 16;
@@ -149,16 +148,22 @@ __device__ __forceinline__ void f16_epilogue_rows(void* out, int ldn, int m0, si
 }
 
 // Wgrad.  The warp's TMEM lanes are gradient rows n0 + lane, its columns k.
-// 128 bytes of every row at a time go through one of two 4 KB boxes (written
-// in the 128-byte swizzle, free of bank conflicts) into a TMA store, which
-// clips at the gradient's bounds; or into an adding store.
+// 128 bytes of every row at a time go through 4 KB of shared memory (16-byte
+// units swizzled by the row: no bank conflicts either way), so that eight lanes
+// store one row's 128 contiguous bytes.  With accumulate the same lanes read
+// what is there and add: one addition per element.
 __device__ __forceinline__ void f16_epilogue_wgrad(const F16Params& p, int g, int n0, int k0,
-                                                   bool empty, uint32_t taddr, uint32_t stage,
-                                                   uint32_t& box) {
+                                                   bool empty, uint32_t taddr, uint8_t* stage) {
   const int lane = threadIdx.x & 31;
-  const int cw = p.out_fp32 ? 32 : 64;  // columns per box
+  const int eb = p.out_fp32 ? 4 : 2;
+  const int cw = 128 / eb;  // columns per step
   const int kcols = min(256, p.c_ext - k0);
   if (n0 >= p.m_ext) return;
+  uint8_t* const out = static_cast<uint8_t*>(p.out) +
+                       ((size_t(g) * size_t(p.m_ext) + size_t(n0)) * size_t(p.c_ext) + size_t(k0)) *
+                           size_t(eb);
+  const size_t pitch = size_t(p.c_ext) * size_t(eb);
+  const int unit = lane & 7;
   for (int c0 = 0; c0 < kcols; c0 += cw) {
     uint32_t v[32];
     if (empty) {
@@ -179,27 +184,38 @@ __device__ __forceinline__ void f16_epilogue_wgrad(const F16Params& p, int g, in
                                   p.bf16 != 0);
       }
     }
-    // the store issued from this box two steps ago has read it
-    if (lane == 0) bulk_wait_read<1>();
-    __syncwarp();
-    const uint32_t at = stage + (box & 1u) * 4096u + uint32_t(lane) * 128u;
 #pragma unroll
     for (int u = 0; u < 8; ++u)
-      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + ((u ^ (lane & 7)) << 4)),
-                   "r"(v[4 * u]), "r"(v[4 * u + 1]), "r"(v[4 * u + 2]), "r"(v[4 * u + 3])
-                   : "memory");
-    fence_async_shared();
+      *reinterpret_cast<uint4*>(stage + lane * 128 + ((u ^ (lane & 7)) << 4)) =
+          make_uint4(v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]);
     __syncwarp();
-    if (lane == 0) {
-      const uint32_t src = stage + (box & 1u) * 4096u;
-      if (p.accumulate)
-        tma_add_3d(&p.tmap_out, src, k0 + c0, n0, g);
-      else
-        tma_store_3d(&p.tmap_out, src, k0 + c0, n0, g);
-      bulk_commit();
+    const bool col_ok = c0 + unit * (16 / eb) < kcols;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int row = 4 * i + (lane >> 3);
+      if (col_ok && n0 + row < p.m_ext) {
+        uint4 q = *reinterpret_cast<const uint4*>(stage + row * 128 + ((unit ^ (row & 7)) << 4));
+        uint4* const dst =
+            reinterpret_cast<uint4*>(out + size_t(row) * pitch + size_t(c0) * eb + unit * 16);
+        if (p.accumulate) {  // fp32
+          const uint4 old = *dst;
+          q.x = __float_as_uint(__uint_as_float(old.x) + __uint_as_float(q.x));
+          q.y = __float_as_uint(__uint_as_float(old.y) + __uint_as_float(q.y));
+          q.z = __float_as_uint(__uint_as_float(old.z) + __uint_as_float(q.z));
+          q.w = __float_as_uint(__uint_as_float(old.w) + __uint_as_float(q.w));
+        }
+        *dst = q;
+      }
     }
-    ++box;
+    __syncwarp();
   }
+}
+
+// Steps of the contraction over a group of m rows (wgrad): 64 rows each, then
+// the whole sixteens of what is left, then the last m % 16 rows' copy.
+__device__ __forceinline__ int wgrad_flat_steps(int m) { return (m / 16 + 3) / 4; }
+__device__ __forceinline__ int wgrad_steps(int m) {
+  return wgrad_flat_steps(m) + ((m & 15) != 0 ? 1 : 0);
 }
 
 // ------------------------------------------------------------ the kernel
@@ -225,7 +241,8 @@ __device__ __forceinline__ F16Slot f16_make_slot(const F16Params& p, int t, int 
     const int local = t - s.g * per;
     s.mt = local / p.cts;
     s.ct = local - s.mt * p.cts;
-    s.rows = __ldg(p.offsets + s.g + 1) - __ldg(p.offsets + s.g);
+    s.row0 = __ldg(p.offsets + s.g);
+    s.rows = __ldg(p.offsets + s.g + 1) - s.row0;
   } else {
     const uint64_t tile = __ldg(p.tiles + t);
     s.g = int(tile >> 48);
@@ -276,7 +293,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
     return C::MODE == kWgrad ? C::BN : min(C::BN, (rows + 31) & ~31);
   };
   auto tile_ksteps = [&](int rows) -> int {
-    return C::MODE == kWgrad ? (rows + C::KS - 1) / C::KS : p.ksteps;
+    return C::MODE == kWgrad ? wgrad_steps(rows) : p.ksteps;
   };
 
   if (threadIdx.x == 0) {
@@ -308,8 +325,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
     if (lane == 0) mbar_arrive(tmem_ready_bar);
   }
 
-  // the tile list, the tensor maps and the status words come from the prepare
-  // kernel just before this launch, which it may overlap until here
+  // the tile list, the copies of last rows and the status words come from the
+  // prepare kernel just before this launch, which it may overlap until here
   griddep_wait();
   const uint32_t leader_schede0 = mapa_shared(schede_bar(0), 0);
   const uint32_t leader_acce0 = mapa_shared(acce_bar(0), 0);
@@ -363,9 +380,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
     int slot = 0;
     uint32_t sphase = 0;
     uint32_t arms = 0;
-    if (C::MODE != kWgrad && lane == 0) {
-      prefetch_tensormap(&p.tmap_w);
-      prefetch_tensormap(&p.tmap_tok[kTokenMaps - 1]);
+    if (lane == 0) {
+      if constexpr (C::MODE == kWgrad) {
+        prefetch_tensormap(&p.tmap_a);
+        prefetch_tensormap(&p.tmap_b);
+      } else {
+        prefetch_tensormap(&p.tmap_w);
+        prefetch_tensormap(&p.tmap_tok[kTokenMaps - 1]);
+      }
     }
     while (true) {
       if (!mbar_wait<true>(schedf_bar(slot), sphase, abort_flag, p.status,
@@ -388,30 +410,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
         if (lane == 0) griddep_launch_dependents();  // no new tiles for this CTA
         break;
       }
-      if (g >= p.num_groups) {  // the group indexes descriptor arrays: never trusted blindly
-        if (lane == 0) {
-          atomicCAS(p.status, 0, kStatusBadTile);
-          *abort_flag = 1;
-        }
-        break;
-      }
       const int half = tile_ncols(rows) >> 1;
       const int ksteps = tile_ksteps(rows);
       // bytes that both CTAs' loads of one step deliver to the leader's barrier
       const uint32_t tx_step = 2u * (C::A_BYTES + uint32_t(half) * 128u);
+      const int flat_steps = C::MODE == kWgrad ? wgrad_flat_steps(rows) : ksteps;
       const int m0 = mt * 256 + int(rank) * 128;     // this CTA's rows of the M axis
       const int tok = row0 + int(rank) * half;       // forward, dgrad: its tokens
       const int c0 = ct * 256 + int(rank) * 128;     // wgrad: its columns k
-      const CUtensorMap* ta = nullptr;
-      const CUtensorMap* tb = nullptr;
-      if constexpr (C::MODE == kWgrad) {
-        ta = p.tmap_a + g;
-        tb = p.tmap_b + g;
-        tensormap_acquire(ta);
-        tensormap_acquire(tb);
-      } else {
-        tb = &p.tmap_tok[half / 16 - 1];
-      }
+      const CUtensorMap* const tb =
+          C::MODE == kWgrad ? &p.tmap_b : &p.tmap_tok[half / 16 - 1];
       bool ok = true;
       for (int ks = 0; ks < ksteps; ++ks) {
         if (!mbar_wait(empty_bar(stage), phase ^ 1, abort_flag, p.status,
@@ -423,7 +431,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
         const int x = ks * C::KS;
         const bool arm = (p.debug_flags & kDebugNoLoads) == 0;
         if (arm && elect_one()) {
-          if (leader) mbar_arrive_expect_tx(full_bar(stage), tx_step);
+          // the copy of a group's last rows comes in boxes of 16 rows
+          const bool tail = C::MODE == kWgrad && ks >= flat_steps;
+          if (leader) mbar_arrive_expect_tx(full_bar(stage), tail ? tx_step / 4 : tx_step);
           if constexpr (C::MODE == kFwd) {
             tma_load_3d_pair(sA(stage), &p.tmap_w, fb, x, m0, g);
             tma_load_2d_pair(sB(stage), tb, fb, x, tok);
@@ -432,10 +442,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
             tma_load_3d_pair(sA(stage) + 8192u, &p.tmap_w, fb, m0 + 64, x, g);
             tma_load_2d_pair(sB(stage), tb, fb, x, tok);
           } else {
-            tma_load_2d_pair(sA(stage), ta, fb, m0, x);
-            tma_load_2d_pair(sA(stage) + 8192u, ta, fb, m0 + 64, x);
-            tma_load_2d_pair(sB(stage), tb, fb, c0, x);
-            tma_load_2d_pair(sB(stage) + 8192u, tb, fb, c0 + 64, x);
+            const CUtensorMap* const ma = tail ? &p.tmap_ta : &p.tmap_a;
+            const CUtensorMap* const mb = tail ? &p.tmap_tb : tb;
+            const int y = tail ? 16 * g : row0 + x;
+            tma_load_2d_pair(sA(stage), ma, fb, m0, y);
+            tma_load_2d_pair(sA(stage) + 8192u, ma, fb, m0 + 64, y);
+            tma_load_2d_pair(sB(stage), mb, fb, c0, y);
+            tma_load_2d_pair(sB(stage) + 8192u, mb, fb, c0 + 64, y);
           }
         }
         __syncwarp();
@@ -496,11 +509,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
         // 16 of the contraction: 32 bytes of a K-major row, 16 rows of an MN-major tile
         constexpr uint32_t kStepA = C::A_MN ? 2048u >> 4 : 32u >> 4;
         constexpr uint32_t kStepB = C::B_MN ? 2048u >> 4 : 32u >> 4;
+        // wgrad: the whole sixteens of rows that this step holds; its last, the copy
+        const int nj = C::MODE == kWgrad
+                           ? (ks < wgrad_flat_steps(rows) ? min(4, rows / 16 - 4 * ks) : 1)
+                           : 4;
         if (elect_one()) {
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            tc_mma_f16_pair(d_tmem, adesc + kStepA * j, bdesc + kStepB * j, idesc,
-                            (ks | j) != 0 ? 1u : 0u);
+            if (j < nj)
+              tc_mma_f16_pair(d_tmem, adesc + kStepA * j, bdesc + kStepB * j, idesc,
+                              (ks | j) != 0 ? 1u : 0u);
           tc_commit_pair(empty_bar(stage), 0x3);
           if (ks + 1 == ksteps) tc_commit_pair(accf_bar(b), 0x3);
         }
@@ -538,7 +556,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
     int slot = 0;
     uint32_t sphase = 0;
     uint32_t lt = 0;
-    uint32_t box = 0;
     while (ok) {
       if (!mbar_wait<true>(schedf_bar(slot), sphase, abort_flag, p.status,
                            kStatusTimeoutEpilogue))
@@ -559,7 +576,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
       const uint32_t taddr = tmem + (uint32_t(q * 32) << 16) + b * C::BN;
       if constexpr (C::MODE == kWgrad) {
         if (s.rows > 0 || !p.accumulate)
-          f16_epilogue_wgrad(p, s.g, m0, s.ct * 256, s.rows == 0, taddr, base + stage_off, box);
+          f16_epilogue_wgrad(p, s.g, m0, s.ct * 256, s.rows == 0, taddr, gbase + stage_off);
       } else {
         if (m0 < p.m_ext)
           f16_epilogue_rows(p.out, p.m_ext, m0, size_t(s.row0), s.rows, tile_ncols(s.rows),
@@ -575,8 +592,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
       }
       ++lt;
     }
-    // stores in flight read this CTA's shared memory
-    if (C::MODE == kWgrad && lane == 0) bulk_wait<0>();
   }
 
   __syncthreads();
@@ -590,16 +605,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
 
 // ---------------------------------------------------------------- prepare
 struct F16PrepParams {
-  CUtensorMap tmpl_a, tmpl_b;  // wgrad: one group's geometry
   const int32_t* offsets;
-  const uint8_t* a;  // wgrad: dy, x
-  const uint8_t* b;
-  CUtensorMap* tmap_a;
-  CUtensorMap* tmap_b;
+  const uint4* a;  // wgrad: dy, x in 16-byte vectors
+  const uint4* b;
+  uint4* tail_a;   // wgrad: the groups' last rows, 16 rows each
+  uint4* tail_b;
   uint64_t* tiles;
   int32_t* tile_rows;
   int* status;
-  int64_t row_bytes_a, row_bytes_b;
+  int32_t vec_a, vec_b;  // wgrad: vectors per row
   int32_t num_groups, max_rows, mts, tile_cap;
   int32_t wgrad_tiles;  // wgrad: every group's tiles; 0 = forward, dgrad
 };
@@ -614,8 +628,8 @@ __device__ __forceinline__ int f16_tile_height(int m, int count) {
 
 // Every block scans the groups' tile counts (at most 512) in shared memory and
 // writes its share of the tile list, group by group, a weight tile's token
-// tiles next to each other (they share it in L2); or its share of the groups'
-// tensor maps (wgrad).
+// tiles next to each other (they share it in L2); or copies its share of the
+// groups' last rows % 16 rows, with zeros up to 16 (wgrad).
 __global__ void __launch_bounds__(256) f16_prepare_kernel(const __grid_constant__ F16PrepParams p) {
   griddep_launch_dependents();
   griddep_wait();
@@ -623,7 +637,6 @@ __global__ void __launch_bounds__(256) f16_prepare_kernel(const __grid_constant_
   __shared__ int32_t sbegin[FGG_MAX_GROUPS + 1];
   __shared__ int32_t swarp[8];
   __shared__ int s_bad;
-  __shared__ alignas(128) CUtensorMap smap[8];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int G = p.num_groups;
   if (threadIdx.x == 0) s_bad = 0;
@@ -673,24 +686,22 @@ __global__ void __launch_bounds__(256) f16_prepare_kernel(const __grid_constant_
   }
   if (num_tiles == 0) return;
   if (p.wgrad_tiles > 0) {
-    for (int i = blockIdx.x * 8 + warp; i < 2 * G; i += gridDim.x * 8) {
-      const int g = i >> 1;
-      const bool is_b = i & 1;
-      const uint32_t* src = reinterpret_cast<const uint32_t*>(is_b ? &p.tmpl_b : &p.tmpl_a);
-      reinterpret_cast<uint32_t*>(&smap[warp])[lane] = src[lane];
-      __syncwarp();
-      if (lane == 0) {
-        const uint8_t* at = is_b ? p.b + int64_t(soff[g]) * p.row_bytes_b
-                                 : p.a + int64_t(soff[g]) * p.row_bytes_a;
-        // an empty group's maps are never used: any valid address will do
-        const int m = soff[g + 1] - soff[g];
-        tmap_replace_address(smem_u32(&smap[warp]),
-                             reinterpret_cast<uint64_t>(m > 0 ? at : (is_b ? p.b : p.a)));
-        tmap_replace_dim1(smem_u32(&smap[warp]), max(m, 1));
-      }
-      __syncwarp();
-      tmap_publish((is_b ? p.tmap_b : p.tmap_a) + g, smem_u32(&smap[warp]));
-      __syncwarp();
+    const int vecs = p.vec_a + p.vec_b;
+    const int64_t total = int64_t(G) * 16 * vecs;
+    for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < total;
+         i += int64_t(gridDim.x) * 256) {
+      const int64_t r = i / vecs;
+      const int c = int(i - r * vecs);
+      const int g = int(r >> 4), row = int(r & 15);
+      const int rest = (soff[g + 1] - soff[g]) & 15;
+      if (rest == 0) continue;  // never read
+      const bool is_a = c < p.vec_a;
+      const int col = is_a ? c : c - p.vec_a;
+      const int64_t pitch = is_a ? p.vec_a : p.vec_b;
+      const int64_t src = int64_t(soff[g + 1] - rest + row);
+      uint4 v = make_uint4(0u, 0u, 0u, 0u);
+      if (row < rest) v = __ldg((is_a ? p.a : p.b) + src * pitch + col);
+      (is_a ? p.tail_a : p.tail_b)[r * pitch + col] = v;
     }
     return;
   }
@@ -717,7 +728,7 @@ __global__ void __launch_bounds__(256) f16_prepare_kernel(const __grid_constant_
 // ------------------------------------------------------------------- host
 struct F16Layout {
   int mts = 0, cts = 0, tile_cap = 0;
-  size_t status = 0, tiles = 0, tile_rows = 0, tmap_a = 0, tmap_b = 0, total = 0;
+  size_t status = 0, tiles = 0, tile_rows = 0, tail_a = 0, tail_b = 0, total = 0;
 };
 
 int plan_f16(const FggF16RowsProblem* p, int direction, F16Layout* L) {
@@ -747,8 +758,8 @@ int plan_f16(const FggF16RowsProblem* p, int direction, F16Layout* L) {
   int64_t cap;
   if (direction == kWgrad) {
     cap = int64_t(G) * L->mts * L->cts;
-    L->tmap_a = cv.take(size_t(G) * sizeof(CUtensorMap), 128);
-    L->tmap_b = cv.take(size_t(G) * sizeof(CUtensorMap), 128);
+    L->tail_a = cv.take(size_t(G) * 16 * size_t(p->n) * 2, 256);
+    L->tail_b = cv.take(size_t(G) * 16 * size_t(p->k) * 2, 256);
   } else {
     // sum over groups of ceil(m / 256) <= rows / 256 + groups (and <= rows)
     cap = std::min<int64_t>(int64_t(p->max_rows) / 256 + G, p->max_rows) * L->mts;
@@ -838,27 +849,23 @@ int fgg_f16_grouped_gemm_rows(const FggF16RowsProblem* p, int32_t direction, voi
   gp.debug_flags = debug_flags();
   int blocks;
   if (direction == kWgrad) {
-    // one group's maps: the prepare kernel sets each group's base and rows
-    if (int rc = encode_2d(&pp.tmpl_a, kMap16, p->a, N, R, N * 2, 64, 64)) return rc;
-    if (int rc = encode_2d(&pp.tmpl_b, kMap16, p->b, K, R, K * 2, 64, 64)) return rc;
-    pp.a = static_cast<const uint8_t*>(p->a);
-    pp.b = static_cast<const uint8_t*>(p->b);
-    pp.row_bytes_a = int64_t(N) * 2;
-    pp.row_bytes_b = int64_t(K) * 2;
-    pp.tmap_a = reinterpret_cast<CUtensorMap*>(ws + L.tmap_a);
-    pp.tmap_b = reinterpret_cast<CUtensorMap*>(ws + L.tmap_b);
+    pp.a = static_cast<const uint4*>(p->a);
+    pp.b = static_cast<const uint4*>(p->b);
+    pp.tail_a = reinterpret_cast<uint4*>(ws + L.tail_a);
+    pp.tail_b = reinterpret_cast<uint4*>(ws + L.tail_b);
+    pp.vec_a = p->n / 8;
+    pp.vec_b = p->k / 8;
+    if (int rc = encode_2d(&gp.tmap_a, kMap16, p->a, N, R, N * 2, 64, 64)) return rc;
+    if (int rc = encode_2d(&gp.tmap_b, kMap16, p->b, K, R, K * 2, 64, 64)) return rc;
+    if (int rc = encode_2d(&gp.tmap_ta, kMap16, pp.tail_a, N, 16 * G, N * 2, 64, 16)) return rc;
+    if (int rc = encode_2d(&gp.tmap_tb, kMap16, pp.tail_b, K, 16 * G, K * 2, 64, 16)) return rc;
     pp.wgrad_tiles = L.tile_cap;
-    gp.tmap_a = pp.tmap_a;
-    gp.tmap_b = pp.tmap_b;
     gp.m_ext = p->n;
     gp.c_ext = p->k;
     gp.out_fp32 = p->out_dtype == 0 ? 1 : 0;
     gp.accumulate = p->accumulate != 0 ? 1 : 0;
-    const uint64_t eb = gp.out_fp32 ? 4 : 2;
-    if (int rc = encode_3d(&gp.tmap_out, gp.out_fp32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : kMap16,
-                           p->out, K, N, G, K * eb, N * K * eb, gp.out_fp32 ? 32 : 64, 32, 1))
-      return rc;
-    blocks = (2 * p->num_groups + 7) / 8;
+    const int64_t vecs = int64_t(p->num_groups) * 16 * (pp.vec_a + pp.vec_b);
+    blocks = int(std::min<int64_t>((vecs + 255) / 256, 8 * dev.sm_count));
   } else {
     const uint64_t ck = direction == kFwd ? K : N;  // contraction: the tokens' row length
     if (int rc = encode_3d(&gp.tmap_w, kMap16, p->b, K, N, G, K * 2, N * K * 2, 64,
