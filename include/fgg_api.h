@@ -251,6 +251,35 @@ FGG_API int fgg_mx_grouped_gemm(const FggMxProblem* p, void* workspace, size_t w
                         void* stream);
 
 /* ------------------------------------------------------------------------ */
+/* MXFP4: quantisation, its inverse, and MXFP4 x MXFP4 over contiguous rows  */
+/* ------------------------------------------------------------------------ */
+
+/* E2M1 elements, two per byte (element 2j in the LOW nibble of byte j), one
+ * UE8M0 scale byte per 32 consecutive elements: the weight format of the
+ * reference operator (kernel.py:14-26) for both operands.
+ *   byte = max(floor(log2(max |x|)) - 2 + 127, 0); 255 (NaN) for a block with a
+ *   NaN or an infinity;  q = e2m1_rne(x 2^(127 - byte)), saturating at 6
+ * x: count elements (a multiple of 32) of x_dtype 0 fp32, 1 bf16 or 2 fp16,
+ * 16-byte aligned; codes: count/2 bytes, 4-byte aligned; sf: count/32 bytes. */
+FGG_API int fgg_mxfp4_quantize(const void* x, int32_t x_dtype, int64_t count, void* codes, void* sf,
+                               void* stream);
+/* x = e2m1 * 2^(byte - 127), rounded once to x_dtype. */
+FGG_API int fgg_mxfp4_dequantize(const void* codes, const void* sf, int64_t count, void* x,
+                                 int32_t x_dtype, void* stream);
+
+/* The contiguous-rows grouped GEMM (fgg_nvfp4_grouped_gemm_rows) on MXFP4
+ * operands: the same arguments, statuses and alignment, with a_sf and b_sf of
+ * K/32 UE8M0 bytes per row and K a multiple of 128.  Weight packs of the two
+ * formats differ; each call refuses the other's (status 0x201). */
+typedef FggNvfp4RowsProblem FggMxfp4RowsProblem;
+FGG_API size_t fgg_mxfp4_weight_pack_bytes(int32_t num_groups, int32_t n, int32_t k);
+FGG_API int fgg_mxfp4_pack_weights(const FggNvfp4Weights* w, void* pack, size_t pack_bytes,
+                                   void* stream);
+FGG_API size_t fgg_mxfp4_rows_workspace_bytes(const FggMxfp4RowsProblem* p);
+FGG_API int fgg_mxfp4_grouped_gemm_rows(const FggMxfp4RowsProblem* p, const void* pack,
+                                        void* workspace, size_t ws_bytes, void* stream);
+
+/* ------------------------------------------------------------------------ */
 /* bf16 / fp16 products grouped by expert, forward and both gradients        */
 /* ------------------------------------------------------------------------ */
 
@@ -289,6 +318,30 @@ typedef struct FggF16RowsProblem {
 FGG_API size_t fgg_f16_rows_workspace_bytes(const FggF16RowsProblem* p, int32_t direction);
 FGG_API int fgg_f16_grouped_gemm_rows(const FggF16RowsProblem* p, int32_t direction,
                                       void* workspace, size_t ws_bytes, void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* Router of a mixture-of-experts layer                                      */
+/* ------------------------------------------------------------------------ */
+
+/* No counterpart in the reference operator (it takes routed rows).  For every
+ * row l of logits [tokens, experts] (dtype 0 fp32, 1 bf16, 2 fp16):
+ *   s = softmax(l) (score 0) or sigmoid(l) (score 1)
+ *   ids[0..topk) = the experts with the largest s + bias (bias: fp32 [experts] or
+ *   NULL), largest first, ties to the lowest index
+ *   weights[j] = scale * s[ids[j]], over the chosen ones' sum when renormalize != 0
+ * A logit or bias of -inf (or a NaN bias) masks an expert; routes left over get
+ * id -1 and weight 0.  A row with a NaN logit (softmax: or +inf) has NaN weights.
+ * experts <= 1024, topk <= min(experts, 32). */
+FGG_API int fgg_moe_router(const void* logits, int32_t dtype, int32_t tokens, int32_t experts,
+                           int32_t topk, int32_t score, const float* bias, int32_t renormalize,
+                           float scale, int32_t* ids, float* weights, void* stream);
+/* dlogits [tokens, experts] (in dtype, every element written) from dweights fp32
+ * [tokens, topk] and the forward call's logits and ids; an id outside
+ * [0, experts) is an absent route, an id named twice gets both shares. */
+FGG_API int fgg_moe_router_backward(const float* dweights, const void* logits, int32_t dtype,
+                                    const int32_t* ids, int32_t tokens, int32_t experts,
+                                    int32_t topk, int32_t score, int32_t renormalize, float scale,
+                                    void* dlogits, void* stream);
 
 /* ------------------------------------------------------------------------ */
 /* Expert-parallel MoE: the byte-moving kernels around the grouped GEMM      */

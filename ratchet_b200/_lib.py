@@ -103,6 +103,18 @@ _SIGS = {
     "fgg_nvfp4_grouped_gemm_noalloc": (ctypes.c_int, [ctypes.POINTER(FggNvfp4Problem), _VOIDP, _VOIDP, _VOIDP]),
     "fgg_f16_rows_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(FggF16RowsProblem), ctypes.c_int32]),
     "fgg_f16_grouped_gemm_rows": (ctypes.c_int, [ctypes.POINTER(FggF16RowsProblem), ctypes.c_int32, _VOIDP, ctypes.c_size_t, _VOIDP]),
+    "fgg_mxfp4_quantize": (ctypes.c_int, [_VOIDP, ctypes.c_int32, ctypes.c_int64, _VOIDP, _VOIDP, _VOIDP]),
+    "fgg_mxfp4_dequantize": (ctypes.c_int, [_VOIDP, _VOIDP, ctypes.c_int64, _VOIDP, ctypes.c_int32, _VOIDP]),
+    "fgg_mxfp4_weight_pack_bytes": (ctypes.c_size_t, [ctypes.c_int32, ctypes.c_int32, ctypes.c_int32]),
+    "fgg_mxfp4_pack_weights": (ctypes.c_int, [ctypes.POINTER(FggNvfp4Weights), _VOIDP, ctypes.c_size_t, _VOIDP]),
+    "fgg_mxfp4_rows_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(FggNvfp4RowsProblem)]),
+    "fgg_mxfp4_grouped_gemm_rows": (ctypes.c_int, [ctypes.POINTER(FggNvfp4RowsProblem), _VOIDP, _VOIDP, ctypes.c_size_t, _VOIDP]),
+    "fgg_moe_router": (ctypes.c_int, [_VOIDP, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32,
+                                      ctypes.c_int32, _VOIDP, ctypes.c_int32, ctypes.c_float, _VOIDP, _VOIDP,
+                                      _VOIDP]),
+    "fgg_moe_router_backward": (ctypes.c_int, [_VOIDP, _VOIDP, ctypes.c_int32, _VOIDP, ctypes.c_int32,
+                                               ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32,
+                                               ctypes.c_float, _VOIDP, _VOIDP]),
     "fgg_moe_plan": (ctypes.c_int, [_VOIDP, ctypes.c_int32, ctypes.c_int32, _VOIDP, _VOIDP, ctypes.c_int32,
                                     ctypes.c_int32, ctypes.c_int32, _VOIDP, _VOIDP, _VOIDP, _VOIDP, _VOIDP]),
     "fgg_moe_gather_rows": (ctypes.c_int, [_VOIDP, _VOIDP, ctypes.c_int64, ctypes.c_int32, ctypes.c_int32,

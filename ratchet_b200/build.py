@@ -23,7 +23,8 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 LIB = PKG / "_fgg.so"
 SOURCES = ["fgg_common.cu", "fgg_nvfp4.cu", "fgg_mx.cu", "fgg_quant.cu", "fgg_scratch.cu",
-           "fgg_moe.cu", "fgg_peer.cu", "fgg_f16.cu"]
+           "fgg_moe.cu", "fgg_peer.cu", "fgg_f16.cu",
+           "fgg_router.cu", "fgg_mxfp4.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

@@ -38,9 +38,12 @@
 //   fgg_gemm_kernel       one CTA per tile, 128 weight rows x BN tokens
 //   fgg_gemm_pair_kernel  a CTA pair (cta_group::2) per tile, 256 x 224: each
 //                         CTA loads half of the token tile
-// Two kinds (compile-time):
+// Three kinds (compile-time):
 //   NVFP4   .kind::mxf4nvf4 .scale_vec::4X: E2M1 x E2M1, one E4M3 scale per 16
 //           K; K step 256 = 4 MMAs of K 64, one SF slot per MMA.
+//   MXFP4   .kind::mxf4 .scale_vec::2X: E2M1 x E2M1, one UE8M0 scale per 32 K;
+//           the same K step, one SF slot per two MMAs, which pick their two
+//           bytes of it with the SF id.  (MX4 below; MX is the next one.)
 //   MX      .kind::mxf8f6f4: weights E2M1 (4-bit codes unpacked to bytes by
 //           TMA), tokens E4M3, one UE8M0 scale per 32 K; K step 128 = 4 MMAs of
 //           K 32 that share one SF slot and pick their byte with the SF id.
@@ -66,7 +69,8 @@ __host__ __device__ __forceinline__ uint32_t pack_tile(int g, int nt, int xt) {
 }
 constexpr uint32_t kEndTile = 0xFFFFFFFFu;
 
-constexpr uint32_t kPackMagic = 0x46474e34u;  // "FGN4"
+constexpr uint32_t kPackMagic = 0x46474e34u;   // "FGN4"
+constexpr uint32_t kPackMagicMx = 0x46474d34u;  // "FGM4"
 struct PackHeader {
   uint32_t magic;
   int32_t g, n, k;
@@ -314,9 +318,13 @@ __device__ __forceinline__ void epilogue_tile_silu_mul(__nv_bfloat16* out, int l
   }
 }
 
-template <bool MX_, int BN_, int STAGES_, int KSUB_ = 1>
+template <bool MX_, int BN_, int STAGES_, int KSUB_ = 1, bool MX4_ = false>
 struct EngineCfg {
   static constexpr bool MX = MX_;
+  static constexpr bool MX4 = MX4_;
+  static_assert(!(MX && MX4), "one kind");
+  // 512-byte scale atoms per K step and 128 rows, each in a TMEM slot of its own
+  static constexpr int ATOMS = MX ? 1 : MX4 ? 2 : 4;
   static constexpr int BN = BN_;
   static constexpr int STAGES = STAGES_;
   // K steps per pipeline stage (one barrier wait and one commit per stage)
@@ -328,10 +336,10 @@ struct EngineCfg {
   static constexpr uint32_t W_BYTES = 128 * 128;   // smem bytes of the weight tile
   static constexpr uint32_t W_TX = MX ? 64 * 128 : 128 * 128;  // bytes TMA reads from HBM
   static constexpr uint32_t X_BYTES = BN * 128;
-  // NVFP4: 4 atoms (one per K64 MMA); MX: one atom covers the 4 K32 MMAs.
-  static constexpr uint32_t SFW_BYTES = MX ? 512 : 4 * 512;
-  // token scales: CH atoms per MMA (NVFP4) or per K step (MX)
-  static constexpr uint32_t SFX_BYTES = MX ? CH * 512 : 4 * CH * 512;
+  // NVFP4: an atom per K64 MMA; MXFP4: per two of them; MX: one covers the 4 K32 MMAs.
+  static constexpr uint32_t SFW_BYTES = ATOMS * 512;
+  // token scales: CH atoms for each of the weights'
+  static constexpr uint32_t SFX_BYTES = ATOMS * CH * 512;
   static constexpr uint32_t TX_BYTES = W_TX + X_BYTES + SFW_BYTES + SFX_BYTES;
   // Shared memory of one K step: its two operand tiles (1024 B aligned for
   // the 128-byte swizzle) in one region, its scale atoms in another, so that
@@ -345,7 +353,7 @@ struct EngineCfg {
   static_assert(SF_BYTES % 128 == 0, "scale atoms must stay 128 B aligned");
   // TMEM columns: two accumulators of BN fp32 columns, then a ring of scale
   // slots (4 columns of weight scales + 4 per token atom).  NVFP4 takes one
-  // slot per MMA, MX one per K step.
+  // slot per MMA, MXFP4 one per two, MX one per K step.
   static constexpr int SF_BASE = ((2 * BN + 3) / 4) * 4;
   static constexpr int SF_SLOT = 4 + 4 * CH;
   static constexpr int NSLOTS_FIT = (512 - SF_BASE) / SF_SLOT;
@@ -426,7 +434,7 @@ __global__ void __launch_bounds__(256, 1) fgg_gemm_kernel(const __grid_constant_
       // A pack built for a different problem is refused before any load.
       const PackHeader h = *p.pack;
       // reported after griddep_wait: the prepare kernel resets the status word
-      if (h.magic != kPackMagic || h.g != p.wg || h.n != p.n || h.k != p.k) *abort_flag = 2;
+      if (h.magic != (C::MX4 ? kPackMagicMx : kPackMagic) || h.g != p.wg || h.n != p.n || h.k != p.k) *abort_flag = 2;
     }
     fence_mbar_init();
   }
@@ -625,6 +633,7 @@ __global__ void __launch_bounds__(256, 1) fgg_gemm_kernel(const __grid_constant_
           break;
         tc_fence_after();
         const uint32_t d_tmem = tmem + b * C::BN;
+        // (MX and MXFP4: one per SF id, below)
         const uint32_t idesc =
             C::MX ? 0u : idesc_block_scaled(kFmtNvf4E2M1, kFmtNvf4E2M1, 0, 128, ncols, 0, 0);
         for (int ks0 = 0; ks0 < p.ksteps; ks0 += C::KSUB) {
@@ -633,8 +642,8 @@ __global__ void __launch_bounds__(256, 1) fgg_gemm_kernel(const __grid_constant_
             break;
           }
           tc_fence_after();
-          // scale slots of this stage's MMAs (NVFP4: one per MMA; MX: one per K step)
-          constexpr int kSlots = C::KSUB * (C::MX ? 1 : 4);
+          // scale slots of this stage's MMAs
+          constexpr int kSlots = C::KSUB * C::ATOMS;
           uint32_t col[kSlots];
 #pragma unroll
           for (int i = 0; i < kSlots; ++i) {
@@ -668,6 +677,25 @@ __global__ void __launch_bounds__(256, 1) fgg_gemm_kernel(const __grid_constant_
                   tc_mma_mxf8f6f4(d_tmem, adesc + 2u * j, bdesc + 2u * j, idj,
                                   c0 | (uint32_t(j) << 30), (c0 + 4) | (uint32_t(j) << 30),
                                   (ks | j) != 0 ? 1u : 0u);
+                }
+              } else if constexpr (C::MX4) {
+#pragma unroll
+                for (int a = 0; a < 2; ++a) {
+                  const uint32_t c0 = col[sub * 2 + a];
+                  tc_cp_sf(c0, desc_sf_atom(sSFW(q) + a * 512));
+#pragma unroll
+                  for (int c = 0; c < C::CH; ++c)
+                    if (c == 0 || ncols > 128 * c)
+                      tc_cp_sf(c0 + 4 + 4 * c, desc_sf_atom(sSFX(q) + (a * C::CH + c) * 512));
+#pragma unroll
+                  for (int h = 0; h < 2; ++h) {
+                    // SF id 0 or 2: the scales of the atom's first or second 64 K elements
+                    const int j = 2 * a + h;
+                    const uint32_t id = 2u * h;
+                    tc_mma_mxf4(d_tmem, adesc + 2u * j, bdesc + 2u * j,
+                                idesc_block_scaled(kFmtNvf4E2M1, kFmtNvf4E2M1, 1, 128, ncols, id, id),
+                                c0 | (id << 30), (c0 + 4) | (id << 30), (ks | j) != 0 ? 1u : 0u);
+                  }
                 }
               } else {
 #pragma unroll
@@ -783,9 +811,11 @@ __global__ void __launch_bounds__(256, 1) fgg_gemm_kernel(const __grid_constant_
 // schedule ring, whose slots the leader writes into the follower's shared
 // memory: those waits acquire at cluster scope.
 // ====================================================================
-template <bool MX_, int STAGES_, int KSUB_ = 1>
+template <bool MX_, int STAGES_, int KSUB_ = 1, bool MX4_ = false>
 struct PairCfg {
   static constexpr bool MX = MX_;
+  static constexpr bool MX4 = MX4_;
+  static constexpr int ATOMS = MX ? 1 : MX4 ? 2 : 4;  // as in EngineCfg
   static constexpr int BN = 224;   // tokens per pair tile = MMA N
   static constexpr int BNH = 112;  // token rows one CTA loads
   static constexpr int STAGES = STAGES_;
@@ -798,11 +828,10 @@ struct PairCfg {
   static constexpr uint32_t W_BYTES = 128 * 128;
   static constexpr uint32_t W_TX = MX ? 64 * 128 : 128 * 128;
   static constexpr uint32_t X_BYTES = BNH * 128;
-  // Weight scales of a K step (this CTA's 128 rows).  MX: one atom for the 4
-  // MMAs.  NVFP4: one atom per MMA.
-  static constexpr uint32_t SFW_BYTES = MX ? 512 : 4 * 512;
-  // token scales of all 224 tokens: two atoms per MMA (NVFP4) or per K step (MX)
-  static constexpr uint32_t SFX_BYTES = MX ? 2 * 512 : 4 * 2 * 512;
+  // weight scales of a K step (this CTA's 128 rows)
+  static constexpr uint32_t SFW_BYTES = ATOMS * 512;
+  // token scales of all 224 tokens: two atoms for each of the weights'
+  static constexpr uint32_t SFX_BYTES = ATOMS * 2 * 512;
   // SF atoms travel as 2-D uint64 boxes {ROW_U64, BOX_ROWS}
   static constexpr uint32_t SFW_ROW_U64 = SFW_BYTES / 8 > 256 ? 256 : SFW_BYTES / 8;
   static constexpr uint32_t SFW_BOX_ROWS = SFW_BYTES / (8 * SFW_ROW_U64);
@@ -816,7 +845,7 @@ struct PairCfg {
   static_assert(OP_BYTES % 1024 == 0, "operand tiles must stay 1024 B aligned");
   static_assert(SF_BYTES % 128 == 0, "scale atoms must stay 128 B aligned");
   static constexpr int SF_BASE = 2 * BN;          // 448
-  // [weights 4 | tokens 8]: per MMA (NVFP4) or per K step (MX)
+  // [weights 4 | tokens 8] per atom
   static constexpr int SF_SLOT = 12;
   static constexpr int NSLOTS = (512 - SF_BASE) / SF_SLOT;
   static_assert(NSLOTS >= 2, "not enough TMEM for the scale ring");
@@ -896,7 +925,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
     if constexpr (!C::MX) {
       const PackHeader h = *p.pack;
       // reported after griddep_wait: the prepare kernel resets the status word
-      if (h.magic != kPackMagic || h.g != p.wg || h.n != p.n || h.k != p.k) *abort_flag = 2;
+      if (h.magic != (C::MX4 ? kPackMagicMx : kPackMagic) || h.g != p.wg || h.n != p.n || h.k != p.k) *abort_flag = 2;
     }
     fence_mbar_init();
   }
@@ -1131,8 +1160,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
             break;
           }
           tc_fence_after();
-          // scale slots of this stage's MMAs (NVFP4: one per MMA; MX: one per K step)
-          constexpr int kSlots = C::KSUB * (C::MX ? 1 : 4);
+          // scale slots of this stage's MMAs
+          constexpr int kSlots = C::KSUB * C::ATOMS;
           uint32_t col[kSlots];
 #pragma unroll
           for (int i = 0; i < kSlots; ++i) {
@@ -1162,6 +1191,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
                   tc_mma_mxf8f6f4_pair(d_tmem, adesc + 2u * j, bdesc + 2u * j, idj,
                                        c0 | (uint32_t(j) << 30), (c0 + 4) | (uint32_t(j) << 30),
                                        (ks | j) != 0 ? 1u : 0u);
+                }
+              } else if constexpr (C::MX4) {
+#pragma unroll
+                for (int a = 0; a < 2; ++a) {
+                  const uint32_t c0 = col[sub * 2 + a];
+                  tc_cp_sf_pair(c0, desc_sf_atom(sSFW(q) + a * 512));
+                  tc_cp_sf_pair(c0 + 4, desc_sf_atom(sSFX(q) + (2 * a) * 512));
+                  if (ncols > 128) tc_cp_sf_pair(c0 + 8, desc_sf_atom(sSFX(q) + (2 * a + 1) * 512));
+#pragma unroll
+                  for (int h = 0; h < 2; ++h) {
+                    const int j = 2 * a + h;
+                    const uint32_t id = 2u * h;
+                    tc_mma_mxf4_pair(
+                        d_tmem, adesc + 2u * j, bdesc + 2u * j,
+                        idesc_block_scaled(kFmtNvf4E2M1, kFmtNvf4E2M1, 1, 256, ncols, id, id),
+                        c0 | (id << 30), (c0 + 4) | (id << 30), (ks | j) != 0 ? 1u : 0u);
+                  }
                 }
               } else {
 #pragma unroll

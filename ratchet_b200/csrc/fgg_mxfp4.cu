@@ -1,0 +1,232 @@
+// fgg_mxfp4.cu - MXFP4 quantisation on the device and its inverse.
+//
+// The format (OCP microscaling, E2M1 elements): 32 consecutive elements share a
+// power-of-two scale, stored as an UE8M0 byte.
+//   e    = floor(log2(max |x|)) - 2      (2: the exponent of E2M1's largest, 6)
+//   byte = max(e + 127, 0)               (0 for a block of zeros)
+//   q    = e2m1_rne(x 2^-e)              ties to the even code, saturating at 6
+// A block that holds a NaN or an infinity has the NaN scale 0xFF, so that it
+// reads back as NaN.  e comes from the exponent bits of the maximum, and x 2^-e
+// is exact in fp32 but where it vanishes, so every step is exact up to the one
+// rounding to E2M1.  The exact rounding of the value's 4 bits is the hardware's
+// (cvt.rn.satfinite.e2m1x2).
+//
+// Both kernels are HBM-bound copies: one pass, 16-byte loads, four lanes per
+// 32-element block.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "fgg_host.cuh"
+#include "fgg_ptx.cuh"
+
+namespace fgg {
+namespace {
+
+// Eight consecutive values as fp32, and eight fp32 as values (16-byte aligned).
+template <typename T>
+struct Vec8;
+template <>
+struct Vec8<float> {
+  uint4 a, b;
+  __device__ __forceinline__ void load(const float* p) {
+    a = __ldg(reinterpret_cast<const uint4*>(p));
+    b = __ldg(reinterpret_cast<const uint4*>(p) + 1);
+  }
+  __device__ __forceinline__ void get(float (&v)[8]) const {
+    v[0] = __uint_as_float(a.x); v[1] = __uint_as_float(a.y);
+    v[2] = __uint_as_float(a.z); v[3] = __uint_as_float(a.w);
+    v[4] = __uint_as_float(b.x); v[5] = __uint_as_float(b.y);
+    v[6] = __uint_as_float(b.z); v[7] = __uint_as_float(b.w);
+  }
+  static __device__ __forceinline__ void store(float* p, const float (&v)[8]) {
+    reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+    reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+  }
+};
+template <>
+struct Vec8<__nv_bfloat16> {
+  uint4 a;
+  __device__ __forceinline__ void load(const __nv_bfloat16* p) {
+    a = __ldg(reinterpret_cast<const uint4*>(p));
+  }
+  __device__ __forceinline__ void get(float (&v)[8]) const {
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&a);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = __bfloat1622float2(h[i]);
+      v[2 * i] = f.x;
+      v[2 * i + 1] = f.y;
+    }
+  }
+  static __device__ __forceinline__ void store(__nv_bfloat16* p, const float (&v)[8]) {
+    uint4 o;
+    __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&o);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+    *reinterpret_cast<uint4*>(p) = o;
+  }
+};
+template <>
+struct Vec8<__half> {
+  uint4 a;
+  __device__ __forceinline__ void load(const __half* p) {
+    a = __ldg(reinterpret_cast<const uint4*>(p));
+  }
+  __device__ __forceinline__ void get(float (&v)[8]) const {
+    const __half2* h = reinterpret_cast<const __half2*>(&a);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = __half22float2(h[i]);
+      v[2 * i] = f.x;
+      v[2 * i + 1] = f.y;
+    }
+  }
+  static __device__ __forceinline__ void store(__half* p, const float (&v)[8]) {
+    uint4 o;
+    __half2* h = reinterpret_cast<__half2*>(&o);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+    *reinterpret_cast<uint4*>(p) = o;
+  }
+};
+
+// E2M1 codes of eight values, the first in the lowest four bits.
+__device__ __forceinline__ uint32_t e2m1x8(const float (&v)[8]) {
+  uint32_t w;
+  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
+      "mov.b32 %0, {a, b, c, d};\n\t}"
+      : "=r"(w)
+      : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
+  return w;
+}
+
+// Two E2M1 values of a byte.
+__device__ __forceinline__ float2 e2m1x2_values(uint32_t byte) {
+  uint32_t h;
+  asm("{\n\t.reg .b8 a, z;\n\t"
+      "mov.b32 {a, z, z, z}, %1;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, a;\n\t}"
+      : "=r"(h)
+      : "r"(byte));
+  return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
+
+// 2^(b - 127) for a scale byte b; NaN for 255.
+__device__ __forceinline__ float ue8m0_value(uint32_t b) {
+  return __uint_as_float(b == 0 ? 0x00400000u : b == 255u ? 0x7fc00000u : b << 23);
+}
+
+// Four lanes per 32-element block, eight elements each.
+template <typename T>
+__global__ void __launch_bounds__(256)
+    mxfp4_quant_kernel(const T* __restrict__ x, int64_t blocks, uint8_t* __restrict__ codes,
+                       uint8_t* __restrict__ sf) {
+  const int64_t h = int64_t(blockIdx.x) * 256 + threadIdx.x;  // index of the 8 elements
+  const bool live = h < 4 * blocks;
+  Vec8<T> in;
+  float v[8];
+  uint32_t top = 0;
+  if (live) {
+    in.load(x + h * 8);
+    in.get(v);
+    // magnitudes compare as integers, NaN above infinity above every number
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+  }
+  top = max(top, __shfl_xor_sync(kFullMask, top, 1));
+  top = max(top, __shfl_xor_sync(kFullMask, top, 2));
+  if (!live) return;
+  const uint32_t eb = top >> 23;  // exponent + 127; 255: NaN or infinity
+  const uint32_t byte = eb == 255u ? 255u : (eb > 2u ? eb - 2u : 0u);
+  const float inv = byte == 255u ? 0.0f : __uint_as_float((254u - byte) << 23);  // 2^(127 - byte)
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = byte == 255u ? 0.0f : v[i] * inv;
+  reinterpret_cast<uint32_t*>(codes)[h] = e2m1x8(v);
+  if ((h & 3) == 0) sf[h >> 2] = uint8_t(byte);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256)
+    mxfp4_dequant_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ sf,
+                         int64_t blocks, T* __restrict__ x) {
+  const int64_t h = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  if (h >= 4 * blocks) return;
+  const uint32_t w = __ldg(reinterpret_cast<const uint32_t*>(codes) + h);
+  const float s = ue8m0_value(__ldg(sf + (h >> 2)));
+  float v[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = e2m1x2_values(w >> (8 * i) & 0xffu);
+    v[2 * i] = f.x * s;
+    v[2 * i + 1] = f.y * s;
+  }
+  Vec8<T>::store(x + h * 8, v);
+}
+
+int check_mx(const void* x, int dtype, int64_t count, const void* codes, const void* sf) {
+  if (dtype < 0 || dtype > 2)
+    return set_error(FGG_EINVAL, "dtype=%d must be 0 (fp32), 1 (bf16) or 2 (fp16)", dtype);
+  if (count < 0 || count % 32 != 0)
+    return set_error(FGG_EBADSHAPE, "the count of elements must be a multiple of 32");
+  if (count > 0 && (x == nullptr || codes == nullptr || sf == nullptr))
+    return set_error(FGG_EINVAL, "null pointer");
+  if (!aligned16(x)) return set_error(FGG_EALIGN, "x must be 16-byte aligned");
+  if (!aligned4(codes)) return set_error(FGG_EALIGN, "codes must be 4-byte aligned");
+  if (count / 8 > int64_t(INT32_MAX) * 256) return set_error(FGG_EBADSHAPE, "tensor too large");
+  return FGG_OK;
+}
+
+}  // namespace
+}  // namespace fgg
+
+using namespace fgg;
+
+extern "C" {
+
+int fgg_mxfp4_quantize(const void* x, int32_t x_dtype, int64_t count, void* codes, void* sf,
+                       void* stream) {
+  if (int rc = check_mx(x, x_dtype, count, codes, sf)) return rc;
+  if (count == 0) return FGG_OK;
+  DeviceInfo dev;
+  if (int rc = current_device(&dev)) return rc;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  const int64_t blocks = count / 32;
+  const int grid = int((4 * blocks + 255) / 256);
+  auto* c8 = static_cast<uint8_t*>(codes);
+  auto* s8 = static_cast<uint8_t*>(sf);
+  if (x_dtype == 0)
+    mxfp4_quant_kernel<<<grid, 256, 0, s>>>(static_cast<const float*>(x), blocks, c8, s8);
+  else if (x_dtype == 1)
+    mxfp4_quant_kernel<<<grid, 256, 0, s>>>(static_cast<const __nv_bfloat16*>(x), blocks, c8, s8);
+  else
+    mxfp4_quant_kernel<<<grid, 256, 0, s>>>(static_cast<const __half*>(x), blocks, c8, s8);
+  FGG_CUDA_CHECK(cudaGetLastError());
+  return FGG_OK;
+}
+
+int fgg_mxfp4_dequantize(const void* codes, const void* sf, int64_t count, void* x, int32_t x_dtype,
+                         void* stream) {
+  if (int rc = check_mx(x, x_dtype, count, codes, sf)) return rc;
+  if (count == 0) return FGG_OK;
+  DeviceInfo dev;
+  if (int rc = current_device(&dev)) return rc;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  const int64_t blocks = count / 32;
+  const int grid = int((4 * blocks + 255) / 256);
+  const auto* c8 = static_cast<const uint8_t*>(codes);
+  const auto* s8 = static_cast<const uint8_t*>(sf);
+  if (x_dtype == 0)
+    mxfp4_dequant_kernel<<<grid, 256, 0, s>>>(c8, s8, blocks, static_cast<float*>(x));
+  else if (x_dtype == 1)
+    mxfp4_dequant_kernel<<<grid, 256, 0, s>>>(c8, s8, blocks, static_cast<__nv_bfloat16*>(x));
+  else
+    mxfp4_dequant_kernel<<<grid, 256, 0, s>>>(c8, s8, blocks, static_cast<__half*>(x));
+  FGG_CUDA_CHECK(cudaGetLastError());
+  return FGG_OK;
+}
+
+}  // extern "C"

@@ -1,4 +1,7 @@
-// fgg_nvfp4.cu - NVFP4 x NVFP4 grouped GEMM entry points (per-group lists).
+// fgg_nvfp4.cu - NVFP4 x NVFP4 grouped GEMM entry points (per-group lists,
+// contiguous rows) and the MXFP4 x MXFP4 ones (contiguous rows), which differ
+// in the scales only: an UE8M0 byte per 32 elements instead of an E4M3 byte per
+// 16, so half as many 512-byte atoms.
 //
 // Per call:
 //   1. nvfp4_prepare_kernel  per-group TMA descriptors for the token tensors
@@ -220,10 +223,12 @@ struct RowsPrepParams {
   uint32_t* tiles_out;
   uint8_t* sfx_out;
   int* status;             // [0] status [1] tile counter [2] finished CTAs [3] tile count
-  int32_t g, wg, k, bn, ch, nk64p, nt, max_rows;
+  int32_t g, wg, k, bn, ch, nt, max_rows;
+  int32_t kq;     // scales per row: K/16 (NVFP4), K/32 (MXFP4)
+  int32_t nk64p;  // SF atoms per 128 rows: one per 4 scales, padded to K steps
   int32_t tile_cap, xt_cap;  // room in tiles_out / token tiles in sfx_out
   int32_t blocks_tiles;
-  int32_t sf_vec;     // K % 256 == 0 and a_sf 16-byte aligned
+  int32_t sf_vec;     // whole 16-byte runs of scales, 16-byte aligned
   int32_t decode;     // decode tiles: never the across-groups order
 };
 
@@ -302,7 +307,7 @@ __global__ void __launch_bounds__(256)
     const int t = blk * blockDim.x + threadIdx.x;
     if (t >= num_tiles) return;
     const bool across = !p.decode && p.g > 1 &&
-                        int64_t(soff[p.g]) * (p.k / 2 + p.k / 16) <= kAcrossGroupsMaxBytes;
+                        int64_t(soff[p.g]) * (p.k / 2 + p.kq) <= kAcrossGroupsMaxBytes;
     if (across) {
       const int nti = t / xt_total;
       const int X = t - nti * xt_total;
@@ -319,7 +324,7 @@ __global__ void __launch_bounds__(256)
     return;
   }
   blk -= p.blocks_tiles;
-  const int kq = p.k / 16;
+  const int kq = p.kq;
   if (p.sf_vec) {
     const int64_t quad = int64_t(blk) * blockDim.x + threadIdx.x;
     const int nk256 = p.nk64p / 4;
@@ -382,6 +387,8 @@ struct PackParams {
   CUtensorMap* tmap_out;
   uint8_t* sfw_out;
   int32_t g, n, k, nk64p, nt;
+  int32_t kq;  // scales per row
+  uint32_t magic;
   int32_t blocks_tmap;
 };
 
@@ -392,7 +399,7 @@ __global__ void __launch_bounds__(256) nvfp4_pack_weights_kernel(const __grid_co
   if (blk < p.blocks_tmap) {
     if (blk == 0 && threadIdx.x == 0) {
       PackHeader h;
-      h.magic = kPackMagic;
+      h.magic = p.magic;
       h.g = p.g;
       h.n = p.n;
       h.k = p.k;
@@ -419,7 +426,7 @@ __global__ void __launch_bounds__(256) nvfp4_pack_weights_kernel(const __grid_co
   rest /= p.nk64p;
   const int nt = int(rest % p.nt);
   const int g = int(rest / p.nt);
-  const int kq = p.k / 16;
+  const int kq = p.kq;
   uint32_t v[4];
 #pragma unroll
   for (int r1 = 0; r1 < 4; ++r1) {
@@ -438,11 +445,20 @@ using CfgPrefill = EngineCfg<false, 224, 4>;   // one CTA per tile (N % 256 != 0
 using CfgDecode = EngineCfg<false, 16, 4, 2>;  // every group has M <= 16; 2 K steps per stage
 using CfgPair = PairCfg<false, 6>;             // CTA pairs, 256 x 224 tiles
 
+// MXFP4: the same tiles, two SF atoms per K step
+using Mx4Prefill = EngineCfg<false, 224, 4, 1, true>;
+using Mx4Decode = EngineCfg<false, 16, 4, 2, true>;
+using Mx4Pair = PairCfg<false, 6, 1, true>;
+
 struct PackLayout {
   size_t header, tmaps, sfw, total;
 };
-static PackLayout pack_layout(int g, int n, int k) {
-  const int nk64p = ((k / 64) + 3) / 4 * 4;
+// SF atoms of 128 rows of K elements: 4 (MXFP4: 2) per K step of 256
+static int sf_atoms(int k, bool mx4) {
+  return mx4 ? (k / 128 + 1) / 2 * 2 : (k / 64 + 3) / 4 * 4;
+}
+static PackLayout pack_layout(int g, int n, int k, bool mx4 = false) {
+  const int nk64p = sf_atoms(k, mx4);
   Carver cv;
   PackLayout L;
   L.header = cv.take(sizeof(PackHeader), 256);
@@ -553,15 +569,29 @@ size_t fgg_nvfp4_weight_pack_bytes(int32_t num_groups, int32_t n, int32_t k) {
   return pack_layout(num_groups, n, k).total;
 }
 
-int fgg_nvfp4_pack_weights(const FggNvfp4Weights* w, void* pack, size_t pack_bytes, void* stream) {
+size_t fgg_mxfp4_weight_pack_bytes(int32_t num_groups, int32_t n, int32_t k) {
+  if (num_groups < 1 || num_groups > FGG_MAX_GROUPS || n <= 0 || n % 128 != 0 || k <= 0 ||
+      k % 128 != 0)
+    return 0;
+  return pack_layout(num_groups, n, k, true).total;
+}
+
+}  // extern "C"
+
+namespace fgg {
+namespace {
+
+int pack_weights_impl(const FggNvfp4Weights* w, void* pack, size_t pack_bytes, void* stream,
+                      bool mx4) {
   if (w == nullptr || pack == nullptr) return set_error(FGG_EINVAL, "weights or pack is null");
   const int G = w->num_groups;
   if (G < 1 || G > FGG_MAX_GROUPS)
     return set_error(FGG_EINVAL, "num_groups=%d outside [1, %d]", G, FGG_MAX_GROUPS);
   if (w->n <= 0 || w->n % 128 != 0)
     return set_error(FGG_EBADSHAPE, "N=%d must be a positive multiple of 128", w->n);
-  if (w->k < 64 || w->k % 64 != 0)
-    return set_error(FGG_EBADSHAPE, "K=%d must be a positive multiple of 64", w->k);
+  const int kmul = mx4 ? 128 : 64;
+  if (w->k < kmul || w->k % kmul != 0)
+    return set_error(FGG_EBADSHAPE, "K=%d must be a positive multiple of %d", w->k, kmul);
   if (w->b == nullptr || w->b_sf == nullptr) return set_error(FGG_EINVAL, "b / b_sf arrays are null");
   for (int g = 0; g < G; ++g) {
     if (w->b[g] == nullptr || w->b_sf[g] == nullptr)
@@ -570,7 +600,7 @@ int fgg_nvfp4_pack_weights(const FggNvfp4Weights* w, void* pack, size_t pack_byt
     if (!aligned4(w->b_sf[g])) return set_error(FGG_EALIGN, "b_sf[%d] is not 4-byte aligned", g);
   }
   if (!aligned16(pack)) return set_error(FGG_EALIGN, "pack is not 16-byte aligned");
-  const PackLayout L = pack_layout(G, w->n, w->k);
+  const PackLayout L = pack_layout(G, w->n, w->k, mx4);
   if (pack_bytes < L.total)
     return set_error(FGG_EWORKSPACE, "pack has %zu bytes, needs %zu", pack_bytes, L.total);
   DeviceInfo dev;
@@ -591,7 +621,9 @@ int fgg_nvfp4_pack_weights(const FggNvfp4Weights* w, void* pack, size_t pack_byt
   pp.g = G;
   pp.n = w->n;
   pp.k = w->k;
-  pp.nk64p = ((w->k / 64) + 3) / 4 * 4;
+  pp.nk64p = sf_atoms(w->k, mx4);
+  pp.kq = w->k / (mx4 ? 32 : 16);
+  pp.magic = mx4 ? kPackMagicMx : kPackMagic;
   pp.nt = w->n / 128;
   pp.blocks_tmap = (G + 7) / 8;
   const int64_t lines = int64_t(G) * pp.nt * pp.nk64p * 32;
@@ -600,6 +632,19 @@ int fgg_nvfp4_pack_weights(const FggNvfp4Weights* w, void* pack, size_t pack_byt
   nvfp4_pack_weights_kernel<<<int(blocks), 256, 0, reinterpret_cast<cudaStream_t>(stream)>>>(pp);
   FGG_CUDA_CHECK(cudaGetLastError());
   return FGG_OK;
+}
+
+}  // namespace
+}  // namespace fgg
+
+extern "C" {
+
+int fgg_nvfp4_pack_weights(const FggNvfp4Weights* w, void* pack, size_t pack_bytes, void* stream) {
+  return pack_weights_impl(w, pack, pack_bytes, stream, false);
+}
+
+int fgg_mxfp4_pack_weights(const FggNvfp4Weights* w, void* pack, size_t pack_bytes, void* stream) {
+  return pack_weights_impl(w, pack, pack_bytes, stream, true);
 }
 
 size_t fgg_nvfp4_workspace_bytes(const FggNvfp4Problem* p) {
@@ -824,15 +869,17 @@ struct RowsLayout {
   size_t status = 0, ginfo = 0, tiles = 0, sfx = 0, total = 0;
 };
 
-int plan_rows(const FggNvfp4RowsProblem* p, RowsLayout* L) {
+int plan_rows(const FggNvfp4RowsProblem* p, RowsLayout* L, bool mx4) {
   if (p == nullptr) return set_error(FGG_EINVAL, "problem is null");
   const int G = p->num_groups;
   if (G < 1 || G > FGG_MAX_GROUPS)
     return set_error(FGG_EINVAL, "num_groups=%d outside [1, %d]", G, FGG_MAX_GROUPS);
   if (p->n <= 0 || p->n % 128 != 0)
     return set_error(FGG_EBADSHAPE, "N=%d must be a positive multiple of 128", p->n);
-  if (p->k < 64 || p->k % 64 != 0)
-    return set_error(FGG_EBADSHAPE, "K=%d must be a positive multiple of 64", p->k);
+  // whole 4-byte words of scales in a row: 64 elements (NVFP4), 128 (MXFP4)
+  const int kmul = mx4 ? 128 : 64;
+  if (p->k < kmul || p->k % kmul != 0)
+    return set_error(FGG_EBADSHAPE, "K=%d must be a positive multiple of %d", p->k, kmul);
   if (p->n / 128 > 2047) return set_error(FGG_EBADSHAPE, "N=%d too large", p->n);
   if (p->max_rows < 0) return set_error(FGG_EINVAL, "max_rows=%d is negative", p->max_rows);
   if (p->b_index != nullptr &&
@@ -846,7 +893,7 @@ int plan_rows(const FggNvfp4RowsProblem* p, RowsLayout* L) {
   L->ch = L->decode ? CfgDecode::CH : CfgPrefill::CH;
   L->box_rows = L->pair ? CfgPair::BNH : L->bn;
   L->nk256 = (p->k + 255) / 256;
-  L->nk64p = 4 * L->nk256;
+  L->nk64p = sf_atoms(p->k, mx4);
   L->nt128 = p->n / 128;
   L->nt = L->pair ? p->n / 256 : L->nt128;
   // token tiles: sum_g ceil(M_g / BN) <= max_rows / BN + G
@@ -866,21 +913,12 @@ int plan_rows(const FggNvfp4RowsProblem* p, RowsLayout* L) {
   return FGG_OK;
 }
 
-}  // namespace
-}  // namespace fgg
-
-extern "C" {
-
-size_t fgg_nvfp4_rows_workspace_bytes(const FggNvfp4RowsProblem* p) {
+// The rows entry of one format, with that format's three kernels.
+template <bool kMx4, class Pair, class Prefill, class Decode>
+int rows_impl(const FggNvfp4RowsProblem* p, const void* pack, void* workspace, size_t ws_bytes,
+              void* stream) {
   RowsLayout L;
-  if (plan_rows(p, &L) != FGG_OK) return 0;
-  return L.total;
-}
-
-int fgg_nvfp4_grouped_gemm_rows(const FggNvfp4RowsProblem* p, const void* pack, void* workspace,
-                                size_t ws_bytes, void* stream) {
-  RowsLayout L;
-  if (int rc = plan_rows(p, &L)) return rc;
+  if (int rc = plan_rows(p, &L, kMx4)) return rc;
   if (workspace == nullptr) return set_error(FGG_EINVAL, "workspace is null");
   if (!aligned16(workspace)) return set_error(FGG_EALIGN, "workspace must be 16-byte aligned");
   if (ws_bytes < L.total)
@@ -918,6 +956,7 @@ int fgg_nvfp4_grouped_gemm_rows(const FggNvfp4RowsProblem* p, const void* pack, 
   pp.g = G;
   pp.wg = wg;
   pp.k = p->k;
+  pp.kq = p->k / (kMx4 ? 32 : 16);
   pp.bn = L.bn;
   pp.ch = L.ch;
   pp.nk64p = L.nk64p;
@@ -926,7 +965,7 @@ int fgg_nvfp4_grouped_gemm_rows(const FggNvfp4RowsProblem* p, const void* pack, 
   pp.tile_cap = L.tile_cap;
   pp.xt_cap = L.xt_cap;
   pp.blocks_tiles = (L.tile_cap + 255) / 256;
-  pp.sf_vec = (p->k % 256 == 0 && aligned16(p->a_sf)) ? 1 : 0;
+  pp.sf_vec = (pp.kq % 16 == 0 && L.nk64p % 4 == 0 && aligned16(p->a_sf)) ? 1 : 0;
   pp.decode = L.decode ? 1 : 0;
   const int64_t sf_lines = int64_t(L.xt_cap) * L.nk64p * L.ch * 32 / (pp.sf_vec ? 4 : 1);
   const int64_t blocks = 1 + int64_t(pp.blocks_tiles) + (sf_lines + 255) / 256;
@@ -935,7 +974,7 @@ int fgg_nvfp4_grouped_gemm_rows(const FggNvfp4RowsProblem* p, const void* pack, 
   FGG_CUDA_CHECK(cudaGetLastError());
 
   const uint8_t* pk = static_cast<const uint8_t*>(pack);
-  const PackLayout PL = pack_layout(wg, p->n, p->k);
+  const PackLayout PL = pack_layout(wg, p->n, p->k, kMx4);
   GemmParams gp;
   memset(&gp, 0, sizeof(gp));
   if (int rc = encode_u8_2d(&gp.tmap_x_flat, p->a, uint64_t(p->k) / 2, uint64_t(p->max_rows), 128,
@@ -966,12 +1005,12 @@ int fgg_nvfp4_grouped_gemm_rows(const FggNvfp4RowsProblem* p, const void* pack, 
   cudaError_t e;
   if (L.pair) {
     if (int rc = encode_u64_rows(&gp.sfw_map, gp.sfw,
-                                 uint64_t(wg) * L.nt128 * L.nk256 * CfgPair::SFW_BOX_ROWS,
-                                 CfgPair::SFW_ROW_U64, CfgPair::SFW_BOX_ROWS))
+                                 uint64_t(wg) * L.nt128 * L.nk256 * Pair::SFW_BOX_ROWS,
+                                 Pair::SFW_ROW_U64, Pair::SFW_BOX_ROWS))
       return rc;
     if (int rc = encode_u64_rows(&gp.sfx_map, gp.sfx,
-                                 uint64_t(L.xt_cap) * L.nk256 * CfgPair::SFX_BOX_ROWS,
-                                 CfgPair::SFX_ROW_U64, CfgPair::SFX_BOX_ROWS))
+                                 uint64_t(L.xt_cap) * L.nk256 * Pair::SFX_BOX_ROWS,
+                                 Pair::SFX_ROW_U64, Pair::SFX_BOX_ROWS))
       return rc;
     // the narrow token boxes (a tail tile of a group loads only its rows)
     for (int i = 0; i < kXSmallMaps; ++i)
@@ -979,14 +1018,41 @@ int fgg_nvfp4_grouped_gemm_rows(const FggNvfp4RowsProblem* p, const void* pack, 
                                 uint64_t(p->max_rows), 128, uint32_t(16 * (i + 1))))
         return rc;
     gp.x_small = 1;
-    e = launch_pair<CfgPair>(gp, dev.sm_count, s);
+    e = launch_pair<Pair>(gp, dev.sm_count, s);
   } else if (L.decode) {
-    e = launch_engine<CfgDecode>(gp, dev.sm_count, s);
+    e = launch_engine<Decode>(gp, dev.sm_count, s);
   } else {
-    e = launch_engine<CfgPrefill>(gp, dev.sm_count, s);
+    e = launch_engine<Prefill>(gp, dev.sm_count, s);
   }
   if (e != cudaSuccess) return set_error(FGG_ECUDA, "GEMM launch failed: %s", cudaGetErrorString(e));
   return FGG_OK;
+}
+
+}  // namespace
+}  // namespace fgg
+
+extern "C" {
+
+size_t fgg_nvfp4_rows_workspace_bytes(const FggNvfp4RowsProblem* p) {
+  RowsLayout L;
+  if (plan_rows(p, &L, false) != FGG_OK) return 0;
+  return L.total;
+}
+
+size_t fgg_mxfp4_rows_workspace_bytes(const FggMxfp4RowsProblem* p) {
+  RowsLayout L;
+  if (plan_rows(p, &L, true) != FGG_OK) return 0;
+  return L.total;
+}
+
+int fgg_nvfp4_grouped_gemm_rows(const FggNvfp4RowsProblem* p, const void* pack, void* workspace,
+                                size_t ws_bytes, void* stream) {
+  return rows_impl<false, CfgPair, CfgPrefill, CfgDecode>(p, pack, workspace, ws_bytes, stream);
+}
+
+int fgg_mxfp4_grouped_gemm_rows(const FggMxfp4RowsProblem* p, const void* pack, void* workspace,
+                                size_t ws_bytes, void* stream) {
+  return rows_impl<true, Mx4Pair, Mx4Prefill, Mx4Decode>(p, pack, workspace, ws_bytes, stream);
 }
 
 }  // extern "C"

@@ -319,6 +319,18 @@ __device__ __forceinline__ void tc_mma_mxf8f6f4(uint32_t d_tmem, uint64_t adesc,
       "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa_tmem), "r"(sfb_tmem), "r"(accumulate)
       : "memory");
 }
+// MXFP4: E2M1 x E2M1 with one UE8M0 scale per 32 K elements.
+__device__ __forceinline__ void tc_mma_mxf4(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc,
+                                            uint32_t idesc, uint32_t sfa_tmem, uint32_t sfb_tmem,
+                                            uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X"
+      " [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa_tmem), "r"(sfb_tmem), "r"(accumulate)
+      : "memory");
+}
 // ---- CTA-pair (cta_group::2) forms: issued by the pair's leader (alloc and
 // dealloc by the same warp in both CTAs); operands are read from both CTAs'
 // shared memory at the same offsets and results land in both CTAs' TMEM.
@@ -367,6 +379,18 @@ __device__ __forceinline__ void tc_mma_mxf8f6f4_pair(uint32_t d_tmem, uint64_t a
       "{\n\t.reg .pred p;\n\t"
       "setp.ne.b32 p, %6, 0;\n\t"
       "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale"
+      " [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa_tmem), "r"(sfb_tmem), "r"(accumulate)
+      : "memory");
+}
+
+__device__ __forceinline__ void tc_mma_mxf4_pair(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc,
+                                                 uint32_t idesc, uint32_t sfa_tmem,
+                                                 uint32_t sfb_tmem, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X"
       " [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d_tmem),
       "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa_tmem), "r"(sfb_tmem), "r"(accumulate)
       : "memory");
@@ -461,7 +485,7 @@ __host__ __device__ constexpr uint32_t idesc_f16(uint32_t fmt, uint32_t a_mn, ui
   return (1u << 4) | (fmt << 7) | (fmt << 10) | (a_mn << 15) | (b_mn << 16) |
          (uint32_t(n >> 3) << 17) | (uint32_t(m >> 4) << 24);
 }
-constexpr uint32_t kFmtNvf4E2M1 = 1;   // .kind::mxf4nvf4 operand format E2M1
+constexpr uint32_t kFmtNvf4E2M1 = 1;   // .kind::mxf4nvf4 and .kind::mxf4 operand format E2M1
 constexpr uint32_t kFmtF8E4M3 = 0;     // .kind::mxf8f6f4 E4M3
 constexpr uint32_t kFmtF8E2M1 = 5;     // .kind::mxf8f6f4 E2M1 (one element per byte in smem)
 
