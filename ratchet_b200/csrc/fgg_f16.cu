@@ -25,6 +25,13 @@
 //   * n and k need not be multiples of the tile: TMA fills zeros, and the
 //     epilogues clip.
 //
+// The tensor core adds each instruction's sixteen products to its fp32
+// accumulator with truncation, so a long sum drifts towards zero: by 5e-6 of its
+// value on average over groups of 4000 rows, ten times what fp32 additions in
+// order lose.  Against a gradient's fp32 that is visible, so wgrad sums 512 rows
+// at a time in TMEM and the epilogue adds those sums in registers, rounding to
+// nearest; a 16-bit result hides it (forward, dgrad).
+//
 // What bounds it: the tensor pipe for groups of about 200 tokens and more, the
 // weights' HBM stream below that, the gradient's write for wgrad with short
 // groups.
@@ -97,14 +104,24 @@ struct F16Cfg {
   static constexpr int STAGES = 6;
   static constexpr uint32_t TMEM_COLS = 512;  // two accumulators of 256 columns
   static constexpr int SCHED = 8;
-  // readers of a slot: leader producer, MMA warp, 4 epilogue warps; follower
-  // producer and 4 epilogue warps
-  static constexpr uint32_t SCHED_READERS = 11;
+  // Epilogue warps of a CTA: one per TMEM quadrant; wgrad two per quadrant, 128
+  // columns each, which it holds in registers over the chunks of a long group.
+  static constexpr int EPI_WARPS = MODE_ == kWgrad ? 8 : 4;
+  static constexpr int THREADS = 128 + 32 * EPI_WARPS;
+  // wgrad's registers: launched with 168 per thread (384 threads), of which the
+  // four other warps give most to the epilogue's 128 sums
+  static constexpr int REGS_OTHER = 64, REGS_EPI = 216;
+  static constexpr int REGS_TOTAL = 128 * REGS_OTHER + 32 * EPI_WARPS * REGS_EPI;
+  // steps of the contraction that one TMEM accumulator sums
+  static constexpr int CHUNK = MODE_ == kWgrad ? 8 : 1 << 30;
+  // readers of a slot: leader producer, MMA warp, epilogue warps; follower
+  // producer and epilogue warps
+  static constexpr uint32_t SCHED_READERS = 3 + 2 * EPI_WARPS;
   static constexpr uint32_t NBARS = 2 * STAGES + 4 + 2 * SCHED + 3;
   // epilogue staging of a warp: 16 tokens x 64 bytes; wgrad 32 rows x 128 bytes
   static constexpr uint32_t EPI_WARP = MODE_ == kWgrad ? 4096 : 1024;
   static constexpr uint32_t EPI_REGION = STAGES * STAGE_BYTES;  // 1024 B aligned
-  static constexpr uint32_t BAR_REGION = EPI_REGION + 4 * EPI_WARP;
+  static constexpr uint32_t BAR_REGION = EPI_REGION + EPI_WARPS * EPI_WARP;
   static constexpr uint32_t SMEM_BYTES = 1024 + BAR_REGION + 8 * NBARS + 32 * SCHED + 16;
   static_assert(SMEM_BYTES <= 232448, "shared memory budget exceeded");
 };
@@ -147,64 +164,58 @@ __device__ __forceinline__ void f16_epilogue_rows(void* out, int ldn, int m0, si
   }
 }
 
-// Wgrad.  The warp's TMEM lanes are gradient rows n0 + lane, its columns k.
-// 128 bytes of every row at a time go through 4 KB of shared memory (16-byte
-// units swizzled by the row: no bank conflicts either way), so that eight lanes
-// store one row's 128 contiguous bytes.  With accumulate the same lanes read
+// Wgrad.  The warp's lanes hold gradient rows n0 + lane, `acc` 128 columns from
+// k0 of each.  128 bytes of every row at a time go through 4 KB of shared memory
+// (16-byte units swizzled by the row: no bank conflicts either way), so that eight
+// lanes store one row's 128 contiguous bytes.  With accumulate the same lanes read
 // what is there and add: one addition per element.
-__device__ __forceinline__ void f16_epilogue_wgrad(const F16Params& p, int g, int n0, int k0,
-                                                   bool empty, uint32_t taddr, uint8_t* stage) {
+template <bool kFp32>
+__device__ __forceinline__ void f16_store_wgrad(const F16Params& p, int g, int n0, int k0,
+                                                const float (&acc)[128], uint8_t* stage) {
   const int lane = threadIdx.x & 31;
-  const int eb = p.out_fp32 ? 4 : 2;
-  const int cw = 128 / eb;  // columns per step
-  const int kcols = min(256, p.c_ext - k0);
-  if (n0 >= p.m_ext) return;
+  const int kcols = min(128, p.c_ext - k0);
+  if (n0 >= p.m_ext || kcols <= 0) return;
+  constexpr int eb = kFp32 ? 4 : 2;
+  constexpr int cw = 128 / eb;  // columns per step
+  const size_t pitch = size_t(p.c_ext) * eb;
+  const int unit = lane & 7, r0 = lane >> 3;
   uint8_t* const out = static_cast<uint8_t*>(p.out) +
-                       ((size_t(g) * size_t(p.m_ext) + size_t(n0)) * size_t(p.c_ext) + size_t(k0)) *
-                           size_t(eb);
-  const size_t pitch = size_t(p.c_ext) * size_t(eb);
-  const int unit = lane & 7;
-  for (int c0 = 0; c0 < kcols; c0 += cw) {
-    uint32_t v[32];
-    if (empty) {
+                       (size_t(g) * size_t(p.m_ext) + size_t(n0 + r0)) * pitch + size_t(k0) * eb +
+                       unit * 16;
 #pragma unroll
-      for (int j = 0; j < 32; ++j) v[j] = 0u;
-    } else if (p.out_fp32) {
-      tmem_ld32(taddr + c0, v);
-      tmem_wait_ld();
-    } else {
+  for (int i = 0; i < 128 / cw; ++i) {
+    if (i * cw >= kcols) break;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t r[32];
-        tmem_ld32(taddr + c0 + 32 * h, r);
-        tmem_wait_ld();
-#pragma unroll
-        for (int j = 0; j < 16; ++j)
-          v[16 * h + j] = pack_16(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]),
-                                  p.bf16 != 0);
+    for (int u = 0; u < 8; ++u) {
+      uint4 q;
+      if constexpr (kFp32) {
+        const int c = cw * i + 4 * u;
+        q = make_uint4(__float_as_uint(acc[c]), __float_as_uint(acc[c + 1]),
+                       __float_as_uint(acc[c + 2]), __float_as_uint(acc[c + 3]));
+      } else {
+        const int c = cw * i + 8 * u;
+        const bool b = p.bf16 != 0;
+        q = make_uint4(pack_16(acc[c], acc[c + 1], b), pack_16(acc[c + 2], acc[c + 3], b),
+                       pack_16(acc[c + 4], acc[c + 5], b), pack_16(acc[c + 6], acc[c + 7], b));
       }
+      *reinterpret_cast<uint4*>(stage + lane * 128 + ((u ^ (lane & 7)) << 4)) = q;
     }
-#pragma unroll
-    for (int u = 0; u < 8; ++u)
-      *reinterpret_cast<uint4*>(stage + lane * 128 + ((u ^ (lane & 7)) << 4)) =
-          make_uint4(v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]);
     __syncwarp();
-    const bool col_ok = c0 + unit * (16 / eb) < kcols;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int row = 4 * i + (lane >> 3);
+    const bool col_ok = i * cw + unit * (16 / eb) < kcols;
+    uint8_t* at = out + i * 128;
+#pragma unroll 2
+    for (int row = r0; row < 32; row += 4, at += 4 * pitch) {
       if (col_ok && n0 + row < p.m_ext) {
         uint4 q = *reinterpret_cast<const uint4*>(stage + row * 128 + ((unit ^ (row & 7)) << 4));
-        uint4* const dst =
-            reinterpret_cast<uint4*>(out + size_t(row) * pitch + size_t(c0) * eb + unit * 16);
-        if (p.accumulate) {  // fp32
-          const uint4 old = *dst;
+        uint4* const d = reinterpret_cast<uint4*>(at);
+        if (kFp32 && p.accumulate) {
+          const uint4 old = *d;
           q.x = __float_as_uint(__uint_as_float(old.x) + __uint_as_float(q.x));
           q.y = __float_as_uint(__uint_as_float(old.y) + __uint_as_float(q.y));
           q.z = __float_as_uint(__uint_as_float(old.z) + __uint_as_float(q.z));
           q.w = __float_as_uint(__uint_as_float(old.w) + __uint_as_float(q.w));
         }
-        *dst = q;
+        *d = q;
       }
     }
     __syncwarp();
@@ -255,9 +266,9 @@ __device__ __forceinline__ F16Slot f16_make_slot(const F16Params& p, int t, int 
 
 // Roles as in the block-scaled pair kernel (fgg_engine.cuh): warp 0 producer in
 // both CTAs, warp 1 MMA issuer in the leader, warp 2 TMEM, warp 3 scheduler in
-// the leader, warps 4-7 epilogue.
+// the leader, the others epilogue.
 template <class C>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(C::THREADS, 1)
     f16_pair_kernel(const __grid_constant__ F16Params p) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
@@ -303,7 +314,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(accf_bar(b), 1);
-      mbar_init(acce_bar(b), 8);  // 4 epilogue warps in each CTA (leader's barrier)
+      mbar_init(acce_bar(b), 2 * C::EPI_WARPS);  // both CTAs' (leader's barrier)
     }
     for (int i = 0; i < C::SCHED; ++i) {
       mbar_init(schedf_bar(i), 1);
@@ -338,221 +349,232 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
       mbar_arrive_remote(leader_schede0 + 8u * slot);
   };
 
-  if (warp == 3) {
-    // ---------------------------------------------- scheduler (leader only)
-    if (lane == 0 && leader) {
+  // the register split comes first in each branch: the compiler allots by branch
+  if (warp < 4) {
+    if constexpr (C::MODE == kWgrad) regs_dec<C::REGS_OTHER>();
+    if (warp == 3) {
+      // ---------------------------------------------- scheduler (leader only)
+      if (lane == 0 && leader) {
+        int slot = 0;
+        uint32_t sphase = 0;
+        const int num_tiles = p.status[3];
+        const uint32_t remote_ring0 = mapa_shared(smem_u32(const_cast<F16Slot*>(ring)), peer);
+        const uint32_t remote_schedf0 = mapa_shared(schedf_bar(0), peer);
+        for (uint32_t n = 0;; ++n) {
+          // at most one tile per pair that it has not started
+          if (n > 0 && !mbar_wait1(taken_bar, (n - 1) & 1u, abort_flag, p.status,
+                                   kStatusTimeoutProducer))
+            break;
+          const int t = atomicAdd(p.status + 1, 1);
+          const F16Slot s = f16_make_slot<C::MODE>(p, t, num_tiles);
+          if (!mbar_wait1<true>(schede_bar(slot), sphase ^ 1, abort_flag, p.status,
+                                kStatusTimeoutProducer))
+            break;
+          const uint32_t words[5] = {uint32_t(s.g), uint32_t(s.mt), uint32_t(s.row0),
+                                     uint32_t(s.rows), uint32_t(s.ct)};
+  #pragma unroll
+          for (int i = 0; i < 5; ++i) {
+            reinterpret_cast<volatile uint32_t*>(ring + slot)[i] = words[i];
+            st_shared_remote_u32(remote_ring0 + 32u * slot + 4u * i, words[i]);
+          }
+          mbar_arrive(schedf_bar(slot));
+          mbar_arrive_remote(remote_schedf0 + 8u * slot);
+          if (++slot == C::SCHED) {
+            slot = 0;
+            sphase ^= 1;
+          }
+          if (s.g < 0) break;
+        }
+      }
+      __syncwarp();
+    } else if (warp == 0) {
+      // ------------------------------------------------- producer (both CTAs)
+      int stage = 0;
+      uint32_t phase = 0;
       int slot = 0;
       uint32_t sphase = 0;
-      const int num_tiles = p.status[3];
-      const uint32_t remote_ring0 = mapa_shared(smem_u32(const_cast<F16Slot*>(ring)), peer);
-      const uint32_t remote_schedf0 = mapa_shared(schedf_bar(0), peer);
-      for (uint32_t n = 0;; ++n) {
-        // at most one tile per pair that it has not started
-        if (n > 0 && !mbar_wait1(taken_bar, (n - 1) & 1u, abort_flag, p.status,
-                                 kStatusTimeoutProducer))
-          break;
-        const int t = atomicAdd(p.status + 1, 1);
-        const F16Slot s = f16_make_slot<C::MODE>(p, t, num_tiles);
-        if (!mbar_wait1<true>(schede_bar(slot), sphase ^ 1, abort_flag, p.status,
-                              kStatusTimeoutProducer))
-          break;
-        const uint32_t words[5] = {uint32_t(s.g), uint32_t(s.mt), uint32_t(s.row0),
-                                   uint32_t(s.rows), uint32_t(s.ct)};
-#pragma unroll
-        for (int i = 0; i < 5; ++i) {
-          reinterpret_cast<volatile uint32_t*>(ring + slot)[i] = words[i];
-          st_shared_remote_u32(remote_ring0 + 32u * slot + 4u * i, words[i]);
+      uint32_t arms = 0;
+      if (lane == 0) {
+        if constexpr (C::MODE == kWgrad) {
+          prefetch_tensormap(&p.tmap_a);
+          prefetch_tensormap(&p.tmap_b);
+        } else {
+          prefetch_tensormap(&p.tmap_w);
+          prefetch_tensormap(&p.tmap_tok[kTokenMaps - 1]);
         }
-        mbar_arrive(schedf_bar(slot));
-        mbar_arrive_remote(remote_schedf0 + 8u * slot);
+      }
+      while (true) {
+        if (!mbar_wait<true>(schedf_bar(slot), sphase, abort_flag, p.status,
+                             kStatusTimeoutProducer))
+          break;
+        const int g = __shfl_sync(kFullMask, ring[slot].g, 0);
+        const int mt = __shfl_sync(kFullMask, ring[slot].mt, 0);
+        const int row0 = __shfl_sync(kFullMask, ring[slot].row0, 0);
+        const int rows = __shfl_sync(kFullMask, ring[slot].rows, 0);
+        const int ct = __shfl_sync(kFullMask, ring[slot].ct, 0);
+        if (lane == 0) {
+          release_slot(slot);
+          if (leader) mbar_arrive(taken_bar);
+        }
         if (++slot == C::SCHED) {
           slot = 0;
           sphase ^= 1;
         }
-        if (s.g < 0) break;
-      }
-    }
-    __syncwarp();
-  } else if (warp == 0) {
-    // ------------------------------------------------- producer (both CTAs)
-    int stage = 0;
-    uint32_t phase = 0;
-    int slot = 0;
-    uint32_t sphase = 0;
-    uint32_t arms = 0;
-    if (lane == 0) {
-      if constexpr (C::MODE == kWgrad) {
-        prefetch_tensormap(&p.tmap_a);
-        prefetch_tensormap(&p.tmap_b);
-      } else {
-        prefetch_tensormap(&p.tmap_w);
-        prefetch_tensormap(&p.tmap_tok[kTokenMaps - 1]);
-      }
-    }
-    while (true) {
-      if (!mbar_wait<true>(schedf_bar(slot), sphase, abort_flag, p.status,
-                           kStatusTimeoutProducer))
-        break;
-      const int g = __shfl_sync(kFullMask, ring[slot].g, 0);
-      const int mt = __shfl_sync(kFullMask, ring[slot].mt, 0);
-      const int row0 = __shfl_sync(kFullMask, ring[slot].row0, 0);
-      const int rows = __shfl_sync(kFullMask, ring[slot].rows, 0);
-      const int ct = __shfl_sync(kFullMask, ring[slot].ct, 0);
-      if (lane == 0) {
-        release_slot(slot);
-        if (leader) mbar_arrive(taken_bar);
-      }
-      if (++slot == C::SCHED) {
-        slot = 0;
-        sphase ^= 1;
-      }
-      if (g < 0) {
-        if (lane == 0) griddep_launch_dependents();  // no new tiles for this CTA
-        break;
-      }
-      const int half = tile_ncols(rows) >> 1;
-      const int ksteps = tile_ksteps(rows);
-      // bytes that both CTAs' loads of one step deliver to the leader's barrier
-      const uint32_t tx_step = 2u * (C::A_BYTES + uint32_t(half) * 128u);
-      const int flat_steps = C::MODE == kWgrad ? wgrad_flat_steps(rows) : ksteps;
-      const int m0 = mt * 256 + int(rank) * 128;     // this CTA's rows of the M axis
-      const int tok = row0 + int(rank) * half;       // forward, dgrad: its tokens
-      const int c0 = ct * 256 + int(rank) * 128;     // wgrad: its columns k
-      const CUtensorMap* const tb =
-          C::MODE == kWgrad ? &p.tmap_b : &p.tmap_tok[half / 16 - 1];
-      bool ok = true;
-      for (int ks = 0; ks < ksteps; ++ks) {
-        if (!mbar_wait(empty_bar(stage), phase ^ 1, abort_flag, p.status,
-                       kStatusTimeoutProducer)) {
-          ok = false;
+        if (g < 0) {
+          if (lane == 0) griddep_launch_dependents();  // no new tiles for this CTA
           break;
         }
-        const uint32_t fb = leader_full0 + 8u * stage;
-        const int x = ks * C::KS;
-        const bool arm = (p.debug_flags & kDebugNoLoads) == 0;
-        if (arm && elect_one()) {
-          // the copy of a group's last rows comes in boxes of 16 rows
-          const bool tail = C::MODE == kWgrad && ks >= flat_steps;
-          if (leader) mbar_arrive_expect_tx(full_bar(stage), tail ? tx_step / 4 : tx_step);
-          if constexpr (C::MODE == kFwd) {
-            tma_load_3d_pair(sA(stage), &p.tmap_w, fb, x, m0, g);
-            tma_load_2d_pair(sB(stage), tb, fb, x, tok);
-          } else if constexpr (C::MODE == kDgrad) {
-            tma_load_3d_pair(sA(stage), &p.tmap_w, fb, m0, x, g);
-            tma_load_3d_pair(sA(stage) + 8192u, &p.tmap_w, fb, m0 + 64, x, g);
-            tma_load_2d_pair(sB(stage), tb, fb, x, tok);
-          } else {
-            const CUtensorMap* const ma = tail ? &p.tmap_ta : &p.tmap_a;
-            const CUtensorMap* const mb = tail ? &p.tmap_tb : tb;
-            const int y = tail ? 16 * g : row0 + x;
-            tma_load_2d_pair(sA(stage), ma, fb, m0, y);
-            tma_load_2d_pair(sA(stage) + 8192u, ma, fb, m0 + 64, y);
-            tma_load_2d_pair(sB(stage), mb, fb, c0, y);
-            tma_load_2d_pair(sB(stage) + 8192u, mb, fb, c0 + 64, y);
+        const int half = tile_ncols(rows) >> 1;
+        const int ksteps = tile_ksteps(rows);
+        // bytes that both CTAs' loads of one step deliver to the leader's barrier
+        const uint32_t tx_step = 2u * (C::A_BYTES + uint32_t(half) * 128u);
+        const int flat_steps = C::MODE == kWgrad ? wgrad_flat_steps(rows) : ksteps;
+        const int m0 = mt * 256 + int(rank) * 128;     // this CTA's rows of the M axis
+        const int tok = row0 + int(rank) * half;       // forward, dgrad: its tokens
+        const int c0 = ct * 256 + int(rank) * 128;     // wgrad: its columns k
+        const CUtensorMap* const tb =
+            C::MODE == kWgrad ? &p.tmap_b : &p.tmap_tok[half / 16 - 1];
+        bool ok = true;
+        for (int ks = 0; ks < ksteps; ++ks) {
+          if (!mbar_wait(empty_bar(stage), phase ^ 1, abort_flag, p.status,
+                         kStatusTimeoutProducer)) {
+            ok = false;
+            break;
+          }
+          const uint32_t fb = leader_full0 + 8u * stage;
+          const int x = ks * C::KS;
+          const bool arm = (p.debug_flags & kDebugNoLoads) == 0;
+          if (arm && elect_one()) {
+            // the copy of a group's last rows comes in boxes of 16 rows
+            const bool tail = C::MODE == kWgrad && ks >= flat_steps;
+            if (leader) mbar_arrive_expect_tx(full_bar(stage), tail ? tx_step / 4 : tx_step);
+            if constexpr (C::MODE == kFwd) {
+              tma_load_3d_pair(sA(stage), &p.tmap_w, fb, x, m0, g);
+              tma_load_2d_pair(sB(stage), tb, fb, x, tok);
+            } else if constexpr (C::MODE == kDgrad) {
+              tma_load_3d_pair(sA(stage), &p.tmap_w, fb, m0, x, g);
+              tma_load_3d_pair(sA(stage) + 8192u, &p.tmap_w, fb, m0 + 64, x, g);
+              tma_load_2d_pair(sB(stage), tb, fb, x, tok);
+            } else {
+              const CUtensorMap* const ma = tail ? &p.tmap_ta : &p.tmap_a;
+              const CUtensorMap* const mb = tail ? &p.tmap_tb : tb;
+              const int y = tail ? 16 * g : row0 + x;
+              tma_load_2d_pair(sA(stage), ma, fb, m0, y);
+              tma_load_2d_pair(sA(stage) + 8192u, ma, fb, m0 + 64, y);
+              tma_load_2d_pair(sB(stage), mb, fb, c0, y);
+              tma_load_2d_pair(sB(stage) + 8192u, mb, fb, c0 + 64, y);
+            }
+          }
+          __syncwarp();
+          if (arm) ++arms;
+          if (++stage == C::STAGES) {
+            stage = 0;
+            phase ^= 1;
           }
         }
-        __syncwarp();
-        if (arm) ++arms;
-        if (++stage == C::STAGES) {
-          stage = 0;
-          phase ^= 1;
-        }
+        if (!ok) break;
       }
-      if (!ok) break;
-    }
-    // the leader's full barriers cover both CTAs' bytes: they land before exit
-    if (leader && lane == 0) {
-      const uint32_t first = arms > uint32_t(C::STAGES) ? arms - C::STAGES : 0u;
-      for (uint32_t a = first; a < arms; ++a)
-        mbar_wait_one(full_bar(int(a % C::STAGES)), (a / C::STAGES) & 1u, 200000000ull);
-    }
-    __syncwarp();
-  } else if (warp == 1 && leader) {
-    // ------------------------------------------------------- MMA issuer
-    bool ok = mbar_wait(tmem_ready_bar, 0, abort_flag, p.status, kStatusTimeoutMma);
-    tc_fence_after();
-    const uint32_t tmem = __shfl_sync(kFullMask, *tmem_holder, 0);
-    int stage = 0;
-    uint32_t phase = 0;
-    int slot = 0;
-    uint32_t sphase = 0;
-    uint32_t lt = 0;
-    bool issued_any = false;
-    while (ok) {
-      if (!mbar_wait<true>(schedf_bar(slot), sphase, abort_flag, p.status, kStatusTimeoutMma))
-        break;
-      const int g = __shfl_sync(kFullMask, ring[slot].g, 0);
-      const int rows = __shfl_sync(kFullMask, ring[slot].rows, 0);
-      if (lane == 0) mbar_arrive(schede_bar(slot));
-      if (++slot == C::SCHED) {
-        slot = 0;
-        sphase ^= 1;
+      // the leader's full barriers cover both CTAs' bytes: they land before exit
+      if (leader && lane == 0) {
+        const uint32_t first = arms > uint32_t(C::STAGES) ? arms - C::STAGES : 0u;
+        for (uint32_t a = first; a < arms; ++a)
+          mbar_wait_one(full_bar(int(a % C::STAGES)), (a / C::STAGES) & 1u, 200000000ull);
       }
-      if (g < 0) break;
-      const int ncols = tile_ncols(rows);
-      const int ksteps = tile_ksteps(rows);
-      const uint32_t b = lt & 1u;
-      if (!mbar_wait(acce_bar(b), ((lt >> 1) & 1u) ^ 1u, abort_flag, p.status, kStatusTimeoutMma))
-        break;
+      __syncwarp();
+    } else if (warp == 1 && leader) {
+      // ------------------------------------------------------- MMA issuer
+      bool ok = mbar_wait(tmem_ready_bar, 0, abort_flag, p.status, kStatusTimeoutMma);
       tc_fence_after();
-      const uint32_t d_tmem = tmem + b * C::BN;
-      const uint32_t idesc =
-          idesc_f16(p.bf16 ? 1u : 0u, C::A_MN ? 1u : 0u, C::B_MN ? 1u : 0u, 256, ncols);
-      for (int ks = 0; ks < ksteps; ++ks) {
-        if (!mbar_wait(full_bar(stage), phase, abort_flag, p.status, kStatusTimeoutMma)) {
-          ok = false;
+      const uint32_t tmem = __shfl_sync(kFullMask, *tmem_holder, 0);
+      int stage = 0;
+      uint32_t phase = 0;
+      int slot = 0;
+      uint32_t sphase = 0;
+      uint32_t lt = 0;
+      bool issued_any = false;
+      while (ok) {
+        if (!mbar_wait<true>(schedf_bar(slot), sphase, abort_flag, p.status, kStatusTimeoutMma))
           break;
+        const int g = __shfl_sync(kFullMask, ring[slot].g, 0);
+        const int rows = __shfl_sync(kFullMask, ring[slot].rows, 0);
+        if (lane == 0) mbar_arrive(schede_bar(slot));
+        if (++slot == C::SCHED) {
+          slot = 0;
+          sphase ^= 1;
         }
-        tc_fence_after();
-        const uint64_t adesc = C::A_MN ? desc_mn_sw128(sA(stage), 8192u) : desc_k_sw128(sA(stage));
-        const uint64_t bdesc = C::B_MN ? desc_mn_sw128(sB(stage), 8192u) : desc_k_sw128(sB(stage));
-        // 16 of the contraction: 32 bytes of a K-major row, 16 rows of an MN-major tile
-        constexpr uint32_t kStepA = C::A_MN ? 2048u >> 4 : 32u >> 4;
-        constexpr uint32_t kStepB = C::B_MN ? 2048u >> 4 : 32u >> 4;
-        // wgrad: the whole sixteens of rows that this step holds; its last, the copy
-        const int nj = C::MODE == kWgrad
-                           ? (ks < wgrad_flat_steps(rows) ? min(4, rows / 16 - 4 * ks) : 1)
-                           : 4;
+        if (g < 0) break;
+        const int ncols = tile_ncols(rows);
+        const int ksteps = tile_ksteps(rows);
+        const uint32_t idesc =
+            idesc_f16(p.bf16 ? 1u : 0u, C::A_MN ? 1u : 0u, C::B_MN ? 1u : 0u, 256, ncols);
+        // an empty group's gradient (wgrad) is a chunk without steps
+        int ks = 0;
+        do {
+          const int chunk0 = ks;
+          const int chunk1 = min(ksteps - chunk0, C::CHUNK) + chunk0;
+          const uint32_t b = lt & 1u;
+          if (!mbar_wait(acce_bar(b), ((lt >> 1) & 1u) ^ 1u, abort_flag, p.status,
+                         kStatusTimeoutMma)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t d_tmem = tmem + b * C::BN;
+          for (; ks < chunk1; ++ks) {
+            if (!mbar_wait(full_bar(stage), phase, abort_flag, p.status, kStatusTimeoutMma)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const uint64_t adesc =
+                C::A_MN ? desc_mn_sw128(sA(stage), 8192u) : desc_k_sw128(sA(stage));
+            const uint64_t bdesc =
+                C::B_MN ? desc_mn_sw128(sB(stage), 8192u) : desc_k_sw128(sB(stage));
+            // 16 of the contraction: 32 bytes of a K-major row, 16 rows of an MN-major tile
+            constexpr uint32_t kStepA = C::A_MN ? 2048u >> 4 : 32u >> 4;
+            constexpr uint32_t kStepB = C::B_MN ? 2048u >> 4 : 32u >> 4;
+            // wgrad: the whole sixteens of rows that this step holds; its last, the copy
+            const int nj = C::MODE == kWgrad
+                               ? (ks < wgrad_flat_steps(rows) ? min(4, rows / 16 - 4 * ks) : 1)
+                               : 4;
+            if (elect_one()) {
+  #pragma unroll
+              for (int j = 0; j < 4; ++j)
+                if (j < nj)
+                  tc_mma_f16_pair(d_tmem, adesc + kStepA * j, bdesc + kStepB * j, idesc,
+                                  ((ks - chunk0) | j) != 0 ? 1u : 0u);
+              tc_commit_pair(empty_bar(stage), 0x3);
+            }
+            __syncwarp();
+            if (++stage == C::STAGES) {
+              stage = 0;
+              phase ^= 1;
+            }
+          }
+          if (!ok) break;
+          if (elect_one()) tc_commit_pair(accf_bar(b), 0x3);
+          __syncwarp();
+          issued_any = true;
+          ++lt;
+        } while (ks < ksteps);
+      }
+      if (issued_any) {
         if (elect_one()) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (j < nj)
-              tc_mma_f16_pair(d_tmem, adesc + kStepA * j, bdesc + kStepB * j, idesc,
-                              (ks | j) != 0 ? 1u : 0u);
-          tc_commit_pair(empty_bar(stage), 0x3);
-          if (ks + 1 == ksteps) tc_commit_pair(accf_bar(b), 0x3);
-        }
-        __syncwarp();
-        issued_any = true;
-        if (++stage == C::STAGES) {
-          stage = 0;
-          phase ^= 1;
+          tc_commit_pair(drain_bar, 0x1);
+          if (!mbar_wait_one(drain_bar, 0, 200000000ull))
+            atomicCAS(p.status, 0, kStatusTimeoutDrain);
         }
       }
-      if (!ok) break;
-      // an empty group's gradient tile (wgrad): nothing to multiply, zeros to store
-      if (ksteps == 0) {
-        if (elect_one()) tc_commit_pair(accf_bar(b), 0x3);
-        __syncwarp();
-        issued_any = true;
-      }
-      ++lt;
+      __syncwarp();
     }
-    if (issued_any) {
-      if (elect_one()) {
-        tc_commit_pair(drain_bar, 0x1);
-        if (!mbar_wait_one(drain_bar, 0, 200000000ull))
-          atomicCAS(p.status, 0, kStatusTimeoutDrain);
-      }
-    }
-    __syncwarp();
-  } else if (warp >= 4) {
+  } else {
     // --------------------------------------------------------- epilogue
+    if constexpr (C::MODE == kWgrad) regs_inc<C::REGS_EPI>();
     const int q = warp & 3;
     bool ok = mbar_wait(tmem_ready_bar, 0, abort_flag, p.status, kStatusTimeoutEpilogue);
     tc_fence_after();
     const uint32_t tmem = *tmem_holder;
-    const uint32_t stage_off = C::EPI_REGION + uint32_t(q) * C::EPI_WARP;
+    const uint32_t stage_off = C::EPI_REGION + uint32_t(warp - 4) * C::EPI_WARP;
     int slot = 0;
     uint32_t sphase = 0;
     uint32_t lt = 0;
@@ -568,29 +590,65 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
         sphase ^= 1;
       }
       if (s.g < 0) break;
-      const uint32_t b = lt & 1u;
-      if (!mbar_wait(accf_bar(b), (lt >> 1) & 1u, abort_flag, p.status, kStatusTimeoutEpilogue))
-        break;
-      tc_fence_after();
       const int m0 = s.mt * 256 + int(rank) * 128 + q * 32;
-      const uint32_t taddr = tmem + (uint32_t(q * 32) << 16) + b * C::BN;
+      auto release_acc = [&](uint32_t b) {  // this warp has read accumulator b
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if (leader)
+            mbar_arrive(acce_bar(b));
+          else
+            mbar_arrive_remote(leader_acce0 + 8u * b);
+        }
+      };
       if constexpr (C::MODE == kWgrad) {
-        if (s.rows > 0 || !p.accumulate)
-          f16_epilogue_wgrad(p, s.g, m0, s.ct * 256, s.rows == 0, taddr, gbase + stage_off);
+        const int part = (warp - 4) >> 2;  // its 128 columns of 256
+        const int ksteps = tile_ksteps(s.rows);
+        float acc[128];
+#pragma unroll
+        for (int j = 0; j < 128; ++j) acc[j] = 0.0f;
+        int ks = 0;
+        do {
+          const uint32_t b = lt & 1u;
+          if (!mbar_wait(accf_bar(b), (lt >> 1) & 1u, abort_flag, p.status,
+                         kStatusTimeoutEpilogue)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t taddr = tmem + (uint32_t(q * 32) << 16) + b * C::BN + 128u * part;
+          if (ksteps > 0) {
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+              uint32_t r[16];
+              tmem_ld16(taddr + 16 * c, r);
+              tmem_wait_ld();
+#pragma unroll
+              for (int j = 0; j < 16; ++j) acc[16 * c + j] += __uint_as_float(r[j]);
+            }
+          }
+          release_acc(b);
+          ++lt;
+          ks += C::CHUNK;
+        } while (ks < ksteps);
+        if (ok && (s.rows > 0 || !p.accumulate)) {
+          if (p.out_fp32)
+            f16_store_wgrad<true>(p, s.g, m0, s.ct * 256 + 128 * part, acc, gbase + stage_off);
+          else
+            f16_store_wgrad<false>(p, s.g, m0, s.ct * 256 + 128 * part, acc, gbase + stage_off);
+        }
       } else {
+        const uint32_t b = lt & 1u;
+        if (!mbar_wait(accf_bar(b), (lt >> 1) & 1u, abort_flag, p.status, kStatusTimeoutEpilogue))
+          break;
+        tc_fence_after();
+        const uint32_t taddr = tmem + (uint32_t(q * 32) << 16) + b * C::BN;
         if (m0 < p.m_ext)
           f16_epilogue_rows(p.out, p.m_ext, m0, size_t(s.row0), s.rows, tile_ncols(s.rows),
                             p.bf16 != 0, taddr, reinterpret_cast<uint32_t*>(gbase + stage_off));
+        release_acc(b);
+        ++lt;
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        if (leader)
-          mbar_arrive(acce_bar(b));
-        else
-          mbar_arrive_remote(leader_acce0 + 8u * b);
-      }
-      ++lt;
     }
   }
 
@@ -781,8 +839,19 @@ int launch_f16(const F16Params& gp, const DeviceInfo& dev, cudaStream_t s) {
   if (int rc = ensure_max_dynamic_smem(reinterpret_cast<const void*>(f16_pair_kernel<C>),
                                        int(C::SMEM_BYTES)))
     return rc;
+  if constexpr (MODE == kWgrad) {
+    // a split of more registers than the block starts with would never be granted
+    static const int regs = [] {
+      cudaFuncAttributes a = {};
+      return cudaFuncGetAttributes(&a, f16_pair_kernel<C>) == cudaSuccess ? a.numRegs : 0;
+    }();
+    if (regs * C::THREADS < C::REGS_TOTAL)
+      return set_error(FGG_ECUDA, "the kernel was built with %d registers per thread, needs %d",
+                       regs, (C::REGS_TOTAL + C::THREADS - 1) / C::THREADS);
+  }
   const int pairs = std::max(1, std::min(gp.grid_tiles, dev.sm_count / 2));
-  const cudaError_t e = launch_dependent(f16_pair_kernel<C>, 2 * pairs, C::SMEM_BYTES, s, gp);
+  const cudaError_t e = launch_pdl(f16_pair_kernel<C>, dim3(2 * pairs), dim3(C::THREADS),
+                                   C::SMEM_BYTES, s, gp);
   if (e != cudaSuccess) return set_error(FGG_ECUDA, "GEMM launch failed: %s", cudaGetErrorString(e));
   return FGG_OK;
 }

@@ -102,3 +102,77 @@ def test_forward_and_gradients(cuda_device, case, dtype):
         for g, a, b in _spans(off):
             if a == b:
                 assert bool((dw[g] == 0).all())
+
+
+@pytest.mark.parametrize("rows", [496, 512, 513, 1024, 1039, 4100])
+def test_wgrad_chunks(cuda_device, rows):
+    """Groups around and past the rows that one accumulator sums; the others of the
+    same call are short."""
+    import ratchet_b200 as rb
+
+    sizes, n, k = [3, rows, 0, 70], 72, 136
+    x, dy, w, offsets, off = _problem(cuda_device, sizes, n, k, torch.bfloat16, seed=rows)
+    dw = rb.grouped_gemm_rows_wgrad(dy, x, offsets)
+    rb.last_status()
+    _check_wgrad(dy, x, dw, off)
+
+
+def test_wgrad_long_sums_do_not_drift(cuda_device):
+    """16384 rows of one sign, where truncating additions would lose the most: 16384 / 16
+    of them 2^-24 each on average, 6e-5 of the sum.  With 512 rows to a chunk it is at
+    most 32 truncations of 2^-23 and 32 roundings of 2^-24 of the sum: 6e-6."""
+    import ratchet_b200 as rb
+
+    g = torch.Generator("cuda").manual_seed(1)
+    rows, n, k = 16384, 64, 64
+    x = torch.rand(rows, k, generator=g, device=cuda_device).bfloat16()
+    dy = torch.rand(rows, n, generator=g, device=cuda_device).bfloat16()
+    off = torch.tensor([0, rows], dtype=torch.int32, device=cuda_device)
+    dw = rb.grouped_gemm_rows_wgrad(dy, x, off)
+    rb.last_status()
+    want = dy.double().T @ x.double()
+    assert float(((dw[0].double() - want).abs() / want).max()) <= 32 * 2.0**-23 + 32 * 2.0**-24
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+def test_wgrad_accumulates(cuda_device, dtype):
+    """Two microbatches into one fp32 gradient; an empty group's is left as it is."""
+    import ratchet_b200 as rb
+
+    sizes, n, k = [33, 0, 300, 5], 264, 72
+    x, dy, w, offsets, off = _problem(cuda_device, sizes, n, k, dtype, seed=3)
+    start = torch.randn(4, n, k, device=cuda_device)
+    dw = start.clone()
+    got = rb.grouped_gemm_rows_wgrad(dy, x, offsets, out=dw, accumulate=True)
+    rb.last_status()
+    assert got is dw
+    _check_wgrad(dy, x, dw, off, start)
+    assert torch.equal(dw[1], start[1])
+    # the same call twice from the same start gives the same bits
+    again = start.clone()
+    rb.grouped_gemm_rows_wgrad(dy, x, offsets, out=again, accumulate=True)
+    assert torch.equal(dw, again)
+
+
+def test_infinities_stay_in_their_group(cuda_device):
+    """Infinities and NaN in the rows of one group, in the rows behind the last and in
+    the neighbours of a ragged tile reach no other group's results."""
+    import ratchet_b200 as rb
+
+    sizes, n, k, spare = [37, 21, 50], 128, 192, 20
+    x, dy, w, offsets, off = _problem(cuda_device, sizes, n, k, torch.bfloat16, spare, seed=8)
+    bad = torch.tensor([float("inf"), float("nan"), -float("inf")], device=cuda_device).bfloat16()
+    for t in (x, dy):
+        t[37:58] = bad[torch.arange(t.shape[1], device=cuda_device) % 3]
+        t[108:] = float("nan")
+    y = rb.grouped_gemm_rows(x, w, offsets)
+    dx = rb.grouped_gemm_rows_dgrad(dy, w, offsets)
+    dw = rb.grouped_gemm_rows_wgrad(dy, x, offsets)
+    rb.last_status()
+    for a, b, g in ((0, 37, 0), (58, 108, 2)):
+        assert bool(torch.isfinite(y[a:b]).all()) and bool(torch.isfinite(dx[a:b]).all())
+        D, X, W = dy[a:b].double(), x[a:b].double(), w[g].double()
+        _close(y[a:b], X @ W.T, X.abs() @ W.abs().T, k, ("fwd", g))
+        _close(dx[a:b], D @ W, D.abs() @ W.abs(), n, ("dgrad", g))
+        _close(dw[g], D.T @ X, D.abs().T @ X.abs(), b - a + 1, ("wgrad", g))
+    assert not bool(torch.isfinite(y[37:58]).any()) and not bool(torch.isfinite(dw[1]).any())
