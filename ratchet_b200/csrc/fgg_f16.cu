@@ -346,7 +346,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(C::THREADS, 1)
     if (leader)
       mbar_arrive(schede_bar(slot));
     else
-      mbar_arrive_remote(leader_schede0 + 8u * slot);
+      mbar_arrive_remote_read(leader_schede0 + 8u * slot);
   };
 
   // the register split comes first in each branch: the compiler allots by branch
@@ -598,7 +598,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(C::THREADS, 1)
           if (leader)
             mbar_arrive(acce_bar(b));
           else
-            mbar_arrive_remote(leader_acce0 + 8u * b);
+            mbar_arrive_remote_read(leader_acce0 + 8u * b);
         }
       };
       if constexpr (C::MODE == kWgrad) {
