@@ -117,7 +117,7 @@ struct F16Cfg {
   // readers of a slot: leader producer, MMA warp, epilogue warps; follower
   // producer and epilogue warps
   static constexpr uint32_t SCHED_READERS = 3 + 2 * EPI_WARPS;
-  static constexpr uint32_t NBARS = 2 * STAGES + 4 + 2 * SCHED + 3;
+  static constexpr uint32_t NBARS = 2 * STAGES + 4 + 2 * SCHED + 4;
   // epilogue staging of a warp: 16 tokens x 64 bytes; wgrad 32 rows x 128 bytes
   static constexpr uint32_t EPI_WARP = MODE_ == kWgrad ? 4096 : 1024;
   static constexpr uint32_t EPI_REGION = STAGES * STAGE_BYTES;  // 1024 B aligned
@@ -165,10 +165,12 @@ __device__ __forceinline__ void f16_epilogue_rows(void* out, int ldn, int m0, si
 }
 
 // Wgrad.  The warp's lanes hold gradient rows n0 + lane, `acc` 128 columns from
-// k0 of each.  128 bytes of every row at a time go through 4 KB of shared memory
-// (16-byte units swizzled by the row: no bank conflicts either way), so that eight
-// lanes store one row's 128 contiguous bytes.  With accumulate the same lanes read
-// what is there and add: one addition per element.
+// k0 of each.  128 bytes of every row at a time are turned through 4 KB of shared
+// memory (16-byte units swizzled by the row: no bank conflicts either way), so that
+// eight lanes store one row's 128 contiguous bytes: whole lines reach 7.5 TB/s of
+// L2 writes over all SMs, where a lane storing 32-byte pieces of its own row
+// reaches 4.6.  With p.accumulate the lanes that store read what is there and add:
+// one addition per element.
 template <bool kFp32>
 __device__ __forceinline__ void f16_store_wgrad(const F16Params& p, int g, int n0, int k0,
                                                 const float (&acc)[128], uint8_t* stage) {
@@ -203,19 +205,25 @@ __device__ __forceinline__ void f16_store_wgrad(const F16Params& p, int g, int n
     __syncwarp();
     const bool col_ok = i * cw + unit * (16 / eb) < kcols;
     uint8_t* at = out + i * 128;
-#pragma unroll 2
-    for (int row = r0; row < 32; row += 4, at += 4 * pitch) {
-      if (col_ok && n0 + row < p.m_ext) {
-        uint4 q = *reinterpret_cast<const uint4*>(stage + row * 128 + ((unit ^ (row & 7)) << 4));
-        uint4* const d = reinterpret_cast<uint4*>(at);
+#pragma unroll
+    for (int h0 = 0; h0 < 8; h0 += 4) {  // four rows' loads, then their stores
+      uint4 q[4];
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {
+        const int row = 4 * (h0 + h) + r0;
+        q[h] = *reinterpret_cast<const uint4*>(stage + row * 128 + ((unit ^ (row & 7)) << 4));
+      }
+#pragma unroll
+      for (int h = 0; h < 4; ++h, at += 4 * pitch) {
+        if (!col_ok || n0 + 4 * (h0 + h) + r0 >= p.m_ext) continue;
         if (kFp32 && p.accumulate) {
-          const uint4 old = *d;
-          q.x = __float_as_uint(__uint_as_float(old.x) + __uint_as_float(q.x));
-          q.y = __float_as_uint(__uint_as_float(old.y) + __uint_as_float(q.y));
-          q.z = __float_as_uint(__uint_as_float(old.z) + __uint_as_float(q.z));
-          q.w = __float_as_uint(__uint_as_float(old.w) + __uint_as_float(q.w));
+          const float4 old = *reinterpret_cast<const float4*>(at);
+          q[h].x = __float_as_uint(old.x + __uint_as_float(q[h].x));
+          q[h].y = __float_as_uint(old.y + __uint_as_float(q[h].y));
+          q[h].z = __float_as_uint(old.z + __uint_as_float(q[h].z));
+          q[h].w = __float_as_uint(old.w + __uint_as_float(q[h].w));
         }
-        *d = q;
+        __stcs(reinterpret_cast<uint4*>(at), q[h]);  // written once: first to leave L2
       }
     }
     __syncwarp();
@@ -284,7 +292,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(C::THREADS, 1)
   auto schede_bar = [&](int i) { return bars + 8u * (2 * C::STAGES + 4 + C::SCHED + i); };
   const uint32_t tmem_ready_bar = bars + 8u * (2 * C::STAGES + 4 + 2 * C::SCHED);
   const uint32_t drain_bar = tmem_ready_bar + 8u;
-  const uint32_t taken_bar = tmem_ready_bar + 16u;
+  auto taken_bar = [&](uint32_t n) { return tmem_ready_bar + 16u + 8u * (n & 1u); };
   uint8_t* const misc = gbase + C::BAR_REGION + 8 * C::NBARS;
   volatile F16Slot* const ring = reinterpret_cast<volatile F16Slot*>(misc);
   volatile uint32_t* const tmem_holder =
@@ -322,7 +330,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(C::THREADS, 1)
     }
     mbar_init(tmem_ready_bar, 1);
     mbar_init(drain_bar, 1);
-    mbar_init(taken_bar, 1);
+    mbar_init(taken_bar(0), 1);
+    mbar_init(taken_bar(1), 1);
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -361,8 +370,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(C::THREADS, 1)
         const uint32_t remote_ring0 = mapa_shared(smem_u32(const_cast<F16Slot*>(ring)), peer);
         const uint32_t remote_schedf0 = mapa_shared(schedf_bar(0), peer);
         for (uint32_t n = 0;; ++n) {
-          // at most one tile per pair that it has not started
-          if (n > 0 && !mbar_wait1(taken_bar, (n - 1) & 1u, abort_flag, p.status,
+          // Claim tile n once the producer has taken tile n - 2 (even and odd tiles
+          // on a barrier each): claiming and publishing take about 3 us (an atomic's
+          // way to L2, the peer's ring), longer than a short tile.  A pair then holds
+          // at most two tiles that it has not started.
+          if (n > 1 && !mbar_wait1(taken_bar(n), ((n >> 1) - 1u) & 1u, abort_flag, p.status,
                                    kStatusTimeoutProducer))
             break;
           const int t = atomicAdd(p.status + 1, 1);
@@ -394,6 +406,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(C::THREADS, 1)
       int slot = 0;
       uint32_t sphase = 0;
       uint32_t arms = 0;
+      uint32_t tiles_taken = 0;
       if (lane == 0) {
         if constexpr (C::MODE == kWgrad) {
           prefetch_tensormap(&p.tmap_a);
@@ -414,8 +427,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(C::THREADS, 1)
         const int ct = __shfl_sync(kFullMask, ring[slot].ct, 0);
         if (lane == 0) {
           release_slot(slot);
-          if (leader) mbar_arrive(taken_bar);
+          if (leader) mbar_arrive(taken_bar(tiles_taken));
         }
+        ++tiles_taken;
         if (++slot == C::SCHED) {
           slot = 0;
           sphase ^= 1;
@@ -578,18 +592,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(C::THREADS, 1)
     int slot = 0;
     uint32_t sphase = 0;
     uint32_t lt = 0;
-    while (ok) {
+    // The next tile's slot (g < 0: none).  A tile takes it before it stores, as
+    // the arrival that frees the slot would otherwise wait behind the stores.
+    auto take = [&]() -> F16Slot {
+      F16Slot t;
+      t.g = -1;
       if (!mbar_wait<true>(schedf_bar(slot), sphase, abort_flag, p.status,
                            kStatusTimeoutEpilogue))
-        break;
-      const F16Slot s = f16_read_slot(ring, slot);
+        return t;
+      t = f16_read_slot(ring, slot);
       __syncwarp();
       if (lane == 0) release_slot(slot);
       if (++slot == C::SCHED) {
         slot = 0;
         sphase ^= 1;
       }
-      if (s.g < 0) break;
+      return t;
+    };
+    F16Slot next;
+    next.g = -1;
+    if (ok) next = take();
+    while (ok && next.g >= 0) {
+      const F16Slot s = next;
       const int m0 = s.mt * 256 + int(rank) * 128 + q * 32;
       auto release_acc = [&](uint32_t b) {  // this warp has read accumulator b
         tc_fence_before();
@@ -631,6 +655,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(C::THREADS, 1)
           ++lt;
           ks += C::CHUNK;
         } while (ks < ksteps);
+        next = take();
         if (ok && (s.rows > 0 || !p.accumulate)) {
           if (p.out_fp32)
             f16_store_wgrad<true>(p, s.g, m0, s.ct * 256 + 128 * part, acc, gbase + stage_off);
@@ -642,6 +667,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(C::THREADS, 1)
         if (!mbar_wait(accf_bar(b), (lt >> 1) & 1u, abort_flag, p.status, kStatusTimeoutEpilogue))
           break;
         tc_fence_after();
+        next = take();
         const uint32_t taddr = tmem + (uint32_t(q * 32) << 16) + b * C::BN;
         if (m0 < p.m_ext)
           f16_epilogue_rows(p.out, p.m_ext, m0, size_t(s.row0), s.rows, tile_ncols(s.rows),
