@@ -71,8 +71,9 @@ struct F16Params {
   const uint64_t* tiles;             // forward, dgrad: group << 48 | mt << 32 | first row
   const int32_t* tile_rows;          // forward, dgrad: tokens of each tile
   const int32_t* offsets;
+  const int32_t* order;  // wgrad: groups, the largest first
   void* out;
-  int* status;  // [0] status [1] tile counter [2] finished CTAs [3] tile count
+  int* status;  // [0] status [1] tile counter [3] tile count
   int32_t num_groups;
   int32_t m_ext;   // extent of the M axis (the output's columns; wgrad: its rows n)
   int32_t c_ext;   // wgrad: extent of the N axis (k)
@@ -256,8 +257,9 @@ __device__ __forceinline__ F16Slot f16_make_slot(const F16Params& p, int t, int 
   if (t >= num_tiles) return s;
   if constexpr (MODE == kWgrad) {
     const int per = p.mts * p.cts;
-    s.g = t / per;
-    const int local = t - s.g * per;
+    const int pos = t / per;
+    const int local = t - pos * per;
+    s.g = __ldg(p.order + pos);
     s.mt = local / p.cts;
     s.ct = local - s.mt * p.cts;
     s.row0 = __ldg(p.offsets + s.g);
@@ -700,6 +702,7 @@ struct F16PrepParams {
   int32_t vec_a, vec_b;  // wgrad: vectors per row
   int32_t num_groups, max_rows, mts, tile_cap;
   int32_t wgrad_tiles;  // wgrad: every group's tiles; 0 = forward, dgrad
+  int32_t* order;       // wgrad: groups, the largest first
 };
 
 // Token tiles of a group of m rows: the fewest of at most 256 rows, of equal
@@ -710,15 +713,21 @@ __device__ __forceinline__ int f16_tile_height(int m, int count) {
   return ((m + count - 1) / count + 31) & ~31;
 }
 
-// Every block scans the groups' tile counts (at most 512) in shared memory and
-// writes its share of the tile list, group by group, a weight tile's token
+// Every block ranks the groups by size (at most 512 of them; the largest go first,
+// so that no long tile starts last) and scans their tile counts in shared memory,
+// and writes its share of the tile list, group by group, a weight tile's token
 // tiles next to each other (they share it in L2); or copies its share of the
-// groups' last rows % 16 rows, with zeros up to 16 (wgrad).
+// groups' last rows % 16 rows, with zeros up to 16 (wgrad).  Running the tiles of
+// small groups, bound by their weights' stream, between those of large ones, bound
+// by the tensor pipe, gained 2 % (dgrad, 64 skewed groups) and is left out: under
+// the power cap their costs add up.
 __global__ void __launch_bounds__(256) f16_prepare_kernel(const __grid_constant__ F16PrepParams p) {
   griddep_launch_dependents();
   griddep_wait();
   __shared__ int32_t soff[FGG_MAX_GROUPS + 1];
-  __shared__ int32_t sbegin[FGG_MAX_GROUPS + 1];
+  __shared__ int32_t srows[FGG_MAX_GROUPS];
+  __shared__ int32_t sorder[FGG_MAX_GROUPS];      // groups, the largest first
+  __shared__ int32_t sbegin[FGG_MAX_GROUPS + 1];  // first tile (per M tile) in that order
   __shared__ int32_t swarp[8];
   __shared__ int s_bad;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -726,20 +735,30 @@ __global__ void __launch_bounds__(256) f16_prepare_kernel(const __grid_constant_
   if (threadIdx.x == 0) s_bad = 0;
   for (int i = threadIdx.x; i <= G; i += 256) soff[i] = __ldg(p.offsets + i);
   __syncthreads();
-  // two groups per thread cover FGG_MAX_GROUPS
+  for (int g = threadIdx.x; g < G; g += 256) {
+    const int lo = soff[g], hi = soff[g + 1];
+    const bool bad = lo < 0 || hi < lo || hi > p.max_rows;
+    srows[g] = bad ? 0 : hi - lo;
+    if (bad) s_bad = 1;
+  }
+  __syncthreads();
+  for (int g = threadIdx.x; g < G; g += 256) {
+    const int m = srows[g];
+    int rank = 0;
+    for (int i = 0; i < G; ++i) {
+      const int o = srows[i];
+      rank += o > m || (o == m && i < g) ? 1 : 0;
+    }
+    sorder[rank] = g;
+  }
+  __syncthreads();
+  // two positions per thread cover FGG_MAX_GROUPS
   static_assert(FGG_MAX_GROUPS <= 512, "two groups per thread");
   int cnt[2], run = 0;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const int g = 2 * threadIdx.x + i;
-    cnt[i] = 0;
-    if (g < G) {
-      const int lo = soff[g], hi = soff[g + 1];
-      if (lo < 0 || hi < lo || hi > p.max_rows)
-        s_bad = 1;
-      else
-        cnt[i] = f16_tile_count(hi - lo);
-    }
+    const int r = 2 * threadIdx.x + i;
+    cnt[i] = r < G ? f16_tile_count(srows[sorder[r]]) : 0;
     run += cnt[i];
   }
   int incl = run;
@@ -754,19 +773,23 @@ __global__ void __launch_bounds__(256) f16_prepare_kernel(const __grid_constant_
   for (int w = 0; w < warp; ++w) acc += swarp[w];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const int g = 2 * threadIdx.x + i;
-    if (g <= G) sbegin[g] = acc;
+    const int r = 2 * threadIdx.x + i;
+    if (r <= G) sbegin[r] = acc;
     acc += cnt[i];
   }
   if (threadIdx.x == 255 && G == 512) sbegin[512] = acc;
   __syncthreads();
   int num_tiles = p.wgrad_tiles > 0 ? p.wgrad_tiles : sbegin[G] * p.mts;
   if (s_bad || num_tiles > p.tile_cap) num_tiles = 0;
-  if (blockIdx.x == 0 && threadIdx.x == 0) {
-    p.status[0] = s_bad ? kF16BadOffsets : 0;
-    p.status[1] = 0;
-    p.status[2] = 0;
-    p.status[3] = num_tiles;
+  if (blockIdx.x == 0) {
+    if (threadIdx.x == 0) {
+      p.status[0] = s_bad ? kF16BadOffsets : 0;
+      p.status[1] = 0;
+      p.status[2] = 0;
+      p.status[3] = num_tiles;
+    }
+    if (p.wgrad_tiles > 0)
+      for (int r = threadIdx.x; r < G; r += 256) p.order[r] = sorder[r];
   }
   if (num_tiles == 0) return;
   if (p.wgrad_tiles > 0) {
@@ -799,12 +822,13 @@ __global__ void __launch_bounds__(256) f16_prepare_kernel(const __grid_constant_
       else
         hi = mid;
     }
-    const int m = soff[lo + 1] - soff[lo];
+    const int g = sorder[lo];
+    const int m = srows[g];
     const int count = sbegin[lo + 1] - sbegin[lo];
     const int height = f16_tile_height(m, count);
     const int local = t - sbegin[lo] * p.mts;
     const int mt = local / count, xt = local - mt * count;
-    p.tiles[t] = (uint64_t(lo) << 48) | (uint64_t(mt) << 32) | uint32_t(soff[lo] + xt * height);
+    p.tiles[t] = (uint64_t(g) << 48) | (uint64_t(mt) << 32) | uint32_t(soff[g] + xt * height);
     p.tile_rows[t] = min(height, m - xt * height);
   }
 }
@@ -812,7 +836,7 @@ __global__ void __launch_bounds__(256) f16_prepare_kernel(const __grid_constant_
 // ------------------------------------------------------------------- host
 struct F16Layout {
   int mts = 0, cts = 0, tile_cap = 0;
-  size_t status = 0, tiles = 0, tile_rows = 0, tail_a = 0, tail_b = 0, total = 0;
+  size_t status = 0, order = 0, tiles = 0, tile_rows = 0, tail_a = 0, tail_b = 0, total = 0;
 };
 
 int plan_f16(const FggF16RowsProblem* p, int direction, F16Layout* L) {
@@ -842,6 +866,7 @@ int plan_f16(const FggF16RowsProblem* p, int direction, F16Layout* L) {
   int64_t cap;
   if (direction == kWgrad) {
     cap = int64_t(G) * L->mts * L->cts;
+    L->order = cv.take(size_t(G) * 4, 256);
     L->tail_a = cv.take(size_t(G) * 16 * size_t(p->n) * 2, 256);
     L->tail_b = cv.take(size_t(G) * 16 * size_t(p->k) * 2, 256);
   } else {
@@ -955,6 +980,8 @@ int fgg_f16_grouped_gemm_rows(const FggF16RowsProblem* p, int32_t direction, voi
     if (int rc = encode_2d(&gp.tmap_ta, kMap16, pp.tail_a, N, 16 * G, N * 2, 64, 16)) return rc;
     if (int rc = encode_2d(&gp.tmap_tb, kMap16, pp.tail_b, K, 16 * G, K * 2, 64, 16)) return rc;
     pp.wgrad_tiles = L.tile_cap;
+    pp.order = reinterpret_cast<int32_t*>(ws + L.order);
+    gp.order = pp.order;
     gp.m_ext = p->n;
     gp.c_ext = p->k;
     gp.out_fp32 = p->out_dtype == 0 ? 1 : 0;
