@@ -269,8 +269,9 @@ FGG_API int fgg_mxfp4_dequantize(const void* codes, const void* sf, int64_t coun
 
 /* The contiguous-rows grouped GEMM (fgg_nvfp4_grouped_gemm_rows) on MXFP4
  * operands: the same arguments, statuses and alignment, with a_sf and b_sf of
- * K/32 UE8M0 bytes per row and K a multiple of 128.  Weight packs of the two
- * formats differ; each call refuses the other's (status 0x201). */
+ * K/32 UE8M0 bytes per row, K a multiple of 128, and alpha optional (NULL = 1).
+ * Weight packs of the two formats differ; each call refuses the other's (status
+ * 0x201). */
 typedef FggNvfp4RowsProblem FggMxfp4RowsProblem;
 FGG_API size_t fgg_mxfp4_weight_pack_bytes(int32_t num_groups, int32_t n, int32_t k);
 FGG_API int fgg_mxfp4_pack_weights(const FggNvfp4Weights* w, void* pack, size_t pack_bytes,

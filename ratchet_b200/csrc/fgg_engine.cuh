@@ -112,7 +112,7 @@ struct GemmParams {
   const uint8_t* sfx;         // [XT][KSTEPS][SFX_BYTES]
   const GroupInfo* ginfo;     // NVFP4: [G]
   const uint32_t* tiles;      // [T]
-  const float* alpha;         // NVFP4: [G]; MX: unused (1)
+  const float* alpha;         // NVFP4, MXFP4: [G], null = 1; MX: unused (1)
   const PackHeader* pack;     // NVFP4: weight pack header; MX: null
   __nv_bfloat16* out;
   int* status;  // [0] status, [1] tile counter, [2] finished CTAs
@@ -176,7 +176,7 @@ __device__ __forceinline__ SchedSlot make_slot(const GemmParams& p, uint32_t til
     const GroupInfo gi = p.ginfo[g];
     s.rows = min(BN, gi.m - xti * BN);
     s.row0 = gi.out_row + xti * BN;
-    s.alpha = p.alpha[g];
+    s.alpha = p.alpha != nullptr ? p.alpha[g] : 1.0f;
     s.xtile_index = gi.xtile_begin + xti;
     s.wgroup = gi.wgroup;
   }
@@ -957,7 +957,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
     if (leader)
       mbar_arrive(schede_bar(slot));
     else
-      mbar_arrive_remote(leader_schede0 + 8u * slot);
+      mbar_arrive_remote_read(leader_schede0 + 8u * slot);
   };
 
   if (warp == 3) {
@@ -1286,7 +1286,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
         if (leader)
           mbar_arrive(acce_bar(b));
         else
-          mbar_arrive_remote(leader_acce0 + 8u * b);
+          mbar_arrive_remote_read(leader_acce0 + 8u * b);
       }
       ++lt;
     }

@@ -929,8 +929,8 @@ int rows_impl(const FggNvfp4RowsProblem* p, const void* pack, void* workspace, s
     FGG_CUDA_CHECK(cudaMemsetAsync(ws + L.status, 0, kStatusBytes, s));
     return FGG_OK;
   }
-  if (p->offsets == nullptr || p->a == nullptr || p->a_sf == nullptr || p->alpha == nullptr ||
-      p->out == nullptr)
+  if (p->offsets == nullptr || p->a == nullptr || p->a_sf == nullptr ||
+      (!kMx4 && p->alpha == nullptr) || p->out == nullptr)
     return set_error(FGG_EINVAL, "offsets / a / a_sf / alpha / out is null");
   if (pack == nullptr) return set_error(FGG_EINVAL, "pack is null");
   if (!aligned16(p->a) || !aligned16(p->out) || !aligned16(pack))
