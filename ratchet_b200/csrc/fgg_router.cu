@@ -12,12 +12,14 @@
 // weight 0.  A row that holds a NaN (softmax: or +inf) logit has no scores: its
 // weights are NaN.
 //
-// One warp per token, its logits in registers (lane l holds experts 32 i + l).
-// Keys are compared in 32 bits; two neighbours of the order that lie closer than
-// the keys' error send the token through the same selection on 64-bit keys, so
-// that the order is that of the definition.  The logits are read once; what
-// bounds the kernels is that read for many tokens and one warp's chain of
-// topk reductions for few.
+// L lanes per token (8, 16 or 32 for up to 64, 128 or 1024 experts), each with V
+// consecutive experts in registers, so that a warp works on up to four tokens and
+// loads 16 bytes per lane.  Keys are compared in 32 bits; two neighbours of the
+// order that lie closer than the keys' error send the tokens of the warp through
+// the selection once more with 64-bit keys, computed for the few experts that can
+// still be chosen, so that the order is that of the definition.  The logits are
+// read once; what bounds the kernels is the chain of topk reductions for few
+// tokens and their instructions for many.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -30,7 +32,7 @@ namespace fgg {
 namespace {
 
 constexpr int kRouterMaxExperts = 1024;
-constexpr int kRouterMaxTopk = 32;  // a lane per route
+constexpr int kRouterMaxTopk = 32;
 constexpr int kRouterWarps = 4;
 constexpr float kNegInf = -__builtin_huge_valf();
 
@@ -51,19 +53,17 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { retu
 template <>
 __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
 
-__device__ __forceinline__ float warp_sum(float v) {
+// Reductions over the L lanes of a token.
+template <int L, typename V>
+__device__ __forceinline__ V sub_sum(V v) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kFullMask, v, o);
+  for (int o = L / 2; o > 0; o >>= 1) v += __shfl_xor_sync(kFullMask, v, o);
   return v;
 }
-__device__ __forceinline__ double warp_sum(double v) {
+template <int L>
+__device__ __forceinline__ float sub_max(float v) {  // NaN loses
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kFullMask, v, o);
-  return v;
-}
-__device__ __forceinline__ float warp_max(float v) {  // NaN loses
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(kFullMask, v, o));
+  for (int o = L / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(kFullMask, v, o));
   return v;
 }
 
@@ -81,60 +81,66 @@ __device__ __forceinline__ uint64_t ordered(double f) {
   const uint64_t b = uint64_t(__double_as_longlong(f + 0.0));
   return b >> 63 ? ~b : b | (1ull << 63);
 }
-__device__ __forceinline__ uint32_t warp_max_key(uint32_t k) { return __reduce_max_sync(kFullMask, k); }
-__device__ __forceinline__ uint64_t warp_max_key(uint64_t k) {
-  const uint32_t hi = __reduce_max_sync(kFullMask, uint32_t(k >> 32));
-  const uint32_t lo = __reduce_max_sync(kFullMask, uint32_t(k >> 32) == hi ? uint32_t(k) : 0u);
-  return uint64_t(hi) << 32 | lo;
+template <int L>
+__device__ __forceinline__ uint32_t sub_max_key(uint32_t k) {
+  if constexpr (L == 32) return __reduce_max_sync(kFullMask, k);
+#pragma unroll
+  for (int o = L / 2; o > 0; o >>= 1) k = max(k, __shfl_xor_sync(kFullMask, k, o));
+  return k;
+}
+template <int L>
+__device__ __forceinline__ uint64_t sub_max_key(uint64_t k) {
+#pragma unroll
+  for (int o = L / 2; o > 0; o >>= 1) {
+    const uint64_t other = __shfl_xor_sync(kFullMask, (unsigned long long)k, o);
+    k = other > k ? other : k;
+  }
+  return k;
 }
 
-// The topk largest of the warp's keys in order; lane j returns the j-th's index
-// (-1 when fewer are eligible).  `runs` topk + 1 rounds are made when `gaps` is
-// asked for: true unless two neighbours lie within the keys' error of each other.
-template <int NV, class K>
-__device__ __forceinline__ int select_topk(const K (&key)[NV], int topk, bool* clear) {
-  const int lane = threadIdx.x & 31;
-  uint32_t taken = 0;  // of this lane's keys
-  K best = 0;
-  int best_i = 0;
-  auto rescan = [&]() {
-    best = 0;
-    best_i = 0;
+// The error that the order of two 32-bit keys must exceed to be trusted: scores are
+// good to 1e-6, keys to that and two roundings.
+__device__ __forceinline__ float key_error(float v) { return 4e-6f + 4e-7f * fabsf(v); }
+
+// The topk largest of a token's keys, in order, into ids[0..topk) of the token (-1
+// where fewer are eligible).  With `check`, one round more: false if two neighbours
+// lie within their error, or one is infinite; *last: the topk-th key (or the
+// smallest eligible).  The keys are used up.
+template <int L, int V, bool check, class K>
+__device__ __forceinline__ bool select_topk(K (&key)[V], int topk, int32_t* ids, K* last) {
+  const int lane = threadIdx.x & 31, sub = lane & (L - 1);
+  const unsigned group = L == 32 ? kFullMask : ((1u << L) - 1u) << (lane & ~(L - 1));
+  K prev = 0;
+  bool ok = true;
+  const int rounds = check ? topk + 1 : topk;
+  for (int j = 0; j < rounds; ++j) {
+    K best = 0;
+    int best_i = 0;
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if (!(taken >> i & 1u) && key[i] > best) {
+    for (int i = 0; i < V; ++i)
+      if (key[i] > best) {  // the lowest index among equal ones
         best = key[i];
         best_i = i;
       }
-  };
-  rescan();
-  int mine = -1;
-  K prev = 0;
-  bool ok = true;
-  const int rounds = clear != nullptr ? topk + 1 : topk;
-  for (int j = 0; j < rounds; ++j) {
-    const K top = warp_max_key(best);
-    if (top == 0) break;
-    if constexpr (sizeof(K) == 4) {
-      if (clear != nullptr && j > 0) {
+    const K top = sub_max_key<L>(best);
+    if constexpr (check) {
+      if (j > 0 && top != 0) {
         const float a = unordered(prev), b = unordered(top);
-        // scores are good to 1e-6, keys to that and two roundings; not clear for infinities
-        ok = ok && a - b > 4e-6f + 4e-7f * fabsf(a);
+        ok = ok && a - b > key_error(a);  // false for infinities
       }
+      if (j == topk) break;
+      if (top != 0) *last = top;
+      prev = top;
     }
-    prev = top;
-    if (j == topk) break;
-    // the lowest index among equal keys: lane l's are 32 i + l
-    const uint32_t e = best == top ? uint32_t(32 * best_i + lane) : 0xffffffffu;
-    const uint32_t win = __reduce_min_sync(kFullMask, e);
-    if (lane == j) mine = int(win);
-    if (e == win) {
-      taken |= 1u << best_i;
-      rescan();
-    }
+    const unsigned same = __ballot_sync(kFullMask, best == top) & group;
+    const bool win = top != 0 && lane == __ffs(same) - 1;  // the lowest lane holds the lowest index
+    if (win) ids[j] = sub * V + best_i;
+    if (top == 0 && sub == 0) ids[j] = -1;
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (win && i == best_i) key[i] = 0;
   }
-  if (clear != nullptr) *clear = ok;
-  return mine;
+  return ok;
 }
 
 struct RouterParams {
@@ -146,17 +152,53 @@ struct RouterParams {
   void* dlogits;
   int32_t tokens, experts, topk;
   int32_t renorm;
+  int32_t vec;  // rows of logits (and dlogits) are whole, aligned 16-byte vectors
   float scale;
 };
 
-// This lane's logits (experts 32 i + lane; -inf behind the last).
-template <typename T, int NV>
-__device__ __forceinline__ void load_logits(const T* row, int experts, float (&l)[NV]) {
-  const int lane = threadIdx.x & 31;
+// This lane's V logits (-inf behind the last expert and for `live` false).  Whole
+// 16-byte vectors where `vec` says that rows consist of them.
+template <typename T, int V>
+__device__ __forceinline__ void load_logits(const T* row, int first, int experts, bool live,
+                                            bool vec, float (&l)[V]) {
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int e = 32 * i + lane;
-    l[i] = e < experts ? to_f32<T>(row[e]) : kNegInf;
+  for (int i = 0; i < V; ++i) l[i] = kNegInf;
+  if (!live) return;
+  constexpr int N = 16 / int(sizeof(T));
+  if (vec && V % N == 0) {
+#pragma unroll
+    for (int i = 0; i + N <= V; i += N)
+      if (first + i < experts) {
+        const uint4 q = __ldg(reinterpret_cast<const uint4*>(row + first + i));
+        const T* v = reinterpret_cast<const T*>(&q);
+#pragma unroll
+        for (int j = 0; j < N; ++j) l[i + j] = to_f32<T>(v[j]);
+      }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (first + i < experts) l[i] = to_f32<T>(row[first + i]);
+  }
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_logits(T* row, int first, int experts, bool live, bool vec,
+                                             const float (&d)[V]) {
+  if (!live) return;
+  constexpr int N = 16 / int(sizeof(T));
+  if (vec && V % N == 0) {
+#pragma unroll
+    for (int i = 0; i + N <= V; i += N)
+      if (first + i < experts) {
+        uint4 q;
+        T* v = reinterpret_cast<T*>(&q);
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[j] = from_f32<T>(d[i + j]);
+        *reinterpret_cast<uint4*>(row + first + i) = q;
+      }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (first + i < experts) row[first + i] = from_f32<T>(d[i]);
   }
 }
 
@@ -170,90 +212,136 @@ __device__ __forceinline__ float chosen_score(float l, float m) {
   return expf(l - fminf(m, 0.0f)) / (1.0f + expf(l));
 }
 
-template <typename T, int NV, bool kSoftmax>
+template <typename T, int L, int V, bool kSoftmax>
 __global__ void __launch_bounds__(32 * kRouterWarps)
     router_kernel(const __grid_constant__ RouterParams p) {
-  const int lane = threadIdx.x & 31;
-  const int64_t t = int64_t(blockIdx.x) * kRouterWarps + (threadIdx.x >> 5);
-  if (t >= p.tokens) return;
-  const T* row = static_cast<const T*>(p.logits) + t * p.experts;
-  float l[NV];
-  load_logits<T, NV>(row, p.experts, l);
+  constexpr int kTokens = kRouterWarps * 32 / L;  // of the block
+  constexpr int R = (kRouterMaxTopk + L - 1) / L;  // routes of a lane: j = r L + sub
+  __shared__ int32_t s_ids[kTokens][kRouterMaxTopk];
+  const int lane = threadIdx.x & 31, sub = lane & (L - 1);
+  const int slot = int(threadIdx.x) / L;
+  const int64_t t = int64_t(blockIdx.x) * kTokens + slot;
+  const bool live = t < p.tokens;
+  const T* const row = static_cast<const T*>(p.logits) + (live ? t : 0) * p.experts;
+  int32_t* const ids = s_ids[slot];
+  float l[V];
+  load_logits<T, V>(row, sub * V, p.experts, live, p.vec != 0, l);
   bool nan = false;
   float m = kNegInf;
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
+  for (int i = 0; i < V; ++i) {
     nan = nan || l[i] != l[i];
     m = fmaxf(m, l[i]);
   }
-  nan = __any_sync(kFullMask, nan);
-  m = warp_max(m);
+  nan = sub_max_key<L>(nan ? 1u : 0u) != 0u;
+  m = sub_max<L>(m);
   if (kSoftmax && m == -kNegInf) nan = true;
 
   float total = 1.0f;  // softmax: sum of exp(l - m)
   if (kSoftmax && (p.bias != nullptr || !p.renorm)) {
     float s = 0.0f;
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
+    for (int i = 0; i < V; ++i)
       if (l[i] > kNegInf) s += expf(l[i] - m);
-    total = warp_sum(s);
+    total = sub_sum<L>(s);
   }
 
-  uint32_t key[NV];
-  int id;
   if (p.bias == nullptr) {
+    uint32_t key[V];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) key[i] = ordered(l[i]);
-    id = select_topk<NV, uint32_t>(key, p.topk, nullptr);
+    for (int i = 0; i < V; ++i) key[i] = ordered(l[i]);
+    select_topk<L, V, false>(key, p.topk, ids, static_cast<uint32_t*>(nullptr));
   } else {
-    float b[NV];
+    uint32_t key[V], used[V];
+    float b[V];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int e = 32 * i + lane;
+    for (int i = 0; i < V; ++i) {
+      const int e = sub * V + i;
       b[i] = e < p.experts ? __ldg(p.bias + e) : 0.0f;
       // a masked expert (-inf) stays out whatever its bias
       key[i] = 0u;
       if (l[i] > kNegInf)
         key[i] = ordered((kSoftmax ? expf(l[i] - m) / total : 1.0f / (1.0f + expf(-l[i]))) + b[i]);
+      used[i] = key[i];
     }
-    bool clear;
-    id = select_topk<NV, uint32_t>(key, p.topk, &clear);
-    if (!clear) {
-      uint64_t key64[NV];
-      double s64 = 0.0;
+    uint32_t last = 0;
+    const bool clear = select_topk<L, V, true>(used, p.topk, ids, &last);
+    if (__any_sync(kFullMask, !clear)) {
+      // whoever can still be chosen has a key within both errors of the last one's
+      const float v = unordered(last);
+      const float least = v - 2.0f * key_error(v);
+      uint64_t key64[V];
+      double s64 = 1.0;
       if (kSoftmax) {
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
+        s64 = 0.0;
+#pragma unroll 1
+        for (int i = 0; i < V; ++i)
           if (l[i] > kNegInf) s64 += exp(double(l[i]) - double(m));
-        s64 = warp_sum(s64);
+        s64 = sub_sum<L>(s64);
       }
+      uint32_t todo = 0;
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
+      for (int i = 0; i < V; ++i) {
         key64[i] = 0ull;
-        if (l[i] > kNegInf)
-          key64[i] = ordered((kSoftmax ? exp(double(l[i]) - double(m)) / s64
-                                       : 1.0 / (1.0 + exp(-double(l[i])))) + double(b[i]));
+        // (an infinite last key leaves its equals)
+        if (key[i] != 0u && (key[i] >= last || unordered(key[i]) >= least)) todo |= 1u << i;
       }
-      id = select_topk<NV, uint64_t>(key64, p.topk, nullptr);
+      while (__any_sync(kFullMask, todo != 0u)) {
+        const int at = todo != 0u ? __ffs(todo) - 1 : -1;
+        todo &= todo - 1u;
+        float li = 0.0f, bi = 0.0f;
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          if (i == at) {
+            li = l[i];
+            bi = b[i];
+          }
+        const double s = kSoftmax ? exp(double(li) - double(m)) / s64 : 1.0 / (1.0 + exp(-double(li)));
+        const uint64_t k = ordered(s + double(bi));
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          if (i == at) key64[i] = k;
+      }
+      __syncwarp();
+      select_topk<L, V, false>(key64, p.topk, ids, static_cast<uint64_t*>(nullptr));
     }
   }
+  __syncwarp();
 
-  // lane j: the weight of route j
-  const float lj = id >= 0 ? to_f32<T>(row[id]) : kNegInf;
-  const float mj = warp_max(lj);  // the largest chosen logit
-  float w = 0.0f;
-  if (p.renorm) {
-    const float s = id >= 0 ? chosen_score<kSoftmax>(lj, mj) : 0.0f;
-    const float sum = warp_sum(s);
-    w = id >= 0 ? s / sum : 0.0f;
-  } else if (id >= 0) {
-    w = kSoftmax ? expf(lj - m) / total : chosen_score<false>(lj, 0.0f);
+  // the weights of this lane's routes
+  int id[R];
+  float lr[R], w[R];
+  float mj = kNegInf;  // the largest chosen logit
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int j = r * L + sub;
+    id[r] = j < p.topk ? ids[j] : -1;
+    lr[r] = id[r] >= 0 && live ? to_f32<T>(row[id[r]]) : kNegInf;
+    mj = fmaxf(mj, lr[r]);
   }
-  w *= p.scale;
-  if (nan) w = __int_as_float(0x7fc00000);
-  if (lane < p.topk) {
-    p.ids[t * p.topk + lane] = id;
-    p.weights[t * p.topk + lane] = w;
+  mj = sub_max<L>(mj);
+  float sum = 0.0f;
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    w[r] = 0.0f;
+    if (id[r] >= 0) {
+      if (p.renorm)
+        w[r] = chosen_score<kSoftmax>(lr[r], mj);
+      else
+        w[r] = kSoftmax ? expf(lr[r] - m) / total : chosen_score<false>(lr[r], 0.0f);
+    }
+    sum += w[r];
+  }
+  if (p.renorm) sum = sub_sum<L>(sum);
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int j = r * L + sub;
+    if (!live || j >= p.topk) continue;
+    float v = id[r] >= 0 ? w[r] * p.scale : 0.0f;
+    if (p.renorm && id[r] >= 0) v = w[r] / sum * p.scale;
+    if (nan) v = __int_as_float(0x7fc00000);
+    p.ids[t * p.topk + j] = id[r];
+    p.weights[t * p.topk + j] = v;
   }
 }
 
@@ -264,95 +352,141 @@ __global__ void __launch_bounds__(32 * kRouterWarps)
 //   sigmoid                               c_j = dw_j s_j (1 - s_j)
 // (w normalised, without the scale), dl_e = sum of c_j over the routes to e,
 // minus s_e sum_j c_j for the whole softmax.
-template <typename T, int NV, bool kSoftmax>
+template <typename T, int L, int V, bool kSoftmax>
 __global__ void __launch_bounds__(32 * kRouterWarps)
     router_backward_kernel(const __grid_constant__ RouterParams p) {
-  const int lane = threadIdx.x & 31;
-  const int64_t t = int64_t(blockIdx.x) * kRouterWarps + (threadIdx.x >> 5);
-  if (t >= p.tokens) return;
-  const T* row = static_cast<const T*>(p.logits) + t * p.experts;
-  int id = -1;
-  float dw = 0.0f;
-  if (lane < p.topk) {
-    id = p.ids[t * p.topk + lane];
-    dw = p.dweights[t * p.topk + lane] * p.scale;
-  }
-  if (id < 0 || id >= p.experts) {  // an absent route
-    id = -1;
-    dw = 0.0f;
-  }
-  const float lj = id >= 0 ? to_f32<T>(row[id]) : kNegInf;
-  float l[NV];
-  float m = 0.0f, total = 1.0f, c = 0.0f, whole = 0.0f;
+  constexpr int kTokens = kRouterWarps * 32 / L;
+  constexpr int R = (kRouterMaxTopk + L - 1) / L;
+  __shared__ int2 s_share[kTokens][kRouterMaxTopk];  // (expert, share) of each route
+  const int sub = threadIdx.x & (L - 1);
+  const int slot = int(threadIdx.x) / L;
+  const int64_t t = int64_t(blockIdx.x) * kTokens + slot;
+  const bool live = t < p.tokens;
+  const T* const row = static_cast<const T*>(p.logits) + (live ? t : 0) * p.experts;
   const bool dense = kSoftmax && !p.renorm;  // every expert's logit has a gradient
+  int id[R];
+  float dw[R], lr[R], c[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int j = r * L + sub;
+    id[r] = -1;
+    dw[r] = 0.0f;
+    if (live && j < p.topk) {
+      id[r] = __ldg(p.ids + t * p.topk + j);
+      dw[r] = __ldg(p.dweights + t * p.topk + j) * p.scale;
+    }
+    if (id[r] < 0 || id[r] >= p.experts) {  // an absent route
+      id[r] = -1;
+      dw[r] = 0.0f;
+    }
+  }
+  float d[V];
+  float m = 0.0f, total = 1.0f;
   if (dense) {
-    load_logits<T, NV>(row, p.experts, l);
+    load_logits<T, V>(row, sub * V, p.experts, live, p.vec != 0, d);
     m = kNegInf;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) m = fmaxf(m, l[i]);
-    m = warp_max(m);
+    for (int i = 0; i < V; ++i) m = fmaxf(m, d[i]);
+    m = sub_max<L>(m);
     float s = 0.0f;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      l[i] = l[i] == kNegInf ? 0.0f : expf(l[i] - m);
-      s += l[i];
+    for (int i = 0; i < V; ++i) {
+      d[i] = d[i] == kNegInf ? 0.0f : expf(d[i] - m);
+      s += d[i];
     }
-    total = warp_sum(s);
-#pragma unroll
-    for (int i = 0; i < NV; ++i) l[i] = total > 0.0f ? l[i] / total : l[i] + (total - total);
-    c = id >= 0 && lj != kNegInf ? expf(lj - m) / total * dw : 0.0f;
-    whole = warp_sum(c);
-  } else if (p.renorm) {
-    const float mj = warp_max(lj);
-    const float s = id >= 0 && lj != kNegInf ? chosen_score<kSoftmax>(lj, mj) : 0.0f;
-    const float sum = warp_sum(s);
-    const float w = sum == 0.0f ? 0.0f : s / sum;
-    const float dot = warp_sum(w * dw);
-    c = w * (dw - dot);
-    if (!kSoftmax && id >= 0) c *= lj >= 0.0f ? expf(-lj) / (1.0f + expf(-lj)) : 1.0f / (1.0f + expf(lj));
-  } else if (id >= 0) {
-    const float x = expf(-fabsf(lj));
-    c = dw * (x / ((1.0f + x) * (1.0f + x)));
+    total = sub_sum<L>(s);
   }
-  T* out = static_cast<T*>(p.dlogits) + t * p.experts;
-  float d[NV];
 #pragma unroll
-  for (int i = 0; i < NV; ++i) d[i] = dense ? -l[i] * whole : 0.0f;
+  for (int r = 0; r < R; ++r) lr[r] = id[r] >= 0 ? to_f32<T>(row[id[r]]) : kNegInf;
+  float whole = 0.0f;
+  if (dense) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      c[r] = id[r] >= 0 && lr[r] != kNegInf ? expf(lr[r] - m) / total * dw[r] : 0.0f;
+      whole += c[r];
+    }
+    whole = sub_sum<L>(whole);
+    // scores, all zero for a row that is masked whole (total 0), NaN for a NaN total
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+#pragma unroll
+    for (int i = 0; i < V; ++i) d[i] = -(d[i] * inv) * whole;
+  } else {
+    float mj = kNegInf, sum = 0.0f, dot = 0.0f;
+    if (p.renorm) {
+#pragma unroll
+      for (int r = 0; r < R; ++r) mj = fmaxf(mj, lr[r]);
+      mj = sub_max<L>(mj);
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        c[r] = id[r] >= 0 && lr[r] != kNegInf ? chosen_score<kSoftmax>(lr[r], mj) : 0.0f;
+        sum += c[r];
+      }
+      sum = sub_sum<L>(sum);
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        c[r] = sum == 0.0f ? 0.0f : c[r] / sum;
+        dot += c[r] * dw[r];
+      }
+      dot = sub_sum<L>(dot);
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const float x = expf(-fabsf(lr[r]));
+      if (p.renorm) {
+        c[r] *= dw[r] - dot;
+        // 1 - sigmoid(l)
+        if (!kSoftmax && id[r] >= 0) c[r] *= lr[r] >= 0.0f ? x / (1.0f + x) : 1.0f / (1.0f + x);
+      } else {
+        c[r] = id[r] >= 0 ? dw[r] * (x / ((1.0f + x) * (1.0f + x))) : 0.0f;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) d[i] = 0.0f;
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int j = r * L + sub;
+    if (j < p.topk) s_share[slot][j] = make_int2(id[r], __float_as_int(c[r]));
+  }
+  __syncwarp();
+  // in the routes' order, so that an expert named twice always gets the same sum
   for (int j = 0; j < p.topk; ++j) {
-    const int ij = __shfl_sync(kFullMask, id, j);
-    const float cj = __shfl_sync(kFullMask, c, j);
-    if (ij >= 0 && (ij & 31) == lane) {
+    const int2 q = s_share[slot][j];
+    const int at = q.x - sub * V;
+    if (q.x >= 0 && at >= 0 && at < V) {
 #pragma unroll
-      for (int i = 0; i < NV; ++i)
-        if (i == ij >> 5) d[i] += cj;
+      for (int i = 0; i < V; ++i)
+        if (i == at) d[i] += __int_as_float(q.y);
     }
   }
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int e = 32 * i + lane;
-    if (e < p.experts) out[e] = from_f32<T>(d[i]);
-  }
+  store_logits<T, V>(static_cast<T*>(p.dlogits) + (live ? t : 0) * p.experts, sub * V, p.experts,
+                     live, p.vec != 0, d);
 }
 
-// Registers for 32, 64, 128, 256, 512 or 1024 experts.
+// Lanes per token and experts per lane by the number of experts.
 template <typename T, bool kSoftmax, bool kBackward>
 cudaError_t launch_router(const RouterParams& p, cudaStream_t s) {
-  const int blocks = (p.tokens + kRouterWarps - 1) / kRouterWarps;
-  const int v = (p.experts + 31) / 32;
-  auto go = [&](auto nv) {
-    constexpr int NV = decltype(nv)::value;
+  auto go = [&](auto lanes, auto values) {
+    constexpr int L = decltype(lanes)::value, V = decltype(values)::value;
+    constexpr int kTokens = kRouterWarps * 32 / L;
+    const int blocks = int((int64_t(p.tokens) + kTokens - 1) / kTokens);
     if constexpr (kBackward)
-      router_backward_kernel<T, NV, kSoftmax><<<blocks, 32 * kRouterWarps, 0, s>>>(p);
+      router_backward_kernel<T, L, V, kSoftmax><<<blocks, 32 * kRouterWarps, 0, s>>>(p);
     else
-      router_kernel<T, NV, kSoftmax><<<blocks, 32 * kRouterWarps, 0, s>>>(p);
+      router_kernel<T, L, V, kSoftmax><<<blocks, 32 * kRouterWarps, 0, s>>>(p);
   };
-  if (v <= 1) go(std::integral_constant<int, 1>());
-  else if (v <= 2) go(std::integral_constant<int, 2>());
-  else if (v <= 4) go(std::integral_constant<int, 4>());
-  else if (v <= 8) go(std::integral_constant<int, 8>());
-  else if (v <= 16) go(std::integral_constant<int, 16>());
-  else go(std::integral_constant<int, 32>());
+  using std::integral_constant;
+  if (p.experts <= 64) go(integral_constant<int, 8>(), integral_constant<int, 8>());
+  else if (p.experts <= 128) go(integral_constant<int, 16>(), integral_constant<int, 8>());
+  else if (p.experts <= 256) go(integral_constant<int, 32>(), integral_constant<int, 8>());
+  else if (p.experts <= 512) go(integral_constant<int, 32>(), integral_constant<int, 16>());
+  else go(integral_constant<int, 32>(), integral_constant<int, 32>());
   return cudaGetLastError();
+}
+
+// Rows of whole, aligned 16-byte vectors.
+bool rows_of_vectors(const void* a, const void* b, int experts, int dtype) {
+  return experts % (dtype == 0 ? 4 : 8) == 0 && aligned16(a) && aligned16(b);
 }
 
 template <bool kBackward>
@@ -411,6 +545,7 @@ int fgg_moe_router(const void* logits, int32_t dtype, int32_t tokens, int32_t ex
   p.experts = experts;
   p.topk = topk;
   p.renorm = renormalize != 0;
+  p.vec = rows_of_vectors(logits, nullptr, experts, dtype);
   p.scale = scale;
   FGG_CUDA_CHECK(launch_router<false>(p, dtype, score == 0, reinterpret_cast<cudaStream_t>(stream)));
   return FGG_OK;
@@ -439,6 +574,7 @@ int fgg_moe_router_backward(const float* dweights, const void* logits, int32_t d
   p.experts = experts;
   p.topk = topk;
   p.renorm = renormalize != 0;
+  p.vec = rows_of_vectors(logits, dlogits, experts, dtype);
   p.scale = scale;
   FGG_CUDA_CHECK(launch_router<true>(p, dtype, score == 0, reinterpret_cast<cudaStream_t>(stream)));
   return FGG_OK;

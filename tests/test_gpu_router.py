@@ -72,6 +72,9 @@ def _check(logits, topk, score, bias, renorm, scale, ids, weights):
     (9, 256, 8, torch.float32),
     (5, 500, 32, torch.bfloat16),
     (6, 1024, 16, torch.float32),
+    (21, 60, 32, torch.float32),      # more routes than a token has lanes
+    (4, 128, 17, torch.float16),
+    (3, 512, 9, torch.bfloat16),
 ])
 def test_forward(cuda_device, score, biased, t, e, topk, dtype):
     import ratchet_b200 as rb
@@ -212,6 +215,8 @@ def _grad(l, ids, dw, score, renorm, scale):
     (7, 130, 5, torch.float16),
     (4, 512, 32, torch.bfloat16),
     (3, 1000, 9, torch.float32),
+    (18, 61, 32, torch.bfloat16),     # more routes than a token has lanes, odd rows
+    (5, 128, 17, torch.float16),
 ])
 def test_backward(cuda_device, score, renorm, t, e, topk, dtype):
     import ratchet_b200 as rb
