@@ -9,12 +9,13 @@
 // reads back as NaN.  e comes from the exponent bits of the maximum, and x 2^-e
 // is exact in fp32 but where it vanishes, so every step is exact up to the one
 // rounding to E2M1.  The exact rounding of the value's 4 bits is the hardware's
-// (cvt.rn.satfinite.e2m1x2).
+// (cuda_fp4.h's conversion).
 //
 // Both kernels are HBM-bound copies: one pass, 16-byte loads, four lanes per
 // 32-element block.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+#include <cuda_fp4.h>
 
 #include "fgg_host.cuh"
 #include "fgg_ptx.cuh"
@@ -92,27 +93,19 @@ struct Vec8<__half> {
 
 // E2M1 codes of eight values, the first in the lowest four bits.
 __device__ __forceinline__ uint32_t e2m1x8(const float (&v)[8]) {
-  uint32_t w;
-  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
-      "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\t"
-      "cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
-      "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\t"
-      "cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
-      "mov.b32 %0, {a, b, c, d};\n\t}"
-      : "=r"(w)
-      : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
+  uint32_t w = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    w |= uint32_t(__nv_cvt_float2_to_fp4x2(make_float2(v[2 * i], v[2 * i + 1]), __NV_E2M1,
+                                           cudaRoundNearest))
+         << (8 * i);
   return w;
 }
 
-// Two E2M1 values of a byte.
+// Two E2M1 values of a byte, the low half first.
 __device__ __forceinline__ float2 e2m1x2_values(uint32_t byte) {
-  uint32_t h;
-  asm("{\n\t.reg .b8 a, z;\n\t"
-      "mov.b32 {a, z, z, z}, %1;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %0, a;\n\t}"
-      : "=r"(h)
-      : "r"(byte));
-  return __half22float2(*reinterpret_cast<const __half2*>(&h));
+  const __half2_raw h = __nv_cvt_fp4x2_to_halfraw2(__nv_fp4x2_storage_t(byte), __NV_E2M1);
+  return __half22float2(__half2(h));
 }
 
 // 2^(b - 127) for a scale byte b; NaN for 255.

@@ -50,10 +50,15 @@ def _run(direction: int, a, b, out, offsets, G, n, k, rows, accumulate=False) ->
     nbytes = int(L.fgg_f16_rows_workspace_bytes(prob, direction))
     if nbytes == 0:
         _lib.check(L.fgg_f16_grouped_gemm_rows(prob, direction, None, 0, None), "grouped_gemm_rows")
-    with ops._on(dev):
+    if ops._is_current(dev):
         stream = ops._stream_ptr(dev)
         ws = ops._workspace(dev, stream, nbytes)
         rc = L.fgg_f16_grouped_gemm_rows(prob, direction, ws.data_ptr(), nbytes, stream)
+    else:
+        with torch.cuda.device(dev):
+            stream = ops._stream_ptr(dev)
+            ws = ops._workspace(dev, stream, nbytes)
+            rc = L.fgg_f16_grouped_gemm_rows(prob, direction, ws.data_ptr(), nbytes, stream)
     _lib.check(rc, "grouped_gemm_rows")
     ops._set_last_ws(ws)
 

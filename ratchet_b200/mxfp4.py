@@ -33,16 +33,22 @@ def quantize_mxfp4(x: torch.Tensor):
     with a NaN or an infinity has a NaN scale."""
     if x.dtype not in _DTYPES or not x.is_cuda or not x.is_contiguous() or x.dim() < 1:
         raise ValueError("x must be a contiguous fp32, bf16 or fp16 CUDA tensor")
-    k = int(x.shape[-1])
-    if k % 32 != 0 or k == 0:
-        raise ValueError(f"K={k} must be a positive multiple of 32")
+    if x.shape[-1] % 32 != 0 or x.shape[-1] == 0:
+        raise ValueError(f"K={x.shape[-1]} must be a positive multiple of 32")
     dev = x.device
-    with ops._on(dev):
-        codes = torch.empty((*x.shape[:-1], k // 2), dtype=torch.uint8, device=dev)
-        sf = torch.empty((*x.shape[:-1], k // 32), dtype=torch.float8_e8m0fnu, device=dev)
-        _lib.check(_lib.lib().fgg_mxfp4_quantize(x.data_ptr(), _DTYPES[x.dtype], x.numel(),
-                                                 codes.data_ptr(), sf.data_ptr(),
-                                                 ops._stream_ptr(dev)), "quantize_mxfp4")
+    if ops._is_current(dev):
+        return _quantize_on(x, dev)
+    with torch.cuda.device(dev):
+        return _quantize_on(x, dev)
+
+
+def _quantize_on(x, dev):
+    *lead, k = x.shape
+    codes = torch.empty((*lead, k // 2), dtype=torch.uint8, device=dev)
+    sf = torch.empty((*lead, k // 32), dtype=torch.float8_e8m0fnu, device=dev)
+    _lib.check(_lib.lib().fgg_mxfp4_quantize(x.data_ptr(), _DTYPES[x.dtype], x.numel(),
+                                             codes.data_ptr(), sf.data_ptr(),
+                                             ops._stream_ptr(dev)), "quantize_mxfp4")
     return codes, sf
 
 
@@ -52,19 +58,27 @@ def dequantize_mxfp4(codes: torch.Tensor, sf: torch.Tensor,
     to dtype (bf16 holds each of them exactly down to its subnormals)."""
     if dtype not in _DTYPES:
         raise ValueError(f"dtype {dtype} must be float32, bfloat16 or float16")
-    c, s = ops._as_u8(codes, "codes"), _sf_u8(sf, "sf")
-    if c.dim() < 1 or int(c.shape[-1]) % 16 != 0 or int(c.shape[-1]) == 0:
-        raise ValueError(f"codes {list(c.shape)} must be [..., K/2] with K a multiple of 32")
-    if tuple(s.shape) != (*c.shape[:-1], int(c.shape[-1]) // 16):
-        raise ValueError(f"sf {list(s.shape)} does not match codes {list(c.shape)}")
-    dev = c.device
-    if not (c.is_cuda and s.device == dev and c.is_contiguous() and s.is_contiguous()):
+    if codes.dtype not in ops._U8_DTYPES or sf.dtype not in _SF_DTYPES:
+        raise ValueError(f"codes {codes.dtype} / sf {sf.dtype} must be codes and UE8M0 scales as bytes")
+    if codes.dim() < 1 or codes.shape[-1] % 16 != 0 or codes.shape[-1] == 0:
+        raise ValueError(f"codes {list(codes.shape)} must be [..., K/2] with K a multiple of 32")
+    *lead, kh = codes.shape
+    if list(sf.shape) != [*lead, kh // 16]:
+        raise ValueError(f"sf {list(sf.shape)} does not match codes {list(codes.shape)}")
+    dev = codes.device
+    if not (codes.is_cuda and sf.device == dev and codes.is_contiguous() and sf.is_contiguous()):
         raise ValueError("codes and sf must be contiguous tensors on one CUDA device")
-    with ops._on(dev):
-        x = torch.empty((*c.shape[:-1], int(c.shape[-1]) * 2), dtype=dtype, device=dev)
-        _lib.check(_lib.lib().fgg_mxfp4_dequantize(c.data_ptr(), s.data_ptr(), x.numel(),
-                                                   x.data_ptr(), _DTYPES[dtype],
-                                                   ops._stream_ptr(dev)), "dequantize_mxfp4")
+    if ops._is_current(dev):
+        return _dequantize_on(codes, sf, dtype, (*lead, 2 * kh), dev)
+    with torch.cuda.device(dev):
+        return _dequantize_on(codes, sf, dtype, (*lead, 2 * kh), dev)
+
+
+def _dequantize_on(codes, sf, dtype, shape, dev):
+    x = torch.empty(shape, dtype=dtype, device=dev)
+    _lib.check(_lib.lib().fgg_mxfp4_dequantize(codes.data_ptr(), sf.data_ptr(), x.numel(),
+                                               x.data_ptr(), _DTYPES[dtype],
+                                               ops._stream_ptr(dev)), "dequantize_mxfp4")
     return x
 
 
@@ -128,46 +142,51 @@ def mxfp4_grouped_gemm_rows(a: torch.Tensor, a_sf: torch.Tensor, offsets: torch.
     if not isinstance(pack, Mxfp4WeightPack):
         raise ValueError("pack must come from pack_mxfp4_weights")
     n, k, dev = pack.n, pack.k, pack.device
-    codes, sf = ops._as_u8(a, "a"), _sf_u8(a_sf, "a_sf")
-    if (codes.dim() != 2 or int(codes.shape[1]) != k // 2
-            or tuple(sf.shape) != (int(codes.shape[0]), k // 32)):
-        raise ValueError(f"a {list(codes.shape)} / a_sf {list(sf.shape)} do not match "
+    if a.dtype not in ops._U8_DTYPES or a_sf.dtype not in _SF_DTYPES:
+        raise ValueError(f"a {a.dtype} / a_sf {a_sf.dtype} must be codes and UE8M0 scales as bytes")
+    if (a.dim() != 2 or a.shape[1] != k // 2 or a_sf.dim() != 2 or a_sf.shape[0] != a.shape[0]
+            or a_sf.shape[1] != k // 32):
+        raise ValueError(f"a {list(a.shape)} / a_sf {list(a_sf.shape)} do not match "
                          f"[R, {k // 2}] / [R, {k // 32}] for K={k}")
-    rows = int(codes.shape[0])
-    if offsets.dim() != 1 or offsets.shape[0] < 2:
+    if offsets.dtype is not torch.int32 or offsets.dim() != 1 or offsets.shape[0] < 2:
         raise ValueError("offsets must be int32 [G + 1]")
-    G = int(offsets.shape[0]) - 1
+    rows, G = int(a.shape[0]), int(offsets.shape[0]) - 1
     if b_index is None and G != pack.G:
         raise ValueError(f"{G} groups but {pack.G} packed weight groups (pass b_index to map them)")
     if rows > _I32_MAX or not 0 <= max_group_rows <= _I32_MAX:
         raise ValueError(f"{rows} rows / max_group_rows={max_group_rows} out of range")
+    for name, t, dt, shape in (("alpha", alpha, torch.float32, (G,)),
+                               ("out", out, torch.bfloat16, (rows, n)),
+                               ("row_scale", row_scale, torch.float32, (rows,)),
+                               ("b_index", b_index, torch.int32, (G,))):
+        if t is not None and (t.dtype is not dt or tuple(t.shape) != shape):
+            raise ValueError(f"{name} must be {dt} {list(shape)}, got {t.dtype} {list(t.shape)}")
+    di = dev.index  # on the host: -1
+    for t in (a, a_sf, offsets, alpha, out, row_scale, b_index):
+        if t is not None and (t.get_device() != di or not t.is_contiguous()):
+            raise ValueError(f"every tensor must be contiguous and on {dev}")
+    if ops._is_current(dev):
+        return _product_on(a, a_sf, offsets, pack, alpha, out, row_scale, b_index, max_group_rows)
+    with torch.cuda.device(dev):
+        return _product_on(a, a_sf, offsets, pack, alpha, out, row_scale, b_index, max_group_rows)
+
+
+def _product_on(a, a_sf, offsets, pack, alpha, out, row_scale, b_index, max_group_rows):
+    rows, n, dev = a.shape[0], pack.n, pack.device
     if out is None:
         out = torch.empty((rows, n), dtype=torch.bfloat16, device=dev)
-    with ops._on(dev):
-        if alpha is None:
-            alpha = torch.ones(G, dtype=torch.float32, device=dev)
-        for name, t, dt, shape in (("a", codes, torch.uint8, codes.shape),
-                                   ("a_sf", sf, torch.uint8, sf.shape),
-                                   ("offsets", offsets, torch.int32, (G + 1,)),
-                                   ("alpha", alpha, torch.float32, (G,)),
-                                   ("out", out, torch.bfloat16, (rows, n)),
-                                   ("row_scale", row_scale, torch.float32, (rows,)),
-                                   ("b_index", b_index, torch.int32, (G,))):
-            if t is not None and (t.dtype is not dt or tuple(t.shape) != tuple(shape)
-                                  or t.device != dev or not t.is_contiguous()):
-                raise ValueError(f"{name} must be a contiguous {dt} {list(shape)} tensor on {dev}")
-        L = _lib.lib()
-        prob = _lib.FggNvfp4RowsProblem(
-            G, n, k, rows, offsets.data_ptr(), codes.data_ptr(), sf.data_ptr(), alpha.data_ptr(),
-            out.data_ptr(), None if row_scale is None else row_scale.data_ptr(),
-            None if b_index is None else b_index.data_ptr(), pack.G, int(max_group_rows))
-        nbytes = int(L.fgg_mxfp4_rows_workspace_bytes(prob))
-        if nbytes == 0:
-            _lib.check(L.fgg_mxfp4_grouped_gemm_rows(prob, None, None, 0, None),
-                       "mxfp4_grouped_gemm_rows")
-        stream = ops._stream_ptr(dev)
-        ws = ops._workspace(dev, stream, nbytes)
-        _lib.check(L.fgg_mxfp4_grouped_gemm_rows(prob, pack.buf.data_ptr(), ws.data_ptr(), nbytes,
-                                                 stream), "mxfp4_grouped_gemm_rows")
+    L = _lib.lib()
+    ptr = lambda t: None if t is None else t.data_ptr()
+    prob = _lib.FggNvfp4RowsProblem(
+        offsets.shape[0] - 1, n, pack.k, rows, offsets.data_ptr(), a.data_ptr(), a_sf.data_ptr(),
+        ptr(alpha), out.data_ptr(), ptr(row_scale), ptr(b_index), pack.G, int(max_group_rows))
+    nbytes = int(L.fgg_mxfp4_rows_workspace_bytes(prob))
+    if nbytes == 0:
+        _lib.check(L.fgg_mxfp4_grouped_gemm_rows(prob, None, None, 0, None),
+                   "mxfp4_grouped_gemm_rows")
+    stream = ops._stream_ptr(dev)
+    ws = ops._workspace(dev, stream, nbytes)
+    _lib.check(L.fgg_mxfp4_grouped_gemm_rows(prob, pack.buf.data_ptr(), ws.data_ptr(), nbytes,
+                                             stream), "mxfp4_grouped_gemm_rows")
     ops._set_last_ws(ws)
     return out

@@ -22,6 +22,7 @@ from __future__ import annotations
 
 from collections import OrderedDict
 from contextlib import nullcontext
+from threading import get_ident
 from typing import Sequence
 
 import numpy as np
@@ -69,10 +70,12 @@ def _on(device: torch.device):
     return nullcontext() if _is_current(device) else torch.cuda.device(device)
 
 
-# Workspaces reused per (device, stream): calls on one stream are ordered, so
-# the next call's prepare kernel (which waits for the previous GEMM before it
-# touches memory) may overwrite the previous call's workspace.  Not used while
-# the stream is being captured into a CUDA graph (the graph keeps its own).
+# Workspaces reused per (device, stream, host thread): a thread's calls on one
+# stream are ordered, so the next call's prepare kernel (which waits for the
+# previous GEMM before it touches memory) may overwrite the previous call's
+# workspace; another thread's launches may come between a prepare kernel and its
+# GEMM, so they get their own.  Not used while the stream is being captured into
+# a CUDA graph (the graph keeps its own).
 _WS: OrderedDict = OrderedDict()
 _WS_MAX = 8
 
@@ -80,7 +83,7 @@ _WS_MAX = 8
 def _workspace(device: torch.device, stream: int, nbytes: int) -> torch.Tensor:
     if _capturing is not None and _capturing():
         return torch.empty(nbytes, dtype=torch.uint8, device=device)
-    key = (device.index, stream)
+    key = (device.index, stream, get_ident())
     ws = _WS.get(key)
     if ws is None or ws.numel() < nbytes:
         ws = torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
