@@ -249,6 +249,18 @@ __device__ __forceinline__ F16Slot f16_read_slot(const volatile F16Slot* ring, i
   return s;
 }
 
+// Tile `local` of a group's rows x cols tiles: strips of eight columns, row by row.
+// The 74 pairs then work on about nine rows and eight columns at a time, whose
+// operands they share in L2, whatever the grid's shape.
+constexpr int kStrip = 8;
+__device__ __forceinline__ void f16_place(int local, int rows, int cols, int* row, int* col) {
+  const int strip = local / (kStrip * rows);
+  const int rest = local - strip * kStrip * rows;
+  const int width = min(kStrip, cols - strip * kStrip);
+  *row = rest / width;
+  *col = strip * kStrip + rest - *row * width;
+}
+
 template <int MODE>
 __device__ __forceinline__ F16Slot f16_make_slot(const F16Params& p, int t, int num_tiles) {
   F16Slot s;
@@ -260,8 +272,7 @@ __device__ __forceinline__ F16Slot f16_make_slot(const F16Params& p, int t, int 
     const int pos = t / per;
     const int local = t - pos * per;
     s.g = __ldg(p.order + pos);
-    s.mt = local / p.cts;
-    s.ct = local - s.mt * p.cts;
+    f16_place(local, p.mts, p.cts, &s.mt, &s.ct);
     s.row0 = __ldg(p.offsets + s.g);
     s.rows = __ldg(p.offsets + s.g + 1) - s.row0;
   } else {
@@ -715,9 +726,8 @@ __device__ __forceinline__ int f16_tile_height(int m, int count) {
 
 // Every block ranks the groups by size (at most 512 of them; the largest go first,
 // so that no long tile starts last) and scans their tile counts in shared memory,
-// and writes its share of the tile list, group by group, a weight tile's token
-// tiles next to each other (they share it in L2); or copies its share of the
-// groups' last rows % 16 rows, with zeros up to 16 (wgrad).  Running the tiles of
+// and writes its share of the tile list, group by group; or copies its share of
+// the groups' last rows % 16 rows, with zeros up to 16 (wgrad).  Running the tiles of
 // small groups, bound by their weights' stream, between those of large ones, bound
 // by the tensor pipe, gained 2 % (dgrad, 64 skewed groups) and is left out: under
 // the power cap their costs add up.
@@ -827,7 +837,8 @@ __global__ void __launch_bounds__(256) f16_prepare_kernel(const __grid_constant_
     const int count = sbegin[lo + 1] - sbegin[lo];
     const int height = f16_tile_height(m, count);
     const int local = t - sbegin[lo] * p.mts;
-    const int mt = local / count, xt = local - mt * count;
+    int mt, xt;
+    f16_place(local, p.mts, count, &mt, &xt);
     p.tiles[t] = (uint64_t(g) << 48) | (uint64_t(mt) << 32) | uint32_t(soff[g] + xt * height);
     p.tile_rows[t] = min(height, m - xt * height);
   }
