@@ -267,15 +267,22 @@ FGG_API int fgg_mxfp4_quantize(const void* x, int32_t x_dtype, int64_t count, vo
 FGG_API int fgg_mxfp4_dequantize(const void* codes, const void* sf, int64_t count, void* x,
                                  int32_t x_dtype, void* stream);
 
-/* The contiguous-rows grouped GEMM (fgg_nvfp4_grouped_gemm_rows) on MXFP4
- * operands: the same arguments, statuses and alignment, with a_sf and b_sf of
- * K/32 UE8M0 bytes per row, K a multiple of 128, and alpha optional (NULL = 1).
- * Weight packs of the two formats differ; each call refuses the other's (status
- * 0x201). */
-typedef FggNvfp4RowsProblem FggMxfp4RowsProblem;
+/* Packed MXFP4 weights: the scales of num_groups x [N, K/32] UE8M0 bytes (device,
+ * contiguous, 4-byte aligned) in the MMA's 512-byte atoms.  N and K are multiples
+ * of 128; the codes are read where they lie. */
 FGG_API size_t fgg_mxfp4_weight_pack_bytes(int32_t num_groups, int32_t n, int32_t k);
-FGG_API int fgg_mxfp4_pack_weights(const FggNvfp4Weights* w, void* pack, size_t pack_bytes,
-                                   void* stream);
+FGG_API int fgg_mxfp4_pack_weights(const void* b_sf, int32_t num_groups, int32_t n, int32_t k,
+                                   void* pack, size_t pack_bytes, void* stream);
+
+/* The contiguous-rows grouped GEMM (fgg_nvfp4_grouped_gemm_rows) on MXFP4
+ * operands: the same arguments, statuses and alignment, with K/32 UE8M0 bytes per
+ * row of a_sf, K a multiple of 128, alpha optional (NULL = 1), and the weights'
+ * codes b [num_weight_groups, N, K/2] beside their pack.  A pack of another
+ * problem or of the NVFP4 format is refused by the kernel (status 0x201). */
+typedef struct FggMxfp4RowsProblem {
+  FggNvfp4RowsProblem rows;
+  const void* b;
+} FggMxfp4RowsProblem;
 FGG_API size_t fgg_mxfp4_rows_workspace_bytes(const FggMxfp4RowsProblem* p);
 FGG_API int fgg_mxfp4_grouped_gemm_rows(const FggMxfp4RowsProblem* p, const void* pack,
                                         void* workspace, size_t ws_bytes, void* stream);

@@ -45,6 +45,10 @@ class FggNvfp4RowsProblem(ctypes.Structure):
                 ("num_weight_groups", ctypes.c_int32), ("max_group_rows", ctypes.c_int32)]
 
 
+class FggMxfp4RowsProblem(ctypes.Structure):
+    _fields_ = [("rows", FggNvfp4RowsProblem), ("b", _VOIDP)]
+
+
 class FggMxProblem(ctypes.Structure):
     _fields_ = [("m_total", ctypes.c_int32), ("n", ctypes.c_int32), ("k", ctypes.c_int32),
                 ("num_groups", ctypes.c_int32), ("a", _VOIDP), ("a_sf", _VOIDP), ("b", _VOIDP),
@@ -106,9 +110,9 @@ _SIGS = {
     "fgg_mxfp4_quantize": (ctypes.c_int, [_VOIDP, ctypes.c_int32, ctypes.c_int64, _VOIDP, _VOIDP, _VOIDP]),
     "fgg_mxfp4_dequantize": (ctypes.c_int, [_VOIDP, _VOIDP, ctypes.c_int64, _VOIDP, ctypes.c_int32, _VOIDP]),
     "fgg_mxfp4_weight_pack_bytes": (ctypes.c_size_t, [ctypes.c_int32, ctypes.c_int32, ctypes.c_int32]),
-    "fgg_mxfp4_pack_weights": (ctypes.c_int, [ctypes.POINTER(FggNvfp4Weights), _VOIDP, ctypes.c_size_t, _VOIDP]),
-    "fgg_mxfp4_rows_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(FggNvfp4RowsProblem)]),
-    "fgg_mxfp4_grouped_gemm_rows": (ctypes.c_int, [ctypes.POINTER(FggNvfp4RowsProblem), _VOIDP, _VOIDP, ctypes.c_size_t, _VOIDP]),
+    "fgg_mxfp4_pack_weights": (ctypes.c_int, [_VOIDP, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, _VOIDP, ctypes.c_size_t, _VOIDP]),
+    "fgg_mxfp4_rows_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(FggMxfp4RowsProblem)]),
+    "fgg_mxfp4_grouped_gemm_rows": (ctypes.c_int, [ctypes.POINTER(FggMxfp4RowsProblem), _VOIDP, _VOIDP, ctypes.c_size_t, _VOIDP]),
     "fgg_moe_router": (ctypes.c_int, [_VOIDP, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32,
                                       ctypes.c_int32, _VOIDP, ctypes.c_int32, ctypes.c_float, _VOIDP, _VOIDP,
                                       _VOIDP]),

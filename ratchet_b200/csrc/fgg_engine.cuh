@@ -96,7 +96,7 @@ static_assert(sizeof(SchedSlot) == 32, "slot is 8 words");
 constexpr int kXSmallMaps = 6;
 
 struct GemmParams {
-  CUtensorMap mx_tmap_w;      // MX: 3-D map of the [G, N, K] weight codes
+  CUtensorMap mx_tmap_w;      // MX, MXFP4: 3-D map of the [G, N, K] weight codes
   // One 2-D map over contiguous token rows: MX [M_total, K] fp8 activations;
   // NVFP4 with x_flat set: [max_rows, K/2] codes of every group
   CUtensorMap tmap_x_flat;
@@ -497,7 +497,7 @@ __global__ void __launch_bounds__(256, 1) fgg_gemm_kernel(const __grid_constant_
       uint32_t sphase = 0;
       uint32_t arms = 0;
       if (lane == 0) {
-        if constexpr (C::MX) prefetch_tensormap(&p.mx_tmap_w);
+        if constexpr (C::MX || C::MX4) prefetch_tensormap(&p.mx_tmap_w);
         if (C::MX || p.x_flat) prefetch_tensormap(&p.tmap_x_flat);
       }
       while (true) {
@@ -537,7 +537,7 @@ __global__ void __launch_bounds__(256, 1) fgg_gemm_kernel(const __grid_constant_
         const CUtensorMap* tx;
         // first token row of the tile in the map's coordinates
         const int xrow = (C::MX || p.x_flat) ? row0 : xti * C::BN;
-        if constexpr (C::MX) {
+        if constexpr (C::MX || C::MX4) {
           tw = &p.mx_tmap_w;
           tx = &p.tmap_x_flat;
         } else {
@@ -576,6 +576,8 @@ __global__ void __launch_bounds__(256, 1) fgg_gemm_kernel(const __grid_constant_
               const int q = stage * C::KSUB + sub;
               if constexpr (C::MX)
                 tma_load_3d(sW(q), tw, fb, ks * C::K_STEP, nti * 128, g);
+              else if constexpr (C::MX4)
+                tma_load_3d(sW(q), tw, fb, ks * 128, nti * 128, wgroup);
               else
                 tma_load_2d(sW(q), tw, fb, ks * 128, nti * 128);
               tma_load_2d(sX(q), tx, fb, ks * 128, xrow);
@@ -1002,7 +1004,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
       uint32_t sphase = 0;
       uint32_t arms = 0;
       if (lane == 0) {
-        if constexpr (C::MX) prefetch_tensormap(&p.mx_tmap_w);
+        if constexpr (C::MX || C::MX4) prefetch_tensormap(&p.mx_tmap_w);
         if (C::MX || p.x_flat) prefetch_tensormap(&p.tmap_x_flat);
         prefetch_tensormap(&p.sfw_map);
         prefetch_tensormap(&p.sfx_map);
@@ -1048,8 +1050,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
           tw = &p.mx_tmap_w;
           tx = &p.tmap_x_flat;
         } else {
-          tw = p.tmap_w + wgroup;
-          tensormap_acquire(tw);  // every lane: the issuing one among them
+          if constexpr (C::MX4) {
+            tw = &p.mx_tmap_w;
+          } else {
+            tw = p.tmap_w + wgroup;
+            tensormap_acquire(tw);  // every lane: the issuing one among them
+          }
           if (p.x_flat) {
             tx = &p.tmap_x_flat;
             // a narrow tile (half a multiple of 16 below BNH) loads its rows only
@@ -1095,6 +1101,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
               const int q = stage * C::KSUB + sub;
               if constexpr (C::MX)
                 tma_load_3d_pair(sW(q), tw, fb, ks * C::K_STEP, wrow, g);
+              else if constexpr (C::MX4)
+                tma_load_3d_pair(sW(q), tw, fb, ks * 128, wrow, wgroup);
               else
                 tma_load_2d_pair(sW(q), tw, fb, ks * 128, wrow);
               tma_load_2d_pair(sX(q), tx, fb, ks * 128, xrow);

@@ -384,7 +384,7 @@ struct PackParams {
   const uint8_t* b[FGG_MAX_GROUPS];
   const uint8_t* b_sf[FGG_MAX_GROUPS];
   PackHeader* header;
-  CUtensorMap* tmap_out;
+  CUtensorMap* tmap_out;  // null: MXFP4, whose weights are one tensor with one map
   uint8_t* sfw_out;
   int32_t g, n, k, nk64p, nt;
   int32_t kq;  // scales per row
@@ -406,7 +406,7 @@ __global__ void __launch_bounds__(256) nvfp4_pack_weights_kernel(const __grid_co
       *p.header = h;
     }
     const int g = blk * 8 + warp;
-    if (g < p.g) {
+    if (p.tmap_out != nullptr && g < p.g) {
       reinterpret_cast<uint32_t*>(&smap[warp])[lane] =
           reinterpret_cast<const uint32_t*>(&p.tmpl)[lane];
       __syncwarp();
@@ -462,7 +462,7 @@ static PackLayout pack_layout(int g, int n, int k, bool mx4 = false) {
   Carver cv;
   PackLayout L;
   L.header = cv.take(sizeof(PackHeader), 256);
-  L.tmaps = cv.take(size_t(g) * sizeof(CUtensorMap), 128);
+  L.tmaps = cv.take(mx4 ? 0 : size_t(g) * sizeof(CUtensorMap), 128);
   L.sfw = cv.take(size_t(g) * (n / 128) * nk64p * 512, 256);
   L.total = cv.off;
   return L;
@@ -569,29 +569,15 @@ size_t fgg_nvfp4_weight_pack_bytes(int32_t num_groups, int32_t n, int32_t k) {
   return pack_layout(num_groups, n, k).total;
 }
 
-size_t fgg_mxfp4_weight_pack_bytes(int32_t num_groups, int32_t n, int32_t k) {
-  if (num_groups < 1 || num_groups > FGG_MAX_GROUPS || n <= 0 || n % 128 != 0 || k <= 0 ||
-      k % 128 != 0)
-    return 0;
-  return pack_layout(num_groups, n, k, true).total;
-}
-
-}  // extern "C"
-
-namespace fgg {
-namespace {
-
-int pack_weights_impl(const FggNvfp4Weights* w, void* pack, size_t pack_bytes, void* stream,
-                      bool mx4) {
+int fgg_nvfp4_pack_weights(const FggNvfp4Weights* w, void* pack, size_t pack_bytes, void* stream) {
   if (w == nullptr || pack == nullptr) return set_error(FGG_EINVAL, "weights or pack is null");
   const int G = w->num_groups;
   if (G < 1 || G > FGG_MAX_GROUPS)
     return set_error(FGG_EINVAL, "num_groups=%d outside [1, %d]", G, FGG_MAX_GROUPS);
   if (w->n <= 0 || w->n % 128 != 0)
     return set_error(FGG_EBADSHAPE, "N=%d must be a positive multiple of 128", w->n);
-  const int kmul = mx4 ? 128 : 64;
-  if (w->k < kmul || w->k % kmul != 0)
-    return set_error(FGG_EBADSHAPE, "K=%d must be a positive multiple of %d", w->k, kmul);
+  if (w->k < 64 || w->k % 64 != 0)
+    return set_error(FGG_EBADSHAPE, "K=%d must be a positive multiple of 64", w->k);
   if (w->b == nullptr || w->b_sf == nullptr) return set_error(FGG_EINVAL, "b / b_sf arrays are null");
   for (int g = 0; g < G; ++g) {
     if (w->b[g] == nullptr || w->b_sf[g] == nullptr)
@@ -600,7 +586,7 @@ int pack_weights_impl(const FggNvfp4Weights* w, void* pack, size_t pack_bytes, v
     if (!aligned4(w->b_sf[g])) return set_error(FGG_EALIGN, "b_sf[%d] is not 4-byte aligned", g);
   }
   if (!aligned16(pack)) return set_error(FGG_EALIGN, "pack is not 16-byte aligned");
-  const PackLayout L = pack_layout(G, w->n, w->k, mx4);
+  const PackLayout L = pack_layout(G, w->n, w->k);
   if (pack_bytes < L.total)
     return set_error(FGG_EWORKSPACE, "pack has %zu bytes, needs %zu", pack_bytes, L.total);
   DeviceInfo dev;
@@ -621,9 +607,9 @@ int pack_weights_impl(const FggNvfp4Weights* w, void* pack, size_t pack_bytes, v
   pp.g = G;
   pp.n = w->n;
   pp.k = w->k;
-  pp.nk64p = sf_atoms(w->k, mx4);
-  pp.kq = w->k / (mx4 ? 32 : 16);
-  pp.magic = mx4 ? kPackMagicMx : kPackMagic;
+  pp.nk64p = sf_atoms(w->k, false);
+  pp.kq = w->k / 16;
+  pp.magic = kPackMagic;
   pp.nt = w->n / 128;
   pp.blocks_tmap = (G + 7) / 8;
   const int64_t lines = int64_t(G) * pp.nt * pp.nk64p * 32;
@@ -634,17 +620,48 @@ int pack_weights_impl(const FggNvfp4Weights* w, void* pack, size_t pack_bytes, v
   return FGG_OK;
 }
 
-}  // namespace
-}  // namespace fgg
-
-extern "C" {
-
-int fgg_nvfp4_pack_weights(const FggNvfp4Weights* w, void* pack, size_t pack_bytes, void* stream) {
-  return pack_weights_impl(w, pack, pack_bytes, stream, false);
+size_t fgg_mxfp4_weight_pack_bytes(int32_t num_groups, int32_t n, int32_t k) {
+  if (num_groups < 1 || num_groups > FGG_MAX_GROUPS || n <= 0 || n % 128 != 0 || k <= 0 ||
+      k % 128 != 0)
+    return 0;
+  return pack_layout(num_groups, n, k, true).total;
 }
 
-int fgg_mxfp4_pack_weights(const FggNvfp4Weights* w, void* pack, size_t pack_bytes, void* stream) {
-  return pack_weights_impl(w, pack, pack_bytes, stream, true);
+int fgg_mxfp4_pack_weights(const void* b_sf, int32_t num_groups, int32_t n, int32_t k, void* pack,
+                           size_t pack_bytes, void* stream) {
+  if (b_sf == nullptr || pack == nullptr) return set_error(FGG_EINVAL, "b_sf or pack is null");
+  if (num_groups < 1 || num_groups > FGG_MAX_GROUPS)
+    return set_error(FGG_EINVAL, "num_groups=%d outside [1, %d]", num_groups, FGG_MAX_GROUPS);
+  if (n <= 0 || n % 128 != 0 || k <= 0 || k % 128 != 0)
+    return set_error(FGG_EBADSHAPE, "N=%d and K=%d must be positive multiples of 128", n, k);
+  if (!aligned4(b_sf)) return set_error(FGG_EALIGN, "b_sf is not 4-byte aligned");
+  if (!aligned16(pack)) return set_error(FGG_EALIGN, "pack is not 16-byte aligned");
+  const PackLayout L = pack_layout(num_groups, n, k, true);
+  if (pack_bytes < L.total)
+    return set_error(FGG_EWORKSPACE, "pack has %zu bytes, needs %zu", pack_bytes, L.total);
+  DeviceInfo dev;
+  if (int rc = current_device(&dev)) return rc;
+  PackParams pp;
+  memset(&pp, 0, sizeof(pp));
+  for (int g = 0; g < num_groups; ++g)
+    pp.b_sf[g] = static_cast<const uint8_t*>(b_sf) + size_t(g) * n * (k / 32);
+  uint8_t* base = static_cast<uint8_t*>(pack);
+  pp.header = reinterpret_cast<PackHeader*>(base + L.header);
+  pp.sfw_out = base + L.sfw;
+  pp.g = num_groups;
+  pp.n = n;
+  pp.k = k;
+  pp.nk64p = sf_atoms(k, true);
+  pp.kq = k / 32;
+  pp.magic = kPackMagicMx;
+  pp.nt = n / 128;
+  pp.blocks_tmap = 1;  // the header; no descriptors
+  const int64_t lines = int64_t(num_groups) * pp.nt * pp.nk64p * 32;
+  const int64_t blocks = pp.blocks_tmap + (lines + 255) / 256;
+  if (blocks > INT32_MAX) return set_error(FGG_EBADSHAPE, "weights too large");
+  nvfp4_pack_weights_kernel<<<int(blocks), 256, 0, reinterpret_cast<cudaStream_t>(stream)>>>(pp);
+  FGG_CUDA_CHECK(cudaGetLastError());
+  return FGG_OK;
 }
 
 size_t fgg_nvfp4_workspace_bytes(const FggNvfp4Problem* p) {
@@ -915,8 +932,8 @@ int plan_rows(const FggNvfp4RowsProblem* p, RowsLayout* L, bool mx4) {
 
 // The rows entry of one format, with that format's three kernels.
 template <bool kMx4, class Pair, class Prefill, class Decode>
-int rows_impl(const FggNvfp4RowsProblem* p, const void* pack, void* workspace, size_t ws_bytes,
-              void* stream) {
+int rows_impl(const FggNvfp4RowsProblem* p, const void* b, const void* pack, void* workspace,
+              size_t ws_bytes, void* stream) {
   RowsLayout L;
   if (int rc = plan_rows(p, &L, kMx4)) return rc;
   if (workspace == nullptr) return set_error(FGG_EINVAL, "workspace is null");
@@ -933,8 +950,9 @@ int rows_impl(const FggNvfp4RowsProblem* p, const void* pack, void* workspace, s
       (!kMx4 && p->alpha == nullptr) || p->out == nullptr)
     return set_error(FGG_EINVAL, "offsets / a / a_sf / alpha / out is null");
   if (pack == nullptr) return set_error(FGG_EINVAL, "pack is null");
-  if (!aligned16(p->a) || !aligned16(p->out) || !aligned16(pack))
-    return set_error(FGG_EALIGN, "a, out and pack must be 16-byte aligned");
+  if (kMx4 && b == nullptr) return set_error(FGG_EINVAL, "b is null");
+  if (!aligned16(p->a) || !aligned16(p->out) || !aligned16(pack) || !aligned16(b))
+    return set_error(FGG_EALIGN, "a, out, pack and b must be 16-byte aligned");
   if (!aligned4(p->a_sf) || !aligned4(p->offsets) || !aligned4(p->alpha) ||
       (p->row_scale != nullptr && !aligned4(p->row_scale)) ||
       (p->b_index != nullptr && !aligned4(p->b_index)))
@@ -981,6 +999,11 @@ int rows_impl(const FggNvfp4RowsProblem* p, const void* pack, void* workspace, s
                             uint32_t(L.box_rows)))
     return rc;
   gp.x_flat = 1;
+  if (kMx4)
+    if (int rc = encode_3d(&gp.mx_tmap_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, b, uint64_t(p->k) / 2,
+                           uint64_t(p->n), uint64_t(wg), uint64_t(p->k) / 2,
+                           uint64_t(p->n) * uint64_t(p->k) / 2, 128, 128, 1))
+      return rc;
   gp.tmap_w = reinterpret_cast<const CUtensorMap*>(pk + PL.tmaps);
   gp.sfw = pk + PL.sfw;
   gp.sfx = ws + L.sfx;
@@ -1041,18 +1064,21 @@ size_t fgg_nvfp4_rows_workspace_bytes(const FggNvfp4RowsProblem* p) {
 
 size_t fgg_mxfp4_rows_workspace_bytes(const FggMxfp4RowsProblem* p) {
   RowsLayout L;
-  if (plan_rows(p, &L, true) != FGG_OK) return 0;
+  if (plan_rows(p != nullptr ? &p->rows : nullptr, &L, true) != FGG_OK) return 0;
   return L.total;
 }
 
 int fgg_nvfp4_grouped_gemm_rows(const FggNvfp4RowsProblem* p, const void* pack, void* workspace,
                                 size_t ws_bytes, void* stream) {
-  return rows_impl<false, CfgPair, CfgPrefill, CfgDecode>(p, pack, workspace, ws_bytes, stream);
+  return rows_impl<false, CfgPair, CfgPrefill, CfgDecode>(p, nullptr, pack, workspace, ws_bytes,
+                                                          stream);
 }
 
 int fgg_mxfp4_grouped_gemm_rows(const FggMxfp4RowsProblem* p, const void* pack, void* workspace,
                                 size_t ws_bytes, void* stream) {
-  return rows_impl<true, Mx4Pair, Mx4Prefill, Mx4Decode>(p, pack, workspace, ws_bytes, stream);
+  if (p == nullptr) return set_error(FGG_EINVAL, "problem is null");
+  return rows_impl<true, Mx4Pair, Mx4Prefill, Mx4Decode>(&p->rows, p->b, pack, workspace, ws_bytes,
+                                                         stream);
 }
 
 }  // extern "C"

@@ -83,9 +83,9 @@ def _dequantize_on(codes, sf, dtype, shape, dev):
 
 
 class Mxfp4WeightPack:
-    """Device-side packed MXFP4 weights: per-group TMA descriptors plus the scales
-    in the MMA's 512-byte SF atoms.  The codes are read where they lie (the pack
-    keeps them alive); pack again after changing codes or scales in place."""
+    """Device-side packed MXFP4 weights: the scales in the MMA's 512-byte SF atoms.
+    The codes are read where they lie (the pack keeps them alive); pack again after
+    changing scales in place."""
 
     def __init__(self, w: torch.Tensor, w_sf: torch.Tensor):
         codes, sf = ops._as_u8(w, "w"), _sf_u8(w_sf, "w_sf")
@@ -97,8 +97,9 @@ class Mxfp4WeightPack:
             raise ValueError(f"w_sf {list(sf.shape)} must be [{G}, {n}, K/32] with K={k} a "
                              "multiple of 128")
         if not (codes.is_cuda and sf.device == codes.device and codes.is_contiguous()
-                and sf.is_contiguous()):
-            raise ValueError("w and w_sf must be contiguous tensors on one CUDA device")
+                and sf.is_contiguous() and codes.data_ptr() % 16 == 0):
+            raise ValueError("w (16-byte aligned) and w_sf must be contiguous tensors on one CUDA "
+                             "device")
         if max(G, n, k) > _I32_MAX:
             raise ValueError(f"weights {list(codes.shape)} are too large")
         self.G, self.n, self.k = G, n, k
@@ -111,9 +112,7 @@ class Mxfp4WeightPack:
                              f"{_lib.FGG_MAX_GROUPS} groups, N and K multiples of 128")
         with ops._on(self.device):
             self.buf = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
-            pb, psf = ops._ptr_array(codes.unbind(0)), ops._ptr_array(sf.unbind(0))
-            desc = _lib.FggNvfp4Weights(G, n, k, pb.ctypes.data, psf.ctypes.data)
-            _lib.check(L.fgg_mxfp4_pack_weights(desc, self.buf.data_ptr(), nbytes,
+            _lib.check(L.fgg_mxfp4_pack_weights(sf.data_ptr(), G, n, k, self.buf.data_ptr(), nbytes,
                                                 ops._stream_ptr(self.device)),
                        "pack_mxfp4_weights")
 
@@ -177,9 +176,10 @@ def _product_on(a, a_sf, offsets, pack, alpha, out, row_scale, b_index, max_grou
         out = torch.empty((rows, n), dtype=torch.bfloat16, device=dev)
     L = _lib.lib()
     ptr = lambda t: None if t is None else t.data_ptr()
-    prob = _lib.FggNvfp4RowsProblem(
-        offsets.shape[0] - 1, n, pack.k, rows, offsets.data_ptr(), a.data_ptr(), a_sf.data_ptr(),
-        ptr(alpha), out.data_ptr(), ptr(row_scale), ptr(b_index), pack.G, int(max_group_rows))
+    prob = _lib.FggMxfp4RowsProblem(
+        (offsets.shape[0] - 1, n, pack.k, rows, offsets.data_ptr(), a.data_ptr(), a_sf.data_ptr(),
+         ptr(alpha), out.data_ptr(), ptr(row_scale), ptr(b_index), pack.G, int(max_group_rows)),
+        pack.sources[0].data_ptr())
     nbytes = int(L.fgg_mxfp4_rows_workspace_bytes(prob))
     if nbytes == 0:
         _lib.check(L.fgg_mxfp4_grouped_gemm_rows(prob, None, None, 0, None),

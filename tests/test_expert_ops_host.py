@@ -1,7 +1,5 @@
 """Refusals of the router, the 16-bit grouped products and MXFP4, without a GPU: the
 C entries check their arguments before any device call, the Python ones before that."""
-import ctypes
-
 import pytest
 import torch
 
@@ -147,8 +145,9 @@ def test_mxfp4_quantise_refusals(L):
         assert f(n=(1 << 31) * 8 * 256) == _lib.FGG_EBADSHAPE
 
 
-def _rows(G=2, n=256, k=512, rows=300, wg=2, most=0, off=P, a=P, sf=P, alpha=P, out=P, idx=None):
-    return _lib.FggNvfp4RowsProblem(G, n, k, rows, off, a, sf, alpha, out, None, idx, wg, most)
+def _rows(G=2, n=256, k=512, rows=300, wg=2, most=0, off=P, a=P, sf=P, alpha=P, out=P, idx=None,
+          b=P):
+    return _lib.FggMxfp4RowsProblem((G, n, k, rows, off, a, sf, alpha, out, None, idx, wg, most), b)
 
 
 @pytest.mark.parametrize("change,code", [
@@ -168,7 +167,7 @@ def test_mxfp4_bad_problems(L, change, code):
 def test_mxfp4_bad_buffers(L):
     p = _rows()
     need = L.fgg_mxfp4_rows_workspace_bytes(p)
-    nv = L.fgg_nvfp4_rows_workspace_bytes(p)
+    nv = L.fgg_nvfp4_rows_workspace_bytes(p.rows)
     assert 0 < need < nv                           # half the scale atoms
     call = lambda q, pack=P, ws=P, size=need: L.fgg_mxfp4_grouped_gemm_rows(q, pack, ws, size, None)
     assert call(p, ws=None) == _lib.FGG_EINVAL
@@ -176,21 +175,30 @@ def test_mxfp4_bad_buffers(L):
     assert call(p, pack=None) == _lib.FGG_EINVAL
     assert call(_rows(off=None)) == _lib.FGG_EINVAL
     assert call(_rows(a=P + 8)) == _lib.FGG_EALIGN
+    assert call(_rows(b=None)) == _lib.FGG_EINVAL
+    assert call(_rows(b=P + 4)) == _lib.FGG_EALIGN
     # alpha is optional here, and only here
-    nvfp4 = L.fgg_nvfp4_grouped_gemm_rows(_rows(alpha=None), P, P, nv, None)
+    nvfp4 = L.fgg_nvfp4_grouped_gemm_rows(_rows(alpha=None).rows, P, P, nv, None)
     assert nvfp4 == _lib.FGG_EINVAL and b"alpha" in L.fgg_last_error_detail()
 
 
 def test_mxfp4_weight_pack_bytes(L):
-    """Header, one descriptor per group, two 512-byte scale atoms per 128 rows and 256 K."""
-    up = lambda x, a: (x + a - 1) // a * a
+    """A header and two 512-byte scale atoms per 128 rows and 256 K."""
     for g, n, k in ((1, 128, 128), (3, 256, 640), (8, 4096, 7168)):
-        want = up(128 + g * 128, 256) + g * (n // 128) * ((k + 255) // 256) * 2 * 512
+        want = 256 + g * (n // 128) * ((k + 255) // 256) * 2 * 512
         assert L.fgg_mxfp4_weight_pack_bytes(g, n, k) == want
     for bad in ((0, 128, 128), (1, 100, 128), (1, 128, 64), (_lib.FGG_MAX_GROUPS + 1, 128, 128)):
         assert L.fgg_mxfp4_weight_pack_bytes(*bad) == 0
-    w = _lib.FggNvfp4Weights(1, 128, 64, P, P)
-    assert L.fgg_mxfp4_pack_weights(ctypes.byref(w), P, 1 << 20, None) == _lib.FGG_EBADSHAPE
+    pack = lambda sf=P, g=1, n=128, k=128, to=P, size=1 << 20: L.fgg_mxfp4_pack_weights(
+        sf, g, n, k, to, size, None)
+    assert pack(k=64) == _lib.FGG_EBADSHAPE
+    assert pack(n=64) == _lib.FGG_EBADSHAPE
+    assert pack(g=0) == _lib.FGG_EINVAL
+    assert pack(sf=None) == _lib.FGG_EINVAL
+    assert pack(to=None) == _lib.FGG_EINVAL
+    assert pack(sf=P + 2) == _lib.FGG_EALIGN
+    assert pack(to=P + 8) == _lib.FGG_EALIGN
+    assert pack(size=1279) == _lib.FGG_EWORKSPACE
 
 
 def test_mxfp4_python_refusals():

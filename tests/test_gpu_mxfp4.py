@@ -232,8 +232,10 @@ def test_packs_of_the_other_format_are_refused(cuda_device):
     L = _lib.lib()
     qx, sx = rb.quantize_mxfp4(x)
     alpha = torch.ones(1, device=cuda_device)
-    prob = _lib.FggNvfp4RowsProblem(1, 256, 512, 64, off.data_ptr(), qx.data_ptr(), sx.data_ptr(),
-                                    alpha.data_ptr(), out.data_ptr(), None, None, 1, 0)
+    wc, ws_ = rb.quantize_mxfp4(w)
+    prob = _lib.FggMxfp4RowsProblem((1, 256, 512, 64, off.data_ptr(), qx.data_ptr(), sx.data_ptr(),
+                                     alpha.data_ptr(), out.data_ptr(), None, None, 1, 0),
+                                    wc.data_ptr())
     stream = torch.cuda.current_stream(cuda_device).cuda_stream
     # the larger (NVFP4) pack holds every byte that the MXFP4 call could read
     ws = torch.empty(int(L.fgg_mxfp4_rows_workspace_bytes(prob)), dtype=torch.uint8, device=cuda_device)
