@@ -102,7 +102,7 @@ struct F16Cfg {
   static constexpr uint32_t A_BYTES = 128 * 128;
   static constexpr uint32_t B_BYTES = 128 * 128;  // half of 256 columns
   static constexpr uint32_t STAGE_BYTES = A_BYTES + B_BYTES;
-  static constexpr int STAGES = 6;
+  static constexpr int STAGES = MODE_ == kWgrad ? 7 : 6;  // wgrad stages no results
   static constexpr uint32_t TMEM_COLS = 512;  // two accumulators of 256 columns
   static constexpr int SCHED = 8;
   // Epilogue warps of a CTA: one per TMEM quadrant; wgrad two per quadrant, 128
@@ -119,8 +119,8 @@ struct F16Cfg {
   // producer and epilogue warps
   static constexpr uint32_t SCHED_READERS = 3 + 2 * EPI_WARPS;
   static constexpr uint32_t NBARS = 2 * STAGES + 4 + 2 * SCHED + 4;
-  // epilogue staging of a warp: 16 tokens x 64 bytes; wgrad 32 rows x 128 bytes
-  static constexpr uint32_t EPI_WARP = MODE_ == kWgrad ? 4096 : 1024;
+  // epilogue staging of a warp (forward, dgrad): 16 tokens x 64 bytes
+  static constexpr uint32_t EPI_WARP = MODE_ == kWgrad ? 0 : 1024;
   static constexpr uint32_t EPI_REGION = STAGES * STAGE_BYTES;  // 1024 B aligned
   static constexpr uint32_t BAR_REGION = EPI_REGION + EPI_WARPS * EPI_WARP;
   static constexpr uint32_t SMEM_BYTES = 1024 + BAR_REGION + 8 * NBARS + 32 * SCHED + 16;
@@ -165,69 +165,76 @@ __device__ __forceinline__ void f16_epilogue_rows(void* out, int ldn, int m0, si
   }
 }
 
+// 32 bytes of one lane to a 16-byte aligned address (one store where it is
+// 32-byte aligned), of which the first `bytes` (32 or 16) are the tensor's.
+template <bool kFp32>
+__device__ __forceinline__ void store_sector(uint8_t* at, uint32_t (&v)[8], int bytes,
+                                             bool accumulate) {
+  if (kFp32 && accumulate) {  // whole sectors
+    const float4 lo = *reinterpret_cast<const float4*>(at);
+    const float4 hi = *reinterpret_cast<const float4*>(at + 16);
+    const float old[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = __float_as_uint(old[j] + __uint_as_float(v[j]));
+  }
+  if (bytes == 32 && (reinterpret_cast<uintptr_t>(at) & 31u) == 0) {
+    asm volatile("st.global.cs.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(at), "r"(v[0]),
+                 "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+  } else {
+    __stcs(reinterpret_cast<uint4*>(at), make_uint4(v[0], v[1], v[2], v[3]));
+    if (bytes == 32) __stcs(reinterpret_cast<uint4*>(at) + 1, make_uint4(v[4], v[5], v[6], v[7]));
+  }
+}
+
 // Wgrad.  The warp's lanes hold gradient rows n0 + lane, `acc` 128 columns from
-// k0 of each.  128 bytes of every row at a time are turned through 4 KB of shared
-// memory (16-byte units swizzled by the row: no bank conflicts either way), so that
-// eight lanes store one row's 128 contiguous bytes: whole lines reach 7.5 TB/s of
-// L2 writes over all SMs, where a lane storing 32-byte pieces of its own row
-// reaches 4.6.  With p.accumulate the lanes that store read what is there and add:
-// one addition per element.
+// k0 of each.  Neighbouring lanes swap halves of 64 bytes, so that the two of them
+// store 64 contiguous bytes of one row and then of the other: 6.7 TB/s of L2 writes
+// over all SMs (32-byte pieces of 32 rows: 4.6; whole 128-byte lines: 7.5).  Lines
+// would take a turn through shared memory, whose bandwidth is what short tiles run
+// out of: the operands written by TMA and read by the tensor core are 4096 cycles
+// of it in a tile of 512 rows, the turn 2048 more, the stores themselves 1024.
+// With accumulate the lane that stores reads what is there and adds: one addition
+// per element.
 template <bool kFp32>
 __device__ __forceinline__ void f16_store_wgrad(const F16Params& p, int g, int n0, int k0,
-                                                const float (&acc)[128], uint8_t* stage) {
+                                                const float (&acc)[128]) {
   const int lane = threadIdx.x & 31;
+  const bool odd = lane & 1;
   const int kcols = min(128, p.c_ext - k0);
   if (n0 >= p.m_ext || kcols <= 0) return;
   constexpr int eb = kFp32 ? 4 : 2;
-  constexpr int cw = 128 / eb;  // columns per step
   const size_t pitch = size_t(p.c_ext) * eb;
-  const int unit = lane & 7, r0 = lane >> 3;
+  const int row = n0 + (lane & ~1);
   uint8_t* const out = static_cast<uint8_t*>(p.out) +
-                       (size_t(g) * size_t(p.m_ext) + size_t(n0 + r0)) * pitch + size_t(k0) * eb +
-                       unit * 16;
+                       (size_t(g) * size_t(p.m_ext) + size_t(row)) * pitch + size_t(k0) * eb +
+                       (odd ? 32 : 0);
 #pragma unroll
-  for (int i = 0; i < 128 / cw; ++i) {
-    if (i * cw >= kcols) break;
+  for (int c = 0; c < 2 * eb; ++c) {  // 64 bytes of each row
+    if (c * (64 / eb) >= kcols) break;
+    uint32_t first[8], second[8];  // the even lane's row, the odd lane's
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      uint4 q;
+    for (int j = 0; j < 8; ++j) {
+      uint32_t lo, hi;
       if constexpr (kFp32) {
-        const int c = cw * i + 4 * u;
-        q = make_uint4(__float_as_uint(acc[c]), __float_as_uint(acc[c + 1]),
-                       __float_as_uint(acc[c + 2]), __float_as_uint(acc[c + 3]));
+        lo = __float_as_uint(acc[16 * c + j]);
+        hi = __float_as_uint(acc[16 * c + 8 + j]);
       } else {
-        const int c = cw * i + 8 * u;
         const bool b = p.bf16 != 0;
-        q = make_uint4(pack_16(acc[c], acc[c + 1], b), pack_16(acc[c + 2], acc[c + 3], b),
-                       pack_16(acc[c + 4], acc[c + 5], b), pack_16(acc[c + 6], acc[c + 7], b));
+        lo = pack_16(acc[32 * c + 2 * j], acc[32 * c + 2 * j + 1], b);
+        hi = pack_16(acc[32 * c + 16 + 2 * j], acc[32 * c + 17 + 2 * j], b);
       }
-      *reinterpret_cast<uint4*>(stage + lane * 128 + ((u ^ (lane & 7)) << 4)) = q;
+      const uint32_t got = __shfl_xor_sync(kFullMask, odd ? lo : hi, 1);
+      first[j] = odd ? got : lo;
+      second[j] = odd ? hi : got;
     }
-    __syncwarp();
-    const bool col_ok = i * cw + unit * (16 / eb) < kcols;
-    uint8_t* at = out + i * 128;
-#pragma unroll
-    for (int h0 = 0; h0 < 8; h0 += 4) {  // four rows' loads, then their stores
-      uint4 q[4];
-#pragma unroll
-      for (int h = 0; h < 4; ++h) {
-        const int row = 4 * (h0 + h) + r0;
-        q[h] = *reinterpret_cast<const uint4*>(stage + row * 128 + ((unit ^ (row & 7)) << 4));
-      }
-#pragma unroll
-      for (int h = 0; h < 4; ++h, at += 4 * pitch) {
-        if (!col_ok || n0 + 4 * (h0 + h) + r0 >= p.m_ext) continue;
-        if (kFp32 && p.accumulate) {
-          const float4 old = *reinterpret_cast<const float4*>(at);
-          q[h].x = __float_as_uint(old.x + __uint_as_float(q[h].x));
-          q[h].y = __float_as_uint(old.y + __uint_as_float(q[h].y));
-          q[h].z = __float_as_uint(old.z + __uint_as_float(q[h].z));
-          q[h].w = __float_as_uint(old.w + __uint_as_float(q[h].w));
-        }
-        __stcs(reinterpret_cast<uint4*>(at), q[h]);  // written once: first to leave L2
-      }
+    // columns are a multiple of 8: a 16-bit sector may be half the tensor's
+    const int bytes = min(32, (kcols - c * (64 / eb)) * eb - (odd ? 32 : 0));
+    if (bytes > 0) {
+      if (row < p.m_ext) store_sector<kFp32>(out + c * 64, first, bytes, p.accumulate != 0);
+      if (row + 1 < p.m_ext)
+        store_sector<kFp32>(out + pitch + c * 64, second, bytes, p.accumulate != 0);
     }
-    __syncwarp();
   }
 }
 
@@ -671,9 +678,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(C::THREADS, 1)
         next = take();
         if (ok && (s.rows > 0 || !p.accumulate)) {
           if (p.out_fp32)
-            f16_store_wgrad<true>(p, s.g, m0, s.ct * 256 + 128 * part, acc, gbase + stage_off);
+            f16_store_wgrad<true>(p, s.g, m0, s.ct * 256 + 128 * part, acc);
           else
-            f16_store_wgrad<false>(p, s.g, m0, s.ct * 256 + 128 * part, acc, gbase + stage_off);
+            f16_store_wgrad<false>(p, s.g, m0, s.ct * 256 + 128 * part, acc);
         }
       } else {
         const uint32_t b = lt & 1u;
