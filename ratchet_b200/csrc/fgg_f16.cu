@@ -102,12 +102,12 @@ struct F16Cfg {
   static constexpr uint32_t A_BYTES = 128 * 128;
   static constexpr uint32_t B_BYTES = 128 * 128;  // half of 256 columns
   static constexpr uint32_t STAGE_BYTES = A_BYTES + B_BYTES;
-  static constexpr int STAGES = MODE_ == kWgrad ? 7 : 6;  // wgrad stages no results
+  static constexpr int STAGES = 7;
   static constexpr uint32_t TMEM_COLS = 512;  // two accumulators of 256 columns
   static constexpr int SCHED = 8;
-  // Epilogue warps of a CTA: one per TMEM quadrant; wgrad two per quadrant, 128
-  // columns each, which it holds in registers over the chunks of a long group.
-  static constexpr int EPI_WARPS = MODE_ == kWgrad ? 8 : 4;
+  // Epilogue warps of a CTA: two per TMEM quadrant.  In wgrad each holds 128
+  // columns in registers over the chunks of a long group.
+  static constexpr int EPI_WARPS = 8;
   static constexpr int THREADS = 128 + 32 * EPI_WARPS;
   // wgrad's registers: launched with 168 per thread (384 threads), of which the
   // four other warps give most to the epilogue's 128 sums
@@ -119,49 +119,56 @@ struct F16Cfg {
   // producer and epilogue warps
   static constexpr uint32_t SCHED_READERS = 3 + 2 * EPI_WARPS;
   static constexpr uint32_t NBARS = 2 * STAGES + 4 + 2 * SCHED + 4;
-  // epilogue staging of a warp (forward, dgrad): 16 tokens x 64 bytes
-  static constexpr uint32_t EPI_WARP = MODE_ == kWgrad ? 0 : 1024;
-  static constexpr uint32_t EPI_REGION = STAGES * STAGE_BYTES;  // 1024 B aligned
-  static constexpr uint32_t BAR_REGION = EPI_REGION + EPI_WARPS * EPI_WARP;
+  static constexpr uint32_t BAR_REGION = STAGES * STAGE_BYTES;
   static constexpr uint32_t SMEM_BYTES = 1024 + BAR_REGION + 8 * NBARS + 32 * SCHED + 16;
   static_assert(SMEM_BYTES <= 232448, "shared memory budget exceeded");
 };
 
 // ------------------------------------------------------------- epilogues
-// Forward, dgrad.  The warp's 32 TMEM lanes are the output columns m0 + lane,
-// its TMEM columns the tile's tokens.  Sixteen tokens at a time are transposed
-// through 1 KB of the warp's shared memory so that every lane stores 16
-// contiguous bytes (see epilogue_tile of the block-scaled kernels, whose
-// layout this shares); columns past the output's edge are not stored.
+// Forward, dgrad.  The warp's 32 TMEM lanes are the output columns m0 + lane, its
+// TMEM columns the tile's tokens.  They are turned by three rounds of swaps between
+// lanes 1, 2 and 4 apart, after which lane l holds columns (l & ~7) .. + 7 of every
+// eighth token from l & 7 on: 16 contiguous bytes to store, 64 of each token per
+// instruction.  Columns past the output's edge are not stored.
 __device__ __forceinline__ void f16_epilogue_rows(void* out, int ldn, int m0, size_t row0, int rows,
-                                                  int ncols, bool bf16, uint32_t taddr,
-                                                  uint32_t* stage) {
+                                                  int ncols, int part, bool bf16,
+                                                  uint32_t taddr) {
   const int lane = threadIdx.x & 31;
-  const bool odd = lane & 1;
-  const int seg = lane & 3;
-  const bool col_ok = m0 + 8 * seg < ldn;
-  uint16_t* const o = static_cast<uint16_t*>(out);
-  for (int c0 = 0; c0 < ncols; c0 += 16) {
-    uint32_t r[16];
-    tmem_ld16(taddr + c0, r);
+  const bool b0 = lane & 1, b1 = lane & 2, b2 = lane & 4;
+  const int col = m0 + (lane & ~7);
+  const bool col_ok = col < ldn;
+  uint16_t* const o = static_cast<uint16_t*>(out) + size_t(col);
+  // the quadrant's two warps by turns, 32 tokens each; the next ones are read while
+  // these are turned and stored
+  uint32_t r[32];
+  int c0 = 32 * part;
+  if (c0 < ncols) tmem_ld32(taddr + c0, r);
+  for (; c0 < ncols; c0 += 64) {
     tmem_wait_ld();
+    uint32_t w[16];  // columns (l & ~1, + 1) of token 2 i + b0
 #pragma unroll
-    for (int j = 0; j < 16; j += 2) {
-      const float v0 = __uint_as_float(r[j]), v1 = __uint_as_float(r[j + 1]);
-      const float got = __shfl_xor_sync(kFullMask, odd ? v0 : v1, 1);
-      stage[(j + (odd ? 1 : 0)) * 16 + (lane >> 1)] =
-          odd ? pack_16(got, v1, bf16) : pack_16(v0, got, bf16);
+    for (int i = 0; i < 16; ++i) {
+      const float v0 = __uint_as_float(r[2 * i]), v1 = __uint_as_float(r[2 * i + 1]);
+      const float got = __shfl_xor_sync(kFullMask, b0 ? v0 : v1, 1);
+      w[i] = b0 ? pack_16(got, v1, bf16) : pack_16(v0, got, bf16);
     }
-    __syncwarp();
+    if (c0 + 64 < ncols) tmem_ld32(taddr + c0 + 64, r);
+    uint32_t x[8][2];  // columns (l & ~3) .. + 3 of token 4 i + 2 b1 + b0
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int t = (lane >> 2) + 8 * h;
-      const uint4 q = *reinterpret_cast<const uint4*>(stage + t * 16 + 4 * seg);
-      if (c0 + t < rows && col_ok)
-        *reinterpret_cast<uint4*>(o + (row0 + size_t(c0 + t)) * size_t(ldn) + size_t(m0 + 8 * seg)) =
-            q;
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t got = __shfl_xor_sync(kFullMask, b1 ? w[2 * i] : w[2 * i + 1], 2);
+      x[i][0] = b1 ? got : w[2 * i];
+      x[i][1] = b1 ? w[2 * i + 1] : got;
     }
-    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t g0 = __shfl_xor_sync(kFullMask, b2 ? x[2 * i][0] : x[2 * i + 1][0], 4);
+      const uint32_t g1 = __shfl_xor_sync(kFullMask, b2 ? x[2 * i][1] : x[2 * i + 1][1], 4);
+      const uint4 q = b2 ? make_uint4(g0, g1, x[2 * i + 1][0], x[2 * i + 1][1])
+                         : make_uint4(x[2 * i][0], x[2 * i][1], g0, g1);
+      const int t = c0 + 8 * i + (lane & 7);
+      if (t < rows && col_ok) *reinterpret_cast<uint4*>(o + (row0 + size_t(t)) * size_t(ldn)) = q;
+    }
   }
 }
 
@@ -604,11 +611,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(C::THREADS, 1)
   } else {
     // --------------------------------------------------------- epilogue
     if constexpr (C::MODE == kWgrad) regs_inc<C::REGS_EPI>();
-    const int q = warp & 3;
+    const int q = warp & 3, part = (warp - 4) >> 2;
     bool ok = mbar_wait(tmem_ready_bar, 0, abort_flag, p.status, kStatusTimeoutEpilogue);
     tc_fence_after();
     const uint32_t tmem = *tmem_holder;
-    const uint32_t stage_off = C::EPI_REGION + uint32_t(warp - 4) * C::EPI_WARP;
     int slot = 0;
     uint32_t sphase = 0;
     uint32_t lt = 0;
@@ -646,7 +652,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(C::THREADS, 1)
         }
       };
       if constexpr (C::MODE == kWgrad) {
-        const int part = (warp - 4) >> 2;  // its 128 columns of 256
         const int ksteps = tile_ksteps(s.rows);
         float acc[128];
 #pragma unroll
@@ -691,7 +696,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(C::THREADS, 1)
         const uint32_t taddr = tmem + (uint32_t(q * 32) << 16) + b * C::BN;
         if (m0 < p.m_ext)
           f16_epilogue_rows(p.out, p.m_ext, m0, size_t(s.row0), s.rows, tile_ncols(s.rows),
-                            p.bf16 != 0, taddr, reinterpret_cast<uint32_t*>(gbase + stage_off));
+                            part, p.bf16 != 0, taddr);
         release_acc(b);
         ++lt;
       }
