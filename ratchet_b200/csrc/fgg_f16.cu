@@ -32,13 +32,24 @@
 // at a time in TMEM and the epilogue adds those sums in registers, rounding to
 // nearest; a 16-bit result hides it (forward, dgrad).
 //
-// What bounds it: the tensor pipe for groups of about 200 tokens and more, the
-// weights' HBM stream below that, the gradient's write for wgrad with short
-// groups.
+// What bounds it: the tensor pipe for groups of about 250 tokens and more, the
+// weights' HBM stream below that, shared-memory bandwidth and the gradient's write
+// for wgrad with short groups; and in seconds-long runs of any of them but the
+// decode shapes the 1000 W cap (clocks of 1.0 to 1.5 GHz), under which what counts
+// is energy: the bytes moved as much as the products.  Measured, bf16, K 2048 to
+// 8192, short bursts / under the cap:
+//   forward 8192^3                             1.37 / 1.35 PFLOP/s (the library's
+//                                              product 1.63 / 1.35)
+//   forward 8 groups, 4352 rows, 4096 x 7168   204 / 238 us, tensor pipe 88 % active,
+//                                              582 MB of DRAM reads (541 MB needed)
+//   forward 64 groups, 544 rows, 7168 x 2048   283 us, 6.7 TB/s
+//   dgrad 64 skewed groups, 16384 rows         0.90 / 1.08 ms
+//   wgrad 64 skewed groups, 32768 rows, fp32   1.09 / 1.32 ms
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cstring>
 
 #include "fgg_engine.cuh"
@@ -401,9 +412,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(C::THREADS, 1)
           // on a barrier each): claiming and publishing take about 3 us (an atomic's
           // way to L2, the peer's ring), longer than a short tile.  A pair then holds
           // at most two tiles that it has not started.
-          if (n > 1 && !mbar_wait1(taken_bar(n), ((n >> 1) - 1u) & 1u, abort_flag, p.status,
-                                   kStatusTimeoutProducer))
+          // A tile of wgrad is as long as its group: this wait alone may take a minute.
+          bool taken = n < 2;
+          for (int tries = 0; !taken && tries < 60 && *abort_flag == 0; ++tries)
+            taken = mbar_wait_one(taken_bar(n), ((n >> 1) - 1u) & 1u, kWaitLimitNs);
+          if (!taken) {
+            atomicCAS(p.status, 0, kStatusTimeoutProducer);
+            *abort_flag = 1;
             break;
+          }
           const int t = atomicAdd(p.status + 1, 1);
           const F16Slot s = f16_make_slot<C::MODE>(p, t, num_tiles);
           if (!mbar_wait1<true>(schede_bar(slot), sphase ^ 1, abort_flag, p.status,
@@ -411,7 +428,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(C::THREADS, 1)
             break;
           const uint32_t words[5] = {uint32_t(s.g), uint32_t(s.mt), uint32_t(s.row0),
                                      uint32_t(s.rows), uint32_t(s.ct)};
-  #pragma unroll
+#pragma unroll
           for (int i = 0; i < 5; ++i) {
             reinterpret_cast<volatile uint32_t*>(ring + slot)[i] = words[i];
             st_shared_remote_u32(remote_ring0 + 32u * slot + 4u * i, words[i]);
@@ -579,7 +596,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(C::THREADS, 1)
                                ? (ks < wgrad_flat_steps(rows) ? min(4, rows / 16 - 4 * ks) : 1)
                                : 4;
             if (elect_one()) {
-  #pragma unroll
+#pragma unroll
               for (int j = 0; j < 4; ++j)
                 if (j < nj)
                   tc_mma_f16_pair(d_tmem, adesc + kStepA * j, bdesc + kStepB * j, idesc,
@@ -587,6 +604,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(C::THREADS, 1)
               tc_commit_pair(empty_bar(stage), 0x3);
             }
             __syncwarp();
+            issued_any = true;
             if (++stage == C::STAGES) {
               stage = 0;
               phase ^= 1;
@@ -915,10 +933,14 @@ int launch_f16(const F16Params& gp, const DeviceInfo& dev, cudaStream_t s) {
     return rc;
   if constexpr (MODE == kWgrad) {
     // a split of more registers than the block starts with would never be granted
-    static const int regs = [] {
+    static std::atomic<int> known{0};
+    int regs = known.load(std::memory_order_relaxed);
+    if (regs == 0) {
       cudaFuncAttributes a = {};
-      return cudaFuncGetAttributes(&a, f16_pair_kernel<C>) == cudaSuccess ? a.numRegs : 0;
-    }();
+      FGG_CUDA_CHECK(cudaFuncGetAttributes(&a, f16_pair_kernel<C>));
+      regs = a.numRegs;
+      known.store(regs, std::memory_order_relaxed);
+    }
     if (regs * C::THREADS < C::REGS_TOTAL)
       return set_error(FGG_ECUDA, "the kernel was built with %d registers per thread, needs %d",
                        regs, (C::REGS_TOTAL + C::THREADS - 1) / C::THREADS);

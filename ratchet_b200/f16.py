@@ -92,6 +92,7 @@ def grouped_gemm_rows(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, *
         out = torch.empty((rows, n), dtype=x.dtype, device=x.device)
     else:
         _check("out", out, (rows, n), x.dtype, x.device)
+        ops._disjoint(out, x, w)
     _run(0, x, w, out, offsets, G, n, k, rows)
     return out
 
@@ -111,6 +112,7 @@ def grouped_gemm_rows_dgrad(dy: torch.Tensor, w: torch.Tensor, offsets: torch.Te
         out = torch.empty((rows, k), dtype=dy.dtype, device=dy.device)
     else:
         _check("out", out, (rows, k), dy.dtype, dy.device)
+        ops._disjoint(out, dy, w)
     _run(1, dy, w, out, offsets, G, n, k, rows)
     return out
 
@@ -140,6 +142,7 @@ def grouped_gemm_rows_wgrad(dy: torch.Tensor, x: torch.Tensor, offsets: torch.Te
         if out.dtype not in (torch.float32, dy.dtype):
             raise ValueError(f"out dtype {out.dtype} must be float32 or {dy.dtype}")
         _check("out", out, (G, n, k), out.dtype, dy.device)
+        ops._disjoint(out, dy, x)
         if accumulate and out.dtype is not torch.float32:
             raise ValueError("accumulate=True needs a float32 out")
     _run(2, dy, x, out, offsets, G, n, k, rows, accumulate)

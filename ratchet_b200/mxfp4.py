@@ -164,6 +164,8 @@ def mxfp4_grouped_gemm_rows(a: torch.Tensor, a_sf: torch.Tensor, offsets: torch.
     for t in (a, a_sf, offsets, alpha, out, row_scale, b_index):
         if t is not None and (t.get_device() != di or not t.is_contiguous()):
             raise ValueError(f"every tensor must be contiguous and on {dev}")
+    if out is not None:
+        ops._disjoint(out, a, a_sf, pack.sources[0])
     if ops._is_current(dev):
         return _product_on(a, a_sf, offsets, pack, alpha, out, row_scale, b_index, max_group_rows)
     with torch.cuda.device(dev):

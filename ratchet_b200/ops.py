@@ -22,7 +22,7 @@ from __future__ import annotations
 
 from collections import OrderedDict
 from contextlib import nullcontext
-from threading import get_ident
+from threading import Lock, get_ident
 from typing import Sequence
 
 import numpy as np
@@ -70,6 +70,16 @@ def _on(device: torch.device):
     return nullcontext() if _is_current(device) else torch.cuda.device(device)
 
 
+def _disjoint(out: torch.Tensor, *others) -> None:
+    """Refuse an output that shares memory with an operand (both contiguous)."""
+    lo = out.data_ptr()
+    hi = lo + out.numel() * out.element_size()
+    for t in others:
+        p = t.data_ptr()
+        if p < hi and lo < p + t.numel() * t.element_size():
+            raise ValueError("out shares memory with an operand")
+
+
 # Workspaces reused per (device, stream, host thread): a thread's calls on one
 # stream are ordered, so the next call's prepare kernel (which waits for the
 # previous GEMM before it touches memory) may overwrite the previous call's
@@ -78,20 +88,22 @@ def _on(device: torch.device):
 # a CUDA graph (the graph keeps its own).
 _WS: OrderedDict = OrderedDict()
 _WS_MAX = 8
+_WS_LOCK = Lock()
 
 
 def _workspace(device: torch.device, stream: int, nbytes: int) -> torch.Tensor:
     if _capturing is not None and _capturing():
         return torch.empty(nbytes, dtype=torch.uint8, device=device)
     key = (device.index, stream, get_ident())
-    ws = _WS.get(key)
-    if ws is None or ws.numel() < nbytes:
-        ws = torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
-        _WS[key] = ws
-        while len(_WS) > _WS_MAX:  # the oldest stream's buffer returns to torch's allocator
-            _WS.popitem(last=False)
-    else:
-        _WS.move_to_end(key)
+    with _WS_LOCK:
+        ws = _WS.get(key)
+        if ws is None or ws.numel() < nbytes:
+            ws = torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
+            _WS[key] = ws
+            while len(_WS) > _WS_MAX:  # the oldest stream's buffer returns to torch's allocator
+                _WS.popitem(last=False)
+        else:
+            _WS.move_to_end(key)
     return ws
 
 

@@ -367,6 +367,173 @@ def test_long_buffers(cuda_device):
     assert torch.equal(v[-4096:], rb.dequantize_mxfp4(c2, s2))
 
 
+def test_rows_before_the_first_group(cuda_device):
+    """offsets[0] need not be 0: the rows before it are left as they are."""
+    import ratchet_b200 as rb
+
+    dev = cuda_device
+    x, dy, w = _rand(dev, 90, 64, seed=1), _rand(dev, 90, 40, seed=2), _rand(dev, 2, 40, 64, seed=3)
+    off = torch.tensor([13, 50, 83], dtype=torch.int32, device=dev)
+    y = torch.full((90, 40), 7.0, dtype=torch.bfloat16, device=dev)
+    rb.grouped_gemm_rows(x, w, off, out=y)
+    dw = rb.grouped_gemm_rows_wgrad(dy, x, off)
+    rb.last_status()
+    assert bool((y[:13] == 7.0).all()) and bool((y[83:] == 7.0).all())
+    for g, (lo, hi) in enumerate(((13, 50), (50, 83))):
+        X, D, W = x[lo:hi].double(), dy[lo:hi].double(), w[g].double()
+        assert _bound(y[lo:hi], X @ W.T, X.abs() @ W.abs().T, 64)
+        assert _bound(dw[g], D.T @ X, D.abs().T @ X.abs(), hi - lo + 1)
+
+
+def test_waits_that_run_out(cuda_device):
+    """With the test hook that arms no load, every wait of the 16-bit kernels runs out
+    after about a second: a status, nothing written, and a clean call after it."""
+    import ratchet_b200 as rb
+    from ratchet_b200 import _lib
+
+    dev = cuda_device
+    x, dy, w = _rand(dev, 700, 1024), _rand(dev, 700, 520), _rand(dev, 2, 520, 1024)
+    off = torch.tensor([0, 300, 700], dtype=torch.int32, device=dev)
+    y = torch.full((700, 520), 7.0, dtype=torch.bfloat16, device=dev)
+    dw = torch.full((2, 520, 1024), 7.0, device=dev)
+    L = _lib.lib()
+    for call, out in ((lambda: rb.grouped_gemm_rows(x, w, off, out=y), y),
+                      (lambda: rb.grouped_gemm_rows_wgrad(dy, x, off, out=dw), dw)):
+        L.fgg_debug_set_flags(_lib.FGG_DEBUG_NO_LOADS)
+        try:
+            call()
+            torch.cuda.synchronize()
+        finally:
+            L.fgg_debug_set_flags(0)
+        with pytest.raises(rb.FggError, match="0x10"):
+            rb.last_status()
+        assert bool((out == 7.0).all())
+        call()
+        rb.last_status()
+        assert not bool((out == 7.0).all())
+
+
+def test_first_calls_inside_a_capture(cuda_device):
+    """A process whose very first calls are captured: no warm-up is needed."""
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    code = """
+import torch, ratchet_b200 as rb
+d = "cuda"
+x = torch.randn(50, 64, device=d).bfloat16(); dy = torch.randn(50, 40, device=d).bfloat16()
+w = torch.randn(2, 40, 64, device=d).bfloat16()
+off = torch.tensor([0, 20, 50], dtype=torch.int32, device=d)
+l = torch.randn(50, 9, device=d); q = torch.randn(50, 128, device=d)
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    out = (rb.grouped_gemm_rows(x, w, off), rb.grouped_gemm_rows_dgrad(dy, w, off),
+           rb.grouped_gemm_rows_wgrad(dy, x, off), *rb.moe_router(l, 2), *rb.quantize_mxfp4(q))
+g.replay(); torch.cuda.synchronize()
+again = (rb.grouped_gemm_rows(x, w, off), rb.grouped_gemm_rows_dgrad(dy, w, off),
+         rb.grouped_gemm_rows_wgrad(dy, x, off), *rb.moe_router(l, 2), *rb.quantize_mxfp4(q))
+rb.last_status()
+for a, b in zip(out, again):
+    a, b = (t.view(torch.uint8) if t.element_size() == 1 else t for t in (a, b))
+    assert torch.equal(a, b)
+print("captured")
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=180,
+                       cwd=Path(__file__).resolve().parents[1])
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
+
+
+def test_every_group_empty(cuda_device):
+    """Rows, but none in a group: nothing is written, gradients are zero."""
+    import ratchet_b200 as rb
+
+    dev = cuda_device
+    x, dy, w = _rand(dev, 20, 64), _rand(dev, 20, 40), _rand(dev, 3, 40, 64)
+    for at in (0, 20):
+        off = torch.full((4,), at, dtype=torch.int32, device=dev)
+        y = torch.full((20, 40), 7.0, dtype=torch.bfloat16, device=dev)
+        dx = torch.full((20, 64), 7.0, dtype=torch.bfloat16, device=dev)
+        rb.grouped_gemm_rows(x, w, off, out=y)
+        rb.grouped_gemm_rows_dgrad(dy, w, off, out=dx)
+        assert bool((y == 7.0).all()) and bool((dx == 7.0).all())
+        assert bool((rb.grouped_gemm_rows_wgrad(dy, x, off) == 0).all())
+        rb.last_status()
+
+
+def test_views_at_odd_places(cuda_device):
+    """Tensors that start 16 bytes (the router: an element) into their storage give the
+    bits of those that start it."""
+    import ratchet_b200 as rb
+
+    dev = cuda_device
+
+    def shift(t, by):
+        buf = torch.zeros(t.numel() + by, dtype=t.dtype, device=dev)
+        buf[by:].copy_(t.reshape(-1))
+        return buf[by:].view(t.shape)
+
+    off = torch.tensor([0, 33, 90], dtype=torch.int32, device=dev)
+    x, dy, w = _rand(dev, 90, 72, seed=1), _rand(dev, 90, 40, seed=2), _rand(dev, 2, 40, 72, seed=3)
+    xs, ds, ws = shift(x, 8), shift(dy, 8), shift(w, 8)
+    assert torch.equal(rb.grouped_gemm_rows(x, w, off), rb.grouped_gemm_rows(xs, ws, off))
+    assert torch.equal(rb.grouped_gemm_rows_dgrad(dy, w, off), rb.grouped_gemm_rows_dgrad(ds, ws, off))
+    for dt, by in ((torch.float32, 4), (torch.bfloat16, 8)):
+        want = rb.grouped_gemm_rows_wgrad(dy, x, off, out_dtype=dt)
+        out = shift(torch.zeros_like(want), by)
+        rb.grouped_gemm_rows_wgrad(ds, xs, off, out=out)
+        assert torch.equal(out, want)
+        if dt is torch.float32:
+            rb.grouped_gemm_rows_wgrad(ds, xs, off, out=out, accumulate=True)
+            assert torch.equal(out, want + want)
+    rb.last_status()
+    for dt in (torch.float32, torch.bfloat16):
+        logits = _rand(dev, 70, 64, seed=4, dtype=dt)
+        moved = shift(logits, 1)
+        a, b = rb.moe_router(logits, 6, renormalize=False), rb.moe_router(moved, 6, renormalize=False)
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+        assert torch.equal(rb.moe_router_backward(a[1], logits, a[0], renormalize=False),
+                           rb.moe_router_backward(a[1], moved, a[0], renormalize=False))
+    q = rb.quantize_mxfp4(_rand(dev, 5, 96, seed=5))
+    assert torch.equal(rb.dequantize_mxfp4(*q), rb.dequantize_mxfp4(shift(q[0], 4), shift(
+        q[1].view(torch.uint8), 1)))
+
+
+def test_an_index_outside_the_weights(cuda_device):
+    """A device b_index that names no packed group stops the product with status 0x202
+    before any load of that tile; the next call is clean."""
+    import ratchet_b200 as rb
+
+    dev = cuda_device
+    pack = rb.pack_mxfp4_weights(*rb.quantize_mxfp4(_rand(dev, 2, 256, 256)))
+    q = rb.quantize_mxfp4(_rand(dev, 40, 256))
+    off = torch.tensor([0, 20, 40], dtype=torch.int32, device=dev)
+    for bad in ([0, 2], [-1, 1]):
+        rb.mxfp4_grouped_gemm_rows(*q, off, pack, b_index=torch.tensor(bad, dtype=torch.int32, device=dev))
+        with pytest.raises(rb.FggError, match="0x202"):
+            rb.last_status()
+    rb.mxfp4_grouped_gemm_rows(*q, off, pack, b_index=torch.tensor([1, 0], dtype=torch.int32, device=dev))
+    rb.last_status()
+
+
+def test_outputs_that_share_memory_are_refused(cuda_device):
+    import ratchet_b200 as rb
+
+    dev = cuda_device
+    off = torch.tensor([0, 4, 16], dtype=torch.int32, device=dev)
+    buf = torch.zeros(4 * 16 * 64, dtype=torch.bfloat16, device=dev)
+    x, w = buf[:1024].view(16, 64), _rand(dev, 2, 64, 64)
+    with pytest.raises(ValueError, match="shares"):
+        rb.grouped_gemm_rows(x, w, off, out=x)
+    with pytest.raises(ValueError, match="shares"):
+        rb.grouped_gemm_rows(x, w, off, out=buf[512:1536].view(16, 64))
+    with pytest.raises(ValueError, match="shares"):
+        rb.grouped_gemm_rows_dgrad(x, w, off, out=w[0, :16])
+    rb.grouped_gemm_rows(x, w, off, out=buf[1024:2048].view(16, 64))
+    rb.last_status()
+
+
 def test_python_refusals_on_the_device(cuda_device):
     import ratchet_b200 as rb
 
