@@ -349,9 +349,9 @@ __global__ void __launch_bounds__(32 * kRouterWarps)
 }
 
 // dlogits from dweights.  With c_j the share of route j,
-//   softmax, normalised over the chosen   c_j = w_j (dw_j - sum_i dw_i w_i)
+//   softmax, normalised over the chosen   c_j = w_j sum_i w_i (dw_j - dw_i)
 //   softmax                               c_j = s_j dw_j
-//   sigmoid, normalised                   c_j = w_j (dw_j - sum_i dw_i w_i) (1 - s_j)
+//   sigmoid, normalised                   c_j = w_j sum_i w_i (dw_j - dw_i) (1 - s_j)
 //   sigmoid                               c_j = dw_j s_j (1 - s_j)
 // (w normalised, without the scale), dl_e = sum of c_j over the routes to e,
 // minus s_e sum_j c_j for the whole softmax.
@@ -360,7 +360,7 @@ __global__ void __launch_bounds__(32 * kRouterWarps)
     router_backward_kernel(const __grid_constant__ RouterParams p) {
   constexpr int kTokens = kRouterWarps * 32 / L;
   constexpr int R = (kRouterMaxTopk + L - 1) / L;
-  __shared__ int2 s_share[kTokens][kRouterMaxTopk];  // (expert, share) of each route
+  __shared__ int2 s_share[kTokens][kRouterMaxTopk];  // each route's (weight, dw), (expert, share)
   const int sub = threadIdx.x & (L - 1);
   const int slot = int(threadIdx.x) / L;
   const int64_t t = int64_t(blockIdx.x) * kTokens + slot;
@@ -414,7 +414,7 @@ __global__ void __launch_bounds__(32 * kRouterWarps)
 #pragma unroll
     for (int i = 0; i < V; ++i) d[i] = -(d[i] * inv) * whole;
   } else {
-    float mj = kNegInf, sum = 0.0f, dot = 0.0f;
+    float mj = kNegInf, sum = 0.0f;
     if (p.renorm) {
 #pragma unroll
       for (int r = 0; r < R; ++r) mj = fmaxf(mj, lr[r]);
@@ -427,16 +427,30 @@ __global__ void __launch_bounds__(32 * kRouterWarps)
       sum = sub_sum<L>(sum);
 #pragma unroll
       for (int r = 0; r < R; ++r) {
+        const int j = r * L + sub;
         c[r] = sum == 0.0f ? 0.0f : c[r] / sum;
-        dot += c[r] * dw[r];
+        if (j < p.topk) s_share[slot][j] = make_int2(__float_as_int(c[r]), __float_as_int(dw[r]));
       }
-      dot = sub_sum<L>(dot);
+      __syncwarp();
+      // w_j (dw_j - sum_i w_i dw_i) as w_j sum_i w_i (dw_j - dw_i): where one route has
+      // nearly all the weight, the difference of the sum would be its rounding
+      float to[R];
+#pragma unroll
+      for (int r = 0; r < R; ++r) to[r] = 0.0f;
+      for (int i = 0; i < p.topk; ++i) {
+        const int2 q = s_share[slot][i];
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+          to[r] = fmaf(__int_as_float(q.x), dw[r] - __int_as_float(q.y), to[r]);
+      }
+#pragma unroll
+      for (int r = 0; r < R; ++r) c[r] *= to[r];
+      __syncwarp();  // the shares are written over below
     }
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const float x = expf(-fabsf(lr[r]));
       if (p.renorm) {
-        c[r] *= dw[r] - dot;
         // 1 - sigmoid(l)
         if (!kSoftmax && id[r] >= 0) c[r] *= lr[r] >= 0.0f ? x / (1.0f + x) : 1.0f / (1.0f + x);
       } else {

@@ -273,6 +273,25 @@ def test_backward_against_differences(cuda_device, score, renorm):
             assert abs(float(got[r, i]) - want) <= 1e-6, (r, i)
 
 
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_gradient_where_one_route_has_nearly_all_the_weight(cuda_device, score):
+    """Weights 1 - 1e-5 and 1e-5: the gradient w_0 w_1 (dw_0 - dw_1) keeps its relative
+    accuracy, which the difference dw_0 - (w_0 dw_0 + w_1 dw_1) would lose."""
+    import ratchet_b200 as rb
+
+    logits = torch.tensor([[-2.0, -14.0, -30.0]], device=cuda_device)
+    ids = torch.tensor([[0, 1]], dtype=torch.int32, device=cuda_device)
+    dw = torch.tensor([[1.25, 0.5]], device=cuda_device)
+    d = rb.moe_router_backward(dw, logits, ids, score=score).double().cpu()[0]
+    s = _scores(logits[0].double().tolist(), score)
+    w = [s[0] / (s[0] + s[1]), s[1] / (s[0] + s[1])]
+    for i, sign in ((0, 1), (1, -1)):
+        want = sign * w[0] * w[1] * 0.75 * (1.0 if score == "softmax" else 1 - s[i])
+        # expf of up to 28 twice, quotients, products: test_backward's share of the value
+        assert abs(float(d[i]) - want) <= (32 + 8 * 28 + 12) * 2.0**-24 * abs(want)
+    assert float(d[2]) == 0.0
+
+
 def test_masked_rows_have_no_gradient(cuda_device):
     import ratchet_b200 as rb
 
