@@ -137,10 +137,11 @@ struct F16Cfg {
 
 // ------------------------------------------------------------- epilogues
 // Forward, dgrad.  The warp's 32 TMEM lanes are the output columns m0 + lane, its
-// TMEM columns the tile's tokens.  They are turned by three rounds of swaps between
-// lanes 1, 2 and 4 apart, after which lane l holds columns (l & ~7) .. + 7 of every
-// eighth token from l & 7 on: 16 contiguous bytes to store, 64 of each token per
-// instruction.  Columns past the output's edge are not stored.
+// TMEM columns the tile's tokens.  A word of two tokens' results per column goes
+// through three rounds of swaps between lanes 1, 2 and 4 apart, after which lane l
+// holds columns (l & ~7) .. + 7 of tokens 2 (l & 7), 2 (l & 7) + 1 and those 16
+// further on: 16 contiguous bytes to store, 64 of each token per instruction.
+// Columns past the output's edge are not stored.
 __device__ __forceinline__ void f16_epilogue_rows(void* out, int ldn, int m0, size_t row0, int rows,
                                                   int ncols, int part, bool bf16,
                                                   uint32_t taddr) {
@@ -156,29 +157,46 @@ __device__ __forceinline__ void f16_epilogue_rows(void* out, int ldn, int m0, si
   if (c0 < ncols) tmem_ld32(taddr + c0, r);
   for (; c0 < ncols; c0 += 64) {
     tmem_wait_ld();
-    uint32_t w[16];  // columns (l & ~1, + 1) of token 2 i + b0
+    uint32_t w[16];  // tokens 2 i, 2 i + 1 of column l
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const float v0 = __uint_as_float(r[2 * i]), v1 = __uint_as_float(r[2 * i + 1]);
-      const float got = __shfl_xor_sync(kFullMask, b0 ? v0 : v1, 1);
-      w[i] = b0 ? pack_16(got, v1, bf16) : pack_16(v0, got, bf16);
-    }
+    for (int i = 0; i < 16; ++i)
+      w[i] = pack_16(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]), bf16);
     if (c0 + 64 < ncols) tmem_ld32(taddr + c0 + 64, r);
-    uint32_t x[8][2];  // columns (l & ~3) .. + 3 of token 4 i + 2 b1 + b0
+    uint32_t x[8][2];  // token pair 2 i + b0 of columns (l & ~1) + 0, 1
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const uint32_t got = __shfl_xor_sync(kFullMask, b1 ? w[2 * i] : w[2 * i + 1], 2);
-      x[i][0] = b1 ? got : w[2 * i];
-      x[i][1] = b1 ? w[2 * i + 1] : got;
+      const uint32_t got = __shfl_xor_sync(kFullMask, b0 ? w[2 * i] : w[2 * i + 1], 1);
+      x[i][0] = b0 ? got : w[2 * i];
+      x[i][1] = b0 ? w[2 * i + 1] : got;
     }
+    uint32_t y[4][4];  // token pair 4 i + 2 b1 + b0 of columns (l & ~3) + 0 .. 3
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t g0 = __shfl_xor_sync(kFullMask, b2 ? x[2 * i][0] : x[2 * i + 1][0], 4);
-      const uint32_t g1 = __shfl_xor_sync(kFullMask, b2 ? x[2 * i][1] : x[2 * i + 1][1], 4);
-      const uint4 q = b2 ? make_uint4(g0, g1, x[2 * i + 1][0], x[2 * i + 1][1])
-                         : make_uint4(x[2 * i][0], x[2 * i][1], g0, g1);
-      const int t = c0 + 8 * i + (lane & 7);
-      if (t < rows && col_ok) *reinterpret_cast<uint4*>(o + (row0 + size_t(t)) * size_t(ldn)) = q;
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const uint32_t got = __shfl_xor_sync(kFullMask, b1 ? x[2 * i][j] : x[2 * i + 1][j], 2);
+        y[i][j] = b1 ? got : x[2 * i][j];
+        y[i][2 + j] = b1 ? x[2 * i + 1][j] : got;
+      }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      uint32_t z[8];  // token pair 8 i + (l & 7) of columns (l & ~7) + 0 .. 7
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t got = __shfl_xor_sync(kFullMask, b2 ? y[2 * i][j] : y[2 * i + 1][j], 4);
+        z[j] = b2 ? got : y[2 * i][j];
+        z[4 + j] = b2 ? y[2 * i + 1][j] : got;
+      }
+      const int t = c0 + 16 * i + 2 * (lane & 7);
+      uint16_t* const at = o + (row0 + size_t(t)) * size_t(ldn);
+      if (t < rows && col_ok)
+        *reinterpret_cast<uint4*>(at) =
+            make_uint4(__byte_perm(z[0], z[1], 0x5410), __byte_perm(z[2], z[3], 0x5410),
+                       __byte_perm(z[4], z[5], 0x5410), __byte_perm(z[6], z[7], 0x5410));
+      if (t + 1 < rows && col_ok)
+        *reinterpret_cast<uint4*>(at + size_t(ldn)) =
+            make_uint4(__byte_perm(z[0], z[1], 0x7632), __byte_perm(z[2], z[3], 0x7632),
+                       __byte_perm(z[4], z[5], 0x7632), __byte_perm(z[6], z[7], 0x7632));
     }
   }
 }
