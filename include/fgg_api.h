@@ -305,7 +305,9 @@ FGG_API int fgg_mxfp4_grouped_gemm_rows(const FggMxfp4RowsProblem* p, const void
  *                         to what out holds.
  * N and K are multiples of 8; every tensor is contiguous and 16-byte aligned.
  * Sums are held in fp32 and rounded once (fp16 results past 65504 become
- * infinite).  Rows outside every group are neither read for any output nor
+ * infinite).  A call's results do not vary; as a call of few tiles splits its sums
+ * over the GPU, the same rows may differ in the last fp32 bits, before that rounding,
+ * between calls with other groups beside them.  Rows outside every group are neither read for any output nor
  * written.  Malformed offsets (decreasing, negative, past max_rows) run no
  * tile and leave status 0x203 in the workspace. */
 typedef struct FggF16RowsProblem {
@@ -322,7 +324,9 @@ typedef struct FggF16RowsProblem {
   void* out;
 } FggF16RowsProblem;
 
-/* Workspace (128-byte aligned) of one call; 0 for a bad problem. */
+/* Workspace (128-byte aligned) of one call; 0 for a bad problem.  Where tiles may be
+ * split (at most 48 in a call's smallest form, 64 steps of 64 or more) up to 24 MB of
+ * it hold partial sums. */
 FGG_API size_t fgg_f16_rows_workspace_bytes(const FggF16RowsProblem* p, int32_t direction);
 FGG_API int fgg_f16_grouped_gemm_rows(const FggF16RowsProblem* p, int32_t direction,
                                       void* workspace, size_t ws_bytes, void* stream);

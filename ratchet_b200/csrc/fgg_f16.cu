@@ -32,6 +32,14 @@
 // at a time in TMEM and the epilogue adds those sums in registers, rounding to
 // nearest; a 16-bit result hides it (forward, dgrad).
 //
+// A few tiles, or a few long ones (a small expert's gradient over all its rows, one
+// expert's tokens), leave pairs idle: the prepare kernel cuts such a tile along the
+// contraction into up to 16 slices, units of work like the other tiles.  Their fp32
+// sums are joined two by two: of two neighbours the warp that is done first leaves its
+// sums in the workspace and goes on, the other adds them to its own and stands for
+// both.  Nothing waits, and as a + b = b + a the results do not depend on timing.  They
+// may depend, in the last fp32 bits before the rounding, on the call's number of tiles.
+//
 // What bounds it: the tensor pipe for groups of about 250 tokens and more, the
 // weights' HBM stream below that, shared-memory bandwidth and the gradient's write
 // for wgrad with short groups; and in seconds-long runs of any of them but the
@@ -65,14 +73,34 @@ constexpr int kF16BadOffsets = 0x203;  // offsets decreasing, negative or past m
 constexpr int kTokenMaps = 8;
 
 struct F16Slot {
-  int32_t g;     // group, -1 = no more tiles
-  int32_t mt;    // tile of the M axis
-  int32_t row0;  // first token row of the tile (wgrad: of the group)
-  int32_t rows;  // tokens of the tile (forward, dgrad) / of the group (wgrad)
-  int32_t ct;    // tile of the N axis (wgrad)
-  int32_t pad[3];
+  int32_t g;       // group, -1 = no more tiles
+  int32_t mt;      // tile of the M axis
+  int32_t row0;    // first token row of the tile (wgrad: of the group)
+  int32_t rows;    // tokens of the tile (forward, dgrad) / of the group (wgrad)
+  int32_t ct;      // tile of the N axis (wgrad)
+  int32_t k0, k1;  // its steps of the contraction
+  uint32_t split;  // 0 = all of them, else the unit's word (see split_word)
 };
 static_assert(sizeof(F16Slot) == 32, "slot is 8 words");
+
+// A tile is split if a pair's share of the call's steps is at most half of its own,
+// into slices of about that share: the units of split tiles are at most as many as
+// pairs.  A join costs 4 to 5 us, up to 9 where all pairs join at once after few
+// steps, and a step about 0.26 us of a pair.  Unsplit -> split, cold L2: one tile of 64
+// steps in two (a gradient of 64 x 64 over 4096 rows) 30.5 -> 26.4 us, of 128 in four
+// (one token, K 8192) 34.2 -> 22.6; 470 steps in 14 (30000 rows) 143 -> 36; 32 tiles of 64
+// in two, which is not done, 36.9 -> 41.5, of 128 in two 53.2 -> 47.1.  Slices of at least
+// 16 steps: 25.4 -> 31.6 us for 16 tiles of 32; of 64: 143 -> 44 for the 30000 rows.
+constexpr int kMaxSplitUnits = 96;
+constexpr int kMaxSlices = 16;
+constexpr int kMinSlice = 32;
+// 128 fp32 sums per lane and epilogue warp of a pair
+constexpr int kWarpSums = 2 * 8;
+constexpr int kUnitFloats = kWarpSums * 128 * 32;
+// Unit of a split tile: tile, slice, slices, the tile's first unit.
+__host__ __device__ constexpr uint32_t split_word(int tile, int slice, int slices, int first) {
+  return uint32_t(tile) | uint32_t(slice) << 8 | uint32_t(slices) << 16 | uint32_t(first) << 24;
+}
 
 struct F16Params {
   CUtensorMap tmap_w;                // forward, dgrad: [G, N, K] weights
@@ -84,13 +112,16 @@ struct F16Params {
   const int32_t* offsets;
   const int32_t* order;  // wgrad: groups, the largest first
   void* out;
-  int* status;  // [0] status [1] tile counter [3] tile count
+  const uint32_t* units;  // of the split tiles, which are the list's first
+  int32_t* arrived;       // per unit and epilogue warp: sides that came to that join
+  float* partial;         // per unit: the epilogue warps' sums
+  int* status;  // [0] status [1] unit counter [3] tiles [4] split tiles [5] their units
   int32_t num_groups;
   int32_t m_ext;   // extent of the M axis (the output's columns; wgrad: its rows n)
   int32_t c_ext;   // wgrad: extent of the N axis (k)
   int32_t ksteps;  // forward, dgrad: 64-element steps of the contraction
   int32_t mts, cts;
-  int32_t grid_tiles;  // host bound on the tiles
+  int32_t grid_units;  // host bound on the tiles and slices
   int32_t bf16;        // operands bf16 (1) or fp16 (0)
   int32_t out_fp32;    // wgrad: fp32 gradient
   int32_t accumulate;  // wgrad, fp32: add to the gradient
@@ -103,9 +134,15 @@ __device__ __forceinline__ uint32_t pack_16(float lo, float hi, bool bf16) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-template <int MODE_>
+template <int MODE_, bool SPLIT_>
 struct F16Cfg {
   static constexpr int MODE = MODE_;
+  // Tiles may be split.  A build of its own, for problems whose sizes allow it: with the
+  // joins' registers the unsplit gradient of 64 skewed experts, 32768 rows, 7168 x 2048
+  // took 1368 us in place of 1319.  Whole tiles of a
+  // problem that may have split ones pay up to 1 us (16 skewed groups, 4096 rows,
+  // 1024 x 512: 26.7 -> 27.8 us).
+  static constexpr bool SPLIT = SPLIT_;
   static constexpr bool A_MN = MODE_ != kFwd;
   static constexpr bool B_MN = MODE_ == kWgrad;
   static constexpr int BN = 256;   // N axis of a pair tile
@@ -142,63 +179,115 @@ struct F16Cfg {
 // holds columns (l & ~7) .. + 7 of tokens 2 (l & 7), 2 (l & 7) + 1 and those 16
 // further on: 16 contiguous bytes to store, 64 of each token per instruction.
 // Columns past the output's edge are not stored.
-__device__ __forceinline__ void f16_epilogue_rows(void* out, int ldn, int m0, size_t row0, int rows,
-                                                  int ncols, int part, bool bf16,
-                                                  uint32_t taddr) {
+struct F16Rows {
+  uint16_t* out;  // at column m0 + (lane & ~7)
+  size_t row0, ldn;
+  int rows;
+  bool col_ok, bf16;
+};
+__device__ __forceinline__ void f16_pack_block(const uint32_t (&r)[32], bool bf16,
+                                               uint32_t (&w)[16]) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i)  // tokens 2 i, 2 i + 1 of column l
+    w[i] = pack_16(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]), bf16);
+}
+__device__ __forceinline__ void f16_turn_block(const F16Rows& d, int c0, const uint32_t (&w)[16]) {
   const int lane = threadIdx.x & 31;
   const bool b0 = lane & 1, b1 = lane & 2, b2 = lane & 4;
-  const int col = m0 + (lane & ~7);
-  const bool col_ok = col < ldn;
-  uint16_t* const o = static_cast<uint16_t*>(out) + size_t(col);
-  // the quadrant's two warps by turns, 32 tokens each; the next ones are read while
-  // these are turned and stored
+  uint32_t x[8][2];  // token pair 2 i + b0 of columns (l & ~1) + 0, 1
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t got = __shfl_xor_sync(kFullMask, b0 ? w[2 * i] : w[2 * i + 1], 1);
+    x[i][0] = b0 ? got : w[2 * i];
+    x[i][1] = b0 ? w[2 * i + 1] : got;
+  }
+  uint32_t y[4][4];  // token pair 4 i + 2 b1 + b0 of columns (l & ~3) + 0 .. 3
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const uint32_t got = __shfl_xor_sync(kFullMask, b1 ? x[2 * i][j] : x[2 * i + 1][j], 2);
+      y[i][j] = b1 ? got : x[2 * i][j];
+      y[i][2 + j] = b1 ? x[2 * i + 1][j] : got;
+    }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    uint32_t z[8];  // token pair 8 i + (l & 7) of columns (l & ~7) + 0 .. 7
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t got = __shfl_xor_sync(kFullMask, b2 ? y[2 * i][j] : y[2 * i + 1][j], 4);
+      z[j] = b2 ? got : y[2 * i][j];
+      z[4 + j] = b2 ? y[2 * i + 1][j] : got;
+    }
+    const int t = c0 + 16 * i + 2 * (lane & 7);
+    uint16_t* const at = d.out + (d.row0 + size_t(t)) * d.ldn;
+    if (t < d.rows && d.col_ok)
+      *reinterpret_cast<uint4*>(at) =
+          make_uint4(__byte_perm(z[0], z[1], 0x5410), __byte_perm(z[2], z[3], 0x5410),
+                     __byte_perm(z[4], z[5], 0x5410), __byte_perm(z[6], z[7], 0x5410));
+    if (t + 1 < d.rows && d.col_ok)
+      *reinterpret_cast<uint4*>(at + d.ldn) =
+          make_uint4(__byte_perm(z[0], z[1], 0x7632), __byte_perm(z[2], z[3], 0x7632),
+                     __byte_perm(z[4], z[5], 0x7632), __byte_perm(z[6], z[7], 0x7632));
+  }
+}
+
+// A whole tile: the quadrant's two warps by turns, 32 tokens each; the next ones are
+// read while these are turned and stored.
+__device__ __forceinline__ void f16_epilogue_rows(const F16Rows& d, int ncols, int part,
+                                                  uint32_t taddr) {
   uint32_t r[32];
   int c0 = 32 * part;
   if (c0 < ncols) tmem_ld32(taddr + c0, r);
   for (; c0 < ncols; c0 += 64) {
     tmem_wait_ld();
-    uint32_t w[16];  // tokens 2 i, 2 i + 1 of column l
-#pragma unroll
-    for (int i = 0; i < 16; ++i)
-      w[i] = pack_16(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]), bf16);
+    uint32_t w[16];
+    f16_pack_block(r, d.bf16, w);
     if (c0 + 64 < ncols) tmem_ld32(taddr + c0 + 64, r);
-    uint32_t x[8][2];  // token pair 2 i + b0 of columns (l & ~1) + 0, 1
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t got = __shfl_xor_sync(kFullMask, b0 ? w[2 * i] : w[2 * i + 1], 1);
-      x[i][0] = b0 ? got : w[2 * i];
-      x[i][1] = b0 ? w[2 * i + 1] : got;
-    }
-    uint32_t y[4][4];  // token pair 4 i + 2 b1 + b0 of columns (l & ~3) + 0 .. 3
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const uint32_t got = __shfl_xor_sync(kFullMask, b1 ? x[2 * i][j] : x[2 * i + 1][j], 2);
-        y[i][j] = b1 ? got : x[2 * i][j];
-        y[i][2 + j] = b1 ? x[2 * i + 1][j] : got;
-      }
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      uint32_t z[8];  // token pair 8 i + (l & 7) of columns (l & ~7) + 0 .. 7
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t got = __shfl_xor_sync(kFullMask, b2 ? y[2 * i][j] : y[2 * i + 1][j], 4);
-        z[j] = b2 ? got : y[2 * i][j];
-        z[4 + j] = b2 ? y[2 * i + 1][j] : got;
-      }
-      const int t = c0 + 16 * i + 2 * (lane & 7);
-      uint16_t* const at = o + (row0 + size_t(t)) * size_t(ldn);
-      if (t < rows && col_ok)
-        *reinterpret_cast<uint4*>(at) =
-            make_uint4(__byte_perm(z[0], z[1], 0x5410), __byte_perm(z[2], z[3], 0x5410),
-                       __byte_perm(z[4], z[5], 0x5410), __byte_perm(z[6], z[7], 0x5410));
-      if (t + 1 < rows && col_ok)
-        *reinterpret_cast<uint4*>(at + size_t(ldn)) =
-            make_uint4(__byte_perm(z[0], z[1], 0x7632), __byte_perm(z[2], z[3], 0x7632),
-                       __byte_perm(z[4], z[5], 0x7632), __byte_perm(z[6], z[7], 0x7632));
-    }
+    f16_turn_block(d, c0, w);
   }
+}
+
+// ----------------------------------------------------------- split tiles
+// The tree over a split tile's slices, walked by one warp.  At height h it stands for
+// the slices first .. first + 2^h - 1, as far as there are so many; its neighbour's
+// begin where bit h of `first` is the other way.  A join is known by the first slice
+// of its right side.
+struct F16Tree {
+  float* sums;       // this warp's and lane's, of the tile's slice 0
+  int32_t* arrived;  // this warp's, of the tile's slice 0
+  int first, slices, h;
+  __device__ __forceinline__ float* mine() const { return sums + size_t(first) * kUnitFloats; }
+  __device__ __forceinline__ float* other() const {
+    return sums + size_t(first ^ (1 << h)) * kUnitFloats;
+  }
+  // Up to the next join; false at the top.
+  __device__ __forceinline__ bool next() {
+    while ((1 << h) < slices && (first ^ (1 << h)) >= slices) ++h;
+    return (1 << h) < slices;
+  }
+  // This side's sums are in mine().  True if the other's are in other(): go on for both.
+  __device__ __forceinline__ bool arrive() {
+    __threadfence();
+    __syncwarp();
+    int before = 0;
+    if ((threadIdx.x & 31) == 0) before = atomicAdd(arrived + (first | 1 << h) * kWarpSums, 1);
+    before = __shfl_sync(kFullMask, before, 0);
+    __threadfence();
+    return before != 0;
+  }
+  __device__ __forceinline__ void joined() { first &= ~(1 << h++); }
+};
+// Of epilogue warp `ewarp` (0 .. 15 over both CTAs) of the unit.
+__device__ __forceinline__ F16Tree f16_tree(const F16Params& p, uint32_t unit, int ewarp) {
+  F16Tree t;
+  const size_t unit0 = unit >> 24;
+  t.sums = p.partial + unit0 * kUnitFloats + ewarp * 4096 + (threadIdx.x & 31);
+  t.arrived = p.arrived + unit0 * kWarpSums + ewarp;
+  t.first = int(unit >> 8 & 0xFFu);
+  t.slices = int(unit >> 16 & 0xFFu);
+  t.h = 0;
+  return t;
 }
 
 // 32 bytes of one lane to a 16-byte aligned address (one store where it is
@@ -282,6 +371,7 @@ __device__ __forceinline__ int wgrad_steps(int m) {
 }
 
 // ------------------------------------------------------------ the kernel
+// The words from k0 on are published where tiles may be split.
 __device__ __forceinline__ F16Slot f16_read_slot(const volatile F16Slot* ring, int slot) {
   F16Slot s;
   s.g = ring[slot].g;
@@ -289,6 +379,9 @@ __device__ __forceinline__ F16Slot f16_read_slot(const volatile F16Slot* ring, i
   s.row0 = ring[slot].row0;
   s.rows = ring[slot].rows;
   s.ct = ring[slot].ct;
+  s.k0 = ring[slot].k0;
+  s.k1 = ring[slot].k1;
+  s.split = ring[slot].split;
   return s;
 }
 
@@ -304,13 +397,23 @@ __device__ __forceinline__ void f16_place(int local, int rows, int cols, int* ro
   *col = strip * kStrip + rest - *row * width;
 }
 
-template <int MODE>
-__device__ __forceinline__ F16Slot f16_make_slot(const F16Params& p, int t, int num_tiles) {
+template <class C>
+__device__ __forceinline__ F16Slot f16_make_slot(const F16Params& p, int unit, int num_tiles,
+                                                 int split_tiles, int split_units) {
   F16Slot s;
   s.g = -1;
-  s.mt = s.row0 = s.rows = s.ct = 0;
+  s.mt = s.row0 = s.rows = s.ct = s.k0 = s.k1 = 0;
+  s.split = 0;
+  int t = unit;
+  if constexpr (C::SPLIT) {
+    t += split_tiles - split_units;
+    if (unit < split_units) {
+      s.split = __ldg(p.units + unit);
+      t = int(s.split & 0xFFu);
+    }
+  }
   if (t >= num_tiles) return s;
-  if constexpr (MODE == kWgrad) {
+  if constexpr (C::MODE == kWgrad) {
     const int per = p.mts * p.cts;
     const int pos = t / per;
     const int local = t - pos * per;
@@ -324,6 +427,12 @@ __device__ __forceinline__ F16Slot f16_make_slot(const F16Params& p, int t, int 
     s.mt = int((tile >> 32) & 0xFFFFu);
     s.row0 = int(uint32_t(tile));
     s.rows = __ldg(p.tile_rows + t);
+  }
+  s.k1 = C::MODE == kWgrad ? wgrad_steps(s.rows) : p.ksteps;
+  if (C::SPLIT && s.split != 0) {
+    const int64_t steps = s.k1, slice = s.split >> 8 & 0xFFu, slices = s.split >> 16 & 0xFFu;
+    s.k0 = int(steps * slice / slices);
+    s.k1 = int(steps * (slice + 1) / slices);
   }
   return s;
 }
@@ -367,7 +476,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(C::THREADS, 1)
   auto tile_ncols = [&](int rows) -> int {
     return C::MODE == kWgrad ? C::BN : min(C::BN, (rows + 31) & ~31);
   };
-  auto tile_ksteps = [&](int rows) -> int {
+
+  // steps of a unit
+  auto unit_k0 = [&](int slot) -> int {
+    return C::SPLIT ? __shfl_sync(kFullMask, ring[slot].k0, 0) : 0;
+  };
+  auto unit_k1 = [&](int slot, int rows) -> int {
+    if constexpr (C::SPLIT) return __shfl_sync(kFullMask, ring[slot].k1, 0);
     return C::MODE == kWgrad ? wgrad_steps(rows) : p.ksteps;
   };
 
@@ -423,6 +538,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(C::THREADS, 1)
         int slot = 0;
         uint32_t sphase = 0;
         const int num_tiles = p.status[3];
+        const int split_tiles = C::SPLIT ? p.status[4] : 0;
+        const int split_units = C::SPLIT ? p.status[5] : 0;
+        const int num_units = num_tiles - split_tiles + split_units;
+        const bool few = C::SPLIT && num_units <= int(gridDim.x >> 1);
         const uint32_t remote_ring0 = mapa_shared(smem_u32(const_cast<F16Slot*>(ring)), peer);
         const uint32_t remote_schedf0 = mapa_shared(schedf_bar(0), peer);
         for (uint32_t n = 0;; ++n) {
@@ -439,15 +558,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(C::THREADS, 1)
             *abort_flag = 1;
             break;
           }
-          const int t = atomicAdd(p.status + 1, 1);
-          const F16Slot s = f16_make_slot<C::MODE>(p, t, num_tiles);
+          // few units: one for each pair, none claimed ahead of a pair that has none
+          const int unit = few ? (n == 0 ? int(blockIdx.x >> 1) : num_units)
+                               : atomicAdd(p.status + 1, 1);
+          const F16Slot s =
+              f16_make_slot<C>(p, unit, num_tiles, split_tiles, split_units);
           if (!mbar_wait1<true>(schede_bar(slot), sphase ^ 1, abort_flag, p.status,
                                 kStatusTimeoutProducer))
             break;
-          const uint32_t words[5] = {uint32_t(s.g), uint32_t(s.mt), uint32_t(s.row0),
-                                     uint32_t(s.rows), uint32_t(s.ct)};
+          const uint32_t words[8] = {uint32_t(s.g),    uint32_t(s.mt), uint32_t(s.row0),
+                                     uint32_t(s.rows), uint32_t(s.ct), uint32_t(s.k0),
+                                     uint32_t(s.k1),   s.split};
 #pragma unroll
-          for (int i = 0; i < 5; ++i) {
+          for (int i = 0; i < (C::SPLIT ? 8 : 5); ++i) {
             reinterpret_cast<volatile uint32_t*>(ring + slot)[i] = words[i];
             st_shared_remote_u32(remote_ring0 + 32u * slot + 4u * i, words[i]);
           }
@@ -487,6 +610,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(C::THREADS, 1)
         const int row0 = __shfl_sync(kFullMask, ring[slot].row0, 0);
         const int rows = __shfl_sync(kFullMask, ring[slot].rows, 0);
         const int ct = __shfl_sync(kFullMask, ring[slot].ct, 0);
+        const int k0 = unit_k0(slot);
+        const int k1 = unit_k1(slot, rows);
         if (lane == 0) {
           release_slot(slot);
           if (leader) mbar_arrive(taken_bar(tiles_taken));
@@ -501,17 +626,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(C::THREADS, 1)
           break;
         }
         const int half = tile_ncols(rows) >> 1;
-        const int ksteps = tile_ksteps(rows);
         // bytes that both CTAs' loads of one step deliver to the leader's barrier
         const uint32_t tx_step = 2u * (C::A_BYTES + uint32_t(half) * 128u);
-        const int flat_steps = C::MODE == kWgrad ? wgrad_flat_steps(rows) : ksteps;
+        const int flat_steps = C::MODE == kWgrad ? wgrad_flat_steps(rows) : k1;
         const int m0 = mt * 256 + int(rank) * 128;     // this CTA's rows of the M axis
         const int tok = row0 + int(rank) * half;       // forward, dgrad: its tokens
         const int c0 = ct * 256 + int(rank) * 128;     // wgrad: its columns k
         const CUtensorMap* const tb =
             C::MODE == kWgrad ? &p.tmap_b : &p.tmap_tok[half / 16 - 1];
         bool ok = true;
-        for (int ks = 0; ks < ksteps; ++ks) {
+        for (int ks = k0; ks < k1; ++ks) {
           if (!mbar_wait(empty_bar(stage), phase ^ 1, abort_flag, p.status,
                          kStatusTimeoutProducer)) {
             ok = false;
@@ -573,6 +697,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(C::THREADS, 1)
           break;
         const int g = __shfl_sync(kFullMask, ring[slot].g, 0);
         const int rows = __shfl_sync(kFullMask, ring[slot].rows, 0);
+        const int k0 = unit_k0(slot);
+        const int k1 = unit_k1(slot, rows);
         if (lane == 0) mbar_arrive(schede_bar(slot));
         if (++slot == C::SCHED) {
           slot = 0;
@@ -580,14 +706,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(C::THREADS, 1)
         }
         if (g < 0) break;
         const int ncols = tile_ncols(rows);
-        const int ksteps = tile_ksteps(rows);
         const uint32_t idesc =
             idesc_f16(p.bf16 ? 1u : 0u, C::A_MN ? 1u : 0u, C::B_MN ? 1u : 0u, 256, ncols);
         // an empty group's gradient (wgrad) is a chunk without steps
-        int ks = 0;
+        int ks = k0;
         do {
           const int chunk0 = ks;
-          const int chunk1 = min(ksteps - chunk0, C::CHUNK) + chunk0;
+          const int chunk1 = min(k1 - chunk0, C::CHUNK) + chunk0;
           const uint32_t b = lt & 1u;
           if (!mbar_wait(acce_bar(b), ((lt >> 1) & 1u) ^ 1u, abort_flag, p.status,
                          kStatusTimeoutMma)) {
@@ -633,7 +758,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(C::THREADS, 1)
           __syncwarp();
           issued_any = true;
           ++lt;
-        } while (ks < ksteps);
+        } while (ks < k1);
       }
       if (issued_any) {
         if (elect_one()) {
@@ -688,11 +813,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(C::THREADS, 1)
         }
       };
       if constexpr (C::MODE == kWgrad) {
-        const int ksteps = tile_ksteps(s.rows);
         float acc[128];
 #pragma unroll
         for (int j = 0; j < 128; ++j) acc[j] = 0.0f;
-        int ks = 0;
+        const int k0 = C::SPLIT ? s.k0 : 0;
+        const int k1 = C::SPLIT ? s.k1 : wgrad_steps(s.rows);
+        int ks = k0;
         do {
           const uint32_t b = lt & 1u;
           if (!mbar_wait(accf_bar(b), (lt >> 1) & 1u, abort_flag, p.status,
@@ -702,7 +828,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(C::THREADS, 1)
           }
           tc_fence_after();
           const uint32_t taddr = tmem + (uint32_t(q * 32) << 16) + b * C::BN + 128u * part;
-          if (ksteps > 0) {
+          if (k1 > 0) {
 #pragma unroll
             for (int c = 0; c < 8; ++c) {
               uint32_t r[16];
@@ -715,9 +841,30 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(C::THREADS, 1)
           release_acc(b);
           ++lt;
           ks += C::CHUNK;
-        } while (ks < ksteps);
+        } while (ks < k1);
         next = take();
-        if (ok && (s.rows > 0 || !p.accumulate)) {
+        bool store = s.rows > 0 || !p.accumulate;
+        if (C::SPLIT && (m0 >= p.m_ext || s.ct * 256 + 128 * part >= p.c_ext)) store = false;
+        if (C::SPLIT && ok && s.split != 0) {
+          F16Tree tree = f16_tree(p, s.split, int(rank) * C::EPI_WARPS + warp - 4);
+          while (store && tree.next()) {
+#pragma unroll
+            for (int j = 0; j < 128; ++j) __stcg(tree.mine() + 32 * j, acc[j]);
+            store = tree.arrive();
+            if (store) {
+#pragma unroll
+              for (int j = 0; j < 128; j += 32) {
+                float o[32];
+#pragma unroll
+                for (int i = 0; i < 32; ++i) o[i] = __ldcg(tree.other() + 32 * (j + i));
+#pragma unroll
+                for (int i = 0; i < 32; ++i) acc[j + i] += o[i];
+              }
+              tree.joined();
+            }
+          }
+        }
+        if (ok && store) {
           if (p.out_fp32)
             f16_store_wgrad<true>(p, s.g, m0, s.ct * 256 + 128 * part, acc);
           else
@@ -730,10 +877,53 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(C::THREADS, 1)
         tc_fence_after();
         next = take();
         const uint32_t taddr = tmem + (uint32_t(q * 32) << 16) + b * C::BN;
-        if (m0 < p.m_ext)
-          f16_epilogue_rows(p.out, p.m_ext, m0, size_t(s.row0), s.rows, tile_ncols(s.rows),
-                            part, p.bf16 != 0, taddr);
-        release_acc(b);
+        const int ncols = tile_ncols(s.rows);
+        const int col = m0 + (lane & ~7);
+        const F16Rows d = {static_cast<uint16_t*>(p.out) + col, size_t(s.row0), size_t(p.m_ext),
+                           s.rows, col < p.m_ext, p.bf16 != 0};
+        if (C::SPLIT && s.split != 0) {
+          // blocks of 32 tokens as in f16_epilogue_rows, 1024 sums each
+          F16Tree tree = f16_tree(p, s.split, int(rank) * C::EPI_WARPS + warp - 4);
+          bool more = m0 < p.m_ext;
+          if (more)
+            for (int c0 = 32 * part, at = 0; c0 < ncols; c0 += 64, at += 1024) {
+              uint32_t r[32];
+              tmem_ld32(taddr + c0, r);
+              tmem_wait_ld();
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                __stcg(tree.mine() + at + 32 * j, __uint_as_float(r[j]));
+            }
+          release_acc(b);
+          while (more && tree.next() && (more = tree.arrive())) {
+            const float* const lo = tree.mine();
+            const float* const hi = tree.other();
+            tree.joined();
+            const bool top = !tree.next();
+            for (int c0 = 32 * part, at = 0; c0 < ncols; c0 += 64, at += 1024) {
+              uint32_t r[32], w[16];
+              float o[32];
+#pragma unroll
+              for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__ldcg(lo + at + 32 * j));
+#pragma unroll
+              for (int j = 0; j < 32; ++j) o[j] = __ldcg(hi + at + 32 * j);
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                r[j] = __float_as_uint(__uint_as_float(r[j]) + o[j]);
+              if (top) {
+                f16_pack_block(r, d.bf16, w);
+                f16_turn_block(d, c0, w);
+              } else {
+#pragma unroll
+                for (int j = 0; j < 32; ++j)
+                  __stcg(tree.mine() + at + 32 * j, __uint_as_float(r[j]));
+              }
+            }
+          }
+        } else {
+          if (m0 < p.m_ext) f16_epilogue_rows(d, ncols, part, taddr);
+          release_acc(b);
+        }
         ++lt;
       }
     }
@@ -762,7 +952,20 @@ struct F16PrepParams {
   int32_t num_groups, max_rows, mts, tile_cap;
   int32_t wgrad_tiles;  // wgrad: every group's tiles; 0 = forward, dgrad
   int32_t* order;       // wgrad: groups, the largest first
+  uint32_t* units;      // split tiles'
+  int32_t* arrived;
+  int32_t split_pairs;  // pairs that will run; 0 = no tile of this problem is split
+  int32_t ksteps;       // forward, dgrad: steps of the contraction
 };
+
+// Slices of a tile of `steps` steps whose call has a share of `total` / pairs for each
+// pair.  At most 2^31 rows in steps of 64 (wgrad), 2^31 / 64 steps of a row (the
+// others), 48 tiles and 96 pairs: products stay below 2^32.
+__device__ __forceinline__ int f16_slices(uint32_t steps, uint32_t total, uint32_t pairs) {
+  const uint32_t share = steps * pairs / max(total, 1u);
+  if (share < 3 && steps < 4 * kMinSlice) return 1;
+  return int(min(min(share, steps / kMinSlice), uint32_t(kMaxSlices)));
+}
 
 // Token tiles of a group of m rows: the fewest of at most 256 rows, of equal
 // size up to a multiple of 32 (two of 160 and 140 for 300 rows, not 256 and 44:
@@ -788,16 +991,21 @@ __global__ void __launch_bounds__(256) f16_prepare_kernel(const __grid_constant_
   __shared__ int32_t sbegin[FGG_MAX_GROUPS + 1];  // first tile (per M tile) in that order
   __shared__ int32_t swarp[8];
   __shared__ int s_bad;
+  __shared__ int s_steps;  // wgrad: of all groups
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int G = p.num_groups;
-  if (threadIdx.x == 0) s_bad = 0;
+  if (threadIdx.x == 0) s_bad = s_steps = 0;
   for (int i = threadIdx.x; i <= G; i += 256) soff[i] = __ldg(p.offsets + i);
+  if (p.split_pairs > 0 && blockIdx.x == 0)
+    for (int i = threadIdx.x; i < kMaxSplitUnits * kWarpSums / 4; i += 256)
+      reinterpret_cast<int4*>(p.arrived)[i] = make_int4(0, 0, 0, 0);
   __syncthreads();
   for (int g = threadIdx.x; g < G; g += 256) {
     const int lo = soff[g], hi = soff[g + 1];
     const bool bad = lo < 0 || hi < lo || hi > p.max_rows;
     srows[g] = bad ? 0 : hi - lo;
     if (bad) s_bad = 1;
+    if (p.wgrad_tiles > 0 && p.split_pairs > 0 && !bad) atomicAdd(&s_steps, wgrad_steps(hi - lo));
   }
   __syncthreads();
   for (int g = threadIdx.x; g < G; g += 256) {
@@ -845,6 +1053,23 @@ __global__ void __launch_bounds__(256) f16_prepare_kernel(const __grid_constant_
       p.status[1] = 0;
       p.status[2] = 0;
       p.status[3] = num_tiles;
+      // the longest tiles come first in the list, so that those to split lead it
+      int tiles = 0, units = 0;
+      const bool wgrad = p.wgrad_tiles > 0;
+      const int per = wgrad ? p.wgrad_tiles / G : num_tiles;
+      while (tiles < num_tiles && per <= p.split_pairs / 2) {
+        const uint32_t steps = wgrad ? wgrad_steps(srows[sorder[tiles / per]]) : p.ksteps;
+        const int slices =
+            f16_slices(steps, (wgrad ? uint32_t(s_steps) : steps) * per, p.split_pairs);
+        if (slices < 2) break;
+        for (int t = 0; t < per; ++t) {
+          for (int i = 0; i < slices; ++i) p.units[units + i] = split_word(tiles, i, slices, units);
+          ++tiles;
+          units += slices;
+        }
+      }
+      p.status[4] = tiles;
+      p.status[5] = units;
     }
     if (p.wgrad_tiles > 0)
       for (int r = threadIdx.x; r < G; r += 256) p.order[r] = sorder[r];
@@ -896,6 +1121,8 @@ __global__ void __launch_bounds__(256) f16_prepare_kernel(const __grid_constant_
 struct F16Layout {
   int mts = 0, cts = 0, tile_cap = 0;
   size_t status = 0, order = 0, tiles = 0, tile_rows = 0, tail_a = 0, tail_b = 0, total = 0;
+  size_t units = 0, arrived = 0, partial = 0;
+  int max_slices = 1;  // of a tile
 };
 
 int plan_f16(const FggF16RowsProblem* p, int direction, F16Layout* L) {
@@ -937,15 +1164,28 @@ int plan_f16(const FggF16RowsProblem* p, int direction, F16Layout* L) {
   // the tile counter runs past the last tile by one claim per pair
   if (cap > INT32_MAX - 4096) return set_error(FGG_EBADSHAPE, "problem too large");
   L->tile_cap = int(cap);
+  // The fewest tiles of a call are those of one group, in wgrad with all the rows; more
+  // than half as many as pairs, or short ones, are never split.
+  const int least = direction == kWgrad ? L->mts * L->cts : L->mts;
+  const int64_t steps = direction == kWgrad ? int64_t(p->max_rows) / 64 + 2
+                                            : ((direction == kFwd ? p->k : p->n) + 63) / 64;
+  if (least * 2 <= kMaxSplitUnits)
+    L->max_slices = int(std::max<int64_t>(1, std::min<int64_t>(steps / kMinSlice, kMaxSlices)));
+  if (L->max_slices > 1) {
+    L->units = cv.take(kMaxSplitUnits * 4, 256);
+    L->arrived = cv.take(kMaxSplitUnits * kWarpSums * 4, 256);
+    const int64_t units = std::min<int64_t>(cap * L->max_slices, kMaxSplitUnits);
+    L->partial = cv.take(size_t(units) * kUnitFloats * 4, 256);
+  }
   L->total = cv.off;
   return FGG_OK;
 }
 
 constexpr CUtensorMapDataType kMap16 = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;  // moved as bits
 
-template <int MODE>
+template <int MODE, bool SPLIT>
 int launch_f16(const F16Params& gp, const DeviceInfo& dev, cudaStream_t s) {
-  using C = F16Cfg<MODE>;
+  using C = F16Cfg<MODE, SPLIT>;
   if (int rc = ensure_max_dynamic_smem(reinterpret_cast<const void*>(f16_pair_kernel<C>),
                                        int(C::SMEM_BYTES)))
     return rc;
@@ -963,7 +1203,7 @@ int launch_f16(const F16Params& gp, const DeviceInfo& dev, cudaStream_t s) {
       return set_error(FGG_ECUDA, "the kernel was built with %d registers per thread, needs %d",
                        regs, (C::REGS_TOTAL + C::THREADS - 1) / C::THREADS);
   }
-  const int pairs = std::max(1, std::min(gp.grid_tiles, dev.sm_count / 2));
+  const int pairs = std::max(1, std::min(gp.grid_units, dev.sm_count / 2));
   const cudaError_t e = launch_pdl(f16_pair_kernel<C>, dim3(2 * pairs), dim3(C::THREADS),
                                    C::SMEM_BYTES, s, gp);
   if (e != cudaSuccess) return set_error(FGG_ECUDA, "GEMM launch failed: %s", cudaGetErrorString(e));
@@ -1026,10 +1266,19 @@ int fgg_f16_grouped_gemm_rows(const FggF16RowsProblem* p, int32_t direction, voi
   pp.max_rows = p->max_rows;
   pp.mts = gp.mts = L.mts;
   gp.cts = L.cts;
-  pp.tile_cap = gp.grid_tiles = L.tile_cap;
+  pp.tile_cap = L.tile_cap;
+  gp.grid_units = int(std::min<int64_t>(int64_t(L.tile_cap) * L.max_slices, INT32_MAX));
   gp.bf16 = p->dtype == 1 ? 1 : 0;
   gp.out = p->out;
   gp.debug_flags = debug_flags();
+  if (L.max_slices > 1) {
+    pp.units = reinterpret_cast<uint32_t*>(ws + L.units);
+    pp.arrived = reinterpret_cast<int32_t*>(ws + L.arrived);
+    pp.split_pairs = std::min(std::min(gp.grid_units, dev.sm_count / 2), kMaxSplitUnits);
+    gp.units = pp.units;
+    gp.arrived = pp.arrived;
+    gp.partial = reinterpret_cast<float*>(ws + L.partial);
+  }
   int blocks;
   if (direction == kWgrad) {
     pp.a = static_cast<const uint4*>(p->a);
@@ -1065,13 +1314,16 @@ int fgg_f16_grouped_gemm_rows(const FggF16RowsProblem* p, int32_t direction, voi
     gp.tiles = pp.tiles;
     gp.tile_rows = pp.tile_rows;
     gp.m_ext = direction == kFwd ? p->n : p->k;
-    gp.ksteps = int((ck + 63) / 64);
+    gp.ksteps = pp.ksteps = int((ck + 63) / 64);
     blocks = std::min((L.tile_cap + 255) / 256, dev.sm_count);
   }
   FGG_CUDA_CHECK(launch_dependent(f16_prepare_kernel, std::max(blocks, 1), 0, s, pp));
-  if (direction == kFwd) return launch_f16<kFwd>(gp, dev, s);
-  if (direction == kDgrad) return launch_f16<kDgrad>(gp, dev, s);
-  return launch_f16<kWgrad>(gp, dev, s);
+  const bool split = L.max_slices > 1;
+  if (direction == kFwd)
+    return split ? launch_f16<kFwd, true>(gp, dev, s) : launch_f16<kFwd, false>(gp, dev, s);
+  if (direction == kDgrad)
+    return split ? launch_f16<kDgrad, true>(gp, dev, s) : launch_f16<kDgrad, false>(gp, dev, s);
+  return split ? launch_f16<kWgrad, true>(gp, dev, s) : launch_f16<kWgrad, false>(gp, dev, s);
 }
 
 }  // extern "C"

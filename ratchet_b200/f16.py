@@ -81,8 +81,10 @@ def grouped_gemm_rows(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, *
             kernel on the stream -- the host never reads it
     out     optional contiguous [R, N] of the same type; rows outside every
             group are left as they are (in a new tensor they are undefined)
-    Sums are held in fp32 and rounded once.  Malformed offsets write nothing and
-    make last_status() raise."""
+    Sums are held in fp32 and rounded once.  A call's results do not vary; a call of
+    few tiles splits its sums over the GPU, so that the same rows may differ in the
+    last bits between calls with other groups beside them.  Malformed offsets write
+    nothing and make last_status() raise."""
     rows, k = _tokens("x", x)
     G = _offsets(offsets, x.device)
     n, kw = _weights(w, x.dtype, x.device, G)

@@ -74,6 +74,30 @@ def test_f16_workspace_bytes(L):
             == 512 + up(3 * 16 * 264 * 2) + 3 * 16 * 520 * 2)
 
 
+@pytest.mark.parametrize("groups,n,k,rows,direction,units", [
+    (1, 256, 4096, 1, 0, 2),          # one tile of 64 steps: two slices of 32
+    (1, 256, 8192, 256, 0, 8),        # of at most 256 / 256 + 1 token tiles
+    (4, 264, 4096, 300, 0, 20),       # at most 5 token tiles x 2
+    (1, 256, 32768, 1, 0, 16),        # at most 16 slices
+    (9, 256, 65536, 4000, 0, 96),     # at most 96 units
+    (1, 256, 4032, 1, 0, 0),          # 63 steps
+    (1, 48 * 256 + 8, 8192, 1, 0, 0),  # 49 tiles or more in every call
+    (1, 4096, 256, 1, 1, 2),
+    (1, 64, 64, 30000, 2, 14),
+    (1, 2056, 1288, 30000, 2, 0),     # 54 tiles
+])
+def test_f16_workspace_of_split_tiles(L, groups, n, k, rows, direction, units):
+    """What units of 256 KB each, their list and the joins' counters add."""
+    up = lambda x: (x + 255) // 256 * 256
+    if direction == 2:
+        base = 256 + up(4 * groups) + up(groups * 16 * n * 2) + groups * 16 * k * 2
+    else:
+        tiles = min(rows // 256 + groups, rows) * -(-(n if direction == 0 else k) // 256)
+        base = 256 + up(8 * tiles) + 4 * tiles
+    want = base if units == 0 else up(base) + up(96 * 4) + 96 * 16 * 4 + units * 256 * 1024
+    assert L.fgg_f16_rows_workspace_bytes(_f16(groups, n, k, rows), direction) == want
+
+
 def test_f16_python_refusals():
     x = torch.zeros(4, 64, dtype=torch.bfloat16)
     w = torch.zeros(2, 32, 64, dtype=torch.bfloat16)

@@ -117,6 +117,68 @@ def test_wgrad_chunks(cuda_device, rows):
     _check_wgrad(dy, x, dw, off)
 
 
+SPLIT = [
+    # sizes, n, k, spare rows: calls of few tiles, or of a few long ones, in which tiles
+    # are cut along the contraction.  A slice's sum has fewer additions than the whole,
+    # and at most four join it to the others: the bound above still holds.
+    ([1], 256, 4096, 0),                 # one token, one tile
+    ([0, 1, 0, 0], 4096, 2056, 3),       # contraction not a multiple of a step
+    ([33, 0, 256], 264, 5128, 0),        # tiles over the output's edge, all columns
+    ([300], 520, 2048, 2),               # several token tiles
+    ([5000], 64, 64, 0),                 # one small gradient over many rows
+    ([4999, 0, 3, 70], 136, 264, 7),     # one of four, with rows left over a sixteen
+    ([2100, 9000, 2099], 72, 8, 1),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("case", range(len(SPLIT)))
+def test_few_tiles(cuda_device, case, dtype):
+    """Right, and the same bits however the slices' ends fall: again and again, and in
+    a captured graph."""
+    import ratchet_b200 as rb
+
+    sizes, n, k, spare = SPLIT[case]
+    x, dy, w, offsets, off = _problem(cuda_device, sizes, n, k, dtype, spare, seed=case)
+    start = torch.randn(len(sizes), n, k, device=cuda_device)
+    outs = [torch.full((x.shape[0], n), 7.0, dtype=dtype, device=cuda_device),
+            torch.full((x.shape[0], k), 7.0, dtype=dtype, device=cuda_device),
+            torch.empty(len(sizes), n, k, device=cuda_device),
+            torch.empty(len(sizes), n, k, dtype=dtype, device=cuda_device), start.clone()]
+
+    def run():
+        rb.grouped_gemm_rows(x, w, offsets, out=outs[0])
+        rb.grouped_gemm_rows_dgrad(dy, w, offsets, out=outs[1])
+        rb.grouped_gemm_rows_wgrad(dy, x, offsets, out=outs[2])
+        rb.grouped_gemm_rows_wgrad(dy, x, offsets, out=outs[3])
+        outs[4].copy_(start)
+        rb.grouped_gemm_rows_wgrad(dy, x, offsets, out=outs[4], accumulate=True)
+
+    run()
+    rb.last_status()
+    _check_fwd(x, w, outs[0], off)
+    _check_dgrad(dy, w, outs[1], off)
+    _check_wgrad(dy, x, outs[2], off)
+    _check_wgrad(dy, x, outs[3], off)
+    _check_wgrad(dy, x, outs[4], off, start)
+    for o in outs[:2]:
+        assert bool((o[off[-1]:] == 7.0).all())
+    first = [o.clone() for o in outs]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run()
+    for i in range(20):
+        for o in outs:
+            o.fill_(float("nan"))
+        if i < 10:
+            run()
+        else:
+            graph.replay()
+        rb.last_status()
+        for o, f, r in zip(outs, first, [off[-1], off[-1], None, None, None]):
+            assert torch.equal(o[:r], f[:r])
+
+
 def test_wgrad_long_sums_do_not_drift(cuda_device):
     """16384 rows of one sign, where truncating additions would lose the most: 16384 / 16
     of them 2^-24 each on average, 6e-5 of the sum.  With 512 rows to a chunk it is at
