@@ -179,6 +179,38 @@ def test_few_tiles(cuda_device, case, dtype):
             assert torch.equal(o[:r], f[:r])
 
 
+def test_few_tiles_on_two_streams(cuda_device):
+    """Two streams' calls at once, each with sums of its own; then offsets that are
+    malformed in a call whose tiles would be split."""
+    import ratchet_b200 as rb
+
+    cases = [_problem(cuda_device, [2000 + 900 * i, 0, 3], 72, 328, torch.bfloat16, seed=i)
+             for i in range(2)]
+    want = [rb.grouped_gemm_rows_wgrad(dy, x, off) for x, dy, _, off, _ in cases]
+    rb.last_status()
+    for (x, dy, _, _, off), w in zip(cases, want):
+        _check_wgrad(dy, x, w, off)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(20):
+        for i, (st, (x, dy, _, off, _)) in enumerate(zip(streams, cases)):
+            with torch.cuda.stream(st):
+                got[i].append(rb.grouped_gemm_rows_wgrad(dy, x, off))
+    torch.cuda.synchronize()
+    for gs, w in zip(got, want):
+        assert all(torch.equal(g, w) for g in gs)
+    x, dy = cases[0][:2]
+    out = torch.full((3, 72, 328), 7.0, device=cuda_device)
+    bad = torch.tensor([0, 2000, 1000, x.shape[0]], dtype=torch.int32, device=cuda_device)
+    rb.grouped_gemm_rows_wgrad(dy, x, bad, out=out)
+    with pytest.raises(rb.FggError):
+        rb.last_status()
+    assert bool((out == 7.0).all())
+    assert torch.equal(rb.grouped_gemm_rows_wgrad(dy, x, cases[0][3]), want[0])
+    rb.last_status()
+
+
 def test_wgrad_long_sums_do_not_drift(cuda_device):
     """16384 rows of one sign, where truncating additions would lose the most: 16384 / 16
     of them 2^-24 each on average, 6e-5 of the sum.  With 512 rows to a chunk it is at
