@@ -305,9 +305,11 @@ FGG_API int fgg_mxfp4_grouped_gemm_rows(const FggMxfp4RowsProblem* p, const void
  *                         to what out holds.
  * N and K are multiples of 8; every tensor is contiguous and 16-byte aligned.
  * Sums are held in fp32 and rounded once (fp16 results past 65504 become
- * infinite).  A call's results do not vary; as a call of few tiles splits its sums
- * over the GPU, the same rows may differ in the last fp32 bits, before that rounding,
- * between calls with other groups beside them.  Rows outside every group are neither read for any output nor
+ * infinite).  A call's results do not vary.  A call of few tiles, or of a few long
+ * ones, splits their sums over the GPU: the same rows may differ in the last fp32
+ * bits, before that rounding, between calls whose other groups have other rows
+ * (empty groups and spare rows change nothing), and between GPUs with other
+ * numbers of SMs.  Rows outside every group are neither read for any output nor
  * written.  Malformed offsets (decreasing, negative, past max_rows) run no
  * tile and leave status 0x203 in the workspace. */
 typedef struct FggF16RowsProblem {

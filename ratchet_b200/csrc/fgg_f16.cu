@@ -38,7 +38,7 @@
 // sums are joined two by two: of two neighbours the warp that is done first leaves its
 // sums in the workspace and goes on, the other adds them to its own and stands for
 // both.  Nothing waits, and as a + b = b + a the results do not depend on timing.  They
-// may depend, in the last fp32 bits before the rounding, on the call's number of tiles.
+// may depend, in the last fp32 bits before the rounding, on the call's other tiles.
 //
 // What bounds it: the tensor pipe for groups of about 250 tokens and more, the
 // weights' HBM stream below that, shared-memory bandwidth and the gradient's write
@@ -83,13 +83,16 @@ struct F16Slot {
 };
 static_assert(sizeof(F16Slot) == 32, "slot is 8 words");
 
-// A tile is split if a pair's share of the call's steps is at most half of its own,
-// into slices of about that share: the units of split tiles are at most as many as
-// pairs.  A join costs 4 to 5 us, up to 9 where all pairs join at once after few
-// steps, and a step about 0.26 us of a pair.  Unsplit -> split, cold L2: one tile of 64
-// steps in two (a gradient of 64 x 64 over 4096 rows) 30.5 -> 26.4 us, of 128 in four
-// (one token, K 8192) 34.2 -> 22.6; 470 steps in 14 (30000 rows) 143 -> 36; 32 tiles of 64
-// in two, which is not done, 36.9 -> 41.5, of 128 in two 53.2 -> 47.1.  Slices of at least
+// A tile is split if a pair's share of the call's steps (over all pairs of the GPU, so
+// that neither spare rows nor empty groups count) is at most half of the tile's own, and
+// for a tile of fewer than 4 kMinSlice steps at most a fifth; into slices of about that
+// share, of at least kMinSlice steps: the units of split tiles are at most as many as
+// pairs.  A join costs 4 to 5 us, up to 9 where all pairs join at once after few steps,
+// and a step about 0.26 us of a pair.  Unsplit -> split, cold L2, a host call's time with
+// it: one tile of 64 steps in two (a gradient of 64 x 64 over 4096 rows) 31.7 -> 27.6 us,
+// 8 of them (one token, 2048 x 4096) 25.1 -> 23.9, 16 of them 25.9 -> 27.0, 24 of them
+// (256 tokens) 36.3 -> 39.0; one of 128 in four (one token, K 8192) 34.1 -> 23.7; of 470
+// in 14 (30000 rows) 144 -> 38; 32 tiles of 128 in two 53.2 -> 47.1.  Slices of at least
 // 16 steps: 25.4 -> 31.6 us for 16 tiles of 32; of 64: 143 -> 44 for the 30000 rows.
 constexpr int kMaxSplitUnits = 96;
 constexpr int kMaxSlices = 16;
@@ -954,7 +957,7 @@ struct F16PrepParams {
   int32_t* order;       // wgrad: groups, the largest first
   uint32_t* units;      // split tiles'
   int32_t* arrived;
-  int32_t split_pairs;  // pairs that will run; 0 = no tile of this problem is split
+  int32_t split_pairs;  // the GPU's pairs; 0 = no tile of this problem is split
   int32_t ksteps;       // forward, dgrad: steps of the contraction
 };
 
@@ -963,7 +966,7 @@ struct F16PrepParams {
 // others), 48 tiles and 96 pairs: products stay below 2^32.
 __device__ __forceinline__ int f16_slices(uint32_t steps, uint32_t total, uint32_t pairs) {
   const uint32_t share = steps * pairs / max(total, 1u);
-  if (share < 3 && steps < 4 * kMinSlice) return 1;
+  if (share < 5 && steps < 4 * kMinSlice) return 1;
   return int(min(min(share, steps / kMinSlice), uint32_t(kMaxSlices)));
 }
 
@@ -1274,7 +1277,9 @@ int fgg_f16_grouped_gemm_rows(const FggF16RowsProblem* p, int32_t direction, voi
   if (L.max_slices > 1) {
     pp.units = reinterpret_cast<uint32_t*>(ws + L.units);
     pp.arrived = reinterpret_cast<int32_t*>(ws + L.arrived);
-    pp.split_pairs = std::min(std::min(gp.grid_units, dev.sm_count / 2), kMaxSplitUnits);
+    // all of the GPU's pairs: a tile's slices are at most max_slices whatever its share, so
+    // that the units stay within grid_units and `partial`
+    pp.split_pairs = std::min(dev.sm_count / 2, kMaxSplitUnits);
     gp.units = pp.units;
     gp.arrived = pp.arrived;
     gp.partial = reinterpret_cast<float*>(ws + L.partial);

@@ -83,7 +83,8 @@ def grouped_gemm_rows(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, *
             group are left as they are (in a new tensor they are undefined)
     Sums are held in fp32 and rounded once.  A call's results do not vary; a call of
     few tiles splits its sums over the GPU, so that the same rows may differ in the
-    last bits between calls with other groups beside them.  Malformed offsets write
+    last bits between calls whose other groups have other rows (empty groups and
+    spare rows change nothing).  Malformed offsets write
     nothing and make last_status() raise."""
     rows, k = _tokens("x", x)
     G = _offsets(offsets, x.device)
