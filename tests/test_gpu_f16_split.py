@@ -86,8 +86,22 @@ def _split(ws):
 CASES = [
     # direction, sizes, n, k, spare rows, tiles cut, units
     (FWD, [1], 256, 4096, 0, 1, 2),               # one token, one tile of 64 steps
+    (FWD, [33], 256, 6144, 2, 1, 3),
+    (FWD, [1, 0, 200], 264, 8192, 0, 4, 16),      # a second tile of 8 columns
+    (FWD, [250], 520, 10240, 5, 3, 15),
+    (FWD, [3], 8, 14336, 0, 1, 7),
+    (FWD, [256, 70], 256, 32768, 0, 2, 32),
     (DGRAD, [1], 4096, 256, 0, 1, 2),
+    (DGRAD, [9], 6144, 520, 3, 3, 9),
+    (DGRAD, [0, 31, 200], 10248, 264, 0, 4, 20),  # the contraction ends inside a step
+    (DGRAD, [2], 14336, 72, 0, 1, 7),
+    (DGRAD, [130], 32776, 8, 1, 1, 16),
     (WGRAD, [4096], 64, 64, 0, 1, 2),             # a gradient of one tile
+    (WGRAD, [6150], 72, 8, 0, 1, 3),
+    (WGRAD, [10247], 264, 8, 4, 2, 10),
+    (WGRAD, [7, 14336, 0], 136, 72, 0, 1, 7),
+    (WGRAD, [33001], 8, 520, 0, 3, 48),
+    (WGRAD, [9000, 100, 9001], 72, 136, 0, 2, 8),  # two of three groups
 ]
 
 
@@ -144,3 +158,36 @@ def test_spare_rows_and_empty_groups_change_nothing(cuda_device, direction, m, n
         got = r.call(direction)[0]
         assert torch.equal(got[g] if direction == WGRAD else got[:m],
                            want[0] if direction == WGRAD else want)
+
+
+def test_split_calls_on_two_streams(cuda_device):
+    """Two streams' split calls at once, each on its own sums."""
+    if _pairs(cuda_device) != 74:
+        pytest.skip("the counts are those of 148 SMs")
+    cases = [_Problem(cuda_device, [9000 + 900 * i, 0, 3], 72, 328, torch.bfloat16, seed=i)
+             for i in range(2)]
+    want = []
+    for q in cases:
+        out, ws = q.call(WGRAD)
+        assert _split(ws) == (0, 2, 8)
+        q.check(WGRAD, out)
+        want.append(out)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(20):
+        for i, (st, q) in enumerate(zip(streams, cases)):
+            with torch.cuda.stream(st):
+                got[i].append(q.call(WGRAD))
+    torch.cuda.synchronize()
+    for outs, w in zip(got, want):
+        for o, ws in outs:
+            assert _split(ws) == (0, 2, 8) and torch.equal(o, w)
+
+
+def test_malformed_offsets_of_a_call_that_would_split(cuda_device):
+    q = _Problem(cuda_device, [9000, 0, 3], 72, 328, torch.bfloat16)
+    bad = torch.tensor([0, 9000, 8000, 9003], dtype=torch.int32, device=cuda_device)
+    out, ws = q.call(WGRAD, off=bad)
+    assert _split(ws) == (0x203, 0, 0) and bool((out == 7.0).all())
+    q.check(WGRAD, q.call(WGRAD)[0])
