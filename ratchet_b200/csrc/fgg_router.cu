@@ -22,7 +22,8 @@
 // tokens and their instructions for many.  Measured, one call of a replayed graph:
 // 24 x 64 fp32 2.8 us; 4096 x 256 fp32 sigmoid 5.4 us, with a bias 10 us (one
 // token in some hundred needs 64-bit keys, and the kernel waits for the last);
-// gradient of 32768 x 64 bf16 softmax 8.4 us (its 10.5 MB take 1.6 us of HBM).
+// gradient of 32768 x 64 bf16, whole softmax, top 8, 7.4 us (its 10.5 MB take 1.6 us of
+// HBM), of 8 normalised weights 8.8.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -350,23 +351,30 @@ __global__ void __launch_bounds__(32 * kRouterWarps)
 
 // dlogits from dweights.  With c_j the share of route j,
 //   softmax, normalised over the chosen   c_j = w_j sum_i w_i (dw_j - dw_i)
-//   softmax                               c_j = s_j dw_j
 //   sigmoid, normalised                   c_j = w_j sum_i w_i (dw_j - dw_i) (1 - s_j)
 //   sigmoid                               c_j = dw_j s_j (1 - s_j)
-// (w normalised, without the scale), dl_e = sum of c_j over the routes to e,
-// minus s_e sum_j c_j for the whole softmax.
-template <typename T, int L, int V, bool kSoftmax>
+// (w normalised, without the scale), dl_e = sum of c_j over the routes to e.  For the
+// whole softmax, with D_e the sum of dw_j over the routes to e,
+//   e not chosen   dl_e = -s_e sum_f s_f D_f                          f over the chosen
+//   e chosen       dl_e = s_e [ D_e (1 - sum_f s_f) + sum_f s_f (D_e - D_f) ]
+// and 1 - sum_f s_f summed over the experts that are not chosen: where one expert has
+// nearly all the score, s_e D_e - s_e sum_f s_f D_f would be the rounding of both.
+// kDense (softmax without renormalisation): every expert's logit has a gradient.
+template <typename T, int L, int V, bool kSoftmax, bool kDense>
 __global__ void __launch_bounds__(32 * kRouterWarps)
     router_backward_kernel(const __grid_constant__ RouterParams p) {
   constexpr int kTokens = kRouterWarps * 32 / L;
   constexpr int R = (kRouterMaxTopk + L - 1) / L;
   __shared__ int2 s_share[kTokens][kRouterMaxTopk];  // each route's (weight, dw), (expert, share)
+  static_assert(kSoftmax || !kDense, "a sigmoid's gradient is the chosen ones' own");
+  // kDense: the chosen experts' gradients, each in its expert's place
+  __shared__ float s_chosen[kDense ? kTokens : 1][kDense ? L * V : 1];
   const int sub = threadIdx.x & (L - 1);
   const int slot = int(threadIdx.x) / L;
   const int64_t t = int64_t(blockIdx.x) * kTokens + slot;
   const bool live = t < p.tokens;
   const T* const row = static_cast<const T*>(p.logits) + (live ? t : 0) * p.experts;
-  const bool dense = kSoftmax && !p.renorm;  // every expert's logit has a gradient
+  const bool renorm = kSoftmax ? !kDense : p.renorm != 0;
   int id[R];
   float dw[R], lr[R], c[R];
 #pragma unroll
@@ -385,7 +393,7 @@ __global__ void __launch_bounds__(32 * kRouterWarps)
   }
   float d[V];
   float m = 0.0f, total = 1.0f;
-  if (dense) {
+  if constexpr (kDense) {
     load_logits<T, V>(row, sub * V, p.experts, live, p.vec != 0, d);
     m = kNegInf;
 #pragma unroll
@@ -401,21 +409,89 @@ __global__ void __launch_bounds__(32 * kRouterWarps)
   }
 #pragma unroll
   for (int r = 0; r < R; ++r) lr[r] = id[r] >= 0 ? to_f32<T>(row[id[r]]) : kNegInf;
-  float whole = 0.0f;
-  if (dense) {
+  if constexpr (kDense) {
+    // a masked expert has no score: its routes are absent
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      c[r] = id[r] >= 0 && lr[r] != kNegInf ? expf(lr[r] - m) / total * dw[r] : 0.0f;
-      whole += c[r];
+      const int j = r * L + sub;
+      if (lr[r] == kNegInf) {
+        id[r] = -1;
+        dw[r] = 0.0f;
+      }
+      if (j < p.topk) s_share[slot][j] = make_int2(id[r], __float_as_int(dw[r]));
     }
-    whole = sub_sum<L>(whole);
+    __syncwarp();
+    uint32_t chosen = 0, twice = 0;  // of this lane's experts
+    for (int i = 0; i < p.topk; ++i) {
+      const unsigned at = unsigned(s_share[slot][i].x - sub * V);  // large for an absent route
+      const uint32_t bit = at < unsigned(V) ? 1u << (at & 31u) : 0u;
+      twice |= chosen & bit;
+      chosen |= bit;
+    }
+    // D of this lane's routes; an expert's first route stands for it
+    float all[R];
+    bool first[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      all[r] = dw[r];
+      first[r] = id[r] >= 0;
+    }
+    if (__any_sync(kFullMask, twice != 0u)) {  // a token of the warp names one twice
+#pragma unroll
+      for (int r = 0; r < R; ++r) all[r] = -0.0f;  // adds nothing, to -0 neither
+      for (int i = 0; i < p.topk; ++i) {  // in the routes' order
+        const int2 q = s_share[slot][i];
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+          if (q.x == id[r]) {
+            all[r] += __int_as_float(q.y);
+            if (i < r * L + sub) first[r] = false;
+          }
+      }
+    }
+    float rest = 0.0f;  // score of the experts that are not chosen
+#pragma unroll
+    for (int i = 0; i < V; ++i) rest += chosen >> i & 1u ? 0.0f : d[i];
     // scores, all zero for a row that is masked whole (total 0), NaN for a NaN total
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+    rest = sub_sum<L>(rest) * inv;
+    float whole = 0.0f;
+    __syncwarp();  // s_share is written over
 #pragma unroll
-    for (int i = 0; i < V; ++i) d[i] = -(d[i] * inv) * whole;
+    for (int r = 0; r < R; ++r) {
+      const int j = r * L + sub;
+      c[r] = 0.0f;
+      if (r * L < p.topk && first[r]) {
+        c[r] = expf(lr[r] - m) * inv;
+        whole += c[r] * all[r];
+      }
+      if (j < p.topk) s_share[slot][j] = make_int2(__float_as_int(c[r]), __float_as_int(all[r]));
+    }
+    whole = sub_sum<L>(whole);
+    __syncwarp();
+    float to[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) to[r] = rest * all[r];
+    auto differences = [&](auto routes) {  // of a lane
+      for (int i = 0; i < p.topk; ++i) {
+        const int2 q = s_share[slot][i];
+#pragma unroll
+        for (int r = 0; r < decltype(routes)::value; ++r)
+          to[r] = fmaf(__int_as_float(q.x), all[r] - __int_as_float(q.y), to[r]);
+      }
+    };
+    if (p.topk <= L) differences(std::integral_constant<int, 1>());
+    else differences(std::integral_constant<int, R>());
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      if (first[r]) s_chosen[slot][id[r]] = c[r] * to[r];
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      d[i] = chosen >> i & 1u ? s_chosen[slot][sub * V + i] : -(d[i] * inv) * whole;
   } else {
     float mj = kNegInf, sum = 0.0f;
-    if (p.renorm) {
+    if (renorm) {
 #pragma unroll
       for (int r = 0; r < R; ++r) mj = fmaxf(mj, lr[r]);
       mj = sub_max<L>(mj);
@@ -450,7 +526,7 @@ __global__ void __launch_bounds__(32 * kRouterWarps)
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const float x = expf(-fabsf(lr[r]));
-      if (p.renorm) {
+      if (renorm) {
         // 1 - sigmoid(l)
         if (!kSoftmax && id[r] >= 0) c[r] *= lr[r] >= 0.0f ? x / (1.0f + x) : 1.0f / (1.0f + x);
       } else {
@@ -460,20 +536,22 @@ __global__ void __launch_bounds__(32 * kRouterWarps)
 #pragma unroll
     for (int i = 0; i < V; ++i) d[i] = 0.0f;
   }
+  if constexpr (!kDense) {
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const int j = r * L + sub;
-    if (j < p.topk) s_share[slot][j] = make_int2(id[r], __float_as_int(c[r]));
-  }
-  __syncwarp();
-  // in the routes' order, so that an expert named twice always gets the same sum
-  for (int j = 0; j < p.topk; ++j) {
-    const int2 q = s_share[slot][j];
-    const int at = q.x - sub * V;
-    if (q.x >= 0 && at >= 0 && at < V) {
+    for (int r = 0; r < R; ++r) {
+      const int j = r * L + sub;
+      if (j < p.topk) s_share[slot][j] = make_int2(id[r], __float_as_int(c[r]));
+    }
+    __syncwarp();
+    // in the routes' order, so that an expert named twice always gets the same sum
+    for (int j = 0; j < p.topk; ++j) {
+      const int2 q = s_share[slot][j];
+      const int at = q.x - sub * V;
+      if (q.x >= 0 && at >= 0 && at < V) {
 #pragma unroll
-      for (int i = 0; i < V; ++i)
-        if (i == at) d[i] += __int_as_float(q.y);
+        for (int i = 0; i < V; ++i)
+          if (i == at) d[i] += __int_as_float(q.y);
+      }
     }
   }
   store_logits<T, V>(static_cast<T*>(p.dlogits) + (live ? t : 0) * p.experts, sub * V, p.experts,
@@ -481,14 +559,14 @@ __global__ void __launch_bounds__(32 * kRouterWarps)
 }
 
 // Lanes per token and experts per lane by the number of experts.
-template <typename T, bool kSoftmax, bool kBackward>
+template <typename T, bool kSoftmax, bool kBackward, bool kDense = false>
 cudaError_t launch_router(const RouterParams& p, cudaStream_t s) {
   auto go = [&](auto lanes, auto values) {
     constexpr int L = decltype(lanes)::value, V = decltype(values)::value;
     constexpr int kTokens = kRouterWarps * 32 / L;
     const int blocks = int((int64_t(p.tokens) + kTokens - 1) / kTokens);
     if constexpr (kBackward)
-      router_backward_kernel<T, L, V, kSoftmax><<<blocks, 32 * kRouterWarps, 0, s>>>(p);
+      router_backward_kernel<T, L, V, kSoftmax, kDense><<<blocks, 32 * kRouterWarps, 0, s>>>(p);
     else
       router_kernel<T, L, V, kSoftmax><<<blocks, 32 * kRouterWarps, 0, s>>>(p);
   };
@@ -506,16 +584,17 @@ bool rows_of_vectors(const void* a, const void* b, int experts, int dtype) {
   return experts % (dtype == 0 ? 4 : 8) == 0 && aligned16(a) && aligned16(b);
 }
 
+template <typename T, bool kBackward>
+cudaError_t launch_router(const RouterParams& p, bool softmax, cudaStream_t s) {
+  if (!softmax) return launch_router<T, false, kBackward>(p, s);
+  if (kBackward && !p.renorm) return launch_router<T, true, kBackward, kBackward>(p, s);
+  return launch_router<T, true, kBackward>(p, s);
+}
 template <bool kBackward>
 cudaError_t launch_router(const RouterParams& p, int dtype, bool softmax, cudaStream_t s) {
-  if (dtype == 0)
-    return softmax ? launch_router<float, true, kBackward>(p, s)
-                   : launch_router<float, false, kBackward>(p, s);
-  if (dtype == 1)
-    return softmax ? launch_router<__nv_bfloat16, true, kBackward>(p, s)
-                   : launch_router<__nv_bfloat16, false, kBackward>(p, s);
-  return softmax ? launch_router<__half, true, kBackward>(p, s)
-                 : launch_router<__half, false, kBackward>(p, s);
+  if (dtype == 0) return launch_router<float, kBackward>(p, softmax, s);
+  if (dtype == 1) return launch_router<__nv_bfloat16, kBackward>(p, softmax, s);
+  return launch_router<__half, kBackward>(p, softmax, s);
 }
 
 int check_router(const void* logits, int dtype, int tokens, int experts, int topk, int score) {

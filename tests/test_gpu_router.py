@@ -314,3 +314,53 @@ def test_no_tokens(cuda_device):
     assert ids.shape == (0, 2) and w.shape == (0, 2)
     d = rb.moe_router_backward(w, torch.empty(0, 8, device=cuda_device), ids)
     assert d.shape == (0, 8)
+
+
+@pytest.mark.parametrize("e", [3, 64, 130, 300, 700])
+@pytest.mark.parametrize("lead", [2.0, 18.0, 25.0, 60.0])
+@pytest.mark.parametrize("chosen", [[0], [0, 2], [2, 0], [1, 2], [0, 0, 2], [0, 1, 2]])
+def test_whole_softmax_gradient_where_one_expert_has_nearly_all_the_score(cuda_device, e, lead,
+                                                                         chosen):
+    """dl_i = s_i [ D_i (1 - S) + sum_f s_f (D_i - D_f) ] of a chosen expert (S the chosen
+    ones' score, D an expert's summed dw), -s_i sum_f s_f D_f of another, to a share of the
+    magnitudes of these terms: a score's error twice (its own and that of s_f or 1 - S),
+    a step for each addition over the routes, one for each difference and product."""
+    import ratchet_b200 as rb
+
+    logits = _logits(cuda_device, 2, e, torch.float32, seed=e, std=0.5)
+    logits[:, 0] = logits[:, 1:].max(1).values + lead
+    topk = len(chosen)
+    ids = torch.tensor([chosen, chosen[::-1]], dtype=torch.int32, device=cuda_device)
+    dw = torch.tensor([[1.25, -0.5, 2.0][:topk], [0.75, 0.5, 1.0][:topk]], device=cuda_device)
+    got = rb.moe_router_backward(dw, logits, ids, renormalize=False, scale=0.5).cpu()
+    for r in range(2):
+        l = logits[r].double().tolist()
+        m = max(l)
+        z = [math.exp(v - m) for v in l]
+        total = math.fsum(z)
+        D = {}
+        for f, v in zip(ids[r].tolist(), dw[r].tolist()):
+            D[f] = D.get(f, 0.0) + 0.5 * v
+        rest = math.fsum(v for i, v in enumerate(z) if i not in D) / total
+        tol = (48 + 8 * (m - min(l)) + 4 * e + topk) * 2.0**-24
+        for i in range(e):
+            s = z[i] / total
+            if i in D:
+                terms = [D[i] * rest] + [z[f] / total * (D[i] - D[f]) for f in D]
+            else:
+                terms = [-z[f] / total * D[f] for f in D]
+            want, mag = s * math.fsum(terms), s * math.fsum(abs(v) for v in terms)
+            assert abs(float(got[r, i]) - want) <= tol * mag + 2.0**-126, (r, i, float(got[r, i]), want)
+
+
+def test_whole_softmax_gradient_of_masked_routes(cuda_device):
+    """A route to a masked expert is absent, whatever its dw."""
+    import ratchet_b200 as rb
+
+    logits = _logits(cuda_device, 2, 12, torch.float32, seed=3)
+    logits[:, 5] = -INF
+    ids = torch.tensor([[1, 5, 2], [1, -1, 2]], dtype=torch.int32, device=cuda_device)
+    dw = torch.tensor([[1.0, INF, -2.0]] * 2, device=cuda_device)
+    logits[1] = logits[0]
+    d = rb.moe_router_backward(dw, logits, ids, renormalize=False)
+    assert bool(torch.isfinite(d).all()) and torch.equal(d[0], d[1]) and float(d[0, 5]) == 0.0
