@@ -805,13 +805,14 @@ __global__ void __launch_bounds__(256, 1) fgg_gemm_kernel(const __grid_constant_
 // its completion there: .cta_group::2 TMA), and issues the scale-factor
 // uploads and MMAs.  Commits arrive in both CTAs (empty stages, accumulator
 // ready); each CTA's epilogue drains its own TMEM (its 128 output columns) and
-// tells the leader's acc-empty barrier when it is done.
+// arrives on its own CTA's acc-empty barrier; the follower's otherwise idle warp 1
+// forwards that, and the slots that its readers free, to the leader's barriers.
 // Scale factors: each CTA holds the atoms of its own weight rows and the atoms
 // of all 224 tokens; the leader's tcgen05.cp.cta_group::2 copies each CTA's
 // atoms into that CTA's TMEM.
-// Waits acquire at CTA scope (TMA / tcgen05 completions), except on the
-// schedule ring, whose slots the leader writes into the follower's shared
-// memory: those waits acquire at cluster scope.
+// Waits acquire at CTA scope (TMA / tcgen05 completions), except on barriers
+// that the other CTA's threads arrive on: the schedule ring's, whose slots the
+// leader writes into the follower's shared memory, and the leader's acc-empty ones.
 // ====================================================================
 template <bool MX_, int STAGES_, int KSUB_ = 1, bool MX4_ = false>
 struct PairCfg {
@@ -854,9 +855,11 @@ struct PairCfg {
   static_assert(SF_BASE + NSLOTS * SF_SLOT <= 512, "TMEM columns exceeded");
   static constexpr uint32_t TMEM_COLS = 512;
   static constexpr int SCHED = 8;
-  // readers of a slot: leader producer, MMA thread, 4 epilogue warps; follower
-  // producer and 4 epilogue warps
-  static constexpr uint32_t SCHED_READERS = 11;
+  // arrivals that free a slot: on the leader its producer, MMA warp and 4 epilogue
+  // warps and the follower's forwarding warp; on the follower its producer and 4
+  // epilogue warps
+  static constexpr uint32_t READERS_LEADER = 7;
+  static constexpr uint32_t READERS_FOLLOWER = 5;
   static constexpr uint32_t NBARS = 2 * STAGES + 4 + 2 * SCHED + 3;
   static constexpr uint32_t MISC_BYTES = 8 * NBARS + 32 * SCHED + 16;
   static constexpr uint32_t SF_REGION = SUB_SLOTS * OP_BYTES;
@@ -914,11 +917,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(accf_bar(b), 1);
-      mbar_init(acce_bar(b), 8);  // 4 epilogue warps in each CTA (leader's barrier)
+      mbar_init(acce_bar(b), leader ? 5 : 4);  // 4 epilogue warps; the forwarder
     }
     for (int i = 0; i < C::SCHED; ++i) {
       mbar_init(schedf_bar(i), 1);
-      mbar_init(schede_bar(i), C::SCHED_READERS);  // used on the leader
+      mbar_init(schede_bar(i), leader ? C::READERS_LEADER : C::READERS_FOLLOWER);
     }
     mbar_init(tmem_ready_bar, 1);
     mbar_init(drain_bar, 1);
@@ -952,15 +955,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
   const uint32_t leader_schede0 = mapa_shared(schede_bar(0), 0);
   const uint32_t leader_acce0 = mapa_shared(acce_bar(0), 0);
   const uint32_t leader_full0 = mapa_shared(full_bar(0), 0);
-
-  // release a slot this thread has read: the leader's ring barrier counts the
-  // readers of both CTAs
-  auto release_slot = [&](int slot) {
-    if (leader)
-      mbar_arrive(schede_bar(slot));
-    else
-      mbar_arrive_remote_read(leader_schede0 + 8u * slot);
-  };
 
   if (warp == 3) {
     // ---------------------------------------------- scheduler (leader only)
@@ -1019,7 +1013,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
         const int wgroup = __shfl_sync(kFullMask, ring[slot].wgroup, 0);
         const int row0 = __shfl_sync(kFullMask, ring[slot].row0, 0);
         if (lane == 0) {
-          release_slot(slot);
+          mbar_arrive(schede_bar(slot));
           if (leader) mbar_arrive(taken_bar);
         }
         if (++slot == C::SCHED) {
@@ -1155,8 +1149,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
         if (tile == kEndTile) break;
         const int ncols = tile_ncols(rows);
         const uint32_t b = lt & 1u;
-        if (!mbar_wait(acce_bar(b), ((lt >> 1) & 1u) ^ 1u, abort_flag, p.status,
-                       kStatusTimeoutMma))
+        if (!mbar_wait<true>(acce_bar(b), ((lt >> 1) & 1u) ^ 1u, abort_flag, p.status,
+                             kStatusTimeoutMma))
           break;
         tc_fence_after();
         const uint32_t d_tmem = tmem + b * C::BN;
@@ -1253,6 +1247,39 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
       }
     }
     __syncwarp();
+  } else if (warp == 1) {
+    // ----------------------------------------- forwarder (follower only)
+    // The leader writes this CTA's slots and its MMAs this CTA's accumulators, so
+    // what frees them for it is released at cluster scope.  That waits for the
+    // warp's global stores, so it is done by a warp that has none, once the readers
+    // have arrived here: both arrivals of a tile at once, as each by itself takes
+    // long enough to hold up tiles of few tokens (64 groups, 544 rows, 7168 x 2048:
+    // 88 -> 96 us with one after the other).
+    if (!aborted_early) {
+      int slot = 0;
+      uint32_t sphase = 0;
+      uint32_t lt = 0;
+      while (true) {
+        if (!mbar_wait<true>(schedf_bar(slot), sphase, abort_flag, p.status,
+                             kStatusTimeoutEpilogue))
+          break;
+        const uint32_t tile = __shfl_sync(kFullMask, ring[slot].tile, 0);
+        if (tile == kEndTile) break;
+        const uint32_t b = lt & 1u;
+        if (!mbar_wait(schede_bar(slot), sphase, abort_flag, p.status, kStatusTimeoutEpilogue) ||
+            !mbar_wait(acce_bar(b), (lt >> 1) & 1u, abort_flag, p.status, kStatusTimeoutEpilogue))
+          break;
+        tc_fence_after();
+        tc_fence_before();
+        if (lane < 2) mbar_arrive_remote(lane == 0 ? leader_acce0 + 8u * b : leader_schede0 + 8u * slot);
+        if (++slot == C::SCHED) {
+          slot = 0;
+          sphase ^= 1;
+        }
+        ++lt;
+      }
+    }
+    __syncwarp();
   } else if (warp >= 4 && !aborted_early) {
     // --------------------------------------------------------- epilogue
     const int q = warp & 3;
@@ -1268,7 +1295,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
         break;
       const SchedSlot s = read_slot(ring, slot);
       __syncwarp();
-      if (lane == 0) release_slot(slot);
+      if (lane == 0) mbar_arrive(schede_bar(slot));
       if (++slot == C::SCHED) {
         slot = 0;
         sphase ^= 1;
@@ -1290,12 +1317,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
                       epi_stage);
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) {
-        if (leader)
-          mbar_arrive(acce_bar(b));
-        else
-          mbar_arrive_remote_read(leader_acce0 + 8u * b);
-      }
+      if (lane == 0) mbar_arrive(acce_bar(b));
       ++lt;
     }
   }

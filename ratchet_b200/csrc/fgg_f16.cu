@@ -166,9 +166,10 @@ struct F16Cfg {
   static constexpr int REGS_TOTAL = 128 * REGS_OTHER + 32 * EPI_WARPS * REGS_EPI;
   // steps of the contraction that one TMEM accumulator sums
   static constexpr int CHUNK = MODE_ == kWgrad ? 8 : 1 << 30;
-  // readers of a slot: leader producer, MMA warp, epilogue warps; follower
-  // producer and epilogue warps
-  static constexpr uint32_t SCHED_READERS = 3 + 2 * EPI_WARPS;
+  // arrivals that free a slot: on the leader its producer, MMA warp and epilogue warps
+  // and the follower's forwarding warp; on the follower its producer and epilogue warps
+  static constexpr uint32_t READERS_LEADER = 3 + EPI_WARPS;
+  static constexpr uint32_t READERS_FOLLOWER = 1 + EPI_WARPS;
   static constexpr uint32_t NBARS = 2 * STAGES + 4 + 2 * SCHED + 4;
   static constexpr uint32_t BAR_REGION = STAGES * STAGE_BYTES;
   static constexpr uint32_t SMEM_BYTES = 1024 + BAR_REGION + 8 * NBARS + 32 * SCHED + 16;
@@ -441,8 +442,8 @@ __device__ __forceinline__ F16Slot f16_make_slot(const F16Params& p, int unit, i
 }
 
 // Roles as in the block-scaled pair kernel (fgg_engine.cuh): warp 0 producer in
-// both CTAs, warp 1 MMA issuer in the leader, warp 2 TMEM, warp 3 scheduler in
-// the leader, the others epilogue.
+// both CTAs, warp 1 MMA issuer in the leader and forwarder of releases in the
+// follower, warp 2 TMEM, warp 3 scheduler in the leader, the others epilogue.
 template <class C>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(C::THREADS, 1)
     f16_pair_kernel(const __grid_constant__ F16Params p) {
@@ -496,11 +497,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(C::THREADS, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(accf_bar(b), 1);
-      mbar_init(acce_bar(b), 2 * C::EPI_WARPS);  // both CTAs' (leader's barrier)
+      mbar_init(acce_bar(b), C::EPI_WARPS + (leader ? 1 : 0));  // and the forwarder
     }
     for (int i = 0; i < C::SCHED; ++i) {
       mbar_init(schedf_bar(i), 1);
-      mbar_init(schede_bar(i), C::SCHED_READERS);  // used on the leader
+      mbar_init(schede_bar(i), leader ? C::READERS_LEADER : C::READERS_FOLLOWER);
     }
     mbar_init(tmem_ready_bar, 1);
     mbar_init(drain_bar, 1);
@@ -525,12 +526,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(C::THREADS, 1)
   const uint32_t leader_schede0 = mapa_shared(schede_bar(0), 0);
   const uint32_t leader_acce0 = mapa_shared(acce_bar(0), 0);
   const uint32_t leader_full0 = mapa_shared(full_bar(0), 0);
-  auto release_slot = [&](int slot) {
-    if (leader)
-      mbar_arrive(schede_bar(slot));
-    else
-      mbar_arrive_remote_read(leader_schede0 + 8u * slot);
-  };
 
   // the register split comes first in each branch: the compiler allots by branch
   if (warp < 4) {
@@ -616,7 +611,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(C::THREADS, 1)
         const int k0 = unit_k0(slot);
         const int k1 = unit_k1(slot, rows);
         if (lane == 0) {
-          release_slot(slot);
+          mbar_arrive(schede_bar(slot));
           if (leader) mbar_arrive(taken_bar(tiles_taken));
         }
         ++tiles_taken;
@@ -717,8 +712,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(C::THREADS, 1)
           const int chunk0 = ks;
           const int chunk1 = min(k1 - chunk0, C::CHUNK) + chunk0;
           const uint32_t b = lt & 1u;
-          if (!mbar_wait(acce_bar(b), ((lt >> 1) & 1u) ^ 1u, abort_flag, p.status,
-                         kStatusTimeoutMma)) {
+          if (!mbar_wait<true>(acce_bar(b), ((lt >> 1) & 1u) ^ 1u, abort_flag, p.status,
+                               kStatusTimeoutMma)) {
             ok = false;
             break;
           }
@@ -771,6 +766,48 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(C::THREADS, 1)
         }
       }
       __syncwarp();
+    } else if (warp == 1) {
+      // --------------------------------------- forwarder (follower only)
+      // The leader writes this CTA's slots and its MMAs this CTA's accumulators, so
+      // what frees them for it is released at cluster scope.  That waits for the
+      // warp's global stores, so it is done by a warp that has none, once the
+      // readers have arrived here: a tile's slot with its first accumulator.
+      int slot = 0;
+      uint32_t sphase = 0;
+      uint32_t lt = 0;
+      bool ok = true;
+      while (ok) {
+        if (!mbar_wait<true>(schedf_bar(slot), sphase, abort_flag, p.status,
+                             kStatusTimeoutEpilogue))
+          break;
+        const int g = __shfl_sync(kFullMask, ring[slot].g, 0);
+        const int rows = __shfl_sync(kFullMask, ring[slot].rows, 0);
+        const int k0 = unit_k0(slot);
+        const int k1 = unit_k1(slot, rows);
+        if (g < 0) break;
+        if (!mbar_wait(schede_bar(slot), sphase, abort_flag, p.status, kStatusTimeoutEpilogue))
+          break;
+        int ks = k0;
+        do {  // the accumulators that the tile takes
+          const uint32_t b = lt & 1u;
+          if (!mbar_wait(acce_bar(b), (lt >> 1) & 1u, abort_flag, p.status,
+                         kStatusTimeoutEpilogue)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          tc_fence_before();
+          if (lane < (ks == k0 ? 2 : 1))
+            mbar_arrive_remote(lane == 0 ? leader_acce0 + 8u * b : leader_schede0 + 8u * slot);
+          ++lt;
+          ks += C::CHUNK;
+        } while (ks < k1);
+        if (++slot == C::SCHED) {
+          slot = 0;
+          sphase ^= 1;
+        }
+      }
+      __syncwarp();
     }
   } else {
     // --------------------------------------------------------- epilogue
@@ -792,7 +829,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(C::THREADS, 1)
         return t;
       t = f16_read_slot(ring, slot);
       __syncwarp();
-      if (lane == 0) release_slot(slot);
+      if (lane == 0) mbar_arrive(schede_bar(slot));
       if (++slot == C::SCHED) {
         slot = 0;
         sphase ^= 1;
@@ -808,12 +845,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(C::THREADS, 1)
       auto release_acc = [&](uint32_t b) {  // this warp has read accumulator b
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) {
-          if (leader)
-            mbar_arrive(acce_bar(b));
-          else
-            mbar_arrive_remote_read(leader_acce0 + 8u * b);
-        }
+        if (lane == 0) mbar_arrive(acce_bar(b));
       };
       if constexpr (C::MODE == kWgrad) {
         float acc[128];

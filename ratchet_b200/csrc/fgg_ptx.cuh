@@ -65,7 +65,8 @@ __device__ __forceinline__ void mbar_arrive_expect_tx(uint32_t bar, uint32_t byt
 constexpr uint32_t kSuspendHintNs = 1000000u;
 
 // kCluster: acquire at cluster scope, for barriers the peer CTA of a pair
-// arrives on after writing this CTA's shared memory.
+// arrives on: after writing this CTA's shared memory, or after reading what this
+// CTA will overwrite.
 template <bool kCluster = false>
 __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
   uint32_t ok;
@@ -233,15 +234,10 @@ __device__ __forceinline__ void cluster_sync() {
                    : "memory");
 }
 // Arrive on an mbarrier of another CTA of the cluster (release at cluster scope
-// orders this thread's earlier shared-memory writes, remote ones included).
+// orders this thread's earlier accesses, remote ones included, and those of the
+// threads that it has synchronised with; it waits for this warp's global stores).
 __device__ __forceinline__ void mbar_arrive_remote(uint32_t cluster_bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar)
-               : "memory");
-}
-// The same without waiting for this thread's global stores (release at CTA scope):
-// for arrivals that publish no memory, only that this thread is done reading.
-__device__ __forceinline__ void mbar_arrive_remote_read(uint32_t cluster_bar) {
-  asm volatile("mbarrier.arrive.release.cta.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar)
                : "memory");
 }
 __device__ __forceinline__ void st_shared_remote_u32(uint32_t cluster_addr, uint32_t v) {

@@ -242,3 +242,20 @@ def test_mxfp4_python_refusals():
                 lambda: rb.mxfp4_grouped_gemm_rows(codes, sf, torch.zeros(2, dtype=torch.int32), None)):
         with pytest.raises(ValueError):
             bad()
+
+
+# ------------------------------------------------------------------------- sources
+def test_arrivals_in_another_cta_release_at_cluster_scope():
+    """An arrival on another CTA's barrier orders this CTA's accesses before what the other
+    does next only if it releases at cluster scope (a scope left out is the CTA's)."""
+    import re
+    from pathlib import Path
+
+    csrc = Path(rb.__file__).resolve().parent / "csrc"
+    found = []
+    for f in sorted(csrc.glob("*.cu*")):
+        found += [(f.name, m) for m in re.findall(r"mbarrier\.arrive[a-z0-9_.:]*shared::cluster[a-z0-9_.]*",
+                                                  f.read_text())]
+    assert found
+    for name, op in found:
+        assert ".release.cluster." in op, (name, op)
