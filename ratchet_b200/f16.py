@@ -60,7 +60,7 @@ def _run(direction: int, a, b, out, offsets, G, n, k, rows, accumulate=False) ->
             ws = ops._workspace(dev, stream, nbytes)
             rc = L.fgg_f16_grouped_gemm_rows(prob, direction, ws.data_ptr(), nbytes, stream)
     _lib.check(rc, "grouped_gemm_rows")
-    ops._set_last_ws(ws)
+    ops._set_last_ws(ws, stream)
 
 
 def _weights(w: torch.Tensor, dtype, dev, G: int):

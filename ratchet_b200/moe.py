@@ -424,7 +424,7 @@ class ExpertParallelMoE:
         _lib.check(L.fgg_nvfp4_grouped_gemm_rows(b["prob"], self.pack.buf.data_ptr(),
                                                  b["ws"].data_ptr(), b["ws"].numel(), stream),
                    "fgg_nvfp4_grouped_gemm_rows")
-        ops._set_last_ws(b["ws"])
+        ops._set_last_ws(b["ws"], stream)
         mark("reduce")
         out = torch.empty((T, n), dtype=torch.bfloat16, device=dev)
         target = b["partial"] if W > 1 else out
@@ -471,7 +471,7 @@ class ExpertParallelMoE:
         _lib.check(L.fgg_nvfp4_grouped_gemm_rows(b["prob"], self.pack.buf.data_ptr(),
                                                  b["ws"].data_ptr(), b["ws"].numel(), stream),
                    "fgg_nvfp4_grouped_gemm_rows")
-        ops._set_last_ws(b["ws"])
+        ops._set_last_ws(b["ws"], stream)
         mark("reduce")
         _lib.check(L.fgg_moe_reduce_peers(b["y"].data_ptr(), b["R"], b["route_row"].data_ptr(), toks,
                                           peers, self.bad.data_ptr(), stream), "fgg_moe_reduce_peers")

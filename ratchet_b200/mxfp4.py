@@ -190,5 +190,5 @@ def _product_on(a, a_sf, offsets, pack, alpha, out, row_scale, b_index, max_grou
     ws = ops._workspace(dev, stream, nbytes)
     _lib.check(L.fgg_mxfp4_grouped_gemm_rows(prob, pack.buf.data_ptr(), ws.data_ptr(), nbytes,
                                              stream), "mxfp4_grouped_gemm_rows")
-    ops._set_last_ws(ws)
+    ops._set_last_ws(ws, stream)
     return out

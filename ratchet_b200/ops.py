@@ -20,6 +20,7 @@ Everything runs on the current CUDA stream; nothing here synchronises the host.
 """
 from __future__ import annotations
 
+import threading
 from collections import OrderedDict
 from contextlib import nullcontext
 from threading import Lock, get_ident
@@ -140,7 +141,17 @@ class _LRU(OrderedDict):
 
 _PACKS = _LRU()
 _MX_PREP = _LRU()
-_last_ws: torch.Tensor | None = None
+
+
+class _Local(threading.local):
+    """What each host thread keeps for itself."""
+
+    def __init__(self):
+        self.last = None  # (workspace, stream) of the thread's latest GEMM call
+
+
+_LOCAL = _Local()
+_latest = None  # the same of any thread, for a thread that made no call
 
 
 class WeightPack:
@@ -284,7 +295,6 @@ def nvfp4_expert_mlp(a_list, a_sf_list, alpha13, w13_list, w13_sf_list, w2_list,
 
 def _nvfp4_grouped(a_list, a_sf_list, b_list, b_sf_list, problem_sizes, alpha, pack, out,
                    b_index, silu_mul: bool) -> list[torch.Tensor]:
-    global _last_ws
     G = len(a_list)
     if G == 0 or G != len(a_sf_list) or len(b_list) != len(b_sf_list) or not b_list:
         raise ValueError("a_list/a_sf_list and b_list/b_sf_list must be non-empty, pairwise equal length")
@@ -371,7 +381,7 @@ def _nvfp4_grouped(a_list, a_sf_list, b_list, b_sf_list, problem_sizes, alpha, p
             ws = _workspace(dev, stream, nbytes)
             rc = entry(prob, pack.buf.data_ptr(), ws.data_ptr(), nbytes, stream)
     _lib.check(rc, "nvfp4_grouped_gemm")
-    _last_ws = ws
+    _set_last_ws(ws, stream)
     return list(out.split_with_sizes(ms))
 
 
@@ -403,7 +413,6 @@ def nvfp4_grouped_gemm_rows(a: torch.Tensor, a_sf: torch.Tensor, offsets: torch.
     [G] naming each group's packed weight group; max_group_rows: a host bound
     on every group's rows (<= 16 selects the decode tiles).  Host work per
     call does not depend on G: no per-group Python."""
-    global _last_ws
     if pack is None:
         if b_list is None or b_sf_list is None:
             raise ValueError("give pack= or b_list / b_sf_list")
@@ -476,7 +485,7 @@ def nvfp4_grouped_gemm_rows(a: torch.Tensor, a_sf: torch.Tensor, offsets: torch.
             rc = L.fgg_nvfp4_grouped_gemm_rows(prob, pack.buf.data_ptr(), ws.data_ptr(), nbytes,
                                                stream)
     _lib.check(rc, "nvfp4_grouped_gemm_rows")
-    _last_ws = ws
+    _set_last_ws(ws, stream)
     return out
 
 
@@ -496,7 +505,6 @@ def fp4_grouped_gemm(a: torch.Tensor, a_sf: torch.Tensor, b: torch.Tensor, b_sf:
     b [G, N, K/2] int8/uint8 packed e2m1, b_sf [G, N, K/32] fp32 powers of two,
     m_indices [M_total] int32 (-1 = padding, segments aligned to 224 rows).
     ValueError for N % 128 or K % 128 (kernel.py:2811-2816)."""
-    global _last_ws
     if a.dim() != 2 or b.dim() != 3:
         raise ValueError("a must be [M_total, K] and b [G, N, K/2]")
     m_total, k = int(a.shape[0]), int(a.shape[1])
@@ -530,14 +538,15 @@ def fp4_grouped_gemm(a: torch.Tensor, a_sf: torch.Tensor, b: torch.Tensor, b_sf:
     prep = _MX_PREP.get_or(key, lambda: _MxPrepared(
         torch.empty(nbytes, dtype=torch.uint8, device=dev), (a_sf, b_sf, m_indices)))
     prob.reuse_prepared = 1 if prep.ready else 0
+    stream = _stream_ptr(dev)
     if _is_current(dev):
-        rc = L.fgg_mx_grouped_gemm(prob, prep.ws.data_ptr(), nbytes, _stream_ptr(dev))
+        rc = L.fgg_mx_grouped_gemm(prob, prep.ws.data_ptr(), nbytes, stream)
     else:
         with torch.cuda.device(dev):
-            rc = L.fgg_mx_grouped_gemm(prob, prep.ws.data_ptr(), nbytes, _stream_ptr(dev))
+            rc = L.fgg_mx_grouped_gemm(prob, prep.ws.data_ptr(), nbytes, stream)
     _lib.check(rc, "fp4_grouped_gemm")
     prep.ready = True
-    _last_ws = prep.ws
+    _set_last_ws(prep.ws, stream)
     return c
 
 
@@ -578,21 +587,28 @@ def _quantize_on(x, amax, dev, rows, k):
     return codes, sf.view(torch.float8_e4m3fn), g
 
 
-def _set_last_ws(ws: torch.Tensor) -> None:
-    """Record the workspace of a GEMM launched outside this module (last_status reads it)."""
-    global _last_ws
-    _last_ws = ws
+def _set_last_ws(ws: torch.Tensor, stream: int) -> None:
+    """Record a GEMM call's workspace and stream (last_status reads it)."""
+    global _latest
+    _LOCAL.last = _latest = (ws, stream)
 
 
 def last_status() -> int:
     """Synchronise the current stream and return the device status word of the
-    most recent GEMM call (0 = ok); raises FggError on a device timeout."""
-    if _last_ws is None:
+    calling thread's most recent GEMM call, or of any thread's where it made none
+    (0 = ok); raises FggError on a device timeout.  A call on another stream than
+    the current one is waited for too (with the whole device)."""
+    last = _LOCAL.last or _latest
+    if last is None:
         return 0
+    ws, stream = last
     L = _lib.lib()
-    dev = _last_ws.device
+    dev = ws.device
     with torch.cuda.device(dev):
-        rc = L.fgg_read_device_status(_last_ws.data_ptr(), _stream_ptr(dev))
+        current = _stream_ptr(dev)
+        if stream != current:
+            torch.cuda.synchronize(dev)
+        rc = L.fgg_read_device_status(ws.data_ptr(), current)
     _lib.check(rc, "device status")
     return 0
 

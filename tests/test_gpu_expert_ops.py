@@ -594,3 +594,56 @@ def test_python_refusals_on_the_device(cuda_device):
     # nothing that was refused left a mark
     rb.grouped_gemm_rows(x, w, off)
     rb.last_status()
+
+
+def test_status_of_a_call_on_another_stream(cuda_device):
+    """last_status waits for a call on another stream than the current one."""
+    import ratchet_b200 as rb
+
+    dev = cuda_device
+    x, w = _rand(dev, 64, 64), _rand(dev, 3, 32, 64)
+    good = torch.tensor([0, 3, 3, 64], dtype=torch.int32, device=dev)
+    bad = torch.tensor([0, 10, 5, 20], dtype=torch.int32, device=dev)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        rb.grouped_gemm_rows(x, w, good)
+        rb.last_status()
+        torch.cuda._sleep(100_000_000)               # about 50 ms
+        rb.grouped_gemm_rows(x, w, bad)
+    with pytest.raises(rb.FggError, match="0x203"):
+        rb.last_status()
+
+
+def test_status_of_two_threads(cuda_device):
+    """Malformed offsets of one thread raise there, and nowhere else."""
+    import ratchet_b200 as rb
+
+    dev = cuda_device
+    x, w = _rand(dev, 64, 64), _rand(dev, 3, 32, 64)
+    offsets = {"good": [0, 3, 3, 64], "bad": [0, 10, 5, 20]}
+    offsets = {n: torch.tensor(v, dtype=torch.int32, device=dev) for n, v in offsets.items()}
+    torch.cuda.synchronize()
+    called, seen = threading.Barrier(2, timeout=30), {}
+
+    def work(name):
+        with torch.cuda.device(dev):
+            wrong = 0
+            for _ in range(20):
+                called.wait()
+                rb.grouped_gemm_rows(x, w, offsets[name])
+                called.wait()
+                try:
+                    rb.last_status()
+                except rb.FggError:
+                    wrong += 1
+            seen[name] = wrong
+
+    threads = [threading.Thread(target=work, args=(n,)) for n in offsets]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(60)
+    assert seen == {"good": 0, "bad": 20}
+    rb.grouped_gemm_rows(x, w, offsets["good"])
+    rb.last_status()

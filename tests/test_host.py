@@ -120,3 +120,46 @@ def test_interleave_gate_up_order():
     assert sfi.view(torch.uint8)[:, 0].tolist() == want
     with pytest.raises(ValueError):
         rb.interleave_gate_up(w[:40], sf[:40])
+
+
+def test_last_status_is_the_calling_threads(monkeypatch):
+    """Each thread's latest call; any thread's for one that made none; a call on another
+    stream than the current one is waited for."""
+    import contextlib
+    import threading
+    from types import SimpleNamespace
+
+    from ratchet_b200 import _lib, ops
+
+    read, waited = [], []
+    fake = SimpleNamespace(fgg_read_device_status=lambda ws, stream: read.append((ws, stream)) or 0)
+    monkeypatch.setattr(_lib, "lib", lambda: fake)
+    monkeypatch.setattr(ops, "_stream_ptr", lambda dev: 5)
+    monkeypatch.setattr(ops.torch.cuda, "device", lambda dev: contextlib.nullcontext())
+    monkeypatch.setattr(ops.torch.cuda, "synchronize", waited.append)
+    monkeypatch.setattr(ops, "_latest", None)
+    monkeypatch.setattr(ops, "_LOCAL", ops._Local())
+    call = lambda n, stream: ops._set_last_ws(SimpleNamespace(device="d", data_ptr=lambda: n), stream)
+
+    def status(*made):
+        out = []
+
+        def work():
+            for c in made:
+                call(*c)
+            ops.last_status()
+            out.append((read.pop(), waited[:]))
+            waited.clear()
+
+        t = threading.Thread(target=work)
+        t.start()
+        t.join()
+        return out[0]
+
+    assert ops.last_status() == 0 and not read      # no call yet
+    call(1, 5)
+    assert status((2, 5)) == ((2, 5), [])
+    ops.last_status()
+    assert read.pop() == (1, 5) and not waited      # not the other thread's
+    assert status((3, 5), (4, 7)) == ((4, 5), ["d"])
+    assert status() == ((4, 5), ["d"])              # a thread without calls: the latest
