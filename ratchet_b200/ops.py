@@ -23,7 +23,6 @@ from __future__ import annotations
 import threading
 from collections import OrderedDict
 from contextlib import nullcontext
-from threading import Lock, get_ident
 from typing import Sequence
 
 import numpy as np
@@ -81,30 +80,39 @@ def _disjoint(out: torch.Tensor, *others) -> None:
             raise ValueError("out shares memory with an operand")
 
 
-# Workspaces reused per (device, stream, host thread): a thread's calls on one
+class _Local(threading.local):
+    """What each host thread keeps for itself."""
+
+    def __init__(self):
+        self.last = None  # (workspace, stream) of the thread's latest GEMM call
+        self.workspaces = OrderedDict()  # by (device, stream)
+
+
+_LOCAL = _Local()
+_latest = None  # _Local.last of any thread, for a thread that made no call
+
+# Workspaces reused per host thread, device and stream: a thread's calls on one
 # stream are ordered, so the next call's prepare kernel (which waits for the
 # previous GEMM before it touches memory) may overwrite the previous call's
 # workspace; another thread's launches may come between a prepare kernel and its
 # GEMM, so they get their own.  Not used while the stream is being captured into
 # a CUDA graph (the graph keeps its own).
-_WS: OrderedDict = OrderedDict()
-_WS_MAX = 8
-_WS_LOCK = Lock()
+_WS_MAX = 8  # of a thread
 
 
 def _workspace(device: torch.device, stream: int, nbytes: int) -> torch.Tensor:
     if _capturing is not None and _capturing():
         return torch.empty(nbytes, dtype=torch.uint8, device=device)
-    key = (device.index, stream, get_ident())
-    with _WS_LOCK:
-        ws = _WS.get(key)
-        if ws is None or ws.numel() < nbytes:
-            ws = torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
-            _WS[key] = ws
-            while len(_WS) > _WS_MAX:  # the oldest stream's buffer returns to torch's allocator
-                _WS.popitem(last=False)
-        else:
-            _WS.move_to_end(key)
+    kept = _LOCAL.workspaces
+    key = (device.index, stream)
+    ws = kept.get(key)
+    if ws is None or ws.numel() < nbytes:
+        ws = torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
+        kept[key] = ws
+        while len(kept) > _WS_MAX:  # the oldest stream's buffer returns to torch's allocator
+            kept.popitem(last=False)
+    else:
+        kept.move_to_end(key)
     return ws
 
 
@@ -141,17 +149,6 @@ class _LRU(OrderedDict):
 
 _PACKS = _LRU()
 _MX_PREP = _LRU()
-
-
-class _Local(threading.local):
-    """What each host thread keeps for itself."""
-
-    def __init__(self):
-        self.last = None  # (workspace, stream) of the thread's latest GEMM call
-
-
-_LOCAL = _Local()
-_latest = None  # the same of any thread, for a thread that made no call
 
 
 class WeightPack:

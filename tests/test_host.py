@@ -163,3 +163,36 @@ def test_last_status_is_the_calling_threads(monkeypatch):
     assert read.pop() == (1, 5) and not waited      # not the other thread's
     assert status((3, 5), (4, 7)) == ((4, 5), ["d"])
     assert status() == ((4, 5), ["d"])              # a thread without calls: the latest
+
+
+def test_workspaces_are_kept_per_thread(monkeypatch):
+    """Nine threads on one stream keep a workspace each, in every later call; a thread
+    keeps those of eight streams."""
+    import threading
+    from types import SimpleNamespace
+
+    from ratchet_b200 import ops
+
+    monkeypatch.setattr(ops, "_capturing", None)
+    monkeypatch.setattr(ops, "_LOCAL", ops._Local())
+    monkeypatch.setattr(ops.torch, "empty", lambda n, **kw: SimpleNamespace(numel=lambda: n))
+    dev = SimpleNamespace(index=0)
+    threads = 9
+    turn, kept = threading.Barrier(threads, timeout=30), [[] for _ in range(threads)]
+
+    def work(i):
+        for _ in range(3):
+            turn.wait()
+            kept[i].append(ops._workspace(dev, 11, 1000 + i))
+
+    pool = [threading.Thread(target=work, args=(i,), daemon=True) for i in range(threads)]
+    for t in pool:
+        t.start()
+    for t in pool:
+        t.join(60)
+    assert all(len(k) == 3 and k[0] is k[1] is k[2] for k in kept)
+    assert len({id(k[0]) for k in kept}) == threads
+    first = [ops._workspace(dev, s, 1000) for s in range(9)]
+    assert all(ops._workspace(dev, s, 1000) is first[s] for s in range(1, 9))
+    assert ops._workspace(dev, 0, 1000) is not first[0]
+    assert ops._workspace(dev, 8, 2 << 20) is not first[8]      # too small
