@@ -86,6 +86,8 @@ class _Local(threading.local):
     def __init__(self):
         self.last = None  # (workspace, stream) of the thread's latest GEMM call
         self.workspaces = OrderedDict()  # by (device, stream)
+        self.scratch = {}  # see _scratch
+        self.rows = OrderedDict()  # see nvfp4_grouped_gemm_rows
 
 
 _LOCAL = _Local()
@@ -117,16 +119,13 @@ def _workspace(device: torch.device, stream: int, nbytes: int) -> torch.Tensor:
 
 
 # Host arrays for the per-group problem description, reused per group count
-# (the C ABI reads them during the call only).
-_SCRATCH: dict = {}
-
-
+# (the C ABI reads them during the call only, in which other threads run).
 def _scratch(G: int):
-    sc = _SCRATCH.get(G)
+    sc = _LOCAL.scratch.get(G)
     if sc is None:
         sc = (np.empty(G, dtype=np.int32), np.empty(G, dtype=np.uint64),
               np.empty(G, dtype=np.uint64))
-        _SCRATCH[G] = sc
+        _LOCAL.scratch[G] = sc
     return sc
 
 
@@ -382,11 +381,6 @@ def _nvfp4_grouped(a_list, a_sf_list, b_list, b_sf_list, problem_sizes, alpha, p
     return list(out.split_with_sizes(ms))
 
 
-# Problem structs and workspaces of the contiguous-rows entry, per geometry:
-# a repeated call only patches pointers (no per-group host work at all).
-_ROWS: OrderedDict = OrderedDict()
-
-
 def nvfp4_grouped_gemm_rows(a: torch.Tensor, a_sf: torch.Tensor, offsets: torch.Tensor,
                             b_list=None, b_sf_list=None, alpha=None, *,
                             pack: WeightPack | None = None, out: torch.Tensor | None = None,
@@ -450,7 +444,10 @@ def nvfp4_grouped_gemm_rows(a: torch.Tensor, a_sf: torch.Tensor, offsets: torch.
                                  f"on {dev}")
     L = _lib.lib()
     key = (dev.index, G, n, k, R, int(max_group_rows), b_index is not None, pack.G)
-    hit = _ROWS.get(key)
+    # a thread's problem structs per geometry: a repeated call only patches pointers
+    # (no per-group host work at all)
+    kept = _LOCAL.rows
+    hit = kept.get(key)
     if hit is None:
         prob = _lib.FggNvfp4RowsProblem(G, n, k, R, 0, 0, 0, 0, 0, 0, 0, pack.G,
                                         int(max_group_rows))
@@ -458,11 +455,11 @@ def nvfp4_grouped_gemm_rows(a: torch.Tensor, a_sf: torch.Tensor, offsets: torch.
         if nbytes == 0:
             _lib.check(L.fgg_nvfp4_grouped_gemm_rows(prob, None, None, 0, None), "grouped GEMM rows")
         hit = [prob, nbytes]
-        _ROWS[key] = hit
-        while len(_ROWS) > _CACHE_MAX:
-            _ROWS.popitem(last=False)
+        kept[key] = hit
+        while len(kept) > _CACHE_MAX:
+            kept.popitem(last=False)
     else:
-        _ROWS.move_to_end(key)
+        kept.move_to_end(key)
     prob, nbytes = hit
     prob.offsets = offsets.data_ptr()
     prob.a = a_u8.data_ptr()
@@ -613,4 +610,4 @@ def last_status() -> int:
 def clear_caches() -> None:
     _PACKS.clear()
     _MX_PREP.clear()
-    _ROWS.clear()
+    _LOCAL.rows.clear()

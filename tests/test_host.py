@@ -196,3 +196,52 @@ def test_workspaces_are_kept_per_thread(monkeypatch):
     assert all(ops._workspace(dev, s, 1000) is first[s] for s in range(1, 9))
     assert ops._workspace(dev, 0, 1000) is not first[0]
     assert ops._workspace(dev, 8, 2 << 20) is not first[8]      # too small
+
+
+def test_threads_describe_their_own_problems(monkeypatch):
+    """Two threads inside the NVFP4 entries at once, with the same geometry: each call's
+    problem keeps its own pointers."""
+    import threading
+    from types import SimpleNamespace
+
+    import torch
+
+    from ratchet_b200 import _lib, ops
+
+    both, got = threading.Barrier(2, timeout=30), {}
+
+    def entry(prob, pack, ws, nbytes, stream):
+        both.wait()          # the other thread has described its problem by now
+        got[threading.current_thread().name] = (prob.a, prob.out)
+        both.wait()
+        return 0
+
+    fake = SimpleNamespace(fgg_nvfp4_rows_workspace_bytes=lambda prob: 64,
+                           fgg_nvfp4_grouped_gemm_rows=entry)
+    monkeypatch.setattr(_lib, "lib", lambda: fake)
+    monkeypatch.setattr(ops, "_is_current", lambda dev: True)
+    monkeypatch.setattr(ops, "_stream_ptr", lambda dev: 0)
+    monkeypatch.setattr(ops, "_capturing", None)
+    monkeypatch.setattr(ops, "_LOCAL", ops._Local())
+    monkeypatch.setattr(ops, "_latest", None)
+    cpu = torch.device("cpu")
+    pack = SimpleNamespace(n=128, k=64, device=cpu, G=1, buf=torch.empty(1))
+    off = torch.tensor([0, 4], dtype=torch.int32)
+    want, scratch = {}, {}
+
+    def work(name):
+        a, sf = torch.zeros(4, 32, dtype=torch.uint8), torch.zeros(4, 4, dtype=torch.uint8)
+        out = torch.zeros(4, 128, dtype=torch.bfloat16)
+        want[name] = (a.data_ptr(), out.data_ptr())
+        scratch[name] = ops._scratch(3)
+        ops.nvfp4_grouped_gemm_rows(a, sf, off, pack=pack, out=out)
+        assert ops._scratch(3) is scratch[name]
+        both.wait()          # the tensors live until both have been read
+
+    pool = [threading.Thread(target=work, args=(n,), name=n, daemon=True) for n in ("x", "y")]
+    for t in pool:
+        t.start()
+    for t in pool:
+        t.join(60)
+    assert len(got) == 2 and got == want
+    assert scratch["x"][0] is not scratch["y"][0]
