@@ -125,20 +125,28 @@ int current_device(DeviceInfo* out) {
 
 // The encoder's arguments, which fully determine its result: a repeated call
 // (the same buffers every step) copies the remembered map instead of
-// encoding again.  Per host thread, a few entries replaced round-robin.
+// encoding again.  Per host thread, kWays entries for each hash of a key, replaced
+// in turn: a search costs a few comparisons, whether it finds the key or not.
 struct EncodeKey {
   int dtype, rank, swz;
   const void* base;
   cuuint64_t dims[3], strides[2];
   cuuint32_t box[3];
   bool operator==(const EncodeKey& o) const { return memcmp(this, &o, sizeof(*this)) == 0; }
+  unsigned hash() const {
+    uint64_t h = uint64_t(reinterpret_cast<uintptr_t>(base)) >> 4;
+    h = (h ^ dims[1] << 20 ^ uint64_t(box[1]) << 44) * 0x9E3779B97F4A7C15ull;
+    return unsigned(h >> 32);
+  }
 };
 struct EncodeMemo {
-  static constexpr int kEntries = 64;
-  EncodeKey key[kEntries];
-  CUtensorMap map[kEntries];
-  bool used[kEntries];
-  int next;
+  static constexpr int kSets = 64, kWays = 4;
+  struct Set {
+    EncodeKey key[kWays];
+    CUtensorMap map[kWays];
+    bool used[kWays];
+    int next;
+  } sets[kSets];
 };
 static thread_local EncodeMemo t_memo;
 
@@ -156,9 +164,9 @@ static int encode(CUtensorMap* out, CUtensorMapDataType dtype, cuuint32_t rank, 
     k.box[i] = box[i];
     if (i + 1 < rank) k.strides[i] = strides[i];
   }
-  EncodeMemo& m = t_memo;
+  EncodeMemo::Set& m = t_memo.sets[k.hash() % EncodeMemo::kSets];
   if (rank <= 3) {
-    for (int i = 0; i < EncodeMemo::kEntries; ++i)
+    for (int i = 0; i < EncodeMemo::kWays; ++i)
       if (m.used[i] && m.key[i] == k) {
         *out = m.map[i];
         return FGG_OK;
@@ -176,7 +184,7 @@ static int encode(CUtensorMap* out, CUtensorMapDataType dtype, cuuint32_t rank, 
                      rank);
   if (rank <= 3) {
     const int i = m.next;
-    m.next = (m.next + 1) % EncodeMemo::kEntries;
+    m.next = (m.next + 1) % EncodeMemo::kWays;
     m.key[i] = k;
     m.map[i] = *out;
     m.used[i] = true;

@@ -51,6 +51,8 @@
 
 #include <cuda_bf16.h>
 
+#include <type_traits>
+
 #include "fgg_host.cuh"
 #include "fgg_ptx.cuh"
 
@@ -78,6 +80,7 @@ struct PackHeader {
 
 constexpr int kStatusBadPack = 0x201;
 constexpr int kStatusBadTile = 0x202;  // a schedule slot named a group outside the problem
+constexpr int kStatusBadTmem = 0x204;  // tensor memory begins where it cannot
 
 // One schedule-ring slot (32 bytes): what every role needs to know about a
 // tile, published by the scheduler warp.
@@ -98,16 +101,15 @@ constexpr int kXSmallMaps = 6;
 struct GemmParams {
   CUtensorMap mx_tmap_w;      // MX, MXFP4: 3-D map of the [G, N, K] weight codes
   // One 2-D map over contiguous token rows: MX [M_total, K] fp8 activations;
-  // NVFP4 with x_flat set: [max_rows, K/2] codes of every group
+  // NVFP4, MXFP4: [rows, K/2] codes of every group (GemmListParams: a map per group)
   CUtensorMap tmap_x_flat;
   CUtensorMap sfw_map;        // pair kernel: the weight SF atoms as a 2-D uint64 tensor
   CUtensorMap sfx_map;        // pair kernel: the token SF atoms as a 2-D uint64 tensor
-  // pair kernel, NVFP4 with x_flat and x_small set: maps over the same token
-  // rows as tmap_x_flat with boxes of 16, 32, ..., 96 rows, so that a tile
-  // whose MMA is narrower than 224 columns loads only the rows it uses
+  // pair kernel with x_small set: maps over the same token rows as tmap_x_flat
+  // with boxes of 16, 32, ..., 96 rows, so that a tile whose MMA is narrower
+  // than 224 columns loads only the rows it uses
   CUtensorMap tmap_x_small[kXSmallMaps];
-  const CUtensorMap* tmap_w;  // NVFP4: [G] per-group maps (global memory)
-  const CUtensorMap* tmap_x;  // NVFP4: [G] per-group maps (global memory)
+  const CUtensorMap* tmap_w;  // NVFP4: [WG] maps of the weight groups (in the pack)
   const uint8_t* sfw;         // [G][NT128][KSTEPS][SFW_BYTES]
   const uint8_t* sfx;         // [XT][KSTEPS][SFX_BYTES]
   const GroupInfo* ginfo;     // NVFP4: [G]
@@ -125,17 +127,24 @@ struct GemmParams {
   int32_t nt128;  // 128-row weight tiles per group (the SF pack's unit)
   int32_t epi;    // kEpiPlain or kEpiSiluMul (NVFP4 only)
   int32_t debug_flags;  // test hooks (kDebugNoLoads); 0 in normal use
-  // NVFP4: 1 = the token rows of all groups lie in one buffer read through
-  // tmap_x_flat, the tile's first row being its output row (group offsets
-  // from the device); 0 = one descriptor per group (tmap_x)
-  int32_t x_flat;
   // optional device [rows] factor per output row (token), applied with alpha:
   // out[t, n] = bf16(alpha_g * row_scale[t] * acc); null = 1
   const float* row_scale;
   // optional device word holding the tile count (written by the prepare
   // kernel); null = num_tiles
   const int32_t* num_tiles_dev;
-  int32_t x_small;  // 1: tmap_x_small is encoded (x_flat only)
+  int32_t x_small;   // 1: tmap_x_small is encoded
+  int32_t out_rows;  // rows of out: no tile ends behind them
+  int32_t xtiles;    // token tiles that sfx has room for
+};
+
+// NVFP4 over groups whose token rows lie in buffers of their own: a map for each of
+// the groups g0 .. g0 + kListMaps - 1, which are those of the launch's tiles.  The maps
+// are encoded on the host and travel as kernel parameters, as every token map does.
+constexpr int kListMaps = 64;
+struct GemmListParams : GemmParams {
+  CUtensorMap tmap_x[kListMaps];
+  int32_t g0;
 };
 
 // Test hook: the producer arms no stage and issues no load, so the MMA role's
@@ -246,7 +255,7 @@ __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
 // broadcast by shuffles.  Rows past `rows` are neither scaled nor stored.
 __device__ __forceinline__ void epilogue_tile(__nv_bfloat16* out, int ldn, int n0, size_t row0,
                                               int rows, int ncols, float alpha,
-                                              const float* __restrict__ row_scale, uint32_t taddr,
+                                              const float* row_scale, uint32_t taddr,
                                               uint32_t* stage) {
   const int lane = threadIdx.x & 31;
   const bool odd = lane & 1;
@@ -255,7 +264,7 @@ __device__ __forceinline__ void epilogue_tile(__nv_bfloat16* out, int ldn, int n
     tmem_ld16(taddr + c0, r);
     float rs = 1.0f;
     if (row_scale != nullptr && lane < 16 && c0 + lane < rows)
-      rs = __ldg(row_scale + row0 + size_t(c0 + lane));
+      rs = row_scale[row0 + size_t(c0 + lane)];
     tmem_wait_ld();
     float v[16];
 #pragma unroll
@@ -318,8 +327,36 @@ __device__ __forceinline__ void epilogue_tile_silu_mul(__nv_bfloat16* out, int l
   }
 }
 
-template <bool MX_, int BN_, int STAGES_, int KSUB_ = 1, bool MX4_ = false>
+// What forms an address is checked before it does: a tile that is not one of the
+// problem's, or tensor memory at an impossible place, ends the kernel with a status.
+template <int BN>
+__device__ __forceinline__ bool slot_in_range(const GemmParams& p, const SchedSlot& s) {
+  const int nti = int((s.tile >> 11) & 0x7FFu);
+  return nti < p.nt && s.rows > 0 && s.rows <= BN && s.row0 >= 0 &&
+         s.row0 <= p.out_rows - s.rows;
+}
+__device__ __forceinline__ bool tmem_in_range(uint32_t base, uint32_t cols) {
+  return base <= 512u - cols;  // the lane is in the upper half
+}
+__device__ __forceinline__ void give_up(int* status, volatile int* abort_flag, int code) {
+  if ((threadIdx.x & 31) == 0) {
+    atomicCAS(status, 0, code);
+    *abort_flag = 1;
+  }
+  __syncwarp();
+}
+
+// The pack is one of this problem's weights.
+template <class C>
+__device__ __forceinline__ bool pack_matches(const GemmParams& p, const PackHeader& h) {
+  return C::MX || (h.magic == (C::MX4 ? kPackMagicMx : kPackMagic) && h.g == p.wg &&
+                   h.n == p.n && h.k == p.k);
+}
+
+template <bool MX_, int BN_, int STAGES_, int KSUB_ = 1, bool MX4_ = false, bool LIST_ = false>
 struct EngineCfg {
+  static constexpr bool LIST = LIST_;
+  using Params = std::conditional_t<LIST, GemmListParams, GemmParams>;
   static constexpr bool MX = MX_;
   static constexpr bool MX4 = MX4_;
   static_assert(!(MX && MX4), "one kind");
@@ -379,7 +416,8 @@ struct EngineCfg {
 };
 
 template <class C>
-__global__ void __launch_bounds__(256, 1) fgg_gemm_kernel(const __grid_constant__ GemmParams p) {
+__global__ void __launch_bounds__(256, 1)
+    fgg_gemm_kernel(const __grid_constant__ typename C::Params p) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
@@ -430,13 +468,8 @@ __global__ void __launch_bounds__(256, 1) fgg_gemm_kernel(const __grid_constant_
     mbar_init(drain_bar, 1);
     mbar_init(taken_bar, 1);
     *abort_flag = 0;
-    if constexpr (!C::MX) {
-      // A pack built for a different problem is refused before any load.
-      const PackHeader h = *p.pack;
-      // reported after griddep_wait: the prepare kernel resets the status word
-      if (h.magic != (C::MX4 ? kPackMagicMx : kPackMagic) || h.g != p.wg || h.n != p.n || h.k != p.k) *abort_flag = 2;
-    }
     fence_mbar_init();
+    if constexpr (!C::MX) prefetch_l2(p.pack);  // read after griddep_wait
   }
   __syncthreads();
 
@@ -448,30 +481,36 @@ __global__ void __launch_bounds__(256, 1) fgg_gemm_kernel(const __grid_constant_
     if (lane == 0) mbar_arrive(tmem_ready_bar);
   }
 
-  // Everything above (barriers, TMEM, the weight pack's header) is ready
-  // before this launch; the schedule, token descriptors and scale repack come
-  // from the prepare kernel just before it on the stream, which this launch
-  // may overlap (programmatic dependent launch).
+  // Everything above is this launch's own; the schedule and the scale repack come
+  // from the prepare kernel just before it on the stream, which this launch may
+  // overlap (programmatic dependent launch).  Nothing in global memory is read
+  // before this, the pack neither: its kernel may have been the one before that.
   griddep_wait();
-  const bool aborted_early = (*abort_flag != 0);
-  if (threadIdx.x == 0 && *abort_flag == 2) atomicCAS(p.status, 0, kStatusBadPack);
 
   if (warp == 3) {
     // ------------------------------------------------------------ scheduler
-    if (lane == 0 && !aborted_early) {
+    if (lane == 0) {
       int slot = 0;
       uint32_t sphase = 0;
-      const int num_tiles = p.num_tiles_dev != nullptr ? *p.num_tiles_dev : p.num_tiles;
+      int num_tiles = p.num_tiles_dev != nullptr ? *p.num_tiles_dev : p.num_tiles;
+      PackHeader header = {};
+      if constexpr (!C::MX) header = *p.pack;
+      int t = atomicAdd(p.status + 1, 1);  // on its way together with the header
+      if (!pack_matches<C>(p, header)) {  // refused before any load
+        atomicCAS(p.status, 0, kStatusBadPack);
+        num_tiles = 0;
+      }
       for (uint32_t n = 0;; ++n) {
         // Claim tile n only once the producer has taken tile n-1: a CTA holds
         // at most one tile it has not started, so the tail of the tile list
         // spreads over every CTA.  (The producer cannot take tile n before it
         // is published, so the parity below is unambiguous.)
-        if (n > 0 && !mbar_wait1(taken_bar, (n - 1) & 1u, abort_flag, p.status,
-                                 kStatusTimeoutProducer))
-          break;
-        const int t = atomicAdd(p.status + 1, 1);
-        const uint32_t tile = (t < num_tiles) ? __ldg(p.tiles + t) : kEndTile;
+        if (n > 0) {
+          if (!mbar_wait1(taken_bar, (n - 1) & 1u, abort_flag, p.status, kStatusTimeoutProducer))
+            break;
+          t = atomicAdd(p.status + 1, 1);
+        }
+        const uint32_t tile = (t < num_tiles) ? p.tiles[t] : kEndTile;
         const SchedSlot s = make_slot<C::MX, C::BN>(p, tile);
         if (!mbar_wait1(schede_bar(slot), sphase ^ 1, abort_flag, p.status,
                         kStatusTimeoutProducer))
@@ -490,116 +529,111 @@ __global__ void __launch_bounds__(256, 1) fgg_gemm_kernel(const __grid_constant_
     // ------------------------------------------------------------- producer
     // The whole warp runs the loop (operands warp-uniform), one elected lane
     // issues the loads.
-    if (!aborted_early) {
-      int stage = 0;
-      uint32_t phase = 0;
-      int slot = 0;
-      uint32_t sphase = 0;
-      uint32_t arms = 0;
+    int stage = 0;
+    uint32_t phase = 0;
+    int slot = 0;
+    uint32_t sphase = 0;
+    uint32_t arms = 0;
+    if (lane == 0) {
+      if constexpr (C::MX || C::MX4) prefetch_tensormap(&p.mx_tmap_w);
+      if constexpr (!C::LIST) prefetch_tensormap(&p.tmap_x_flat);
+    }
+    while (true) {
+      if (!mbar_wait(schedf_bar(slot), sphase, abort_flag, p.status, kStatusTimeoutProducer))
+        break;
+      const uint32_t tile = __shfl_sync(kFullMask, ring[slot].tile, 0);
+      const int xtile_index = __shfl_sync(kFullMask, ring[slot].xtile_index, 0);
+      const int wgroup = __shfl_sync(kFullMask, ring[slot].wgroup, 0);
+      const int row0 = __shfl_sync(kFullMask, ring[slot].row0, 0);
       if (lane == 0) {
-        if constexpr (C::MX || C::MX4) prefetch_tensormap(&p.mx_tmap_w);
-        if (C::MX || p.x_flat) prefetch_tensormap(&p.tmap_x_flat);
+        mbar_arrive(schede_bar(slot));
+        mbar_arrive(taken_bar);
       }
-      while (true) {
-        if (!mbar_wait(schedf_bar(slot), sphase, abort_flag, p.status, kStatusTimeoutProducer))
-          break;
-        const uint32_t tile = __shfl_sync(kFullMask, ring[slot].tile, 0);
-        const int xtile_index = __shfl_sync(kFullMask, ring[slot].xtile_index, 0);
-        const int wgroup = __shfl_sync(kFullMask, ring[slot].wgroup, 0);
-        const int row0 = __shfl_sync(kFullMask, ring[slot].row0, 0);
-        if (lane == 0) {
-          mbar_arrive(schede_bar(slot));
-          mbar_arrive(taken_bar);
-        }
-        if (++slot == C::SCHED) {
-          slot = 0;
-          sphase ^= 1;
-        }
-        if (tile == kEndTile) {
-          // no new tiles for this CTA: the next kernel on the stream (the next
-          // call's prepare kernel) may launch; it waits for this grid's
-          // completion before it touches memory
-          if (lane == 0) griddep_launch_dependents();
-          break;
-        }
-        const int g = int(tile >> 22);
-        const int nti = int((tile >> 11) & 0x7FFu);
-        const int xti = int(tile & 0x7FFu);
-        // the group and weight group index descriptor arrays: never trust them blindly
-        if (g >= p.g || unsigned(wgroup) >= unsigned(p.wg)) {
-          if (lane == 0) {
-            atomicCAS(p.status, 0, kStatusBadTile);
-            *abort_flag = 1;
-          }
-          break;
-        }
-        const CUtensorMap* tw;
-        const CUtensorMap* tx;
-        // first token row of the tile in the map's coordinates
-        const int xrow = (C::MX || p.x_flat) ? row0 : xti * C::BN;
-        if constexpr (C::MX || C::MX4) {
-          tw = &p.mx_tmap_w;
+      if (++slot == C::SCHED) {
+        slot = 0;
+        sphase ^= 1;
+      }
+      if (tile == kEndTile) {
+        // no new tiles for this CTA: the next kernel on the stream (the next
+        // call's prepare kernel) may launch; it waits for this grid's
+        // completion before it touches memory
+        if (lane == 0) griddep_launch_dependents();
+        break;
+      }
+      const int g = int(tile >> 22);
+      const int nti = int((tile >> 11) & 0x7FFu);
+      const int xti = int(tile & 0x7FFu);
+      bool known = g < p.g && unsigned(wgroup) < unsigned(p.wg) && nti < p.nt &&
+                   unsigned(xtile_index) < unsigned(p.xtiles);
+      if constexpr (C::LIST) known = known && unsigned(g - p.g0) < unsigned(kListMaps);
+      if (!known) {
+        give_up(p.status, abort_flag, kStatusBadTile);
+        break;
+      }
+      const CUtensorMap* tw;
+      const CUtensorMap* tx;
+      // first token row of the tile in the map's coordinates
+      const int xrow = C::LIST ? xti * C::BN : row0;
+      if constexpr (C::MX || C::MX4) {
+        tw = &p.mx_tmap_w;
+        tx = &p.tmap_x_flat;
+      } else {
+        tw = p.tmap_w + wgroup;
+        tensormap_acquire(tw);  // every lane: the issuing one among them
+        if constexpr (C::LIST)
+          tx = &p.tmap_x[g - p.g0];
+        else
           tx = &p.tmap_x_flat;
-        } else {
-          tw = p.tmap_w + wgroup;
-          tensormap_acquire(tw);  // every lane: the issuing one among them
-          if (p.x_flat) {
-            tx = &p.tmap_x_flat;
-          } else {
-            tx = p.tmap_x + g;
-            tensormap_acquire(tx);
-          }
+      }
+      const uint8_t* sfx = p.sfx + size_t(xtile_index) * size_t(p.ksteps) * C::SFX_BYTES;
+      const uint8_t* sfw =
+          p.sfw + (size_t(wgroup) * p.nt + nti) * size_t(p.ksteps) * C::SFW_BYTES;
+      bool ok = true;
+      for (int ks0 = 0; ks0 < p.ksteps; ks0 += C::KSUB) {
+        if (!mbar_wait(empty_bar(stage), phase ^ 1, abort_flag, p.status,
+                       kStatusTimeoutProducer)) {
+          ok = false;
+          break;
         }
-        const uint8_t* sfx = p.sfx + size_t(xtile_index) * size_t(p.ksteps) * C::SFX_BYTES;
-        const uint8_t* sfw =
-            p.sfw + (size_t(wgroup) * p.nt + nti) * size_t(p.ksteps) * C::SFW_BYTES;
-        bool ok = true;
-        for (int ks0 = 0; ks0 < p.ksteps; ks0 += C::KSUB) {
-          if (!mbar_wait(empty_bar(stage), phase ^ 1, abort_flag, p.status,
-                         kStatusTimeoutProducer)) {
-            ok = false;
-            break;
-          }
-          const uint32_t fb = full_bar(stage);
-          const bool arm = (p.debug_flags & kDebugNoLoads) == 0;
-          if (arm && elect_one()) {
-            if constexpr (C::KSUB == 1)
-              mbar_arrive_expect_tx(fb, C::TX_BYTES);
-            else
-              mbar_arrive_expect_tx(fb, C::TX_BYTES * uint32_t(min(C::KSUB, p.ksteps - ks0)));
+        const uint32_t fb = full_bar(stage);
+        const bool arm = (p.debug_flags & kDebugNoLoads) == 0;
+        if (arm && elect_one()) {
+          if constexpr (C::KSUB == 1)
+            mbar_arrive_expect_tx(fb, C::TX_BYTES);
+          else
+            mbar_arrive_expect_tx(fb, C::TX_BYTES * uint32_t(min(C::KSUB, p.ksteps - ks0)));
 #pragma unroll
-            for (int sub = 0; sub < C::KSUB; ++sub) {
-              const int ks = ks0 + sub;
-              if constexpr (C::KSUB > 1) {
-                if (ks >= p.ksteps) break;
-              }
-              const int q = stage * C::KSUB + sub;
-              if constexpr (C::MX)
-                tma_load_3d(sW(q), tw, fb, ks * C::K_STEP, nti * 128, g);
-              else if constexpr (C::MX4)
-                tma_load_3d(sW(q), tw, fb, ks * 128, nti * 128, wgroup);
-              else
-                tma_load_2d(sW(q), tw, fb, ks * 128, nti * 128);
-              tma_load_2d(sX(q), tx, fb, ks * 128, xrow);
-              bulk_g2s(sSFW(q), sfw + size_t(ks) * C::SFW_BYTES, C::SFW_BYTES, fb);
-              bulk_g2s(sSFX(q), sfx + size_t(ks) * C::SFX_BYTES, C::SFX_BYTES, fb);
+          for (int sub = 0; sub < C::KSUB; ++sub) {
+            const int ks = ks0 + sub;
+            if constexpr (C::KSUB > 1) {
+              if (ks >= p.ksteps) break;
             }
-          }
-          __syncwarp();
-          if (arm) ++arms;
-          if (++stage == C::STAGES) {
-            stage = 0;
-            phase ^= 1;
+            const int q = stage * C::KSUB + sub;
+            if constexpr (C::MX)
+              tma_load_3d(sW(q), tw, fb, ks * C::K_STEP, nti * 128, g);
+            else if constexpr (C::MX4)
+              tma_load_3d(sW(q), tw, fb, ks * 128, nti * 128, wgroup);
+            else
+              tma_load_2d(sW(q), tw, fb, ks * 128, nti * 128);
+            tma_load_2d(sX(q), tx, fb, ks * 128, xrow);
+            bulk_g2s(sSFW(q), sfw + size_t(ks) * C::SFW_BYTES, C::SFW_BYTES, fb);
+            bulk_g2s(sSFX(q), sfx + size_t(ks) * C::SFX_BYTES, C::SFX_BYTES, fb);
           }
         }
-        if (!ok) break;
+        __syncwarp();
+        if (arm) ++arms;
+        if (++stage == C::STAGES) {
+          stage = 0;
+          phase ^= 1;
+        }
       }
-      // Every armed stage must land before the CTA may exit (normally already so).
-      if (lane == 0) {
-        const uint32_t first = arms > uint32_t(C::STAGES) ? arms - C::STAGES : 0u;
-        for (uint32_t a = first; a < arms; ++a)
-          mbar_wait_one(full_bar(int(a % C::STAGES)), (a / C::STAGES) & 1u, 200000000ull);
-      }
+      if (!ok) break;
+    }
+    // Every armed stage must land before the CTA may exit (normally already so).
+    if (lane == 0) {
+      const uint32_t first = arms > uint32_t(C::STAGES) ? arms - C::STAGES : 0u;
+      for (uint32_t a = first; a < arms; ++a)
+        mbar_wait_one(full_bar(int(a % C::STAGES)), (a / C::STAGES) & 1u, 200000000ull);
     }
     __syncwarp();
   } else if (warp == 1) {
@@ -607,144 +641,154 @@ __global__ void __launch_bounds__(256, 1) fgg_gemm_kernel(const __grid_constant_
     // The whole warp runs the loop; the scale uploads, MMAs and commits of a
     // stage issue from one elect.sync region, with every operand (descriptors,
     // TMEM columns) computed outside it and warp-uniform.
-    if (!aborted_early) {
-      bool ok = mbar_wait(tmem_ready_bar, 0, abort_flag, p.status, kStatusTimeoutMma);
+    bool ok = mbar_wait(tmem_ready_bar, 0, abort_flag, p.status, kStatusTimeoutMma);
+    tc_fence_after();
+    const uint32_t tmem = __shfl_sync(kFullMask, *tmem_holder, 0);
+    if (ok && !tmem_in_range(tmem, C::TMEM_COLS)) {
+      give_up(p.status, abort_flag, kStatusBadTmem);
+      ok = false;
+    }
+    int stage = 0;
+    uint32_t phase = 0;
+    int slot = 0;
+    uint32_t sphase = 0;
+    uint32_t lt = 0;
+    int sfslot = 0;
+    bool issued_any = false;
+    while (ok) {
+      if (!mbar_wait(schedf_bar(slot), sphase, abort_flag, p.status, kStatusTimeoutMma)) break;
+      const uint32_t tile = __shfl_sync(kFullMask, ring[slot].tile, 0);
+      const int rows = __shfl_sync(kFullMask, ring[slot].rows, 0);
+      if (lane == 0) mbar_arrive(schede_bar(slot));
+      if (++slot == C::SCHED) {
+        slot = 0;
+        sphase ^= 1;
+      }
+      if (tile == kEndTile) break;
+      if (rows <= 0 || rows > C::BN) {
+        give_up(p.status, abort_flag, kStatusBadTile);
+        break;
+      }
+      const int ncols = min(C::BN, (rows + 15) & ~15);
+      const uint32_t b = lt & 1u;
+      if (!mbar_wait(acce_bar(b), ((lt >> 1) & 1u) ^ 1u, abort_flag, p.status,
+                     kStatusTimeoutMma))
+        break;
       tc_fence_after();
-      const uint32_t tmem = __shfl_sync(kFullMask, *tmem_holder, 0);
-      int stage = 0;
-      uint32_t phase = 0;
-      int slot = 0;
-      uint32_t sphase = 0;
-      uint32_t lt = 0;
-      int sfslot = 0;
-      bool issued_any = false;
-      while (ok) {
-        if (!mbar_wait(schedf_bar(slot), sphase, abort_flag, p.status, kStatusTimeoutMma)) break;
-        const uint32_t tile = __shfl_sync(kFullMask, ring[slot].tile, 0);
-        const int rows = __shfl_sync(kFullMask, ring[slot].rows, 0);
-        if (lane == 0) mbar_arrive(schede_bar(slot));
-        if (++slot == C::SCHED) {
-          slot = 0;
-          sphase ^= 1;
-        }
-        if (tile == kEndTile) break;
-        const int ncols = min(C::BN, (rows + 15) & ~15);
-        const uint32_t b = lt & 1u;
-        if (!mbar_wait(acce_bar(b), ((lt >> 1) & 1u) ^ 1u, abort_flag, p.status,
-                       kStatusTimeoutMma))
+      const uint32_t d_tmem = tmem + b * C::BN;
+      // (MX and MXFP4: one per SF id, below)
+      const uint32_t idesc =
+          C::MX ? 0u : idesc_block_scaled(kFmtNvf4E2M1, kFmtNvf4E2M1, 0, 128, ncols, 0, 0);
+      for (int ks0 = 0; ks0 < p.ksteps; ks0 += C::KSUB) {
+        if (!mbar_wait(full_bar(stage), phase, abort_flag, p.status, kStatusTimeoutMma)) {
+          ok = false;
           break;
+        }
         tc_fence_after();
-        const uint32_t d_tmem = tmem + b * C::BN;
-        // (MX and MXFP4: one per SF id, below)
-        const uint32_t idesc =
-            C::MX ? 0u : idesc_block_scaled(kFmtNvf4E2M1, kFmtNvf4E2M1, 0, 128, ncols, 0, 0);
-        for (int ks0 = 0; ks0 < p.ksteps; ks0 += C::KSUB) {
-          if (!mbar_wait(full_bar(stage), phase, abort_flag, p.status, kStatusTimeoutMma)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          // scale slots of this stage's MMAs
-          constexpr int kSlots = C::KSUB * C::ATOMS;
-          uint32_t col[kSlots];
+        // scale slots of this stage's MMAs
+        constexpr int kSlots = C::KSUB * C::ATOMS;
+        uint32_t col[kSlots];
 #pragma unroll
-          for (int i = 0; i < kSlots; ++i) {
-            col[i] = tmem + C::SF_BASE + sfslot * C::SF_SLOT;
-            sfslot = (sfslot + 1 == C::NSLOTS) ? 0 : sfslot + 1;
-          }
-          const bool last = ks0 + C::KSUB >= p.ksteps;
-          if (elect_one()) {
+        for (int i = 0; i < kSlots; ++i) {
+          col[i] = tmem + C::SF_BASE + sfslot * C::SF_SLOT;
+          sfslot = (sfslot + 1 == C::NSLOTS) ? 0 : sfslot + 1;
+        }
+        const bool last = ks0 + C::KSUB >= p.ksteps;
+        if (elect_one()) {
 #pragma unroll
-            for (int sub = 0; sub < C::KSUB; ++sub) {
-              const int ks = ks0 + sub;
-              if constexpr (C::KSUB > 1) {
-                if (ks >= p.ksteps) break;
+          for (int sub = 0; sub < C::KSUB; ++sub) {
+            const int ks = ks0 + sub;
+            if constexpr (C::KSUB > 1) {
+              if (ks >= p.ksteps) break;
+            }
+            const int q = stage * C::KSUB + sub;  // this K step's slot in the stage
+            const uint64_t adesc = desc_k_sw128(sW(q));
+            const uint64_t bdesc = desc_k_sw128(sX(q));
+            if constexpr (C::MX) {
+              const uint32_t c0 = col[sub];
+              tc_cp_sf(c0, desc_sf_atom(sSFW(q)));
+#pragma unroll
+              for (int c = 0; c < C::CH; ++c)
+                if (c == 0 || ncols > 128 * c)
+                  tc_cp_sf(c0 + 4 + 4 * c, desc_sf_atom(sSFX(q) + c * 512));
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                // K step of 32 one-byte elements = 32 bytes = +2 in the start field;
+                // SF id j picks byte j of every scale column.
+                const uint32_t idj =
+                    idesc_block_scaled(kFmtF8E2M1, kFmtF8E4M3, 1, 128, ncols, j, j);
+                tc_mma_mxf8f6f4(d_tmem, adesc + 2u * j, bdesc + 2u * j, idj,
+                                c0 | (uint32_t(j) << 30), (c0 + 4) | (uint32_t(j) << 30),
+                                (ks | j) != 0 ? 1u : 0u);
               }
-              const int q = stage * C::KSUB + sub;  // this K step's slot in the stage
-              const uint64_t adesc = desc_k_sw128(sW(q));
-              const uint64_t bdesc = desc_k_sw128(sX(q));
-              if constexpr (C::MX) {
-                const uint32_t c0 = col[sub];
-                tc_cp_sf(c0, desc_sf_atom(sSFW(q)));
+            } else if constexpr (C::MX4) {
+#pragma unroll
+              for (int a = 0; a < 2; ++a) {
+                const uint32_t c0 = col[sub * 2 + a];
+                tc_cp_sf(c0, desc_sf_atom(sSFW(q) + a * 512));
 #pragma unroll
                 for (int c = 0; c < C::CH; ++c)
                   if (c == 0 || ncols > 128 * c)
-                    tc_cp_sf(c0 + 4 + 4 * c, desc_sf_atom(sSFX(q) + c * 512));
+                    tc_cp_sf(c0 + 4 + 4 * c, desc_sf_atom(sSFX(q) + (a * C::CH + c) * 512));
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                  // K step of 32 one-byte elements = 32 bytes = +2 in the start field;
-                  // SF id j picks byte j of every scale column.
-                  const uint32_t idj =
-                      idesc_block_scaled(kFmtF8E2M1, kFmtF8E4M3, 1, 128, ncols, j, j);
-                  tc_mma_mxf8f6f4(d_tmem, adesc + 2u * j, bdesc + 2u * j, idj,
-                                  c0 | (uint32_t(j) << 30), (c0 + 4) | (uint32_t(j) << 30),
-                                  (ks | j) != 0 ? 1u : 0u);
-                }
-              } else if constexpr (C::MX4) {
-#pragma unroll
-                for (int a = 0; a < 2; ++a) {
-                  const uint32_t c0 = col[sub * 2 + a];
-                  tc_cp_sf(c0, desc_sf_atom(sSFW(q) + a * 512));
-#pragma unroll
-                  for (int c = 0; c < C::CH; ++c)
-                    if (c == 0 || ncols > 128 * c)
-                      tc_cp_sf(c0 + 4 + 4 * c, desc_sf_atom(sSFX(q) + (a * C::CH + c) * 512));
-#pragma unroll
-                  for (int h = 0; h < 2; ++h) {
-                    // SF id 0 or 2: the scales of the atom's first or second 64 K elements
-                    const int j = 2 * a + h;
-                    const uint32_t id = 2u * h;
-                    tc_mma_mxf4(d_tmem, adesc + 2u * j, bdesc + 2u * j,
-                                idesc_block_scaled(kFmtNvf4E2M1, kFmtNvf4E2M1, 1, 128, ncols, id, id),
-                                c0 | (id << 30), (c0 + 4) | (id << 30), (ks | j) != 0 ? 1u : 0u);
-                  }
-                }
-              } else {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                  const uint32_t c0 = col[sub * 4 + j];
-                  tc_cp_sf(c0, desc_sf_atom(sSFW(q) + j * 512));
-                  // token scale atom c covers tokens [128 c, 128 c + 128): a tile
-                  // of ncols columns reads only the atoms it reaches
-#pragma unroll
-                  for (int c = 0; c < C::CH; ++c)
-                    if (c == 0 || ncols > 128 * c)
-                      tc_cp_sf(c0 + 4 + 4 * c, desc_sf_atom(sSFX(q) + (j * C::CH + c) * 512));
-                  // K step of 64 fp4 = 32 bytes = +2 in the descriptor's start field.
-                  tc_mma_nvf4(d_tmem, adesc + 2u * j, bdesc + 2u * j, idesc, c0, c0 + 4,
-                              (ks | j) != 0 ? 1u : 0u);
+                for (int h = 0; h < 2; ++h) {
+                  // SF id 0 or 2: the scales of the atom's first or second 64 K elements
+                  const int j = 2 * a + h;
+                  const uint32_t id = 2u * h;
+                  tc_mma_mxf4(d_tmem, adesc + 2u * j, bdesc + 2u * j,
+                              idesc_block_scaled(kFmtNvf4E2M1, kFmtNvf4E2M1, 1, 128, ncols, id, id),
+                              c0 | (id << 30), (c0 + 4) | (id << 30), (ks | j) != 0 ? 1u : 0u);
                 }
               }
+            } else {
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const uint32_t c0 = col[sub * 4 + j];
+                tc_cp_sf(c0, desc_sf_atom(sSFW(q) + j * 512));
+                // token scale atom c covers tokens [128 c, 128 c + 128): a tile
+                // of ncols columns reads only the atoms it reaches
+#pragma unroll
+                for (int c = 0; c < C::CH; ++c)
+                  if (c == 0 || ncols > 128 * c)
+                    tc_cp_sf(c0 + 4 + 4 * c, desc_sf_atom(sSFX(q) + (j * C::CH + c) * 512));
+                // K step of 64 fp4 = 32 bytes = +2 in the descriptor's start field.
+                tc_mma_nvf4(d_tmem, adesc + 2u * j, bdesc + 2u * j, idesc, c0, c0 + 4,
+                            (ks | j) != 0 ? 1u : 0u);
+              }
             }
-            tc_commit(empty_bar(stage));
-            if (last) tc_commit(accf_bar(b));
           }
-          __syncwarp();
-          issued_any = true;
-          if (++stage == C::STAGES) {
-            stage = 0;
-            phase ^= 1;
-          }
+          tc_commit(empty_bar(stage));
+          if (last) tc_commit(accf_bar(b));
         }
-        if (!ok) break;
-        ++lt;
+        __syncwarp();
+        issued_any = true;
+        if (++stage == C::STAGES) {
+          stage = 0;
+          phase ^= 1;
+        }
       }
-      // Drain: every tcgen05 op the warp issued completes before TMEM is freed.
-      if (issued_any) {
-        if (elect_one()) {
-          tc_commit(drain_bar);
-          if (!mbar_wait_one(drain_bar, 0, 200000000ull))
-            atomicCAS(p.status, 0, kStatusTimeoutDrain);
-        }
+      if (!ok) break;
+      ++lt;
+    }
+    // Drain: every tcgen05 op the warp issued completes before TMEM is freed.
+    if (issued_any) {
+      if (elect_one()) {
+        tc_commit(drain_bar);
+        if (!mbar_wait_one(drain_bar, 0, 200000000ull))
+          atomicCAS(p.status, 0, kStatusTimeoutDrain);
       }
     }
     __syncwarp();
-  } else if (warp >= 4 && !aborted_early) {
+  } else if (warp >= 4) {
     // ------------------------------------------------------------- epilogue
     const int q = warp & 3;  // TMEM lane quadrant this warp may read
     bool ok = mbar_wait(tmem_ready_bar, 0, abort_flag, p.status, kStatusTimeoutEpilogue);
     tc_fence_after();
     const uint32_t tmem = *tmem_holder;
+    if (ok && !tmem_in_range(tmem, C::TMEM_COLS)) {
+      give_up(p.status, abort_flag, kStatusBadTmem);
+      ok = false;
+    }
     int slot = 0;
     uint32_t sphase = 0;
     uint32_t lt = 0;
@@ -759,6 +803,10 @@ __global__ void __launch_bounds__(256, 1) fgg_gemm_kernel(const __grid_constant_
         sphase ^= 1;
       }
       if (s.tile == kEndTile) break;
+      if (!slot_in_range<C::BN>(p, s)) {
+        give_up(p.status, abort_flag, kStatusBadTile);
+        break;
+      }
       const int nti = int((s.tile >> 11) & 0x7FFu);
       const int ncols = min(C::BN, (s.rows + 15) & ~15);
       const uint32_t b = lt & 1u;
@@ -814,8 +862,10 @@ __global__ void __launch_bounds__(256, 1) fgg_gemm_kernel(const __grid_constant_
 // that the other CTA's threads arrive on: the schedule ring's, whose slots the
 // leader writes into the follower's shared memory, and the leader's acc-empty ones.
 // ====================================================================
-template <bool MX_, int STAGES_, int KSUB_ = 1, bool MX4_ = false>
+template <bool MX_, int STAGES_, int KSUB_ = 1, bool MX4_ = false, bool LIST_ = false>
 struct PairCfg {
+  static constexpr bool LIST = LIST_;
+  using Params = std::conditional_t<LIST, GemmListParams, GemmParams>;
   static constexpr bool MX = MX_;
   static constexpr bool MX4 = MX4_;
   static constexpr int ATOMS = MX ? 1 : MX4 ? 2 : 4;  // as in EngineCfg
@@ -871,7 +921,7 @@ struct PairCfg {
 
 template <class C>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
-    fgg_gemm_pair_kernel(const __grid_constant__ GemmParams p) {
+    fgg_gemm_pair_kernel(const __grid_constant__ typename C::Params p) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
@@ -927,12 +977,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
     mbar_init(drain_bar, 1);
     mbar_init(taken_bar, 1);
     *abort_flag = 0;
-    if constexpr (!C::MX) {
-      const PackHeader h = *p.pack;
-      // reported after griddep_wait: the prepare kernel resets the status word
-      if (h.magic != (C::MX4 ? kPackMagicMx : kPackMagic) || h.g != p.wg || h.n != p.n || h.k != p.k) *abort_flag = 2;
-    }
     fence_mbar_init();
+    if constexpr (!C::MX) prefetch_l2(p.pack);  // read after griddep_wait
   }
   // barrier inits visible to the peer before any of its loads or arrivals
   cluster_sync();
@@ -945,32 +991,38 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
     if (lane == 0) mbar_arrive(tmem_ready_bar);
   }
 
-  // Everything above (barriers, TMEM, the weight pack's header) is ready
-  // before this launch; the schedule, token descriptors and scale repack come
-  // from the prepare kernel just before it on the stream, which this launch
-  // may overlap (programmatic dependent launch).
+  // Everything above is this launch's own; the schedule and the scale repack come
+  // from the prepare kernel just before it on the stream, which this launch may
+  // overlap (programmatic dependent launch).  Nothing in global memory is read
+  // before this, the pack neither: its kernel may have been the one before that.
   griddep_wait();
-  const bool aborted_early = (*abort_flag != 0);
-  if (threadIdx.x == 0 && *abort_flag == 2) atomicCAS(p.status, 0, kStatusBadPack);
   const uint32_t leader_schede0 = mapa_shared(schede_bar(0), 0);
   const uint32_t leader_acce0 = mapa_shared(acce_bar(0), 0);
   const uint32_t leader_full0 = mapa_shared(full_bar(0), 0);
 
   if (warp == 3) {
     // ---------------------------------------------- scheduler (leader only)
-    if (lane == 0 && leader && !aborted_early) {
+    if (lane == 0 && leader) {
       int slot = 0;
       uint32_t sphase = 0;
-      const int num_tiles = p.num_tiles_dev != nullptr ? *p.num_tiles_dev : p.num_tiles;
+      int num_tiles = p.num_tiles_dev != nullptr ? *p.num_tiles_dev : p.num_tiles;
+      PackHeader header = {};
+      if constexpr (!C::MX) header = *p.pack;
+      int t = atomicAdd(p.status + 1, 1);  // on its way together with the header
+      if (!pack_matches<C>(p, header)) {  // refused before any load
+        atomicCAS(p.status, 0, kStatusBadPack);
+        num_tiles = 0;
+      }
       const uint32_t remote_ring0 = mapa_shared(smem_u32(const_cast<SchedSlot*>(ring)), peer);
       const uint32_t remote_schedf0 = mapa_shared(schedf_bar(0), peer);
       for (uint32_t n = 0;; ++n) {
         // one unstarted tile per pair at most (see the single-CTA kernel)
-        if (n > 0 && !mbar_wait1(taken_bar, (n - 1) & 1u, abort_flag, p.status,
-                                 kStatusTimeoutProducer))
-          break;
-        const int t = atomicAdd(p.status + 1, 1);
-        const uint32_t tile = (t < num_tiles) ? __ldg(p.tiles + t) : kEndTile;
+        if (n > 0) {
+          if (!mbar_wait1(taken_bar, (n - 1) & 1u, abort_flag, p.status, kStatusTimeoutProducer))
+            break;
+          t = atomicAdd(p.status + 1, 1);
+        }
+        const uint32_t tile = (t < num_tiles) ? p.tiles[t] : kEndTile;
         const SchedSlot s = make_slot<C::MX, C::BN>(p, tile);
         if (!mbar_wait1<true>(schede_bar(slot), sphase ^ 1, abort_flag, p.status,
                               kStatusTimeoutProducer))
@@ -991,259 +1043,261 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
     // ------------------------------------------------- producer (both CTAs)
     // The whole warp runs the loop (operands warp-uniform), one elected lane
     // issues the loads.
-    if (!aborted_early) {
-      int stage = 0;
-      uint32_t phase = 0;
-      int slot = 0;
-      uint32_t sphase = 0;
-      uint32_t arms = 0;
+    int stage = 0;
+    uint32_t phase = 0;
+    int slot = 0;
+    uint32_t sphase = 0;
+    uint32_t arms = 0;
+    if (lane == 0) {
+      if constexpr (C::MX || C::MX4) prefetch_tensormap(&p.mx_tmap_w);
+      if constexpr (!C::LIST) prefetch_tensormap(&p.tmap_x_flat);
+      prefetch_tensormap(&p.sfw_map);
+      prefetch_tensormap(&p.sfx_map);
+    }
+    while (true) {
+      if (!mbar_wait<true>(schedf_bar(slot), sphase, abort_flag, p.status,
+                           kStatusTimeoutProducer))
+        break;
+      const uint32_t tile = __shfl_sync(kFullMask, ring[slot].tile, 0);
+      const int rows = __shfl_sync(kFullMask, ring[slot].rows, 0);
+      const int xtile_index = __shfl_sync(kFullMask, ring[slot].xtile_index, 0);
+      const int wgroup = __shfl_sync(kFullMask, ring[slot].wgroup, 0);
+      const int row0 = __shfl_sync(kFullMask, ring[slot].row0, 0);
       if (lane == 0) {
-        if constexpr (C::MX || C::MX4) prefetch_tensormap(&p.mx_tmap_w);
-        if (C::MX || p.x_flat) prefetch_tensormap(&p.tmap_x_flat);
-        prefetch_tensormap(&p.sfw_map);
-        prefetch_tensormap(&p.sfx_map);
+        mbar_arrive(schede_bar(slot));
+        if (leader) mbar_arrive(taken_bar);
       }
-      while (true) {
-        if (!mbar_wait<true>(schedf_bar(slot), sphase, abort_flag, p.status,
-                             kStatusTimeoutProducer))
-          break;
-        const uint32_t tile = __shfl_sync(kFullMask, ring[slot].tile, 0);
-        const int rows = __shfl_sync(kFullMask, ring[slot].rows, 0);
-        const int xtile_index = __shfl_sync(kFullMask, ring[slot].xtile_index, 0);
-        const int wgroup = __shfl_sync(kFullMask, ring[slot].wgroup, 0);
-        const int row0 = __shfl_sync(kFullMask, ring[slot].row0, 0);
-        if (lane == 0) {
-          mbar_arrive(schede_bar(slot));
-          if (leader) mbar_arrive(taken_bar);
-        }
-        if (++slot == C::SCHED) {
-          slot = 0;
-          sphase ^= 1;
-        }
-        if (tile == kEndTile) {
-          if (lane == 0) griddep_launch_dependents();  // as in the single-CTA kernel
-          break;
-        }
-        const int g = int(tile >> 22);
-        const int nti = int((tile >> 11) & 0x7FFu);
-        const int xti = int(tile & 0x7FFu);
-        // the group and weight group index descriptor arrays: never trust them blindly
-        if (g >= p.g || unsigned(wgroup) >= unsigned(p.wg)) {
-          if (lane == 0) {
-            atomicCAS(p.status, 0, kStatusBadTile);
-            *abort_flag = 1;
-          }
-          break;
-        }
-        const int half = tile_ncols(rows) >> 1;
-        const CUtensorMap* tw;
-        const CUtensorMap* tx;
-        // bytes both CTAs' loads of one K step deliver to the leader's barrier
-        uint32_t tx_step = 2u * C::TX_CTA;
-        if constexpr (C::MX) {
+      if (++slot == C::SCHED) {
+        slot = 0;
+        sphase ^= 1;
+      }
+      if (tile == kEndTile) {
+        if (lane == 0) griddep_launch_dependents();  // as in the single-CTA kernel
+        break;
+      }
+      const int g = int(tile >> 22);
+      const int nti = int((tile >> 11) & 0x7FFu);
+      const int xti = int(tile & 0x7FFu);
+      bool known = g < p.g && unsigned(wgroup) < unsigned(p.wg) && nti < p.nt &&
+                   unsigned(xtile_index) < unsigned(p.xtiles);
+      if constexpr (C::LIST) known = known && unsigned(g - p.g0) < unsigned(kListMaps);
+      if (!known) {
+        give_up(p.status, abort_flag, kStatusBadTile);
+        break;
+      }
+      const int half = tile_ncols(rows) >> 1;
+      const CUtensorMap* tw;
+      const CUtensorMap* tx;
+      // bytes both CTAs' loads of one K step deliver to the leader's barrier
+      uint32_t tx_step = 2u * C::TX_CTA;
+      if constexpr (C::MX) {
+        tw = &p.mx_tmap_w;
+        tx = &p.tmap_x_flat;
+      } else {
+        if constexpr (C::MX4) {
           tw = &p.mx_tmap_w;
-          tx = &p.tmap_x_flat;
         } else {
-          if constexpr (C::MX4) {
-            tw = &p.mx_tmap_w;
-          } else {
-            tw = p.tmap_w + wgroup;
-            tensormap_acquire(tw);  // every lane: the issuing one among them
-          }
-          if (p.x_flat) {
-            tx = &p.tmap_x_flat;
-            // a narrow tile (half a multiple of 16 below BNH) loads its rows only
-            if (p.x_small && half >= 16 && half < C::BNH) {
-              tx = &p.tmap_x_small[half / 16 - 1];
-              tx_step = 2u * (C::TX_CTA - C::X_BYTES + uint32_t(half) * 128u);
-            }
-          } else {
-            tx = p.tmap_x + g;
-            tensormap_acquire(tx);
+          tw = p.tmap_w + wgroup;
+          tensormap_acquire(tw);  // every lane: the issuing one among them
+        }
+        if constexpr (C::LIST) {
+          tx = &p.tmap_x[g - p.g0];
+        } else {
+          tx = &p.tmap_x_flat;
+          // a narrow tile (half a multiple of 16 below BNH) loads its rows only
+          if (p.x_small && half >= 16 && half < C::BNH) {
+            tx = &p.tmap_x_small[half / 16 - 1];
+            tx_step = 2u * (C::TX_CTA - C::X_BYTES + uint32_t(half) * 128u);
           }
         }
-        const int wrow = nti * 256 + int(rank) * 128;
-        // this CTA's first token row in the map's coordinates
-        const int xrow = ((C::MX || p.x_flat) ? row0 : xti * C::BN) + int(rank) * half;
-        // this CTA's weight scale atoms of the tile: one row of SFW_BYTES per K step
-        const int sfw_y =
-            ((wgroup * p.nt128 + 2 * nti + int(rank)) * p.ksteps) * int(C::SFW_BOX_ROWS);
-        const int sfx_y = (xtile_index * p.ksteps) * int(C::SFX_BOX_ROWS);
-        bool ok = true;
-        for (int ks0 = 0; ks0 < p.ksteps; ks0 += C::KSUB) {
-          if (!mbar_wait(empty_bar(stage), phase ^ 1, abort_flag, p.status,
-                         kStatusTimeoutProducer)) {
-            ok = false;
-            break;
+      }
+      const int wrow = nti * 256 + int(rank) * 128;
+      // this CTA's first token row in the map's coordinates
+      const int xrow = (C::LIST ? xti * C::BN : row0) + int(rank) * half;
+      // this CTA's weight scale atoms of the tile: one row of SFW_BYTES per K step
+      const int sfw_y =
+          ((wgroup * p.nt128 + 2 * nti + int(rank)) * p.ksteps) * int(C::SFW_BOX_ROWS);
+      const int sfx_y = (xtile_index * p.ksteps) * int(C::SFX_BOX_ROWS);
+      bool ok = true;
+      for (int ks0 = 0; ks0 < p.ksteps; ks0 += C::KSUB) {
+        if (!mbar_wait(empty_bar(stage), phase ^ 1, abort_flag, p.status,
+                       kStatusTimeoutProducer)) {
+          ok = false;
+          break;
+        }
+        const uint32_t fb = leader_full0 + 8u * stage;
+        const bool arm = (p.debug_flags & kDebugNoLoads) == 0;
+        if (arm && elect_one()) {
+          if (leader) {
+            if constexpr (C::KSUB == 1)
+              mbar_arrive_expect_tx(full_bar(stage), tx_step);
+            else
+              mbar_arrive_expect_tx(full_bar(stage),
+                                    tx_step * uint32_t(min(C::KSUB, p.ksteps - ks0)));
           }
-          const uint32_t fb = leader_full0 + 8u * stage;
-          const bool arm = (p.debug_flags & kDebugNoLoads) == 0;
-          if (arm && elect_one()) {
-            if (leader) {
-              if constexpr (C::KSUB == 1)
-                mbar_arrive_expect_tx(full_bar(stage), tx_step);
-              else
-                mbar_arrive_expect_tx(full_bar(stage),
-                                      tx_step * uint32_t(min(C::KSUB, p.ksteps - ks0)));
-            }
 #pragma unroll
-            for (int sub = 0; sub < C::KSUB; ++sub) {
-              const int ks = ks0 + sub;
-              if constexpr (C::KSUB > 1) {
-                if (ks >= p.ksteps) break;
-              }
-              const int q = stage * C::KSUB + sub;
-              if constexpr (C::MX)
-                tma_load_3d_pair(sW(q), tw, fb, ks * C::K_STEP, wrow, g);
-              else if constexpr (C::MX4)
-                tma_load_3d_pair(sW(q), tw, fb, ks * 128, wrow, wgroup);
-              else
-                tma_load_2d_pair(sW(q), tw, fb, ks * 128, wrow);
-              tma_load_2d_pair(sX(q), tx, fb, ks * 128, xrow);
-              tma_load_2d_pair(sSFW(q), &p.sfw_map, fb, 0, sfw_y + ks * int(C::SFW_BOX_ROWS));
-              tma_load_2d_pair(sSFX(q), &p.sfx_map, fb, 0, sfx_y + ks * int(C::SFX_BOX_ROWS));
+          for (int sub = 0; sub < C::KSUB; ++sub) {
+            const int ks = ks0 + sub;
+            if constexpr (C::KSUB > 1) {
+              if (ks >= p.ksteps) break;
             }
-          }
-          __syncwarp();
-          if (arm) ++arms;
-          if (++stage == C::STAGES) {
-            stage = 0;
-            phase ^= 1;
+            const int q = stage * C::KSUB + sub;
+            if constexpr (C::MX)
+              tma_load_3d_pair(sW(q), tw, fb, ks * C::K_STEP, wrow, g);
+            else if constexpr (C::MX4)
+              tma_load_3d_pair(sW(q), tw, fb, ks * 128, wrow, wgroup);
+            else
+              tma_load_2d_pair(sW(q), tw, fb, ks * 128, wrow);
+            tma_load_2d_pair(sX(q), tx, fb, ks * 128, xrow);
+            tma_load_2d_pair(sSFW(q), &p.sfw_map, fb, 0, sfw_y + ks * int(C::SFW_BOX_ROWS));
+            tma_load_2d_pair(sSFX(q), &p.sfx_map, fb, 0, sfx_y + ks * int(C::SFX_BOX_ROWS));
           }
         }
-        if (!ok) break;
+        __syncwarp();
+        if (arm) ++arms;
+        if (++stage == C::STAGES) {
+          stage = 0;
+          phase ^= 1;
+        }
       }
-      // the leader's full barriers cover both CTAs' bytes: drain them before exit
-      if (leader && lane == 0) {
-        const uint32_t first = arms > uint32_t(C::STAGES) ? arms - C::STAGES : 0u;
-        for (uint32_t a = first; a < arms; ++a)
-          mbar_wait_one(full_bar(int(a % C::STAGES)), (a / C::STAGES) & 1u, 200000000ull);
-      }
+      if (!ok) break;
+    }
+    // the leader's full barriers cover both CTAs' bytes: drain them before exit
+    if (leader && lane == 0) {
+      const uint32_t first = arms > uint32_t(C::STAGES) ? arms - C::STAGES : 0u;
+      for (uint32_t a = first; a < arms; ++a)
+        mbar_wait_one(full_bar(int(a % C::STAGES)), (a / C::STAGES) & 1u, 200000000ull);
     }
     __syncwarp();
   } else if (warp == 1 && leader) {
     // ------------------------------------------------------- MMA issuer
     // The whole warp runs the loop; one elect.sync region per stage issues its
     // scale uploads, MMAs and commits with warp-uniform operands.
-    if (!aborted_early) {
-      bool ok = mbar_wait(tmem_ready_bar, 0, abort_flag, p.status, kStatusTimeoutMma);
+    bool ok = mbar_wait(tmem_ready_bar, 0, abort_flag, p.status, kStatusTimeoutMma);
+    tc_fence_after();
+    const uint32_t tmem = __shfl_sync(kFullMask, *tmem_holder, 0);
+    if (ok && !tmem_in_range(tmem, C::TMEM_COLS)) {
+      give_up(p.status, abort_flag, kStatusBadTmem);
+      ok = false;
+    }
+    int stage = 0;
+    uint32_t phase = 0;
+    int slot = 0;
+    uint32_t sphase = 0;
+    uint32_t lt = 0;
+    int sfslot = 0;
+    bool issued_any = false;
+    while (ok) {
+      if (!mbar_wait<true>(schedf_bar(slot), sphase, abort_flag, p.status, kStatusTimeoutMma))
+        break;
+      const uint32_t tile = __shfl_sync(kFullMask, ring[slot].tile, 0);
+      const int rows = __shfl_sync(kFullMask, ring[slot].rows, 0);
+      if (lane == 0) mbar_arrive(schede_bar(slot));
+      if (++slot == C::SCHED) {
+        slot = 0;
+        sphase ^= 1;
+      }
+      if (tile == kEndTile) break;
+      if (rows <= 0 || rows > C::BN) {
+        give_up(p.status, abort_flag, kStatusBadTile);
+        break;
+      }
+      const int ncols = tile_ncols(rows);
+      const uint32_t b = lt & 1u;
+      if (!mbar_wait<true>(acce_bar(b), ((lt >> 1) & 1u) ^ 1u, abort_flag, p.status,
+                           kStatusTimeoutMma))
+        break;
       tc_fence_after();
-      const uint32_t tmem = __shfl_sync(kFullMask, *tmem_holder, 0);
-      int stage = 0;
-      uint32_t phase = 0;
-      int slot = 0;
-      uint32_t sphase = 0;
-      uint32_t lt = 0;
-      int sfslot = 0;
-      bool issued_any = false;
-      while (ok) {
-        if (!mbar_wait<true>(schedf_bar(slot), sphase, abort_flag, p.status, kStatusTimeoutMma))
+      const uint32_t d_tmem = tmem + b * C::BN;
+      const uint32_t idesc =
+          C::MX ? 0u : idesc_block_scaled(kFmtNvf4E2M1, kFmtNvf4E2M1, 0, 256, ncols, 0, 0);
+      for (int ks0 = 0; ks0 < p.ksteps; ks0 += C::KSUB) {
+        if (!mbar_wait(full_bar(stage), phase, abort_flag, p.status, kStatusTimeoutMma)) {
+          ok = false;
           break;
-        const uint32_t tile = __shfl_sync(kFullMask, ring[slot].tile, 0);
-        const int rows = __shfl_sync(kFullMask, ring[slot].rows, 0);
-        if (lane == 0) mbar_arrive(schede_bar(slot));
-        if (++slot == C::SCHED) {
-          slot = 0;
-          sphase ^= 1;
         }
-        if (tile == kEndTile) break;
-        const int ncols = tile_ncols(rows);
-        const uint32_t b = lt & 1u;
-        if (!mbar_wait<true>(acce_bar(b), ((lt >> 1) & 1u) ^ 1u, abort_flag, p.status,
-                             kStatusTimeoutMma))
-          break;
         tc_fence_after();
-        const uint32_t d_tmem = tmem + b * C::BN;
-        const uint32_t idesc =
-            C::MX ? 0u : idesc_block_scaled(kFmtNvf4E2M1, kFmtNvf4E2M1, 0, 256, ncols, 0, 0);
-        for (int ks0 = 0; ks0 < p.ksteps; ks0 += C::KSUB) {
-          if (!mbar_wait(full_bar(stage), phase, abort_flag, p.status, kStatusTimeoutMma)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          // scale slots of this stage's MMAs
-          constexpr int kSlots = C::KSUB * C::ATOMS;
-          uint32_t col[kSlots];
+        // scale slots of this stage's MMAs
+        constexpr int kSlots = C::KSUB * C::ATOMS;
+        uint32_t col[kSlots];
 #pragma unroll
-          for (int i = 0; i < kSlots; ++i) {
-            col[i] = tmem + C::SF_BASE + sfslot * C::SF_SLOT;
-            sfslot = (sfslot + 1 == C::NSLOTS) ? 0 : sfslot + 1;
-          }
-          const bool last = ks0 + C::KSUB >= p.ksteps;
-          if (elect_one()) {
+        for (int i = 0; i < kSlots; ++i) {
+          col[i] = tmem + C::SF_BASE + sfslot * C::SF_SLOT;
+          sfslot = (sfslot + 1 == C::NSLOTS) ? 0 : sfslot + 1;
+        }
+        const bool last = ks0 + C::KSUB >= p.ksteps;
+        if (elect_one()) {
 #pragma unroll
-            for (int sub = 0; sub < C::KSUB; ++sub) {
-              const int ks = ks0 + sub;
-              if constexpr (C::KSUB > 1) {
-                if (ks >= p.ksteps) break;
+          for (int sub = 0; sub < C::KSUB; ++sub) {
+            const int ks = ks0 + sub;
+            if constexpr (C::KSUB > 1) {
+              if (ks >= p.ksteps) break;
+            }
+            const int q = stage * C::KSUB + sub;  // this K step's slot in the stage
+            const uint64_t adesc = desc_k_sw128(sW(q));
+            const uint64_t bdesc = desc_k_sw128(sX(q));
+            if constexpr (C::MX) {
+              const uint32_t c0 = col[sub];
+              tc_cp_sf_pair(c0, desc_sf_atom(sSFW(q)));
+              tc_cp_sf_pair(c0 + 4, desc_sf_atom(sSFX(q)));
+              if (ncols > 128) tc_cp_sf_pair(c0 + 8, desc_sf_atom(sSFX(q) + 512));
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const uint32_t idj =
+                    idesc_block_scaled(kFmtF8E2M1, kFmtF8E4M3, 1, 256, ncols, j, j);
+                tc_mma_mxf8f6f4_pair(d_tmem, adesc + 2u * j, bdesc + 2u * j, idj,
+                                     c0 | (uint32_t(j) << 30), (c0 + 4) | (uint32_t(j) << 30),
+                                     (ks | j) != 0 ? 1u : 0u);
               }
-              const int q = stage * C::KSUB + sub;  // this K step's slot in the stage
-              const uint64_t adesc = desc_k_sw128(sW(q));
-              const uint64_t bdesc = desc_k_sw128(sX(q));
-              if constexpr (C::MX) {
-                const uint32_t c0 = col[sub];
-                tc_cp_sf_pair(c0, desc_sf_atom(sSFW(q)));
-                tc_cp_sf_pair(c0 + 4, desc_sf_atom(sSFX(q)));
-                if (ncols > 128) tc_cp_sf_pair(c0 + 8, desc_sf_atom(sSFX(q) + 512));
+            } else if constexpr (C::MX4) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                  const uint32_t idj =
-                      idesc_block_scaled(kFmtF8E2M1, kFmtF8E4M3, 1, 256, ncols, j, j);
-                  tc_mma_mxf8f6f4_pair(d_tmem, adesc + 2u * j, bdesc + 2u * j, idj,
-                                       c0 | (uint32_t(j) << 30), (c0 + 4) | (uint32_t(j) << 30),
-                                       (ks | j) != 0 ? 1u : 0u);
+              for (int a = 0; a < 2; ++a) {
+                const uint32_t c0 = col[sub * 2 + a];
+                tc_cp_sf_pair(c0, desc_sf_atom(sSFW(q) + a * 512));
+                tc_cp_sf_pair(c0 + 4, desc_sf_atom(sSFX(q) + (2 * a) * 512));
+                if (ncols > 128) tc_cp_sf_pair(c0 + 8, desc_sf_atom(sSFX(q) + (2 * a + 1) * 512));
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                  const int j = 2 * a + h;
+                  const uint32_t id = 2u * h;
+                  tc_mma_mxf4_pair(
+                      d_tmem, adesc + 2u * j, bdesc + 2u * j,
+                      idesc_block_scaled(kFmtNvf4E2M1, kFmtNvf4E2M1, 1, 256, ncols, id, id),
+                      c0 | (id << 30), (c0 + 4) | (id << 30), (ks | j) != 0 ? 1u : 0u);
                 }
-              } else if constexpr (C::MX4) {
+              }
+            } else {
 #pragma unroll
-                for (int a = 0; a < 2; ++a) {
-                  const uint32_t c0 = col[sub * 2 + a];
-                  tc_cp_sf_pair(c0, desc_sf_atom(sSFW(q) + a * 512));
-                  tc_cp_sf_pair(c0 + 4, desc_sf_atom(sSFX(q) + (2 * a) * 512));
-                  if (ncols > 128) tc_cp_sf_pair(c0 + 8, desc_sf_atom(sSFX(q) + (2 * a + 1) * 512));
-#pragma unroll
-                  for (int h = 0; h < 2; ++h) {
-                    const int j = 2 * a + h;
-                    const uint32_t id = 2u * h;
-                    tc_mma_mxf4_pair(
-                        d_tmem, adesc + 2u * j, bdesc + 2u * j,
-                        idesc_block_scaled(kFmtNvf4E2M1, kFmtNvf4E2M1, 1, 256, ncols, id, id),
-                        c0 | (id << 30), (c0 + 4) | (id << 30), (ks | j) != 0 ? 1u : 0u);
-                  }
-                }
-              } else {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                  const uint32_t c0 = col[sub * 4 + j];
-                  tc_cp_sf_pair(c0, desc_sf_atom(sSFW(q) + j * 512));
-                  tc_cp_sf_pair(c0 + 4, desc_sf_atom(sSFX(q) + (2 * j) * 512));
-                  // tokens 128..223: only a tile wider than 128 columns reads them
-                  if (ncols > 128)
-                    tc_cp_sf_pair(c0 + 8, desc_sf_atom(sSFX(q) + (2 * j + 1) * 512));
-                  tc_mma_nvf4_pair(d_tmem, adesc + 2u * j, bdesc + 2u * j, idesc, c0, c0 + 4,
-                                   (ks | j) != 0 ? 1u : 0u);
-                }
+              for (int j = 0; j < 4; ++j) {
+                const uint32_t c0 = col[sub * 4 + j];
+                tc_cp_sf_pair(c0, desc_sf_atom(sSFW(q) + j * 512));
+                tc_cp_sf_pair(c0 + 4, desc_sf_atom(sSFX(q) + (2 * j) * 512));
+                // tokens 128..223: only a tile wider than 128 columns reads them
+                if (ncols > 128)
+                  tc_cp_sf_pair(c0 + 8, desc_sf_atom(sSFX(q) + (2 * j + 1) * 512));
+                tc_mma_nvf4_pair(d_tmem, adesc + 2u * j, bdesc + 2u * j, idesc, c0, c0 + 4,
+                                 (ks | j) != 0 ? 1u : 0u);
               }
             }
-            tc_commit_pair(empty_bar(stage), 0x3);
-            if (last) tc_commit_pair(accf_bar(b), 0x3);
           }
-          __syncwarp();
-          issued_any = true;
-          if (++stage == C::STAGES) {
-            stage = 0;
-            phase ^= 1;
-          }
+          tc_commit_pair(empty_bar(stage), 0x3);
+          if (last) tc_commit_pair(accf_bar(b), 0x3);
         }
-        if (!ok) break;
-        ++lt;
+        __syncwarp();
+        issued_any = true;
+        if (++stage == C::STAGES) {
+          stage = 0;
+          phase ^= 1;
+        }
       }
-      if (issued_any) {
-        if (elect_one()) {
-          tc_commit_pair(drain_bar, 0x1);
-          if (!mbar_wait_one(drain_bar, 0, 200000000ull))
-            atomicCAS(p.status, 0, kStatusTimeoutDrain);
-        }
+      if (!ok) break;
+      ++lt;
+    }
+    if (issued_any) {
+      if (elect_one()) {
+        tc_commit_pair(drain_bar, 0x1);
+        if (!mbar_wait_one(drain_bar, 0, 200000000ull))
+          atomicCAS(p.status, 0, kStatusTimeoutDrain);
       }
     }
     __syncwarp();
@@ -1254,38 +1308,38 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
     // warp's global stores, so it is done by a warp that has none, once the readers
     // have arrived here: both arrivals of a tile at once, as each by itself takes
     // long enough to hold up tiles of few tokens (64 groups, 544 rows, 7168 x 2048:
-    // 88 -> 96 us with one after the other).
-    if (!aborted_early) {
-      int slot = 0;
-      uint32_t sphase = 0;
-      uint32_t lt = 0;
-      while (true) {
-        if (!mbar_wait<true>(schedf_bar(slot), sphase, abort_flag, p.status,
-                             kStatusTimeoutEpilogue))
-          break;
-        const uint32_t tile = __shfl_sync(kFullMask, ring[slot].tile, 0);
-        if (tile == kEndTile) break;
-        const uint32_t b = lt & 1u;
-        if (!mbar_wait(schede_bar(slot), sphase, abort_flag, p.status, kStatusTimeoutEpilogue) ||
-            !mbar_wait(acce_bar(b), (lt >> 1) & 1u, abort_flag, p.status, kStatusTimeoutEpilogue))
-          break;
-        tc_fence_after();
-        tc_fence_before();
-        if (lane < 2) mbar_arrive_remote(lane == 0 ? leader_acce0 + 8u * b : leader_schede0 + 8u * slot);
-        if (++slot == C::SCHED) {
-          slot = 0;
-          sphase ^= 1;
-        }
-        ++lt;
-      }
+    // 88 -> 96 us with one after the other).  What the last tile frees nobody waits
+    // for; the slot after a tile's is published once the producer has the tile.
+    int slot = 0;
+    uint32_t sphase = 0;
+    uint32_t lt = 0;
+    bool ok = mbar_wait<true>(schedf_bar(0), 0, abort_flag, p.status, kStatusTimeoutEpilogue);
+    while (ok && __shfl_sync(kFullMask, ring[slot].tile, 0) != kEndTile) {
+      const uint32_t b = lt & 1u;
+      const int next = slot + 1 == C::SCHED ? 0 : slot + 1;
+      const uint32_t nphase = next == 0 ? sphase ^ 1u : sphase;
+      ok = mbar_wait(schede_bar(slot), sphase, abort_flag, p.status, kStatusTimeoutEpilogue) &&
+           mbar_wait(acce_bar(b), (lt >> 1) & 1u, abort_flag, p.status, kStatusTimeoutEpilogue) &&
+           mbar_wait<true>(schedf_bar(next), nphase, abort_flag, p.status, kStatusTimeoutEpilogue);
+      if (!ok || __shfl_sync(kFullMask, ring[next].tile, 0) == kEndTile) break;
+      tc_fence_after();
+      tc_fence_before();
+      if (lane < 2) mbar_arrive_remote(lane == 0 ? leader_acce0 + 8u * b : leader_schede0 + 8u * slot);
+      slot = next;
+      sphase = nphase;
+      ++lt;
     }
     __syncwarp();
-  } else if (warp >= 4 && !aborted_early) {
+  } else if (warp >= 4) {
     // --------------------------------------------------------- epilogue
     const int q = warp & 3;
     bool ok = mbar_wait(tmem_ready_bar, 0, abort_flag, p.status, kStatusTimeoutEpilogue);
     tc_fence_after();
     const uint32_t tmem = *tmem_holder;
+    if (ok && !tmem_in_range(tmem, C::TMEM_COLS)) {
+      give_up(p.status, abort_flag, kStatusBadTmem);
+      ok = false;
+    }
     int slot = 0;
     uint32_t sphase = 0;
     uint32_t lt = 0;
@@ -1301,6 +1355,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
         sphase ^= 1;
       }
       if (s.tile == kEndTile) break;
+      if (!slot_in_range<C::BN>(p, s)) {
+        give_up(p.status, abort_flag, kStatusBadTile);
+        break;
+      }
       const int nti = int((s.tile >> 11) & 0x7FFu);
       const int ncols = tile_ncols(s.rows);
       const uint32_t b = lt & 1u;
@@ -1362,7 +1420,7 @@ cudaError_t launch_dependent(Kernel kernel, int grid, uint32_t smem, cudaStream_
 // Raise the kernel's dynamic shared memory limit (once per context), then launch
 // one CTA pair per two SMs, or one per tile when there are fewer tiles.  Host only.
 template <class C>
-cudaError_t launch_pair(const GemmParams& gp, int sm_count, cudaStream_t s) {
+cudaError_t launch_pair(const typename C::Params& gp, int sm_count, cudaStream_t s) {
   if (ensure_max_dynamic_smem(reinterpret_cast<const void*>(fgg_gemm_pair_kernel<C>),
                               int(C::SMEM_BYTES)) != FGG_OK)
     return cudaErrorInvalidValue;
@@ -1374,7 +1432,7 @@ cudaError_t launch_pair(const GemmParams& gp, int sm_count, cudaStream_t s) {
 // Raise the kernel's dynamic shared memory limit (once per context), then launch
 // one CTA per SM, or one per tile when there are fewer tiles.  Host only.
 template <class C>
-cudaError_t launch_engine(const GemmParams& gp, int sm_count, cudaStream_t s) {
+cudaError_t launch_engine(const typename C::Params& gp, int sm_count, cudaStream_t s) {
   if (ensure_max_dynamic_smem(reinterpret_cast<const void*>(fgg_gemm_kernel<C>),
                               int(C::SMEM_BYTES)) != FGG_OK)
     return cudaErrorInvalidValue;

@@ -124,6 +124,7 @@ struct F16Params {
   int32_t c_ext;   // wgrad: extent of the N axis (k)
   int32_t ksteps;  // forward, dgrad: 64-element steps of the contraction
   int32_t mts, cts;
+  int32_t max_rows;
   int32_t grid_units;  // host bound on the tiles and slices
   int32_t bf16;        // operands bf16 (1) or fp16 (0)
   int32_t out_fp32;    // wgrad: fp32 gradient
@@ -412,7 +413,7 @@ __device__ __forceinline__ F16Slot f16_make_slot(const F16Params& p, int unit, i
   if constexpr (C::SPLIT) {
     t += split_tiles - split_units;
     if (unit < split_units) {
-      s.split = __ldg(p.units + unit);
+      s.split = p.units[unit];
       t = int(s.split & 0xFFu);
     }
   }
@@ -421,16 +422,16 @@ __device__ __forceinline__ F16Slot f16_make_slot(const F16Params& p, int unit, i
     const int per = p.mts * p.cts;
     const int pos = t / per;
     const int local = t - pos * per;
-    s.g = __ldg(p.order + pos);
+    s.g = p.order[pos];
     f16_place(local, p.mts, p.cts, &s.mt, &s.ct);
-    s.row0 = __ldg(p.offsets + s.g);
-    s.rows = __ldg(p.offsets + s.g + 1) - s.row0;
+    s.row0 = p.offsets[s.g];
+    s.rows = p.offsets[s.g + 1] - s.row0;
   } else {
-    const uint64_t tile = __ldg(p.tiles + t);
+    const uint64_t tile = p.tiles[t];
     s.g = int(tile >> 48);
     s.mt = int((tile >> 32) & 0xFFFFu);
     s.row0 = int(uint32_t(tile));
-    s.rows = __ldg(p.tile_rows + t);
+    s.rows = p.tile_rows[t];
   }
   s.k1 = C::MODE == kWgrad ? wgrad_steps(s.rows) : p.ksteps;
   if (C::SPLIT && s.split != 0) {
@@ -439,6 +440,16 @@ __device__ __forceinline__ F16Slot f16_make_slot(const F16Params& p, int unit, i
     s.k1 = int(steps * (slice + 1) / slices);
   }
   return s;
+}
+
+// What forms addresses is checked before it does: a tile that is not one of the
+// problem's ends the kernel with a status.
+template <class C>
+__device__ __forceinline__ bool f16_slot_in_range(const F16Params& p, const F16Slot& s) {
+  const bool rows = C::MODE == kWgrad ? s.rows >= 0 : s.rows > 0 && s.rows <= C::BN;
+  return rows && unsigned(s.g) < unsigned(p.num_groups) && unsigned(s.mt) < unsigned(p.mts) &&
+         unsigned(s.ct) < unsigned(p.cts) && s.row0 >= 0 && s.row0 <= p.max_rows - s.rows &&
+         (s.split >> 24) + (s.split >> 8 & 0xFFu) < unsigned(kMaxSplitUnits);
 }
 
 // Roles as in the block-scaled pair kernel (fgg_engine.cuh): warp 0 producer in
@@ -559,8 +570,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(C::THREADS, 1)
           // few units: one for each pair, none claimed ahead of a pair that has none
           const int unit = few ? (n == 0 ? int(blockIdx.x >> 1) : num_units)
                                : atomicAdd(p.status + 1, 1);
-          const F16Slot s =
-              f16_make_slot<C>(p, unit, num_tiles, split_tiles, split_units);
+          F16Slot s = f16_make_slot<C>(p, unit, num_tiles, split_tiles, split_units);
+          if (s.g != -1 && !f16_slot_in_range<C>(p, s)) {
+            atomicCAS(p.status, 0, kStatusBadTile);
+            s.g = -1;
+          }
           if (!mbar_wait1<true>(schede_bar(slot), sphase ^ 1, abort_flag, p.status,
                                 kStatusTimeoutProducer))
             break;
@@ -684,6 +698,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(C::THREADS, 1)
       bool ok = mbar_wait(tmem_ready_bar, 0, abort_flag, p.status, kStatusTimeoutMma);
       tc_fence_after();
       const uint32_t tmem = __shfl_sync(kFullMask, *tmem_holder, 0);
+      if (ok && !tmem_in_range(tmem, C::TMEM_COLS)) {
+        give_up(p.status, abort_flag, kStatusBadTmem);
+        ok = false;
+      }
       int stage = 0;
       uint32_t phase = 0;
       int slot = 0;
@@ -771,41 +789,41 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(C::THREADS, 1)
       // The leader writes this CTA's slots and its MMAs this CTA's accumulators, so
       // what frees them for it is released at cluster scope.  That waits for the
       // warp's global stores, so it is done by a warp that has none, once the
-      // readers have arrived here: a tile's slot with its first accumulator.
+      // readers have arrived here: a tile's slot with its first accumulator.  The
+      // last accumulator of the last tile nobody waits for; the slot after a tile's
+      // is published once the producer has the tile.
       int slot = 0;
       uint32_t sphase = 0;
       uint32_t lt = 0;
-      bool ok = true;
-      while (ok) {
-        if (!mbar_wait<true>(schedf_bar(slot), sphase, abort_flag, p.status,
-                             kStatusTimeoutEpilogue))
-          break;
-        const int g = __shfl_sync(kFullMask, ring[slot].g, 0);
+      bool ok = mbar_wait<true>(schedf_bar(0), 0, abort_flag, p.status, kStatusTimeoutEpilogue);
+      bool more = ok && __shfl_sync(kFullMask, ring[0].g, 0) >= 0;
+      while (more) {
         const int rows = __shfl_sync(kFullMask, ring[slot].rows, 0);
         const int k0 = unit_k0(slot);
         const int k1 = unit_k1(slot, rows);
-        if (g < 0) break;
-        if (!mbar_wait(schede_bar(slot), sphase, abort_flag, p.status, kStatusTimeoutEpilogue))
-          break;
-        int ks = k0;
-        do {  // the accumulators that the tile takes
+        const int next = slot + 1 == C::SCHED ? 0 : slot + 1;
+        const uint32_t nphase = next == 0 ? sphase ^ 1u : sphase;
+        ok = mbar_wait(schede_bar(slot), sphase, abort_flag, p.status, kStatusTimeoutEpilogue);
+        for (int ks = k0; ok && more; ks += C::CHUNK) {  // the accumulators of the tile
           const uint32_t b = lt & 1u;
-          if (!mbar_wait(acce_bar(b), (lt >> 1) & 1u, abort_flag, p.status,
-                         kStatusTimeoutEpilogue)) {
-            ok = false;
-            break;
+          ok = mbar_wait(acce_bar(b), (lt >> 1) & 1u, abort_flag, p.status, kStatusTimeoutEpilogue);
+          const bool last = ks + C::CHUNK >= k1;
+          if (ok && last) {
+            ok = mbar_wait<true>(schedf_bar(next), nphase, abort_flag, p.status,
+                                 kStatusTimeoutEpilogue);
+            more = ok && __shfl_sync(kFullMask, ring[next].g, 0) >= 0;
           }
+          if (!ok || !more) break;
           tc_fence_after();
           tc_fence_before();
           if (lane < (ks == k0 ? 2 : 1))
             mbar_arrive_remote(lane == 0 ? leader_acce0 + 8u * b : leader_schede0 + 8u * slot);
           ++lt;
-          ks += C::CHUNK;
-        } while (ks < k1);
-        if (++slot == C::SCHED) {
-          slot = 0;
-          sphase ^= 1;
+          if (last) break;
         }
+        more = more && ok;
+        slot = next;
+        sphase = nphase;
       }
       __syncwarp();
     }
@@ -816,6 +834,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(C::THREADS, 1)
     bool ok = mbar_wait(tmem_ready_bar, 0, abort_flag, p.status, kStatusTimeoutEpilogue);
     tc_fence_after();
     const uint32_t tmem = *tmem_holder;
+    if (ok && !tmem_in_range(tmem, C::TMEM_COLS)) {
+      give_up(p.status, abort_flag, kStatusBadTmem);
+      ok = false;
+    }
     int slot = 0;
     uint32_t sphase = 0;
     uint32_t lt = 0;
@@ -1030,7 +1052,7 @@ __global__ void __launch_bounds__(256) f16_prepare_kernel(const __grid_constant_
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int G = p.num_groups;
   if (threadIdx.x == 0) s_bad = s_steps = 0;
-  for (int i = threadIdx.x; i <= G; i += 256) soff[i] = __ldg(p.offsets + i);
+  for (int i = threadIdx.x; i <= G; i += 256) soff[i] = p.offsets[i];
   if (p.split_pairs > 0 && blockIdx.x == 0)
     for (int i = threadIdx.x; i < kMaxSplitUnits * kWarpSums / 4; i += 256)
       reinterpret_cast<int4*>(p.arrived)[i] = make_int4(0, 0, 0, 0);
@@ -1125,7 +1147,7 @@ __global__ void __launch_bounds__(256) f16_prepare_kernel(const __grid_constant_
       const int64_t pitch = is_a ? p.vec_a : p.vec_b;
       const int64_t src = int64_t(soff[g + 1] - rest + row);
       uint4 v = make_uint4(0u, 0u, 0u, 0u);
-      if (row < rest) v = __ldg((is_a ? p.a : p.b) + src * pitch + col);
+      if (row < rest) v = (is_a ? p.a : p.b)[src * pitch + col];
       (is_a ? p.tail_a : p.tail_b)[r * pitch + col] = v;
     }
     return;
@@ -1300,6 +1322,7 @@ int fgg_f16_grouped_gemm_rows(const FggF16RowsProblem* p, int32_t direction, voi
   pp.num_groups = gp.num_groups = p->num_groups;
   pp.max_rows = p->max_rows;
   pp.mts = gp.mts = L.mts;
+  gp.max_rows = p->max_rows;
   gp.cts = L.cts;
   pp.tile_cap = L.tile_cap;
   gp.grid_units = int(std::min<int64_t>(int64_t(L.tile_cap) * L.max_slices, INT32_MAX));

@@ -61,7 +61,7 @@ __global__ void __launch_bounds__(256) mx_prepare_kernel(const __grid_constant__
     if (t < p.xblocks * p.nt) {
       const int xb = t / p.nt;
       const int nti = t - xb * p.nt;
-      int e = __ldg(p.m_indices + size_t(xb) * kMxBlockM);
+      int e = p.m_indices[size_t(xb) * kMxBlockM];
       e = min(max(e, 0), p.g - 1);  // padding block -> expert 0 (output unchecked)
       p.tiles_out[t] = pack_tile(e, nti, xb);
     }
@@ -86,7 +86,7 @@ __global__ void __launch_bounds__(256) mx_prepare_kernel(const __grid_constant__
       const int row = xb * kMxBlockM + rr;
       v[r1] = 0u;
       if (rr < kMxBlockM && row < p.m_total)
-        v[r1] = e8m0_byte(__ldg(p.a_sf + size_t(row) * kq + ks)) * 0x01010101u;
+        v[r1] = e8m0_byte(p.a_sf[size_t(row) * kq + ks]) * 0x01010101u;
     }
     *reinterpret_cast<uint4*>(p.sfx_out + ((size_t(xb) * p.ksteps + ks) * 2 + c) * 512u +
                               size_t(r0) * 16u) = make_uint4(v[0], v[1], v[2], v[3]);
@@ -107,8 +107,8 @@ __global__ void __launch_bounds__(256) mx_prepare_kernel(const __grid_constant__
 #pragma unroll
     for (int r1 = 0; r1 < 4; ++r1) {
       const int row = nti * 128 + r1 * 32 + r0;
-      const float4 s = __ldg(reinterpret_cast<const float4*>(p.b_sf + (size_t(g) * p.n + row) * kw +
-                                                             size_t(ks) * 4));
+      const float4 s = *reinterpret_cast<const float4*>(p.b_sf + (size_t(g) * p.n + row) * kw +
+                                                      size_t(ks) * 4);
       v[r1] = e8m0_byte(s.x) | (e8m0_byte(s.y) << 8) | (e8m0_byte(s.z) << 16) |
               (e8m0_byte(s.w) << 24);
     }
@@ -239,6 +239,8 @@ int fgg_mx_grouped_gemm(const FggMxProblem* p, void* workspace, size_t ws_bytes,
   gp.n = p->n;
   gp.k = p->k;
   gp.m_total = p->m_total;
+  gp.out_rows = p->m_total;
+  gp.xtiles = L.xblocks;
   gp.num_tiles = L.num_tiles;
   gp.ksteps = L.ksteps;
   gp.nt = L.nt;

@@ -4,13 +4,22 @@
 // 16, so half as many 512-byte atoms.
 //
 // Per call:
-//   1. nvfp4_prepare_kernel  per-group TMA descriptors for the token tensors
-//                            (edited on the device from one host-encoded
-//                            template), the token scales repacked into 512-byte
-//                            SF atoms, the flat tile list, status reset.
+//   1. nvfp4_prepare_kernel  the token scales repacked into 512-byte SF atoms, the
+//                            flat tile list, status reset.
 //   2. fgg_gemm_kernel<NVFP4 cfg>  (fgg_engine.cuh).
-// Weights are packed once by nvfp4_pack_weights_kernel (descriptors + SF
-// atoms) and cached by the caller, as kernel.py:2743-2786 caches its repack.
+// Weights are packed once (descriptors + SF atoms) and cached by the caller, as
+// kernel.py:2743-2786 caches its repack.
+//
+// Every TMA descriptor is encoded on the host.  Those of the tokens are kernel
+// parameters: one map where the groups' rows follow each other in one buffer, else
+// one per group, kListMaps groups to a launch.  Those of the weights lie in the pack.
+// Descriptors edited on the device (one template, an address per group) cost less
+// host time but are not used: the only faults this library has had came from
+// kernels that read such ones, a few in thousands of runs, and their cause was not
+// found.
+//
+// What an earlier kernel of the stream wrote is read by ordinary loads: these kernels
+// start while that one finishes, so that it is not constant for their life.
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -30,21 +39,18 @@ constexpr int64_t kAcrossGroupsMaxBytes = 32ll << 20;
 // small instance for the common few-group call keeps the launch light).
 template <int CAP>
 struct PrepParams {
-  CUtensorMap tmpl;  // token descriptor template (group 0's geometry)
-  const uint8_t* a[CAP];
   const uint8_t* a_sf[CAP];
   int32_t m[CAP];
   int32_t xtile_begin[CAP + 1];
   int32_t tile_begin[CAP + 1];
   int32_t out_row[CAP];
   int32_t wgroup[CAP];  // weight group of each problem group
-  CUtensorMap* tmap_out;
   GroupInfo* ginfo_out;
   uint32_t* tiles_out;
   uint8_t* sfx_out;
   int* status;
   int32_t g, k, bn, ch, nk64p, nt, num_tiles, xt_total;
-  int32_t blocks_tmap, blocks_tiles;
+  int32_t blocks_tiles;
   int32_t across_groups;
   int32_t sf_vec;  // 1: K % 256 == 0 and every a_sf[g] 16-byte aligned (vector repack)  // tile order: 1 weight-tile-major over all groups, 0 group-major
 };
@@ -82,37 +88,25 @@ __global__ void __launch_bounds__(256)
   griddep_launch_dependents();
   // launched early behind the previous GEMM: touch no memory before it is done
   griddep_wait();
-  __shared__ alignas(128) CUtensorMap smap[8];
   __shared__ int32_t sbegin[CAP + 1];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int blk = blockIdx.x;
-  if (blk < p.blocks_tmap) {
-    if (blk == 0 && threadIdx.x == 0) {
+  if (blk == 0) {
+    if (threadIdx.x == 0) {
       p.status[0] = 0;
       p.status[1] = 0;
       p.status[2] = 0;
     }
-    const int g = blk * 8 + warp;
-    if (g < p.g) {
-      const uint32_t* src = reinterpret_cast<const uint32_t*>(&p.tmpl);
-      reinterpret_cast<uint32_t*>(&smap[warp])[lane] = src[lane];
-      __syncwarp();
-      if (lane == 0) {
-        tmap_replace_address(smem_u32(&smap[warp]), reinterpret_cast<uint64_t>(p.a[g]));
-        tmap_replace_dim1(smem_u32(&smap[warp]), max(p.m[g], 1));
-        GroupInfo gi;
-        gi.m = p.m[g];
-        gi.out_row = p.out_row[g];
-        gi.xtile_begin = p.xtile_begin[g];
-        gi.wgroup = p.wgroup[g];
-        p.ginfo_out[g] = gi;
-      }
-      __syncwarp();
-      tmap_publish(p.tmap_out + g, smem_u32(&smap[warp]));
+    for (int g = threadIdx.x; g < p.g; g += blockDim.x) {
+      GroupInfo gi;
+      gi.m = p.m[g];
+      gi.out_row = p.out_row[g];
+      gi.xtile_begin = p.xtile_begin[g];
+      gi.wgroup = p.wgroup[g];
+      p.ginfo_out[g] = gi;
     }
     return;
   }
-  blk -= p.blocks_tmap;
+  --blk;
   if (blk < p.blocks_tiles) {
     if (p.across_groups) {
       // Weight-tile-major over all groups: tile t pairs weight tile
@@ -171,7 +165,7 @@ __global__ void __launch_bounds__(256)
       const int row = xt * p.bn + rr;
       v[r1] = make_uint4(0u, 0u, 0u, 0u);
       if (rr < p.bn && row < p.m[g])
-        v[r1] = __ldg(reinterpret_cast<const uint4*>(p.a_sf[g] + size_t(row) * kq + 16 * s4));
+        v[r1] = *reinterpret_cast<const uint4*>(p.a_sf[g] + size_t(row) * kq + 16 * s4);
     }
     uint8_t* dst = p.sfx_out + ((size_t(X) * p.nk64p + 4 * s4) * p.ch + c) * 512u + size_t(r0) * 16u;
     const size_t jstride = size_t(p.ch) * 512u;
@@ -200,7 +194,7 @@ __global__ void __launch_bounds__(256)
     const int row = xt * p.bn + rr;
     v[r1] = 0u;
     if (rr < p.bn && row < p.m[g] && 4 * j < kq)
-      v[r1] = __ldg(reinterpret_cast<const uint32_t*>(p.a_sf[g] + size_t(row) * kq + 4 * j));
+      v[r1] = *reinterpret_cast<const uint32_t*>(p.a_sf[g] + size_t(row) * kq + 4 * j);
   }
   *reinterpret_cast<uint4*>(p.sfx_out + ((size_t(X) * p.nk64p + j) * p.ch + c) * 512u +
                             size_t(r0) * 16u) = make_uint4(v[0], v[1], v[2], v[3]);
@@ -238,7 +232,7 @@ __device__ int rows_tile_prefix(const RowsPrepParams& p, int32_t* begin, int32_t
   __shared__ int s_bad;
   __shared__ int32_t s_warp[8];
   if (threadIdx.x == 0) s_bad = 0;
-  for (int i = threadIdx.x; i <= p.g; i += blockDim.x) off[i] = __ldg(p.offsets + i);
+  for (int i = threadIdx.x; i <= p.g; i += blockDim.x) off[i] = p.offsets[i];
   __syncthreads();
   // each thread sums the tiles of a contiguous run of groups
   const int per = (p.g + blockDim.x - 1) / blockDim.x;
@@ -295,7 +289,7 @@ __global__ void __launch_bounds__(256)
       gi.m = bad ? 0 : soff[g + 1] - soff[g];
       gi.out_row = soff[g];
       gi.xtile_begin = bad ? 0 : sbegin[g];
-      int wg = p.b_index != nullptr ? __ldg(p.b_index + g) : g;
+      int wg = p.b_index != nullptr ? p.b_index[g] : g;
       gi.wgroup = wg;
       p.ginfo_out[g] = gi;
     }
@@ -345,7 +339,7 @@ __global__ void __launch_bounds__(256)
       const int row = xt * p.bn + rr;
       v[r1] = make_uint4(0u, 0u, 0u, 0u);
       if (rr < p.bn && row < m)
-        v[r1] = __ldg(reinterpret_cast<const uint4*>(p.a_sf + size_t(soff[g] + row) * kq + 16 * s4));
+        v[r1] = *reinterpret_cast<const uint4*>(p.a_sf + size_t(soff[g] + row) * kq + 16 * s4);
     }
     uint8_t* dst = p.sfx_out + ((size_t(X) * p.nk64p + 4 * s4) * p.ch + c) * 512u + size_t(r0) * 16u;
     const size_t jstride = size_t(p.ch) * 512u;
@@ -373,31 +367,41 @@ __global__ void __launch_bounds__(256)
     const int row = xt * p.bn + rr;
     v[r1] = 0u;
     if (rr < p.bn && row < m && 4 * j < kq)
-      v[r1] = __ldg(reinterpret_cast<const uint32_t*>(p.a_sf + size_t(soff[g] + row) * kq + 4 * j));
+      v[r1] = *reinterpret_cast<const uint32_t*>(p.a_sf + size_t(soff[g] + row) * kq + 4 * j);
   }
   *reinterpret_cast<uint4*>(p.sfx_out + ((size_t(X) * p.nk64p + j) * p.ch + c) * 512u +
                             size_t(r0) * 16u) = make_uint4(v[0], v[1], v[2], v[3]);
 }
 
+// The maps of up to kPackMaps weight groups, host-encoded, into the pack.
+constexpr int kPackMaps = 128;
+struct PackMapsParams {
+  CUtensorMap maps[kPackMaps];
+  CUtensorMap* out;
+  int32_t count;
+};
+__global__ void __launch_bounds__(256)
+    nvfp4_pack_maps_kernel(const __grid_constant__ PackMapsParams p) {
+  const uint4* const src = reinterpret_cast<const uint4*>(p.maps);
+  uint4* const dst = reinterpret_cast<uint4*>(p.out);
+  const int words = p.count * int(sizeof(CUtensorMap) / sizeof(uint4));
+  for (int i = threadIdx.x; i < words; i += 256) dst[i] = src[i];
+  tensormap_release();  // its readers acquire
+}
+
 struct PackParams {
-  CUtensorMap tmpl;
-  const uint8_t* b[FGG_MAX_GROUPS];
   const uint8_t* b_sf[FGG_MAX_GROUPS];
   PackHeader* header;
-  CUtensorMap* tmap_out;  // null: MXFP4, whose weights are one tensor with one map
   uint8_t* sfw_out;
   int32_t g, n, k, nk64p, nt;
   int32_t kq;  // scales per row
   uint32_t magic;
-  int32_t blocks_tmap;
 };
 
 __global__ void __launch_bounds__(256) nvfp4_pack_weights_kernel(const __grid_constant__ PackParams p) {
-  __shared__ alignas(128) CUtensorMap smap[8];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int blk = blockIdx.x;
-  if (blk < p.blocks_tmap) {
-    if (blk == 0 && threadIdx.x == 0) {
+  if (blk == 0) {
+    if (threadIdx.x == 0) {
       PackHeader h;
       h.magic = p.magic;
       h.g = p.g;
@@ -405,18 +409,9 @@ __global__ void __launch_bounds__(256) nvfp4_pack_weights_kernel(const __grid_co
       h.k = p.k;
       *p.header = h;
     }
-    const int g = blk * 8 + warp;
-    if (p.tmap_out != nullptr && g < p.g) {
-      reinterpret_cast<uint32_t*>(&smap[warp])[lane] =
-          reinterpret_cast<const uint32_t*>(&p.tmpl)[lane];
-      __syncwarp();
-      if (lane == 0) tmap_replace_address(smem_u32(&smap[warp]), reinterpret_cast<uint64_t>(p.b[g]));
-      __syncwarp();
-      tmap_publish(p.tmap_out + g, smem_u32(&smap[warp]));
-    }
     return;
   }
-  blk -= p.blocks_tmap;
+  --blk;
   const int64_t line = int64_t(blk) * blockDim.x + threadIdx.x;
   const int64_t total = int64_t(p.g) * p.nt * p.nk64p * 32;
   if (line >= total) return;
@@ -432,7 +427,7 @@ __global__ void __launch_bounds__(256) nvfp4_pack_weights_kernel(const __grid_co
   for (int r1 = 0; r1 < 4; ++r1) {
     const int row = nt * 128 + r1 * 32 + r0;
     v[r1] = (4 * j < kq)
-                ? __ldg(reinterpret_cast<const uint32_t*>(p.b_sf[g] + size_t(row) * kq + 4 * j))
+                ? *reinterpret_cast<const uint32_t*>(p.b_sf[g] + size_t(row) * kq + 4 * j)
                 : 0u;
   }
   uint4* dst = reinterpret_cast<uint4*>(p.sfw_out + ((size_t(g) * p.nt + nt) * p.nk64p + j) * 512u +
@@ -444,6 +439,10 @@ __global__ void __launch_bounds__(256) nvfp4_pack_weights_kernel(const __grid_co
 using CfgPrefill = EngineCfg<false, 224, 4>;   // one CTA per tile (N % 256 != 0)
 using CfgDecode = EngineCfg<false, 16, 4, 2>;  // every group has M <= 16; 2 K steps per stage
 using CfgPair = PairCfg<false, 6>;             // CTA pairs, 256 x 224 tiles
+// the same over groups in buffers of their own
+using ListPrefill = EngineCfg<false, 224, 4, 1, false, true>;
+using ListDecode = EngineCfg<false, 16, 4, 2, false, true>;
+using ListPair = PairCfg<false, 6, 1, false, true>;
 
 // MXFP4: the same tiles, two SF atoms per K step.  Measured: 8 groups, 4352 rows,
 // 4096 x 7168 60 us (4.2 PFLOP/s, tensor pipe 64 % active); 64 groups, 544 rows,
@@ -476,7 +475,7 @@ struct WsLayout {
   bool pair = false;
   int box_rows = 0;  // token rows per TMA box (a pair CTA loads half a tile)
   int nk64p = 0, nk256 = 0, nt = 0, nt128 = 0;
-  int num_tiles = 0, xt_total = 0;
+  int num_tiles = 0, xt_total = 0, rows = 0;
   // per-group bookkeeping in fixed arrays: planning a call touches no host heap
   int32_t xtile_begin[FGG_MAX_GROUPS + 1];
   int32_t tile_begin[FGG_MAX_GROUPS + 1];
@@ -489,7 +488,7 @@ struct WsLayout {
   // order stays group-major, so a group's token tiles share each weight tile
   // while it is hot.  Decode tiles stream their weights once in either order.
   bool across_groups = false;
-  size_t status = 0, tmaps = 0, ginfo = 0, tiles = 0, sfx = 0, total = 0;
+  size_t status = 0, ginfo = 0, tiles = 0, sfx = 0, total = 0;
 };
 
 static int plan(const FggNvfp4Problem* p, WsLayout* L) {
@@ -549,9 +548,10 @@ static int plan(const FggNvfp4Problem* p, WsLayout* L) {
   L->tile_begin[G] = int32_t(tiles);
   L->num_tiles = int(tiles);
   L->xt_total = int(xts);
+  L->rows = int(rows);
   Carver cv;
   L->status = cv.take(kStatusBytes, 256);
-  L->tmaps = cv.take(size_t(G) * sizeof(CUtensorMap), 128);
+  cv.take(size_t(G) * sizeof(CUtensorMap), 128);  // not used: callers' sizes stay what they were
   L->ginfo = cv.take(size_t(G) * sizeof(GroupInfo), 256);
   L->tiles = cv.take(size_t(std::max<int64_t>(tiles, 1)) * 4, 256);
   // token scales per (token tile, MMA): ch atoms of 512 B
@@ -594,17 +594,23 @@ int fgg_nvfp4_pack_weights(const FggNvfp4Weights* w, void* pack, size_t pack_byt
   DeviceInfo dev;
   if (int rc = current_device(&dev)) return rc;
 
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  uint8_t* base = static_cast<uint8_t*>(pack);
+  for (int g0 = 0; g0 < G; g0 += kPackMaps) {
+    static thread_local PackMapsParams pm;  // 16 KB: keep it off the stack
+    pm.count = std::min(G - g0, kPackMaps);
+    for (int i = 0; i < pm.count; ++i)
+      if (int rc = encode_u8_2d(&pm.maps[i], w->b[g0 + i], uint64_t(w->k) / 2, uint64_t(w->n), 128,
+                                128))
+        return rc;
+    pm.out = reinterpret_cast<CUtensorMap*>(base + L.tmaps) + g0;
+    nvfp4_pack_maps_kernel<<<1, 256, 0, s>>>(pm);
+    FGG_CUDA_CHECK(cudaGetLastError());
+  }
   PackParams pp;
   memset(&pp, 0, sizeof(pp));
-  if (int rc = encode_u8_2d(&pp.tmpl, w->b[0], uint64_t(w->k) / 2, uint64_t(w->n), 128, 128))
-    return rc;
-  for (int g = 0; g < G; ++g) {
-    pp.b[g] = static_cast<const uint8_t*>(w->b[g]);
-    pp.b_sf[g] = static_cast<const uint8_t*>(w->b_sf[g]);
-  }
-  uint8_t* base = static_cast<uint8_t*>(pack);
+  for (int g = 0; g < G; ++g) pp.b_sf[g] = static_cast<const uint8_t*>(w->b_sf[g]);
   pp.header = reinterpret_cast<PackHeader*>(base + L.header);
-  pp.tmap_out = reinterpret_cast<CUtensorMap*>(base + L.tmaps);
   pp.sfw_out = base + L.sfw;
   pp.g = G;
   pp.n = w->n;
@@ -613,11 +619,10 @@ int fgg_nvfp4_pack_weights(const FggNvfp4Weights* w, void* pack, size_t pack_byt
   pp.kq = w->k / 16;
   pp.magic = kPackMagic;
   pp.nt = w->n / 128;
-  pp.blocks_tmap = (G + 7) / 8;
   const int64_t lines = int64_t(G) * pp.nt * pp.nk64p * 32;
-  const int64_t blocks = pp.blocks_tmap + (lines + 255) / 256;
+  const int64_t blocks = 1 + (lines + 255) / 256;
   if (blocks > INT32_MAX) return set_error(FGG_EBADSHAPE, "weights too large");
-  nvfp4_pack_weights_kernel<<<int(blocks), 256, 0, reinterpret_cast<cudaStream_t>(stream)>>>(pp);
+  nvfp4_pack_weights_kernel<<<int(blocks), 256, 0, s>>>(pp);
   FGG_CUDA_CHECK(cudaGetLastError());
   return FGG_OK;
 }
@@ -657,9 +662,8 @@ int fgg_mxfp4_pack_weights(const void* b_sf, int32_t num_groups, int32_t n, int3
   pp.kq = k / 32;
   pp.magic = kPackMagicMx;
   pp.nt = n / 128;
-  pp.blocks_tmap = 1;  // the header; no descriptors
   const int64_t lines = int64_t(num_groups) * pp.nt * pp.nk64p * 32;
-  const int64_t blocks = pp.blocks_tmap + (lines + 255) / 256;
+  const int64_t blocks = 1 + (lines + 255) / 256;
   if (blocks > INT32_MAX) return set_error(FGG_EBADSHAPE, "weights too large");
   nvfp4_pack_weights_kernel<<<int(blocks), 256, 0, reinterpret_cast<cudaStream_t>(stream)>>>(pp);
   FGG_CUDA_CHECK(cudaGetLastError());
@@ -702,17 +706,21 @@ int check_problem(const FggNvfp4Problem* p, const WsLayout& L, void* workspace, 
   return FGG_OK;
 }
 
+// The buffer that holds every group's rows, one after the other, or null.
+const uint8_t* one_buffer(const FggNvfp4Problem* p, const WsLayout& L, int first) {
+  const uint8_t* const base = static_cast<const uint8_t*>(p->a[first]);
+  for (int g = first + 1; g < p->num_groups; ++g)
+    if (p->m[g] > 0 && p->a[g] != base + size_t(L.out_row[g]) * (p->k / 2)) return nullptr;
+  return base;
+}
+
 template <int CAP>
 int prepare_launch(const FggNvfp4Problem* p, const WsLayout& L, int first, uint8_t* ws,
                    cudaStream_t s) {
   const int G = p->num_groups;
   static thread_local PrepParams<CAP> pp;  // up to ~17 KB: keep it off the stack
   memset(&pp, 0, sizeof(pp));
-  if (int rc = encode_u8_2d(&pp.tmpl, p->a[first], uint64_t(p->k) / 2, uint64_t(p->m[first]), 128,
-                            uint32_t(L.box_rows)))
-    return rc;
   for (int g = 0; g < G; ++g) {
-    pp.a[g] = static_cast<const uint8_t*>(p->a[g]);
     pp.a_sf[g] = static_cast<const uint8_t*>(p->a_sf[g]);
     pp.m[g] = p->m[g];
     pp.out_row[g] = L.out_row[g];
@@ -722,7 +730,6 @@ int prepare_launch(const FggNvfp4Problem* p, const WsLayout& L, int first, uint8
     pp.xtile_begin[g] = L.xtile_begin[g];
     pp.tile_begin[g] = L.tile_begin[g];
   }
-  pp.tmap_out = reinterpret_cast<CUtensorMap*>(ws + L.tmaps);
   pp.ginfo_out = reinterpret_cast<GroupInfo*>(ws + L.ginfo);
   pp.tiles_out = reinterpret_cast<uint32_t*>(ws + L.tiles);
   pp.sfx_out = ws + L.sfx;
@@ -735,16 +742,16 @@ int prepare_launch(const FggNvfp4Problem* p, const WsLayout& L, int first, uint8
   pp.nt = L.nt;
   pp.num_tiles = L.num_tiles;
   pp.xt_total = L.xt_total;
-  pp.blocks_tmap = (G + 7) / 8;
   pp.blocks_tiles = (L.num_tiles + 255) / 256;
-  pp.across_groups = L.across_groups ? 1 : 0;
+  // launches of some groups each need the groups' tiles one after the other
+  pp.across_groups = L.across_groups && (G <= kListMaps || one_buffer(p, L, first) != nullptr);
   bool vec = p->k % 256 == 0;
   for (int g = 0; g < G && vec; ++g)
     vec = p->m[g] == 0 || aligned16(p->a_sf[g]);
   pp.sf_vec = vec ? 1 : 0;
   // threads of the scale repack: one per atom row, or per 4 atom rows (vector)
   const int64_t sf_lines = int64_t(L.xt_total) * L.nk64p * L.ch * 32 / (vec ? 4 : 1);
-  const int64_t blocks = int64_t(pp.blocks_tmap) + pp.blocks_tiles + (sf_lines + 255) / 256;
+  const int64_t blocks = 1 + int64_t(pp.blocks_tiles) + (sf_lines + 255) / 256;
   if (blocks > INT32_MAX) return set_error(FGG_EBADSHAPE, "problem too large");
   FGG_CUDA_CHECK(launch_dependent(nvfp4_prepare_kernel<CAP>, int(blocks), 0, s, pp));
   FGG_CUDA_CHECK(cudaGetLastError());
@@ -763,7 +770,16 @@ int prepare_impl(const FggNvfp4Problem* p, const WsLayout& L, int first, uint8_t
   return prepare_launch<FGG_MAX_GROUPS>(p, L, first, ws, s);
 }
 
-int gemm_impl(const FggNvfp4Problem* p, const WsLayout& L, const void* pack, uint8_t* ws,
+template <class Pair, class Prefill, class Decode, class Params>
+int launch_tiles(const Params& gp, const WsLayout& L, const DeviceInfo& dev, cudaStream_t s) {
+  const cudaError_t e = L.pair                      ? launch_pair<Pair>(gp, dev.sm_count, s)
+                        : L.bn == CfgDecode::BN ? launch_engine<Decode>(gp, dev.sm_count, s)
+                                                : launch_engine<Prefill>(gp, dev.sm_count, s);
+  if (e != cudaSuccess) return set_error(FGG_ECUDA, "GEMM launch failed: %s", cudaGetErrorString(e));
+  return FGG_OK;
+}
+
+int gemm_impl(const FggNvfp4Problem* p, const WsLayout& L, int first, const void* pack, uint8_t* ws,
               const DeviceInfo& dev, cudaStream_t s, int32_t epi = kEpiPlain) {
   if (L.num_tiles == 0) return FGG_OK;
   if (pack == nullptr) return set_error(FGG_EINVAL, "pack is null");
@@ -771,10 +787,9 @@ int gemm_impl(const FggNvfp4Problem* p, const WsLayout& L, const void* pack, uin
   const int G = p->num_groups;
   const uint8_t* pk = static_cast<const uint8_t*>(pack);
   const PackLayout PL = pack_layout(L.wg, p->n, p->k);
-  GemmParams gp;
+  static thread_local GemmListParams gp;  // 10 KB: keep it off the stack
   memset(&gp, 0, sizeof(gp));
   gp.tmap_w = reinterpret_cast<const CUtensorMap*>(pk + PL.tmaps);
-  gp.tmap_x = reinterpret_cast<const CUtensorMap*>(ws + L.tmaps);
   gp.sfw = pk + PL.sfw;
   gp.sfx = ws + L.sfx;
   gp.ginfo = reinterpret_cast<const GroupInfo*>(ws + L.ginfo);
@@ -794,7 +809,8 @@ int gemm_impl(const FggNvfp4Problem* p, const WsLayout& L, const void* pack, uin
   gp.nt = L.nt;
   gp.nt128 = L.nt128;
   gp.debug_flags = debug_flags();
-  cudaError_t e;
+  gp.out_rows = L.rows;
+  gp.xtiles = L.xt_total;
   if (L.pair) {
     // scale atoms as rows of uint64: a CTA's 4 weight atoms of a K step are one
     // 2 KB row of the pack, the 8 token atoms of a K step two 2 KB rows
@@ -806,13 +822,36 @@ int gemm_impl(const FggNvfp4Problem* p, const WsLayout& L, const void* pack, uin
                                  uint64_t(L.xt_total) * L.nk256 * CfgPair::SFX_BOX_ROWS,
                                  CfgPair::SFX_ROW_U64, CfgPair::SFX_BOX_ROWS))
       return rc;
-    e = launch_pair<CfgPair>(gp, dev.sm_count, s);
-  } else if (L.bn == CfgDecode::BN) {
-    e = launch_engine<CfgDecode>(gp, dev.sm_count, s);
-  } else {
-    e = launch_engine<CfgPrefill>(gp, dev.sm_count, s);
   }
-  if (e != cudaSuccess) return set_error(FGG_ECUDA, "GEMM launch failed: %s", cudaGetErrorString(e));
+  const uint64_t row_bytes = uint64_t(p->k) / 2;
+  if (const uint8_t* a = one_buffer(p, L, first)) {
+    if (int rc = encode_u8_2d(&gp.tmap_x_flat, a, row_bytes, uint64_t(L.rows), 128,
+                              uint32_t(L.box_rows)))
+      return rc;
+    if (L.pair) {
+      for (int i = 0; i < kXSmallMaps; ++i)
+        if (int rc = encode_u8_2d(&gp.tmap_x_small[i], a, row_bytes, uint64_t(L.rows), 128,
+                                  uint32_t(16 * (i + 1))))
+          return rc;
+      gp.x_small = 1;
+    }
+    return launch_tiles<CfgPair, CfgPrefill, CfgDecode>(static_cast<const GemmParams&>(gp), L, dev,
+                                                        s);
+  }
+  for (gp.g0 = 0; gp.g0 < G; gp.g0 += kListMaps) {
+    const int g1 = std::min(G, gp.g0 + kListMaps);
+    if (G > kListMaps) {  // the tiles of these groups
+      gp.tiles = reinterpret_cast<const uint32_t*>(ws + L.tiles) + L.tile_begin[gp.g0];
+      gp.num_tiles = L.tile_begin[g1] - L.tile_begin[gp.g0];
+      if (gp.num_tiles == 0) continue;
+    }
+    for (int g = gp.g0; g < g1; ++g)
+      if (p->m[g] > 0)
+        if (int rc = encode_u8_2d(&gp.tmap_x[g - gp.g0], p->a[g], row_bytes, uint64_t(p->m[g]), 128,
+                                  uint32_t(L.box_rows)))
+          return rc;
+    if (int rc = launch_tiles<ListPair, ListPrefill, ListDecode>(gp, L, dev, s)) return rc;
+  }
   return FGG_OK;
 }
 
@@ -840,7 +879,7 @@ int fgg_nvfp4_gemm(const FggNvfp4Problem* p, const void* pack, void* workspace, 
   if (int rc = check_problem(p, L, workspace, ws_bytes, &first)) return rc;
   DeviceInfo dev;
   if (int rc = current_device(&dev)) return rc;
-  return gemm_impl(p, L, pack, static_cast<uint8_t*>(workspace), dev,
+  return gemm_impl(p, L, first, pack, static_cast<uint8_t*>(workspace), dev,
                    reinterpret_cast<cudaStream_t>(stream));
 }
 
@@ -856,7 +895,7 @@ int fgg_nvfp4_grouped_gemm(const FggNvfp4Problem* p, const void* pack, void* wor
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   if (int rc = prepare_impl(p, L, first, ws, s)) return rc;
-  return gemm_impl(p, L, pack, ws, dev, s);
+  return gemm_impl(p, L, first, pack, ws, dev, s);
 }
 
 int fgg_nvfp4_grouped_gemm_silu_mul(const FggNvfp4Problem* p, const void* pack, void* workspace,
@@ -873,7 +912,7 @@ int fgg_nvfp4_grouped_gemm_silu_mul(const FggNvfp4Problem* p, const void* pack, 
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   if (int rc = prepare_impl(p, L, first, ws, s)) return rc;
-  return gemm_impl(p, L, pack, ws, dev, s, kEpiSiluMul);
+  return gemm_impl(p, L, first, pack, ws, dev, s, kEpiSiluMul);
 }
 
 }  // extern "C"
@@ -1000,7 +1039,8 @@ int rows_impl(const FggNvfp4RowsProblem* p, const void* b, const void* pack, voi
   if (int rc = encode_u8_2d(&gp.tmap_x_flat, p->a, uint64_t(p->k) / 2, uint64_t(p->max_rows), 128,
                             uint32_t(L.box_rows)))
     return rc;
-  gp.x_flat = 1;
+  gp.out_rows = p->max_rows;
+  gp.xtiles = L.xt_cap;
   if (kMx4)
     if (int rc = encode_3d(&gp.mx_tmap_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, b, uint64_t(p->k) / 2,
                            uint64_t(p->n), uint64_t(wg), uint64_t(p->k) / 2,
@@ -1113,7 +1153,7 @@ int fgg_nvfp4_grouped_gemm_noalloc(const FggNvfp4Problem* p, const void* pack, v
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   uint8_t* ws = static_cast<uint8_t*>(scratch);
   if (int rc = prepare_impl(p, L, first, ws, s)) return rc;
-  if (int rc = gemm_impl(p, L, pack, ws, dev, s)) return rc;
+  if (int rc = gemm_impl(p, L, first, pack, ws, dev, s)) return rc;
   if (status_out != nullptr)
     FGG_CUDA_CHECK(
         cudaMemcpyAsync(status_out, ws + L.status, sizeof(int32_t), cudaMemcpyDeviceToDevice, s));

@@ -172,6 +172,10 @@ __device__ __forceinline__ void bulk_g2s(uint32_t dst, const void* src, uint32_t
       "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(bar)
       : "memory");
 }
+// A hint: nothing is read.
+__device__ __forceinline__ void prefetch_l2(const void* p) {
+  asm volatile("prefetch.global.L2 [%0];" ::"l"(__cvta_generic_to_global(p)) : "memory");
+}
 __device__ __forceinline__ void prefetch_tensormap(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
 }
@@ -182,27 +186,10 @@ __device__ __forceinline__ void tensormap_acquire(const CUtensorMap* map) {
                : "memory");
 }
 
-// ------------------------------------------------------- tensormap edits
-__device__ __forceinline__ void tmap_replace_address(uint32_t smem_map, uint64_t addr) {
-  asm volatile("tensormap.replace.tile.global_address.shared::cta.b1024.b64 [%0], %1;" ::"r"(
-                   smem_map),
-               "l"(addr)
-               : "memory");
-}
-__device__ __forceinline__ void tmap_replace_dim1(uint32_t smem_map, int32_t extent) {
-  asm volatile("tensormap.replace.tile.global_dim.shared::cta.b1024.b32 [%0], 1, %1;" ::"r"(
-                   smem_map),
-               "r"(extent)
-               : "memory");
-}
-// Warp-collective copy of an edited descriptor from shared to global memory,
-// with the release fence that publishes it to the tensormap proxy.
-__device__ __forceinline__ void tmap_publish(CUtensorMap* gdst, uint32_t smem_map) {
-  asm volatile(
-      "tensormap.cp_fenceproxy.global.shared::cta.tensormap::generic.release.gpu.sync.aligned"
-      " [%0], [%1], 128;" ::"l"(reinterpret_cast<uint64_t>(gdst)),
-      "r"(smem_map)
-      : "memory");
+// The writer's side: this thread's stores to descriptors, through the generic proxy,
+// come before their acquisition elsewhere.
+__device__ __forceinline__ void tensormap_release() {
+  asm volatile("fence.proxy.tensormap::generic.release.gpu;" ::: "memory");
 }
 
 // ------------------------------------------- programmatic dependent launch

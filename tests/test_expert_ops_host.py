@@ -259,3 +259,26 @@ def test_arrivals_in_another_cta_release_at_cluster_scope():
     assert found
     for name, op in found:
         assert ".release.cluster." in op, (name, op)
+
+
+def test_no_descriptor_is_edited_on_the_device():
+    """TMA descriptors are encoded on the host: the kernels that edited them on the device
+    are the only ones that ever faulted."""
+    from pathlib import Path
+
+    csrc = Path(rb.__file__).resolve().parent / "csrc"
+    for f in sorted(csrc.glob("*.cu*")):
+        text = f.read_text()
+        assert "tensormap.replace" not in text and "tensormap.cp_fenceproxy" not in text, f.name
+
+
+def test_what_the_prepare_kernels_write_is_not_read_as_constant():
+    """The products start while their prepare kernel runs, and that one while the kernel
+    before it finishes: neither reads global memory as data that is constant for its life."""
+    from pathlib import Path
+
+    csrc = Path(rb.__file__).resolve().parent / "csrc"
+    for name in ("fgg_engine.cuh", "fgg_nvfp4.cu", "fgg_mx.cu", "fgg_f16.cu"):
+        text = (csrc / name).read_text()
+        assert "griddep_wait()" in text
+        assert "__ldg(" not in text and "ld.global.nc" not in text, name

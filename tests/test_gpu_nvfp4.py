@@ -285,3 +285,76 @@ def test_config2_full_size(cuda_device):
     ms = [int(v) for v in rng.integers(64, 1025, size=8)]
     prob = ref.random_problem(ms, 4096, 7168, seed=0)
     _run_and_check(prob, 4096, 7168, cuda_device)
+
+
+def _list_inputs(ms, n, k, dev, seed):
+    """(separate token buffers, the same rows as slices of one buffer, weights, alpha)"""
+    prob = ref.random_problem(ms, n, k, seed=seed)
+    a, a_sf, b, b_sf, alpha = _dev_problem(prob, dev)
+    cut = np.cumsum([0] + ms).tolist()
+    one = torch.cat(a)
+    return prob, (a, a_sf), ([one[lo:hi] for lo, hi in zip(cut, cut[1:])], a_sf), (b, b_sf), alpha
+
+
+@pytest.mark.parametrize("ms,n,k", [
+    ([300, 17, 64], 512, 1024),                 # pair tiles
+    ([0, 230, 0, 31, 96, 0], 256, 320),         # empty groups first, between, last
+    ([300, 17, 224, 1], 384, 512),              # one CTA per tile
+    ([7, 16, 1, 0, 9], 256, 512),               # decode tiles
+    ([3] * 64 + [20], 256, 256),                # more groups than one launch has maps
+    ([33, 0, 250] * 50, 128, 192),
+    ([5, 0, 2] * 170, 256, 128),                # decode, more than 500 groups
+    ([0] * 70 + [40, 300], 256, 256),           # a first launch without tiles
+])
+def test_buffers_of_their_own_and_one_buffer(cuda_device, ms, n, k):
+    """Token rows in a buffer per group and in one buffer: both right, the same bits; the
+    gated form too."""
+    import ratchet_b200 as rb
+
+    prob, own, one, (b, b_sf), alpha = _list_inputs(ms, n, k, cuda_device, seed=len(ms))
+    pack = rb.pack_weights(b, b_sf)
+    refs = ref.grouped_gemm(prob["a"], prob["a_sf"], prob["b"], prob["b_sf"], prob["alpha"])
+    outs = []
+    for a, a_sf in (own, one):
+        outs.append(rb.nvfp4_grouped_gemm(a, a_sf, b, b_sf, None, alpha, pack=pack))
+        rb.last_status()
+        for o, r in zip(outs[-1], refs):
+            if o.shape[0]:
+                ok, st = ref.check_close(o.cpu(), r)
+                assert ok, st
+    assert all(torch.equal(x, y) for x, y in zip(*outs))
+    gated = [rb.nvfp4_grouped_gemm_silu_mul(a, a_sf, b, b_sf, None, alpha, pack=pack)
+             for a, a_sf in (own, one)]
+    rb.last_status()
+    assert all(torch.equal(x, y) for x, y in zip(*gated))
+
+
+def test_calls_of_other_layouts_in_turn(cuda_device):
+    """Decode, pair and one-CTA calls of few and many groups one after the other on one
+    workspace, each behind another layout's bytes: every call right each time."""
+    import ratchet_b200 as rb
+
+    cases = [([9] * 20, 384, 1024), ([300, 17, 64], 512, 1024), ([12] * 70, 256, 512),
+             ([100, 3], 256, 256), ([300, 17, 224, 1], 384, 512), ([230, 31, 96], 512, 768)]
+    calls, want = [], []
+    for i, (ms, n, k) in enumerate(cases):
+        prob, own, _, (b, b_sf), alpha = _list_inputs(ms, n, k, cuda_device, seed=i)
+        pack = rb.pack_weights(b, b_sf)
+        calls.append((own[0], own[1], b, b_sf, None, alpha, pack))
+        want.append(ref.grouped_gemm(prob["a"], prob["a_sf"], prob["b"], prob["b_sf"], prob["alpha"]))
+    first = None
+    for rep in range(4):
+        outs = []
+        for *args, pack in calls:
+            outs.append(rb.nvfp4_grouped_gemm(*args, pack=pack))
+            if rep == 0:
+                rb.last_status()
+        rb.last_status()
+        if first is None:
+            first = outs
+            for o, r in zip(outs, want):
+                for x, y in zip(o, r):
+                    ok, st = ref.check_close(x.cpu(), y)
+                    assert ok, st
+        else:
+            assert all(torch.equal(x, y) for o, f in zip(outs, first) for x, y in zip(o, f))
