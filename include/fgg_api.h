@@ -108,12 +108,12 @@ typedef struct FggNvfp4Problem {
   int32_t num_weight_groups; /* groups in `pack` when b_index is set */
 } FggNvfp4Problem;
 
-/* Scratch the call needs (token-scale repack, per-group descriptors, tile
- * list, status words).  Replaces the per-call part of `_prepare`
+/* Scratch the call needs (token-scale repack, group table, tile list, status
+ * words).  Replaces the per-call part of `_prepare`
  * (kernels/gemm/fp4_grouped_gemm/b200/kernel.py:2751-2786). */
 FGG_API size_t fgg_nvfp4_workspace_bytes(const FggNvfp4Problem* p);
 /* Replaces `fp4_grouped_gemm` (kernel.py:2788-2862) for the NVFP4 format:
- * validates, repacks the token scales, builds descriptors and launches the
+ * validates, repacks the token scales, encodes descriptors and launches the
  * persistent tcgen05 kernel.  `pack` must come from fgg_nvfp4_pack_weights
  * for the same N, K and G weight groups (num_weight_groups when b_index is
  * set). */
@@ -131,7 +131,7 @@ FGG_API int fgg_nvfp4_grouped_gemm_silu_mul(const FggNvfp4Problem* p, const void
                                             void* workspace, size_t ws_bytes, void* stream);
 /* The two halves of fgg_nvfp4_grouped_gemm, for callers that replay one
  * problem (same pointers, same sizes) many times, e.g. inside a CUDA graph:
- * fgg_nvfp4_prepare fills `workspace` (descriptors, token-scale repack, tile
+ * fgg_nvfp4_prepare fills `workspace` (group table, token-scale repack, tile
  * list); fgg_nvfp4_gemm launches the GEMM kernel on a prepared workspace and
  * may be repeated.  The token scales must not change between the two. */
 FGG_API int fgg_nvfp4_prepare(const FggNvfp4Problem* p, void* workspace, size_t ws_bytes, void* stream);
