@@ -81,7 +81,8 @@ typedef struct FggNvfp4Weights {
 } FggNvfp4Weights;
 
 /* Size of the device buffer fgg_nvfp4_pack_weights fills: per-group TMA
- * descriptors plus the scales repacked into the MMA's 512-byte SF atoms.
+ * descriptors plus the scales repacked into the MMA's 512-byte SF atoms.  The
+ * buffer is 128-byte aligned.
  * Replaces the identity-cached host repack `_prepare` / `_pack_sf_wgt` of
  * kernels/gemm/fp4_grouped_gemm/b200/kernel.py:2709-2786, done on the device. */
 FGG_API size_t fgg_nvfp4_weight_pack_bytes(int32_t num_groups, int32_t n, int32_t k);

@@ -587,7 +587,7 @@ int fgg_nvfp4_pack_weights(const FggNvfp4Weights* w, void* pack, size_t pack_byt
     if (!aligned16(w->b[g])) return set_error(FGG_EALIGN, "b[%d] is not 16-byte aligned", g);
     if (!aligned4(w->b_sf[g])) return set_error(FGG_EALIGN, "b_sf[%d] is not 4-byte aligned", g);
   }
-  if (!aligned16(pack)) return set_error(FGG_EALIGN, "pack is not 16-byte aligned");
+  if (!aligned128(pack)) return set_error(FGG_EALIGN, "pack is not 128-byte aligned");
   const PackLayout L = pack_layout(G, w->n, w->k);
   if (pack_bytes < L.total)
     return set_error(FGG_EWORKSPACE, "pack has %zu bytes, needs %zu", pack_bytes, L.total);
@@ -783,7 +783,7 @@ int gemm_impl(const FggNvfp4Problem* p, const WsLayout& L, int first, const void
               const DeviceInfo& dev, cudaStream_t s, int32_t epi = kEpiPlain) {
   if (L.num_tiles == 0) return FGG_OK;
   if (pack == nullptr) return set_error(FGG_EINVAL, "pack is null");
-  if (!aligned16(pack)) return set_error(FGG_EALIGN, "pack must be 16-byte aligned");
+  if (!aligned128(pack)) return set_error(FGG_EALIGN, "pack must be 128-byte aligned");
   const int G = p->num_groups;
   const uint8_t* pk = static_cast<const uint8_t*>(pack);
   const PackLayout PL = pack_layout(L.wg, p->n, p->k);
@@ -994,6 +994,8 @@ int rows_impl(const FggNvfp4RowsProblem* p, const void* b, const void* pack, voi
   if (kMx4 && b == nullptr) return set_error(FGG_EINVAL, "b is null");
   if (!aligned16(p->a) || !aligned16(p->out) || !aligned16(pack) || !aligned16(b))
     return set_error(FGG_EALIGN, "a, out, pack and b must be 16-byte aligned");
+  if (!kMx4 && !aligned128(pack))
+    return set_error(FGG_EALIGN, "pack must be 128-byte aligned");
   if (!aligned4(p->a_sf) || !aligned4(p->offsets) || !aligned4(p->alpha) ||
       (p->row_scale != nullptr && !aligned4(p->row_scale)) ||
       (p->b_index != nullptr && !aligned4(p->b_index)))

@@ -237,3 +237,16 @@ def test_peer_wait_limit_validated(L):
     p = _peers()
     p.wait_ms = -1
     assert L.fgg_moe_wait_peers(ctypes.byref(p), 0, None) == _lib.FGG_EINVAL
+
+
+def test_a_pack_with_descriptors_is_128_byte_aligned(L):
+    """Its TMA descriptors lie 128 bytes behind its start: a buffer that is only 16- or
+    64-byte aligned is refused, by the calls that fill it and by those that read it."""
+    P = 1 << 20                                    # pointers that are never followed
+    ptrs = (ctypes.c_void_p * 1)(P)
+    addr = ctypes.addressof(ptrs)
+    w = _lib.FggNvfp4Weights(1, 256, 256, addr, addr)
+    rows = _lib.FggNvfp4RowsProblem(1, 256, 256, 16, P, P, P, P, P, None, None, 0, 0)
+    for off in (16, 64):
+        assert L.fgg_nvfp4_pack_weights(w, P + off, 1 << 30, None) == _lib.FGG_EALIGN
+        assert L.fgg_nvfp4_grouped_gemm_rows(rows, P + off, P, 1 << 30, None) == _lib.FGG_EALIGN
