@@ -1304,13 +1304,6 @@ int fgg_f16_grouped_gemm_rows(const FggF16RowsProblem* p, int32_t direction, voi
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   const uint64_t G = uint64_t(p->num_groups), N = uint64_t(p->n), K = uint64_t(p->k);
-  if (p->max_rows == 0) {
-    // no rows: nothing to write but an overwritten gradient, which is zero
-    FGG_CUDA_CHECK(cudaMemsetAsync(ws + L.status, 0, kStatusBytes, s));
-    if (direction == kWgrad && !p->accumulate)
-      FGG_CUDA_CHECK(cudaMemsetAsync(p->out, 0, G * N * K * (p->out_dtype == 0 ? 4 : 2), s));
-    return FGG_OK;
-  }
   const uint64_t R = uint64_t(p->max_rows);
 
   F16PrepParams pp;
@@ -1347,8 +1340,12 @@ int fgg_f16_grouped_gemm_rows(const FggF16RowsProblem* p, int32_t direction, voi
     pp.tail_b = reinterpret_cast<uint4*>(ws + L.tail_b);
     pp.vec_a = p->n / 8;
     pp.vec_b = p->k / 8;
-    if (int rc = encode_2d(&gp.tmap_a, kMap16, p->a, N, R, N * 2, 64, 64)) return rc;
-    if (int rc = encode_2d(&gp.tmap_b, kMap16, p->b, K, R, K * 2, 64, 64)) return rc;
+    // (without rows the token tensors may be null, and no step reads them)
+    const void* const a = R > 0 ? p->a : pp.tail_a;
+    const void* const b = R > 0 ? p->b : pp.tail_b;
+    const uint64_t rows = R > 0 ? R : 16 * G;
+    if (int rc = encode_2d(&gp.tmap_a, kMap16, a, N, rows, N * 2, 64, 64)) return rc;
+    if (int rc = encode_2d(&gp.tmap_b, kMap16, b, K, rows, K * 2, 64, 64)) return rc;
     if (int rc = encode_2d(&gp.tmap_ta, kMap16, pp.tail_a, N, 16 * G, N * 2, 64, 16)) return rc;
     if (int rc = encode_2d(&gp.tmap_tb, kMap16, pp.tail_b, K, 16 * G, K * 2, 64, 16)) return rc;
     pp.wgrad_tiles = L.tile_cap;
@@ -1362,6 +1359,13 @@ int fgg_f16_grouped_gemm_rows(const FggF16RowsProblem* p, int32_t direction, voi
     blocks = int(std::min<int64_t>((vecs + 255) / 256, 8 * dev.sm_count));
   } else {
     const uint64_t ck = direction == kFwd ? K : N;  // contraction: the tokens' row length
+    pp.tiles = reinterpret_cast<uint64_t*>(ws + L.tiles);
+    pp.tile_rows = reinterpret_cast<int32_t*>(ws + L.tile_rows);
+    pp.ksteps = int((ck + 63) / 64);
+    if (R == 0) {  // no tile, but the offsets are looked at
+      FGG_CUDA_CHECK(launch_dependent(f16_prepare_kernel, 1, 0, s, pp));
+      return FGG_OK;
+    }
     if (int rc = encode_3d(&gp.tmap_w, kMap16, p->b, K, N, G, K * 2, N * K * 2, 64,
                            direction == kFwd ? 128 : 64, 1))
       return rc;
@@ -1369,12 +1373,10 @@ int fgg_f16_grouped_gemm_rows(const FggF16RowsProblem* p, int32_t direction, voi
       if (int rc = encode_2d(&gp.tmap_tok[i], kMap16, p->a, ck, R, ck * 2, 64,
                              uint32_t(16 * (i + 1))))
         return rc;
-    pp.tiles = reinterpret_cast<uint64_t*>(ws + L.tiles);
-    pp.tile_rows = reinterpret_cast<int32_t*>(ws + L.tile_rows);
     gp.tiles = pp.tiles;
     gp.tile_rows = pp.tile_rows;
     gp.m_ext = direction == kFwd ? p->n : p->k;
-    gp.ksteps = pp.ksteps = int((ck + 63) / 64);
+    gp.ksteps = pp.ksteps;
     blocks = std::min((L.tile_cap + 255) / 256, dev.sm_count);
   }
   FGG_CUDA_CHECK(launch_dependent(f16_prepare_kernel, std::max(blocks, 1), 0, s, pp));

@@ -647,3 +647,26 @@ def test_status_of_two_threads(cuda_device):
     assert seen == {"good": 0, "bad": 20}
     rb.grouped_gemm_rows(x, w, offsets["good"])
     rb.last_status()
+
+
+@pytest.mark.parametrize("bad", [[0, 5, 5], [1, 1, 1], [0, 3, 0], [-1, 0, 0]])
+def test_malformed_offsets_without_rows(cuda_device, bad):
+    """Offsets past zero rows are malformed like any others: nothing is written, and the
+    status tells."""
+    import ratchet_b200 as rb
+
+    dev = cuda_device
+    x, dy = _rand(dev, 0, 64), _rand(dev, 0, 32)
+    w, off = _rand(dev, 2, 32, 64), torch.tensor(bad, dtype=torch.int32, device=dev)
+    good = torch.zeros(3, dtype=torch.int32, device=dev)
+    dw = torch.full((2, 32, 64), 7.0, device=dev)
+    for call in (lambda o: rb.grouped_gemm_rows(x, w, o),
+                 lambda o: rb.grouped_gemm_rows_dgrad(dy, w, o),
+                 lambda o: rb.grouped_gemm_rows_wgrad(dy, x, o, out=dw)):
+        call(off)
+        with pytest.raises(rb.FggError, match="0x203"):
+            rb.last_status()
+        assert bool((dw == 7.0).all())
+        if call(good) is dw:
+            assert bool((dw == 0).all())
+        rb.last_status()
