@@ -983,8 +983,23 @@ int rows_impl(const FggNvfp4RowsProblem* p, const void* b, const void* pack, voi
     return set_error(FGG_EWORKSPACE, "workspace has %zu bytes, needs %zu", ws_bytes, L.total);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  if (p->max_rows == 0) {
-    FGG_CUDA_CHECK(cudaMemsetAsync(ws + L.status, 0, kStatusBytes, s));
+  if (p->max_rows == 0) {  // no tile, but offsets are looked at
+    if (p->offsets == nullptr) {
+      FGG_CUDA_CHECK(cudaMemsetAsync(ws + L.status, 0, kStatusBytes, s));
+      return FGG_OK;
+    }
+    if (!aligned4(p->offsets) || !aligned4(p->b_index))
+      return set_error(FGG_EALIGN, "offsets and b_index must be 4-byte aligned");
+    RowsPrepParams none;
+    memset(&none, 0, sizeof(none));
+    none.offsets = p->offsets;
+    none.b_index = p->b_index;
+    none.ginfo_out = reinterpret_cast<GroupInfo*>(ws + L.ginfo);
+    none.status = reinterpret_cast<int*>(ws + L.status);
+    none.g = p->num_groups;
+    none.bn = L.bn;
+    none.nt = L.nt;
+    FGG_CUDA_CHECK(launch_dependent(nvfp4_prepare_rows_kernel, 1, 0, s, none));
     return FGG_OK;
   }
   if (p->offsets == nullptr || p->a == nullptr || p->a_sf == nullptr ||

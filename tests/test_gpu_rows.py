@@ -159,3 +159,30 @@ def test_rows_malformed_offsets_refused(cuda_device):
     past[-1] = 301                                 # beyond max_rows
     out, rc, st = _run_rows(P, 256, 512, cuda_device, offsets=past)
     assert st == 0x203 and torch.isnan(out.float()).all()
+
+
+@pytest.mark.parametrize("kind", ["nvfp4", "mxfp4"])
+def test_malformed_offsets_without_rows(cuda_device, kind):
+    """Offsets past zero rows are malformed like any others; good ones leave no status."""
+    import ratchet_b200 as rb
+
+    dev = cuda_device
+    codes = torch.zeros(2, 128, 64, dtype=torch.uint8, device=dev)
+    a = torch.empty(0, 64, dtype=torch.uint8, device=dev)
+    if kind == "nvfp4":
+        sf = torch.zeros(2, 128, 8, dtype=torch.uint8, device=dev)
+        pack = rb.pack_weights(list(codes), list(sf))
+        a_sf = torch.empty(0, 8, dtype=torch.uint8, device=dev)
+        call = lambda off: rb.nvfp4_grouped_gemm_rows(a, a_sf, off, pack=pack)
+    else:
+        sf = torch.zeros(2, 128, 4, dtype=torch.uint8, device=dev)
+        pack = rb.pack_mxfp4_weights(codes, sf)
+        a_sf = torch.empty(0, 4, dtype=torch.uint8, device=dev)
+        call = lambda off: rb.mxfp4_grouped_gemm_rows(a, a_sf, off, pack)
+    good = torch.zeros(3, dtype=torch.int32, device=dev)
+    for bad in ([0, 5, 5], [0, 3, 0], [-1, 0, 0]):
+        call(torch.tensor(bad, dtype=torch.int32, device=dev))
+        with pytest.raises(rb.FggError, match="0x203"):
+            rb.last_status()
+        assert call(good).shape == (0, 128)
+        rb.last_status()
