@@ -40,19 +40,22 @@
 // both.  Nothing waits, and as a + b = b + a the results do not depend on timing.  They
 // may depend, in the last fp32 bits before the rounding, on the call's other tiles.
 //
-// What bounds it: the tensor pipe for groups of about 250 tokens and more, the
-// weights' HBM stream below that, shared-memory bandwidth and the gradient's write
-// for wgrad with short groups; and in seconds-long runs of any of them but the
-// decode shapes the 1000 W cap (clocks of 1.0 to 1.5 GHz), under which what counts
-// is energy: the bytes moved as much as the products.  Measured, bf16, K 2048 to
-// 8192, short bursts / under the cap:
-//   forward 8192^3                             1.37 / 1.35 PFLOP/s (the library's
-//                                              product 1.63 / 1.35)
-//   forward 8 groups, 4352 rows, 4096 x 7168   204 / 238 us, tensor pipe 88 % active,
+// What bounds it: the tensor pipe for groups of about 250 tokens and more (forward,
+// dgrad) or some thousand rows (wgrad), the weights' HBM stream below that in forward
+// and dgrad.  In wgrad with short groups no unit is full: at 256 rows each the SMs' L1,
+// through which the operands come and the gradient leaves, is busiest with 74 %, then
+// DRAM 58 %, L2 52 %, tensor pipe 29 % (groups of 4096 rows: 47, 17, 38 and 73 %).  In
+// seconds-long runs of any of them but the decode shapes it is the 1000 W cap (clocks
+// of 1.0 to 1.5 GHz), under which what counts is energy: the bytes moved as much as
+// the products.  Measured, bf16, short bursts / under the cap (3 to 6 % more on some
+// machines):
+//   forward 8192^3                             1.53 / 1.34 PFLOP/s, tensor pipe 95 %
+//                                              active (the library's product 1.56 / 1.40)
+//   forward 8 groups, 4352 rows, 4096 x 7168   200 / 238 us, tensor pipe 88 % active,
 //                                              582 MB of DRAM reads (541 MB needed)
-//   forward 64 groups, 544 rows, 7168 x 2048   283 us, 6.7 TB/s
-//   dgrad 64 skewed groups, 16384 rows         0.90 / 1.08 ms
-//   wgrad 64 skewed groups, 32768 rows, fp32   1.09 / 1.32 ms
+//   forward 64 groups, 544 rows, 7168 x 2048   280 us, 6.7 TB/s
+//   dgrad 64 skewed groups, 16384 rows         0.90 / 1.10 ms
+//   wgrad 64 skewed groups, 32768 rows, fp32   1.10 / 1.32 ms
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -90,10 +93,12 @@ static_assert(sizeof(F16Slot) == 32, "slot is 8 words");
 // pairs.  A join costs 4 to 5 us, up to 9 where all pairs join at once after few steps,
 // and a step about 0.26 us of a pair.  Unsplit -> split, cold L2, a host call's time with
 // it: one tile of 64 steps in two (a gradient of 64 x 64 over 4096 rows) 31.7 -> 27.6 us,
-// 8 of them (one token, 2048 x 4096) 25.1 -> 23.9, 16 of them 25.9 -> 27.0, 24 of them
-// (256 tokens) 36.3 -> 39.0; one of 128 in four (one token, K 8192) 34.1 -> 23.7; of 470
-// in 14 (30000 rows) 144 -> 38; 32 tiles of 128 in two 53.2 -> 47.1.  Slices of at least
-// 16 steps: 25.4 -> 31.6 us for 16 tiles of 32; of 64: 143 -> 44 for the 30000 rows.
+// 8 of them (one token, 2048 x 4096) 25.6 -> 23.4, 16 of them 25.9 -> 27.0, 24 of them
+// (256 tokens) 36.3 -> 39.0; one of 128 in four (one token, K 8192) 34.1 -> 23.5; of 470
+// in 14 (30000 rows) 144 -> 37; 32 tiles of 128 in two (one token, 8192 x 8192) 50.1 ->
+// 47.9.  With slices of at least 16 steps the 24 tiles of 256 tokens take 43.4 us (36.7),
+// 8 tiles of 94 steps 39.9 (37.8), one tile of 64 steps 25.6 (27.6); of at least 64 the
+// 30000 rows take 43.8 (37.0), one token of 4096 x 14336 60.4 (43.8).
 constexpr int kMaxSplitUnits = 96;
 constexpr int kMaxSlices = 16;
 constexpr int kMinSlice = 32;
@@ -321,9 +326,8 @@ __device__ __forceinline__ void store_sector(uint8_t* at, uint32_t (&v)[8], int 
 // k0 of each.  Neighbouring lanes swap halves of 64 bytes, so that the two of them
 // store 64 contiguous bytes of one row and then of the other: 6.7 TB/s of L2 writes
 // over all SMs (32-byte pieces of 32 rows: 4.6; whole 128-byte lines: 7.5).  Lines
-// would take a turn through shared memory, whose bandwidth is what short tiles run
-// out of: the operands written by TMA and read by the tensor core are 4096 cycles
-// of it in a tile of 512 rows, the turn 2048 more, the stores themselves 1024.
+// would take a turn through shared memory, which made the 64 skewed groups slower
+// (1193 against 1089 us): more traffic of the unit that short groups keep busiest.
 // With accumulate the lane that stores reads what is there and adds: one addition
 // per element.
 template <bool kFp32>
@@ -1037,8 +1041,9 @@ __device__ __forceinline__ int f16_tile_height(int m, int count) {
 // and writes its share of the tile list, group by group; or copies its share of
 // the groups' last rows % 16 rows, with zeros up to 16 (wgrad).  Running the tiles of
 // small groups, bound by their weights' stream, between those of large ones, bound
-// by the tensor pipe, gained 2 % (dgrad, 64 skewed groups) and is left out: under
-// the power cap their costs add up.
+// by the tensor pipe, gained 2 % in dgrad (64 skewed groups) and is left out there:
+// under the power cap their costs add up.  It was not tried in wgrad, where the cap
+// binds less.
 __global__ void __launch_bounds__(256) f16_prepare_kernel(const __grid_constant__ F16PrepParams p) {
   griddep_launch_dependents();
   griddep_wait();
