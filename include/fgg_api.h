@@ -560,8 +560,10 @@ FGG_API int fgg_nvfp4_quantize(const void* x, int32_t x_dtype, int64_t rows, int
 
 /* Synchronises `stream`, then reads the status word a previous GEMM call left
  * in `workspace` (the NVFP4 or MX workspace).  Returns FGG_OK, FGG_ETIMEOUT
- * (a device wait ran out; the kernel stopped early and its output is
- * incomplete) or FGG_ECUDA. */
+ * (the kernel stopped early and its output is incomplete; the detail names the
+ * word: 0x101 to 0x104 a device wait ran out, 0x201 the pack is not of this
+ * problem, 0x202 a tile or weight group outside it, 0x203 malformed offsets,
+ * 0x204 tensor memory at an impossible place) or FGG_ECUDA. */
 FGG_API int fgg_read_device_status(const void* workspace, void* stream);
 
 /* Test hook, no counterpart in the reference: flags applied to every GEMM

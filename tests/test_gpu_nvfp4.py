@@ -358,3 +358,72 @@ def test_calls_of_other_layouts_in_turn(cuda_device):
                     assert ok, st
         else:
             assert all(torch.equal(x, y) for o, f in zip(outs, first) for x, y in zip(o, f))
+
+
+def test_buffers_that_are_shared_reversed_or_apart(cuda_device):
+    """Groups that all read one tensor, that lie in one buffer the other way round, or with
+    rows between them: the results of separate copies."""
+    import ratchet_b200 as rb
+
+    ms, n, k = [40, 40, 40], 256, 512
+    prob, (a, a_sf), _, (b, b_sf), alpha = _list_inputs(ms, n, k, cuda_device, seed=5)
+    pack = rb.pack_weights(b, b_sf)
+    run = lambda x, s: rb.nvfp4_grouped_gemm(x, s, b, b_sf, None, alpha, pack=pack)
+    want = run(a, a_sf)
+    shared = run([a[0]] * 3, [a_sf[0]] * 3)
+    copies = run([a[0].clone() for _ in ms], [a_sf[0].clone() for _ in ms])
+    assert all(torch.equal(x, y) for x, y in zip(shared, copies))
+    back = torch.cat(a[::-1])
+    apart = torch.zeros(3 * 50, k // 2, dtype=torch.uint8, device=cuda_device)
+    for g in range(3):
+        apart[50 * g:50 * g + 40] = a[g]
+    for x in ([back[80:], back[40:80], back[:40]], [apart[50 * g:50 * g + 40] for g in range(3)]):
+        assert all(torch.equal(u, v) for u, v in zip(run(x, a_sf), want))
+    rb.last_status()
+
+
+@pytest.mark.parametrize("one", [False, True], ids=["own buffers", "one buffer"])
+def test_halves_of_a_call_with_many_groups(cuda_device, one):
+    """Prepared once, multiplied several times and in a replayed graph: 130 groups are three
+    launches where each has a buffer of its own."""
+    import ratchet_b200 as rb
+    from ratchet_b200 import _lib, ops
+
+    ms, n, k = [20, 0, 31, 1, 250] * 26, 256, 256
+    prob, own, whole, (b, b_sf), alpha = _list_inputs(ms, n, k, cuda_device, seed=6)
+    a, a_sf = whole if one else own
+    pack = rb.pack_weights(b, b_sf)
+    want = torch.cat(rb.nvfp4_grouped_gemm(a, a_sf, b, b_sf, None, alpha, pack=pack))
+    rb.last_status()
+    L, G = _lib.lib(), len(ms)
+    m = np.asarray(ms, np.int32)
+    pa, psf = ops._ptr_array(a), ops._ptr_array(a_sf)
+    out = torch.full_like(want, float("nan"))
+    p = _lib.FggNvfp4Problem(G, n, k, m.ctypes.data, pa.ctypes.data, psf.ctypes.data,
+                             alpha.data_ptr(), out.data_ptr(), None, G)
+    nbytes = L.fgg_nvfp4_workspace_bytes(p)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=cuda_device)
+
+    def gemm():
+        _lib.check(L.fgg_nvfp4_gemm(p, pack.buf.data_ptr(), ws.data_ptr(), nbytes,
+                                    ops._stream_ptr(cuda_device)), "gemm")
+
+    _lib.check(L.fgg_nvfp4_prepare(p, ws.data_ptr(), nbytes, ops._stream_ptr(cuda_device)), "prepare")
+    for _ in range(3):
+        out.fill_(float("nan"))
+        gemm()
+        assert L.fgg_read_device_status(ws.data_ptr(), ops._stream_ptr(cuda_device)) == 0
+        assert torch.equal(out, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        gemm()
+        gemm()
+    for _ in range(3):
+        out.fill_(float("nan"))
+        graph.replay()
+        assert torch.equal(out, want)
+    status = torch.full((1,), -1, dtype=torch.int32, device=cuda_device)
+    out.fill_(float("nan"))
+    _lib.check(L.fgg_nvfp4_grouped_gemm_noalloc(p, pack.buf.data_ptr(), status.data_ptr(),
+                                                ops._stream_ptr(cuda_device)), "noalloc")
+    assert int(status) == 0 and torch.equal(out, want)
